@@ -11,6 +11,8 @@ device pointers are shared between torch and the kernels.
 import ctypes
 import os
 import subprocess
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 import torch  # noqa: F401  (must precede the CDLL below, see module docstring)
 
@@ -59,11 +61,17 @@ def build(force=False, verbose=False):
     if (not force) and os.path.exists(SO_PATH) and os.path.getmtime(SO_PATH) >= max(
             max(os.path.getmtime(p) for p in SOURCES + HEADERS), os.path.getmtime(os.path.join(INC_PATH, "hpf_hip.h"))):
         return SO_PATH
-    cmd = ["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC", "-I" + INC_PATH,
-           "-o", SO_PATH] + list(SOURCES) + ["-ldl"]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd)
+    # (-packed-fp32-ops: no packed single-precision instructions, some forms of which have given wrong results on this card)
+    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+             "-I" + INC_PATH]
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in SOURCES]
+        cmds = [["hipcc", "-c"] + flags + ["-o", o, s] for s, o in zip(SOURCES, objs)]
+        if verbose:
+            print("\n".join(" ".join(c) for c in cmds))
+        with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+            list(pool.map(subprocess.check_call, cmds))
+        subprocess.check_call(["hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o", SO_PATH] + objs + ["-ldl"])
     return SO_PATH
 
 

@@ -166,8 +166,9 @@ __device__ __forceinline__ float blend_rate(float step, float base, float c, flo
 // a / b for TWO independent pairs, correctly rounded, for operands and quotients in the normal range: the compiler's IEEE
 // expansion of a float32 division (v_div_scale x2, v_rcp, the Newton / residual FMAs, v_div_fmas, v_div_fixup) minus its range
 // handling -- the scale factors are 1 and the fix-up returns the quotient unchanged unless an operand or the quotient is
-// denormal, infinite or NaN -- with the seven FMA-type steps of the two divisions issued as packed instructions
-// (v_pk_fma_f32 / v_pk_mul_f32: two lanes' worth per issue).  The same roundings, so the same bits as `a / b`
+// denormal, infinite or NaN -- with the steps of the two divisions side by side.  (The library is built without packed
+// single-precision instructions, some forms of which have given wrong results on this card: the two-vectors become plain
+// instructions, at the same measured speed.)  The same roundings, so the same bits as `a / b`
 // (tests/test_hip_parity.py::test_lazy_batch_side_kernel_is_the_general_one_bit_for_bit holds the two against each other);
 // a streaming pass over a [rows][256] table does 200 divisions per 832-byte row and was bound by their issue rate, not by
 // memory.  Shapes are >= the prior (0.3) and rates >= a column sum: normal range by construction.
