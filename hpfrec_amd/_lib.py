@@ -25,11 +25,12 @@ SHARD_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_shard.hip")  # host code: one r
 MT_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_mt19937.hip")   # the MT19937 stream of the initial draws (jump-ahead)
 SVI_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_svi_prep.hip") # index structures of a stochastic batch, on the device
 P2P_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_p2p.hip")      # peer-mapped exchange regions (hipIpc*) + their primitives
-SOURCES = (SRC_PATH, SHARD_SRC_PATH, MT_SRC_PATH, SVI_SRC_PATH, P2P_SRC_PATH)
+ADAMW_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_adamw.hip")  # the first-order step over many tensors
+SOURCES = (SRC_PATH, SHARD_SRC_PATH, MT_SRC_PATH, SVI_SRC_PATH, P2P_SRC_PATH, ADAMW_SRC_PATH)
 HEADERS = (os.path.join(_PKG, "csrc", "hpf_p2p_dev.h"),)
 INC_PATH = os.path.join(_ROOT, "include")
 
-HPF_HIP_ABI_VERSION = 24
+HPF_HIP_ABI_VERSION = 25
 
 #: every symbol include/hpf_hip.h declares (tests check the .so exports all of them)
 SYMBOLS = (
@@ -47,6 +48,7 @@ SYMBOLS = (
     "hpf_hip_p2p_region_data", "hpf_hip_p2p_region_set_timeout", "hpf_hip_p2p_region_next_epoch",
     "hpf_hip_p2p_region_status", "hpf_hip_p2p_region_destroy", "hpf_hip_p2p_signal", "hpf_hip_p2p_wait",
     "hpf_hip_p2p_allreduce_vec_f32", "hpf_hip_p2p_pull_f32",
+    "hpf_hip_adamw_step",
 )
 
 _lib = None
@@ -165,6 +167,8 @@ def lib():
     L.hpf_hip_p2p_wait.argtypes = [vp, ci, u32, u32, vp]
     L.hpf_hip_p2p_allreduce_vec_f32.argtypes = [vp, ci, u32, vp, vp]
     L.hpf_hip_p2p_pull_f32.argtypes = [vp, ci, u32, ci, i64, vp, i64, ci, vp]
+    cd, u64 = ctypes.c_double, ctypes.c_uint64
+    L.hpf_hip_adamw_step.argtypes = [vp, ci, ci, ci, ci, vp, ci, vp, cd, cd, cd, cd, u64, ci, vp]
     for s in SYMBOLS:
         getattr(L, s).restype = ci
     L.hpf_hip_p2p_ctrl_bytes.restype = i64

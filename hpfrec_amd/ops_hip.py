@@ -71,6 +71,23 @@ def _svi_coo_struct():
 SviCooDesc = _svi_coo_struct()
 
 
+def _adamw_tensor_struct():
+    import ctypes
+    vp = ctypes.c_void_p
+
+    class AdamwTensor(ctypes.Structure):
+        """hpf_adamw_tensor (include/hpf_hip.h), field for field."""
+        _fields_ = [("param", vp), ("grad", vp), ("m", vp), ("v", vp), ("master", vp), ("m_scale", vp), ("v_scale", vp),
+                    ("n", ctypes.c_int64), ("weight_decay", ctypes.c_double), ("number", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+    return AdamwTensor
+
+
+AdamwTensor = _adamw_tensor_struct()
+
+#: HPF_F32 / HPF_BF16 / HPF_F16
+TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
 class HipOps:
     name = "hip"
 
@@ -86,6 +103,7 @@ class HipOps:
         # guideline 11); 16 rather than 8 evens out the tail: +0.8 % at C3 (6 -- not a multiple -- costs 6 %)
         self.sweep_blocks = max(1, self.cu_count) * int(os.environ.get("HPF_SWEEP_BPC", "16"))
         self.finalize_blocks = max(1, self.cu_count) * int(os.environ.get("HPF_FIN_BPC", "4"))
+        self.adamw_blocks = max(1, self.cu_count) * 8
         self.refresh_blocks = max(1, self.cu_count) * int(os.environ.get("HPF_REFRESH_BPC", "8"))
 
     def _stream(self):
@@ -399,3 +417,16 @@ class HipOps:
                                                     _ptr(rs), _ptr(cs_other), float(top), float(add), float(step),
                                                     float(step_prev), int(mode), k, ld, self._stream()),
                    "hpf_hip_svi_rate_rows_f32")
+
+    # -- first-order training of tables ---------------------------------------------------------
+    def adamw_step(self, tensors, param_type, grad_type, state_bits, step, advance, lr, beta1, beta2, eps, seed):
+        """One AdamW step over `tensors` (rows of AdamwTensor's fields), all of the same types (hpf_hip_adamw_step);
+        hpfrec_amd.adamw.adamw_step checks and groups the arguments."""
+        n = len(tensors)
+        desc = (AdamwTensor * max(1, n))(*tensors)
+        lr_dev = lr if torch.is_tensor(lr) else None
+        with torch.cuda.device(self.device):
+            _lib.check(self.L.hpf_hip_adamw_step(desc, n, TYPE_CODES[param_type], TYPE_CODES[grad_type], int(state_bits),
+                                                 _ptr(step), int(bool(advance)), _ptr(lr_dev), 0.0 if lr_dev is not None else float(lr),
+                                                 float(beta1), float(beta2), float(eps), int(seed) & (2 ** 64 - 1),
+                                                 self.adamw_blocks, self._stream()), "hpf_hip_adamw_step")

@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define HPF_HIP_ABI_VERSION 24
+#define HPF_HIP_ABI_VERSION 25
 
 #define HPF_EINVAL (-1)  /* bad argument (null pointer, k<=0, ld mismatch ...) */
 #define HPF_EUNSUPPORTED (-2) /* k larger than the kernels are instantiated for */
@@ -689,6 +689,41 @@ int hpf_hip_p2p_wait(void *region, int kind, uint32_t epoch, uint32_t src_mask, 
 int hpf_hip_p2p_allreduce_vec_f32(void *region, int which, uint32_t epoch, float *vec, void *stream);
 int hpf_hip_p2p_pull_f32(void *region, int kind, uint32_t epoch, int src_rank, int64_t src_offset_bytes, float *dst,
                          int64_t n, int grid_blocks, void *stream);
+
+/* ---------------------------------------------------------------------------------------------------------------------
+ * First-order training of tables: the step.  (No counterpart in the reference, whose tables only move by natural-gradient
+ * steps: partial_fit, PXI:423-473.)
+ *
+ * One AdamW step (decoupled weight decay) over a list of tensors, up to 40 of them a launch:
+ *   m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g^2
+ *   p <- p (1 - lr weight_decay) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps),   t = *step + 1
+ * `tensors` is read on the HOST during the call; everything it points to is device memory.  step (device, >= 0) becomes t
+ * at the end of the call if `advance` is set, so a captured call counts its replays; lr_dev (device, may be NULL) replaces
+ * lr.  param_type / grad_type: HPF_F32, HPF_BF16 or HPF_F16, alike for all tensors of a call; 16-bit parameters have a
+ * float32 master, which is what the step works on (param = master rounded to nearest).
+ * state_bits 32: m and v float32.  state_bits 8: m and r = sqrt(v) in e4m3 (one byte a value), times the power of two in
+ * m_scale / v_scale that HPF_ADAMW_BLOCK consecutive values share; rounded stochastically with 16 bits that are a function
+ * of (seed, t, number, index) alone; a root above zero keeps at least the smallest code.
+ * A value whose gradient is infinite or NaN gets moments and a parameter that say so; its block's other values do not.
+ */
+#define HPF_F32 0
+#define HPF_BF16 1
+#define HPF_F16 2
+#define HPF_ADAMW_BLOCK 256
+typedef struct hpf_adamw_tensor {
+    void *param;
+    const void *grad;
+    void *m, *v;
+    float *master;            /* float32 master of a 16-bit parameter, else NULL */
+    float *m_scale, *v_scale; /* ceil(n / HPF_ADAMW_BLOCK) each with state_bits 8, else NULL */
+    int64_t n;
+    double weight_decay;
+    int32_t number;           /* part of the key of its random bits */
+    int32_t reserved;
+} hpf_adamw_tensor;
+int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors, int param_type, int grad_type, int state_bits,
+                       int64_t *step, int advance, const float *lr_dev, double lr, double beta1, double beta2, double eps,
+                       uint64_t seed, int grid_blocks, void *stream);
 
 #ifdef __cplusplus
 }
