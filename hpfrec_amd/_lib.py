@@ -26,7 +26,8 @@ MT_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_mt19937.hip")   # the MT19937 stre
 SVI_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_svi_prep.hip") # index structures of a stochastic batch, on the device
 P2P_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_p2p.hip")      # peer-mapped exchange regions (hipIpc*) + their primitives
 ADAMW_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_adamw.hip")  # the first-order step over many tensors
-SOURCES = (SRC_PATH, SHARD_SRC_PATH, MT_SRC_PATH, SVI_SRC_PATH, P2P_SRC_PATH, ADAMW_SRC_PATH)
+SOFTMAX_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_softmax.hip")  # the full-catalogue softmax loss and its gradients
+SOURCES = (SRC_PATH, SHARD_SRC_PATH, MT_SRC_PATH, SVI_SRC_PATH, P2P_SRC_PATH, ADAMW_SRC_PATH, SOFTMAX_SRC_PATH)
 HEADERS = (os.path.join(_PKG, "csrc", "hpf_p2p_dev.h"),)
 INC_PATH = os.path.join(_ROOT, "include")
 
@@ -48,7 +49,7 @@ SYMBOLS = (
     "hpf_hip_p2p_region_data", "hpf_hip_p2p_region_set_timeout", "hpf_hip_p2p_region_next_epoch",
     "hpf_hip_p2p_region_status", "hpf_hip_p2p_region_destroy", "hpf_hip_p2p_signal", "hpf_hip_p2p_wait",
     "hpf_hip_p2p_allreduce_vec_f32", "hpf_hip_p2p_pull_f32",
-    "hpf_hip_adamw_step",
+    "hpf_hip_adamw_step", "hpf_hip_softmax_workspace", "hpf_hip_softmax_nll", "hpf_hip_softmax_nll_grad",
 )
 
 _lib = None
@@ -169,8 +170,12 @@ def lib():
     L.hpf_hip_p2p_pull_f32.argtypes = [vp, ci, u32, ci, i64, vp, i64, ci, vp]
     cd, u64 = ctypes.c_double, ctypes.c_uint64
     L.hpf_hip_adamw_step.argtypes = [vp, ci, ci, ci, ci, vp, ci, vp, cd, cd, cd, cd, u64, ci, vp]
+    L.hpf_hip_softmax_workspace.argtypes = [i64, i64, i64, ci, ci, ci]
+    L.hpf_hip_softmax_nll.argtypes = [vp, i64, vp, i64, vp, vp, cf, i64, i64, i64, ci, vp, vp, vp, i64, ci, vp]
+    L.hpf_hip_softmax_nll_grad.argtypes = [vp, i64, vp, i64, vp, vp, vp, cf, i64, i64, i64, ci, vp, vp, i64, vp, i64, vp, vp, i64, ci, vp]
     for s in SYMBOLS:
         getattr(L, s).restype = ci
+    L.hpf_hip_softmax_workspace.restype = i64
     L.hpf_hip_p2p_ctrl_bytes.restype = i64
     L.hpf_hip_mt19937_scratch_words.restype = i64
     L.hpf_hip_svi_prep_scratch_words.restype = i64

@@ -419,6 +419,31 @@ class HipOps:
                    "hpf_hip_svi_rate_rows_f32")
 
     # -- first-order training of tables ---------------------------------------------------------
+    def _softmax_scratch(self, n, v, k, dtype, grad):
+        size = int(self.L.hpf_hip_softmax_workspace(n, v, k, TYPE_CODES[dtype], int(grad), self.cu_count))
+        _lib.check(min(size, 0), "hpf_hip_softmax_workspace")
+        return torch.empty(size, dtype=torch.uint8, device=self.device)
+
+    def softmax_nll(self, x, ldx, items, ld_items, target, bias, scale, n, v, k, loss, lse):
+        """Loss and log-sum-exp of n rows against a catalogue of v items (hpf_hip_softmax_nll); hpfrec_amd.softmax checks
+        the arguments."""
+        with torch.cuda.device(self.device):
+            ws = self._softmax_scratch(n, v, k, x.dtype, False)
+            _lib.check(self.L.hpf_hip_softmax_nll(_ptr(x), ldx, _ptr(items), ld_items, _ptr(target), _ptr(bias), scale, n, v, k,
+                                                  TYPE_CODES[x.dtype], _ptr(loss), _ptr(lse), _ptr(ws), ws.numel(), self.cu_count,
+                                                  self._stream()), "hpf_hip_softmax_nll")
+
+    def softmax_nll_grad(self, x, ldx, items, ld_items, target, weight, bias, scale, n, v, k, loss, dx, ld_dx, ditems, ld_ditems,
+                         dbias):
+        """softmax_nll with the gradients of sum weight * loss (hpf_hip_softmax_nll_grad); hpfrec_amd.softmax checks the
+        arguments."""
+        with torch.cuda.device(self.device):
+            ws = self._softmax_scratch(n, v, k, x.dtype, True)
+            _lib.check(self.L.hpf_hip_softmax_nll_grad(_ptr(x), ldx, _ptr(items), ld_items, _ptr(target), _ptr(weight), _ptr(bias),
+                                                       scale, n, v, k, TYPE_CODES[x.dtype], _ptr(loss), _ptr(dx), ld_dx, _ptr(ditems),
+                                                       ld_ditems, _ptr(dbias), _ptr(ws), ws.numel(), self.cu_count, self._stream()),
+                       "hpf_hip_softmax_nll_grad")
+
     def adamw_step(self, tensors, param_type, grad_type, state_bits, step, advance, lr, beta1, beta2, eps, seed):
         """One AdamW step over `tensors` (rows of AdamwTensor's fields), all of the same types (hpf_hip_adamw_step);
         hpfrec_amd.adamw.adamw_step checks and groups the arguments."""

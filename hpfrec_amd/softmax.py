@@ -1,0 +1,108 @@
+"""The softmax likelihood of events against the whole catalogue, and its gradients: beside the Poisson likelihood of listed pairs
+(cython_loops_float.calc_llk), what a model is evaluated on and trained with that ranks every item for every event.
+
+Logits are scale * <x[n], items[v]> + bias[v]; they are made and used in pieces and never stored.  Results are torch tensors on
+the device of `ops`; calls are asynchronous on the current stream, take their scratch memory from torch's allocator and keep
+nothing.  The definitions, and what happens to rows without a target, masked items and NaN, are in include/hpf_hip.h
+(hpf_hip_softmax_nll, hpf_hip_softmax_nll_grad).
+"""
+import math
+
+import torch
+
+from .ops_hip import TYPE_CODES
+
+
+def _matrix(t, name, ops, dtype=None, shape=None):
+    """Row stride of a matrix whose rows are contiguous."""
+    if not torch.is_tensor(t) or t.dim() != 2:
+        raise ValueError("%s must be a matrix" % name)
+    if t.dtype not in TYPE_CODES if dtype is None else t.dtype != dtype:
+        raise ValueError("%s must be of %s" % (name, " or ".join(str(d) for d in TYPE_CODES) if dtype is None else dtype))
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), shape))
+    _on(t, name, ops)
+    rows, k = t.shape
+    if k > 1 and t.stride(1) != 1:
+        raise ValueError("%s must have contiguous rows" % name)
+    if rows > 1 and t.stride(0) < k:
+        raise ValueError("%s must have rows that do not overlap" % name)
+    return t.stride(0) if rows > 1 else max(k, t.stride(0))
+
+
+def _vector(t, name, ops, dtype, n):
+    if not torch.is_tensor(t) or t.dtype != dtype or tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous %s vector of %d" % (name, dtype, n))
+    _on(t, name, ops)
+
+
+def _on(t, name, ops):
+    if t.device.type != ops.device.type or ops.device.index not in (None, t.device.index):
+        raise ValueError("%s is on %s, expected %s" % (name, t.device, ops.device))
+
+
+def _inputs(ops, x, items, target, bias, scale):
+    ldx = _matrix(x, "x", ops)
+    n, k = x.shape
+    ldi = _matrix(items, "items", ops, x.dtype, (items.shape[0], k) if torch.is_tensor(items) and items.dim() == 2 else None)
+    v = items.shape[0]
+    if v == 0 or k == 0:
+        raise ValueError("items is empty")
+    if max(n, v) >= 2 ** 30 - 32:
+        raise ValueError("more than 2^30 - 33 rows")
+    _vector(target, "target", ops, torch.int64, n)
+    if bias is not None:
+        _vector(bias, "bias", ops, torch.float32, v)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    return n, v, k, ldx, ldi
+
+
+def softmax_nll(ops, x, items, target, bias=None, scale=1.0):
+    """(loss, lse) of each event: lse[n] = log sum_v exp(scale <x[n], items[v]> + bias[v]), loss[n] = lse[n] minus the
+    target's logit; float32 vectors.
+
+    x       [n, k] float32, bfloat16 or float16, rows contiguous (a stride between them is allowed: `table[:, :k]`)
+    items   [v, k] of the same type
+    target  int64 [n]; negative: no target, loss 0.  An id of v or more gives a loss of NaN
+    bias    float32 [v] or None; -inf (or the type's lowest value) takes an item out.  A masked target's loss is +inf"""
+    n, v, k, ldx, ldi = _inputs(ops, x, items, target, bias, scale)
+    loss, lse = (torch.empty(n, dtype=torch.float32, device=x.device) for _ in range(2))
+    if n:
+        ops.softmax_nll(x, ldx, items, ldi, target, bias, float(scale), n, v, k, loss, lse)
+    return loss, lse
+
+
+def _span(t):
+    if t is None or t.numel() == 0:
+        return None
+    return t.data_ptr(), t.data_ptr() + (sum((s - 1) * d for s, d in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def softmax_nll_grad(ops, x, items, target, weight=None, bias=None, scale=1.0, dx=None, ditems=None, dbias=None):
+    """(loss, dx, ditems, dbias): softmax_nll's loss of each event, and the gradients of sum_n weight[n] * loss[n] in x, items and
+    (None without a bias) bias.  dx and ditems are of x's type, each value rounded once; loss and dbias are float32.
+
+    weight  float32 [n] or None (ones); any sign
+    dx, ditems, dbias  tensors to write to (dx and ditems may have a stride between rows; what lies between is left as it is);
+                       None: new ones.  They must not overlap an input or each other
+
+    A row without a target, with an id of v or more, or with a masked target takes no part in the gradients."""
+    n, v, k, ldx, ldi = _inputs(ops, x, items, target, bias, scale)
+    if weight is not None:
+        _vector(weight, "weight", ops, torch.float32, n)
+    if bias is None and dbias is not None:
+        raise ValueError("dbias without a bias")
+    dx = torch.empty((n, k), dtype=x.dtype, device=x.device) if dx is None else dx
+    ditems = torch.empty((v, k), dtype=x.dtype, device=x.device) if ditems is None else ditems
+    lddx, lddi = _matrix(dx, "dx", ops, x.dtype, (n, k)), _matrix(ditems, "ditems", ops, x.dtype, (v, k))
+    if bias is not None:
+        dbias = torch.empty(v, dtype=torch.float32, device=x.device) if dbias is None else dbias
+        _vector(dbias, "dbias", ops, torch.float32, v)
+    outs, ins = [[s for s in map(_span, ts) if s] for ts in ((dx, ditems, dbias), (x, items, target, bias, weight))]
+    for i, (a, b) in enumerate(outs):
+        if any(a < d and c < b for c, d in outs[:i] + ins):
+            raise ValueError("dx, ditems or dbias overlaps another tensor of the call")
+    loss = torch.empty(n, dtype=torch.float32, device=x.device)
+    ops.softmax_nll_grad(x, ldx, items, ldi, target, weight, bias, float(scale), n, v, k, loss, dx, lddx, ditems, lddi, dbias)
+    return loss, dx, ditems, dbias

@@ -691,8 +691,8 @@ int hpf_hip_p2p_pull_f32(void *region, int kind, uint32_t epoch, int src_rank, i
                          int64_t n, int grid_blocks, void *stream);
 
 /* ---------------------------------------------------------------------------------------------------------------------
- * First-order training of tables: the step.  (No counterpart in the reference, whose tables only move by natural-gradient
- * steps: partial_fit, PXI:423-473.)
+ * First-order training of tables: the step, and the loss that drives it.  (No counterpart in the reference, whose tables
+ * only move by natural-gradient steps: partial_fit, PXI:423-473.)
  *
  * One AdamW step (decoupled weight decay) over a list of tensors, up to 40 of them a launch:
  *   m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g^2
@@ -724,6 +724,30 @@ typedef struct hpf_adamw_tensor {
 int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors, int param_type, int grad_type, int state_bits,
                        int64_t *step, int advance, const float *lr_dev, double lr, double beta1, double beta2, double eps,
                        uint64_t seed, int grid_blocks, void *stream);
+
+/*
+ * Softmax cross entropy of rows against the whole catalogue, and its gradients; the logits are never stored.
+ *   z[i][j] = scale <x[i], items[j]> + bias[j];   lse[i] = log sum_j exp z[i][j];   loss[i] = lse[i] - z[i][target[i]]
+ *   G[i][j] = weight[i] (exp(z[i][j] - lse[i]) - [j == target[i]])
+ *   dx = scale G items;   ditems = scale G^T x;   dbias[j] = sum_i G[i][j]
+ * x [n][k] and items [v][k], both of `type` (HPF_F32 / HPF_BF16 / HPF_F16), with row strides in values; target int64;
+ * weight (NULL: ones), bias (NULL: none), loss, lse (nll only, may be NULL) and dbias (given exactly when bias is) float32.
+ * Sums and statistics are float32; dx and ditems are rounded once, to `type`.  Equal calls give equal results.
+ *   - target < 0: loss 0; target >= v: loss NaN.  Neither takes part in the gradients, whatever its x holds.
+ *   - A logit of -2^126 ln 2 or less is masked (a bias of -inf, or of the type's lowest value): probability zero.  A row
+ *     whose target is masked -- or everything -- has loss +inf and takes no part in the gradients; lse of nothing is -inf.
+ *   - NaN and +inf logits give NaN losses and gradients.
+ * workspace: hpf_hip_softmax_workspace bytes (same sizes, type, grad and cu_count) at a multiple of 256; free again when
+ * the call's work is done.  n, v < 2^30 - 32.  cu_count: compute units the launch grids are made for.
+ */
+int64_t hpf_hip_softmax_workspace(int64_t n, int64_t v, int64_t k, int type, int grad, int cu_count);
+int hpf_hip_softmax_nll(const void *x, int64_t ldx, const void *items, int64_t ld_items, const int64_t *target,
+                        const float *bias, float scale, int64_t n, int64_t v, int64_t k, int type, float *loss, float *lse,
+                        void *workspace, int64_t workspace_bytes, int cu_count, void *stream);
+int hpf_hip_softmax_nll_grad(const void *x, int64_t ldx, const void *items, int64_t ld_items, const int64_t *target,
+                             const float *weight, const float *bias, float scale, int64_t n, int64_t v, int64_t k, int type,
+                             float *loss, void *dx, int64_t ld_dx, void *ditems, int64_t ld_ditems, float *dbias,
+                             void *workspace, int64_t workspace_bytes, int cu_count, void *stream);
 
 #ifdef __cplusplus
 }

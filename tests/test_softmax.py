@@ -1,0 +1,484 @@
+"""The full-catalogue softmax loss and its gradients (hpfrec_amd.softmax, hpf_hip_softmax_nll / _grad): refusals on the CPU,
+results on the GPU against 64-bit arithmetic, alone and followed by the AdamW step."""
+import ctypes
+import math
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+import torch
+
+from hpfrec_amd import _lib, adamw, softmax
+
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+HALF = {F32: U, BF16: 2.0 ** -8, F16: 2.0 ** -11}   # half a step of each type, relative
+
+
+# ---------------------------------------------------------------------------------------------
+# refusals
+# ---------------------------------------------------------------------------------------------
+class _Recorder:
+    device = torch.device("cpu")
+
+    def __init__(self):
+        self.calls = []
+
+    def softmax_nll(self, x, ldx, items, ld_items, *rest):
+        self.calls.append((ldx, ld_items))
+
+    def softmax_nll_grad(self, x, ldx, items, ld_items, target, weight, bias, scale, n, v, k, loss, dx, ld_dx, ditems, ld_ditems, dbias):
+        self.calls.append((ldx, ld_items, ld_dx, ld_ditems))
+
+
+def _good(**change):
+    a = dict(ops=_Recorder(), x=torch.ones(4, 5), items=torch.ones(7, 5), target=torch.zeros(4, dtype=torch.int64), bias=torch.zeros(7))
+    a.update(change)
+    return a
+
+
+def test_row_strides_are_passed_on():
+    a = _good(x=torch.ones(4, 32)[:, :5], items=torch.ones(7, 64)[:, :5])
+    softmax.softmax_nll(**a)
+    softmax.softmax_nll_grad(**a, dx=torch.ones(4, 8)[:, :5])
+    assert a["ops"].calls == [(32, 64), (32, 64, 8, 5)]
+    a = _good(x=torch.ones(1, 32)[:, :5], target=torch.zeros(1, dtype=torch.int64))
+    softmax.softmax_nll(**a)
+    empty = _good(x=torch.ones(0, 5), target=torch.zeros(0, dtype=torch.int64))
+    loss, lse = softmax.softmax_nll(**empty)
+    assert loss.shape == lse.shape == (0,) and empty["ops"].calls == []
+
+
+_REFUSED = [
+    (dict(x=torch.ones(5)), "x must be a matrix"),
+    (dict(x=torch.ones(4, 5, dtype=torch.float64)), "x must be of"),
+    (dict(items=torch.ones(7, 5, dtype=BF16)), "items must be of"),
+    (dict(items=torch.ones(7, 6)), "items has shape"),
+    (dict(items=torch.ones(0, 5), bias=None), "items is empty"),
+    (dict(x=torch.ones(4, 0), items=torch.ones(7, 0)), "items is empty"),
+    (dict(x=torch.ones(5, 4).t()), "contiguous rows"),
+    (dict(x=torch.ones(1, 5).expand(4, 5)), "overlap"),
+    (dict(target=torch.zeros(4, dtype=torch.int32)), "target"),
+    (dict(target=torch.zeros(3, dtype=torch.int64)), "target"),
+    (dict(target=torch.zeros(8, dtype=torch.int64)[::2]), "target"),
+    (dict(bias=torch.zeros(6)), "bias"),
+    (dict(bias=torch.zeros(7, dtype=torch.float64)), "bias"),
+    (dict(scale=float("nan")), "scale"),
+    (dict(scale=float("inf")), "scale"),
+    (dict(ops=SimpleNamespace(device=torch.device("cuda:0"))), "expected cuda"),
+]
+
+
+@pytest.mark.parametrize("call", [softmax.softmax_nll, softmax.softmax_nll_grad])
+@pytest.mark.parametrize("change, words", _REFUSED)
+def test_refusals(call, change, words):
+    with pytest.raises(ValueError, match=words):
+        call(**_good(**change))
+
+
+@pytest.mark.parametrize("change, words", [
+    (dict(weight=torch.ones(5)), "weight"),
+    (dict(weight=torch.ones(4, dtype=torch.int64)), "weight"),
+    (dict(dx=torch.ones(4, 6)), "dx has shape"),
+    (dict(dx=torch.ones(4, 5, dtype=BF16)), "dx must be of"),
+    (dict(ditems=torch.ones(5, 7).t()), "ditems must have contiguous rows"),
+    (dict(dbias=torch.ones(6)), "dbias"),
+    (dict(bias=None, dbias=torch.ones(7)), "dbias without a bias"),
+])
+def test_refusals_of_the_gradients(change, words):
+    with pytest.raises(ValueError, match=words):
+        softmax.softmax_nll_grad(**_good(**change))
+
+
+def test_outputs_that_overlap_are_refused():
+    a = _good()
+    for name, t in (("dx", a["x"]), ("ditems", a["items"]), ("dbias", a["bias"])):
+        with pytest.raises(ValueError, match="overlaps"):
+            softmax.softmax_nll_grad(**a, **{name: t})
+    both = torch.ones(11, 5)
+    with pytest.raises(ValueError, match="overlaps"):
+        softmax.softmax_nll_grad(**a, dx=both[:4], ditems=both[3:10])
+    softmax.softmax_nll_grad(**a, dx=both[:4], ditems=both[4:])
+
+
+def test_c_entries_refuse_before_touching_the_gpu():
+    L = ctypes.CDLL(_lib.build())
+    vp, i64, ci, cf = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+    L.hpf_hip_softmax_workspace.argtypes, L.hpf_hip_softmax_workspace.restype = [i64, i64, i64, ci, ci, ci], i64
+    L.hpf_hip_softmax_nll.argtypes = [vp, i64, vp, i64, vp, vp, cf, i64, i64, i64, ci, vp, vp, vp, i64, ci, vp]
+    L.hpf_hip_softmax_nll_grad.argtypes = [vp, i64, vp, i64, vp, vp, vp, cf, i64, i64, i64, ci, vp, vp, i64, vp, i64, vp, vp, i64, ci, vp]
+    EINVAL, EUNSUPPORTED = -1, -2
+    size = L.hpf_hip_softmax_workspace
+    assert size(-1, 5, 5, 0, 0, 256) == EINVAL and size(5, 0, 5, 0, 0, 256) == EINVAL and size(5, 5, 0, 0, 0, 256) == EINVAL
+    assert size(2 ** 30, 5, 5, 0, 0, 256) == EINVAL and size(5, 5, 5, 0, 0, 0) == EINVAL
+    assert size(5, 5, 5, 3, 0, 256) == EUNSUPPORTED
+    assert size(0, 5, 5, 0, 1, 256) == 0 and size(0, 5, 500, 1, 0, 256) == 0
+    for k in (1, 50, 256, 257, 5000):
+        for kind in (0, 1, 2):
+            assert 0 < size(100, 1000, k, kind, 0, 256) < size(100, 1000, k, kind, 1, 256)
+    buf = ctypes.create_string_buffer(1024)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+
+    def nll(x=p, ldx=5, w=p, ldw=5, t=p, n=4, v=7, k=5, kind=0, loss=p, ws=p, wsize=1 << 40, cus=256):
+        return L.hpf_hip_softmax_nll(x, ldx, w, ldw, t, None, 1.0, n, v, k, kind, loss, None, ws, wsize, cus, None)
+
+    def grad(x=p, ldx=5, w=p, ldw=5, t=p, bias=None, n=4, v=7, k=5, kind=0, loss=p, dx=p, lddx=5, dw=p, lddw=5, db=None, ws=p, wsize=1 << 40):
+        return L.hpf_hip_softmax_nll_grad(x, ldx, w, ldw, t, None, bias, 1.0, n, v, k, kind, loss, dx, lddx, dw, lddw, db, ws, wsize, 256, None)
+
+    for call in (nll, grad):
+        for bad in (dict(x=None), dict(w=None), dict(t=None), dict(loss=None), dict(ws=None), dict(ws=p + 16), dict(ldx=4), dict(ldw=4),
+                    dict(n=-1), dict(v=0), dict(k=0), dict(wsize=1024)):
+            assert call(**bad) == EINVAL, bad
+        assert call(kind=3) == EUNSUPPORTED
+    assert nll(n=0) == 0 and nll(cus=0) == EINVAL
+    for bad in (dict(dx=None), dict(dw=None), dict(lddx=4), dict(lddw=4), dict(bias=p), dict(db=p)):
+        assert grad(**bad) == EINVAL, bad
+
+
+# ---------------------------------------------------------------------------------------------
+# in 64 bits, and how far 32-bit (and 16-bit) arithmetic may be from it
+# ---------------------------------------------------------------------------------------------
+def _exact(x, items, target, weight, bias, scale):
+    x, w = x.double(), items.double()
+    z = scale * (x @ w.t())
+    if bias is not None:
+        z = z + bias.double()
+    lse = torch.logsumexp(z, dim=1)
+    live = target >= 0
+    zt = z.gather(1, target.clamp(min=0)[:, None])[:, 0]
+    loss = torch.where(live, lse - zt, torch.zeros_like(lse))
+    p = torch.exp(z - lse[:, None])
+    g = p.clone()
+    g.scatter_(1, target.clamp(min=0)[:, None], -(p.scatter(1, target.clamp(min=0)[:, None], 0.0).sum(dim=1))[:, None])
+    g = g * (torch.where(live, weight.double() if weight is not None else torch.ones_like(lse), torch.zeros_like(lse)))[:, None]
+    return dict(z=z, lse=lse, loss=loss, g=g, dx=scale * (g @ w), ditems=scale * (g.t() @ x), dbias=g.sum(dim=0), x=x, w=w)
+
+
+def _bounds(e, kind, bias, scale, k, wmax=1.0):
+    """A logit: (6 products x) 2 ceil(k / 32) matrix instructions, each rounding its running sum (by a whole unit at most), what
+    six products of three parts leave out (3 U), the conversion to base 2 (constant, product, sum: 4 U of the size).
+    A share exp(z - lse): twice that error, 2 U of |z - lse| + |lse| for the argument's rounding, 2 U for the function.
+    Sums of V shares (or V, N products): independent roundings, 4 sqrt(count) U; joining pieces a few U more.
+    16-bit types: shares are rounded to the type once more, results too; half's shares below 2^-14 of 2^-14 absolutely."""
+    steps = (6 if kind == F32 else 1) * 2 * max(1, math.ceil(k / 32)) + 4
+    size = abs(scale) * (e["x"].abs() @ e["w"].abs().t())
+    b = torch.where(bias > -1e30, bias, torch.zeros_like(bias)).double().abs() if bias is not None else torch.zeros(e["w"].shape[0], dtype=torch.float64, device=e["x"].device)
+    ez = (2 * U * steps * size + 4 * U * (size + b)).amax(dim=1)                     # per row
+    n, v = e["z"].shape
+    span = torch.where(e["z"] > -1e30, (e["z"] - e["lse"][:, None]).abs(), torch.zeros_like(e["z"]))
+    share = e["g"].abs()
+    total = ez + (16 + 4 * math.sqrt(v)) * U + 2 * U * (torch.exp(-span) * span).sum(dim=1)
+    lse = total + 4 * U * e["lse"].abs()
+    rel = (2 * ez + total + 8 * U * (1 + e["lse"].abs()))[:, None] + 4 * U * span   # of a share, per logit
+    coarse = 0.0 if kind == F32 else HALF[kind]
+    least = 0.0 if kind != F16 else 2.0 ** -38 * wmax
+    long_v, long_n = (32 + 4 * math.sqrt(v)) * U, (32 + 4 * math.sqrt(n)) * U
+    dx = abs(scale) * ((share * (rel + coarse + long_v) + least) @ e["w"].abs()) + HALF[kind] * e["dx"].abs()
+    dw = abs(scale) * ((share * (rel + coarse + long_n) + least).t() @ e["x"].abs()) + HALF[kind] * e["ditems"].abs()
+    if kind == F16:   # subnormal results
+        dx, dw = dx + 2.0 ** -25, dw + 2.0 ** -25
+    db = (share * (rel + long_n)).sum(dim=0) + 4 * U * e["dbias"].abs()
+    return dict(lse=lse, loss=lse + ez + 4 * U * e["loss"].abs(), dx=dx, ditems=dw, dbias=db)
+
+
+def _close(got, e, bounds, names, rows=None):
+    for name, x in zip(names, got):
+        if x is None:
+            continue
+        off = (x.double() - e[name]).abs() - bounds[name]
+        assert bool((off <= 0).all()), (name, float(off.max()), float((off > 0).double().mean()))
+
+
+# ---------------------------------------------------------------------------------------------
+# on the GPU
+# ---------------------------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from hpfrec_amd.ops_hip import HipOps
+    return HipOps("cuda:0")
+
+
+def _case(n, v, k, kind, bias=True, seed=0, spread=2.0, pad=0):
+    gen = torch.Generator(device="cuda:0").manual_seed(seed)
+    normal = lambda *s: torch.randn(s, device="cuda:0", generator=gen)  # noqa: E731
+    s = (spread / math.sqrt(k)) ** 0.5
+    x = torch.full((n, k + pad), 9.0, device="cuda:0").to(kind)[:, :k]
+    w = torch.full((v, k + pad), 9.0, device="cuda:0").to(kind)[:, :k]
+    x.copy_(normal(n, k) * s)
+    w.copy_(normal(v, k) * s)
+    target = torch.randint(0, v, (n,), device="cuda:0", generator=gen)
+    if n > 4:
+        target[::5] = -1
+        target[1::5] = v - 1          # the same item many times
+    weight = normal(n)
+    if n > 4:
+        weight[2::7] = 0.0
+    return dict(x=x, items=w, target=target, weight=weight, bias=normal(v) if bias else None, scale=1.3)
+
+
+def _both(ops, c):
+    nll = softmax.softmax_nll(ops, **{k: v for k, v in c.items() if k != "weight"})
+    grad = softmax.softmax_nll_grad(ops, **c)
+    return nll, grad
+
+
+def _check(ops, c):
+    kind, k = c["x"].dtype, c["x"].shape[1]
+    e = _exact(**c)
+    b = _bounds(e, kind, c["bias"], c["scale"], k, 2 * float(c["weight"].abs().max()) if c["weight"] is not None else 1.0)
+    nll, grad = _both(ops, c)
+    _close(nll, e, b, ("loss", "lse"))
+    _close(grad, e, b, ("loss", "dx", "ditems", "dbias"))
+
+
+SHAPES = [(1, 1, 1), (1, 7, 3), (2, 33, 31), (31, 31, 32), (33, 1000, 50), (32, 32, 64), (65, 97, 33), (129, 4097, 100), (300, 2000, 128),
+          (200, 1500, 200), (77, 640, 256), (40, 500, 257), (100, 1000, 300), (3, 3000, 520), (150, 900, 1000), (1100, 300, 40), (700, 260, 600)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("n, v, k", SHAPES)
+def test_against_64_bits(ops, n, v, k, bias, kind):
+    _check(ops, _case(n, v, k, kind, bias, seed=n + v + k))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("k", [50, 300])
+@pytest.mark.parametrize("scale", [-1.7, 0.0, 1e-3])
+def test_scales_strides_and_no_weights(ops, k, scale, kind):
+    c = _case(70, 500, k, kind, True, seed=3, pad=13)
+    _check(ops, dict(c, scale=scale))
+    _check(ops, dict(c, weight=None))
+    _check(ops, dict(c, weight=c["weight"] * 1e-6))
+    _check(ops, dict(c, weight=torch.zeros_like(c["weight"])))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [20, 200, 400])
+def test_many_rows_and_long_catalogues(ops, k, kind):
+    """Several pieces of both sides, joined."""
+    _check(ops, _case(2500, 6000, k, kind, True, seed=5))
+    _check(ops, _case(40, 60000, k, kind, False, seed=6))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [50, 300])
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("lowest", [float("-inf"), torch.finfo(torch.float32).min])
+def test_masked_items(ops, k, kind, lowest):
+    c = _case(64, 300, k, kind, True, seed=8)
+    out = torch.zeros(300, dtype=torch.bool, device="cuda:0")
+    out[::3] = True
+    out[96:160] = True                       # whole tiles
+    c["bias"] = torch.where(out, lowest, c["bias"])
+    c["target"] = torch.where((c["target"] >= 0) & out[c["target"].clamp(min=0)], 1, c["target"])
+    c["target"][0], c["target"][3] = 0, 99   # masked targets
+    (loss, lse), (gloss, dx, ditems, dbias) = _both(ops, c)
+    gone = torch.zeros(64, dtype=torch.bool, device="cuda:0")
+    gone[0] = gone[3] = True
+    d = dict(c, bias=torch.where(out, float("-inf"), c["bias"]), target=torch.where(gone, -1, c["target"]))
+    e = _exact(**d)
+    b = _bounds(e, kind, d["bias"], c["scale"], k, 2 * float(c["weight"].abs().max()))
+    assert bool(torch.isinf(loss[gone]).all()) and bool((loss[gone] > 0).all()) and torch.equal(loss, gloss)
+    _close((torch.where(gone, 0.0, loss), lse, dx, ditems, dbias), e, b, ("loss", "lse", "dx", "ditems", "dbias"))
+    assert not bool(dx[gone].any()) and not bool(ditems[out].any()) and not bool(dbias[out].any())
+    # nothing left at all
+    c["bias"] = torch.full_like(c["bias"], lowest)
+    (loss, lse), (gloss, dx, ditems, dbias) = _both(ops, c)
+    live = c["target"] >= 0
+    assert bool((lse == float("-inf")).all()) and bool((loss[live] == float("inf")).all()) and not bool(loss[~live].any())
+    assert not bool(dx.any()) and not bool(ditems.any()) and not bool(dbias.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [50, 300])
+@pytest.mark.parametrize("kind", [F32, F16])
+def test_nan_and_padding(ops, k, kind):
+    c = _case(50, 200, k, kind, True, seed=9)
+    clean = _both(ops, c)
+    c["x"][0] = float("nan")                 # row 0 has no target: what it holds reaches no gradient
+    assert c["target"][0] == -1
+    (loss, lse), grad = _both(ops, c)
+    assert float(loss[0]) == 0.0 and math.isnan(float(lse[0])) and torch.equal(lse[1:], clean[0][1][1:])
+    for x, y in zip(grad, clean[1]):
+        assert torch.equal(x, y)
+    c["target"][7] = 200                     # no such item
+    c["x"][7] = float("inf")
+    loss, dx, ditems, dbias = softmax.softmax_nll_grad(ops, **c)
+    d = dict(c, target=c["target"].clone(), x=c["x"].clone())
+    d["target"][7], d["x"][7] = -1, 0.0
+    want = softmax.softmax_nll_grad(ops, **d)
+    assert math.isnan(float(loss[7])) and torch.equal(dx, want[1]) and torch.equal(ditems, want[2]) and torch.equal(dbias, want[3])
+    c["x"][8, k - 1] = float("nan")          # a live row: its loss and dx, and every item
+    loss, dx, ditems, dbias = softmax.softmax_nll_grad(ops, **c)
+    assert math.isnan(float(loss[8])) and bool(torch.isnan(dx[8]).all()) and bool(torch.isfinite(dx[9]).all()) and bool(torch.isnan(ditems).any(dim=1).all())
+    c["x"][8] = 0.0
+    c["items"][5, 0] = float("nan")          # an item: every live row, whether it is the target or not
+    c["target"][9] = 5
+    loss, dx, _, _ = softmax.softmax_nll_grad(ops, **c)
+    live = (c["target"] >= 0)
+    assert bool(torch.isnan(loss[live]).all())
+    loss, lse = softmax.softmax_nll(ops, **{a: b for a, b in c.items() if a != "weight"})
+    assert bool(torch.isnan(loss[live]).all()) and bool(torch.isnan(lse[1:]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [16, 272])
+def test_a_row_that_is_sure_of_its_target(ops, k):
+    """Loss and gradient are far below one and keep their relative accuracy: others / target, not 1 - p."""
+    v = 500
+    x = torch.zeros(4, k, device="cuda:0")
+    items = torch.zeros(v, k, device="cuda:0")
+    items[7, 0] = 1.0
+    items[:, 1] = torch.linspace(-1, 1, v, device="cuda:0")
+    x[:, 0] = torch.tensor([12.0, 25.0, 40.0, 60.0], device="cuda:0")
+    x[:, 1] = 0.5
+    target = torch.full((4,), 7, device="cuda:0")
+    e = _exact(x, items, target, None, None, 1.0)
+    others = torch.exp(e["z"] - e["z"][:, 7:8])[:, torch.arange(v, device="cuda:0") != 7].sum(dim=1)
+    loss, dx, ditems, _ = softmax.softmax_nll_grad(ops, x, items, target)
+    # a logit of 60 is rounded by U of it: 2 x 60 U of the quotient, and some more
+    assert bool(((loss.double() / torch.log1p(others) - 1).abs() <= 400 * U).all())
+    assert bool(((dx[:, 0].double() / (-others / (1 + others)) - 1).abs() <= 400 * U).all())
+    assert bool(((ditems[7, 0].double() / e["ditems"][7, 0] - 1).abs() <= 400 * U))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [24, 290])
+def test_gradients_against_differences(ops, k):
+    """Along random directions: losses are right to 1e-6 of about 7, so that a difference over 2 h = 0.04 is to 4e-4 of N = 60
+    rows' sqrt(60) x 7e-6 / 0.04; third derivatives (of order 1) add h^2 / 6."""
+    c = _case(60, 700, k, F32, True, seed=12)
+    _, dx, ditems, dbias = softmax.softmax_nll_grad(ops, **c)
+    total = lambda d: float((softmax.softmax_nll(ops, **{a: b for a, b in d.items() if a != "weight"})[0].double() * c["weight"].double()).sum())  # noqa: E731
+    gen = torch.Generator(device="cuda:0").manual_seed(1)
+    for name, g in (("x", dx), ("items", ditems), ("bias", dbias)):
+        d = torch.randn(g.shape, device="cuda:0", generator=gen)
+        d /= d.norm()
+        h = 0.02
+        got = (total(dict(c, **{name: c[name] + h * d})) - total(dict(c, **{name: c[name] - h * d}))) / (2 * h)
+        want = float((g.double() * d.double()).sum())
+        assert abs(got - want) <= 1.5e-3, (name, got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, F16])
+@pytest.mark.parametrize("k", [37, 301])
+def test_given_outputs(ops, k, kind):
+    c = _case(45, 130, k, kind, True, seed=13)
+    want = softmax.softmax_nll_grad(ops, **c)
+    dx, dw = torch.full((45, k + 9), 5.0, device="cuda:0").to(kind), torch.full((130, k + 3), 5.0, device="cuda:0").to(kind)
+    db = torch.empty(130, device="cuda:0")
+    got = softmax.softmax_nll_grad(ops, **c, dx=dx[:, :k], ditems=dw[:, :k], dbias=db)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert bool((dx[:, k:] == 5).all()) and bool((dw[:, k:] == 5).all()) and got[3] is db
+
+
+@pytest.mark.gpu
+def test_no_rows(ops):
+    for kind in (F32, BF16):
+        c = _case(1, 40, 10, kind, True)
+        for name in ("x", "target", "weight"):
+            c[name] = c[name][:0]
+        loss, dx, ditems, dbias = softmax.softmax_nll_grad(ops, **c, ditems=torch.full((40, 12), 3.0, device="cuda:0").to(kind)[:, :10])
+        assert loss.shape == (0,) and dx.shape == (0, 10) and not bool(ditems.any()) and not bool(dbias.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind, k", [(F32, 50), (BF16, 200), (F16, 300)])
+def test_equal_calls_streams_and_graphs(ops, kind, k):
+    """Equal bits in every call, on another stream, in two calls at once, and in each replay of a captured call with eager
+    work and synchronisations between them."""
+    c, d = _case(257, 3000, k, kind, True, seed=14), _case(100, 900, k, kind, False, seed=15)
+    want, other = softmax.softmax_nll_grad(ops, **c), softmax.softmax_nll_grad(ops, **d)
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(one):
+            a = softmax.softmax_nll_grad(ops, **c)
+        with torch.cuda.stream(two):
+            b = softmax.softmax_nll_grad(ops, **d)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(a, want)) and all(torch.equal(x, y) for x, y in zip(b[:3], other))
+    inputs = {n: t.clone() if torch.is_tensor(t) else t for n, t in c.items()}
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = softmax.softmax_nll_grad(ops, **inputs)
+        nll = softmax.softmax_nll(ops, **{n: t for n, t in inputs.items() if n != "weight"})
+    for r in range(3):
+        inputs["x"].copy_(c["x"] * (1 + r))
+        graph.replay()
+        d = dict(c, x=(c["x"] * (1 + r)).contiguous())
+        eager, eager_nll = softmax.softmax_nll_grad(ops, **d), softmax.softmax_nll(ops, **{n: t for n, t in d.items() if n != "weight"})
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got + nll, eager + eager_nll))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind, k, bits", [(F32, 30, 32), (F32, 30, 8), (BF16, 260, 32)])
+def test_loss_gradients_and_steps_together(ops, kind, k, bits):
+    """Three training steps -- loss, gradients, AdamW on both tables and the biases -- against the same in 64 bits.  A step moves a
+    value by about lr whatever its gradient's size, so only values whose gradient is far from zero are held: there the
+    gradient's relative error is below 1e-3 (32 bits), and three steps of lr = 1e-3 drift apart by less than 3e-3 lr."""
+    c = _case(90, 400, k, kind, True, seed=16)
+    c["weight"] = c["weight"].abs() + 0.5
+    params = [c["x"], c["items"], c["bias"]]
+    st = adamw.adamw_state(params, bits)
+    wide = [p.double() for p in params]
+    wm, wv = [torch.zeros_like(p) for p in wide], [torch.zeros_like(p) for p in wide]
+    sure = [torch.ones(p.shape, dtype=torch.bool, device="cuda:0") for p in wide]
+    lr, b1, b2, eps, wd = 1e-3, 0.9, 0.999, 1e-8, 0.01
+    for t in range(1, 4):
+        loss, *grads = softmax.softmax_nll_grad(ops, **c)
+        adamw.adamw_step(ops, params, grads, lr=lr, betas=(b1, b2), eps=eps, weight_decay=[wd, wd, 0.0], seed=3, **st)
+        e = _exact(wide[0], wide[1], c["target"], c["weight"], wide[2], c["scale"])
+        for i, g in enumerate((e["dx"], e["ditems"], e["dbias"])):
+            wm[i], wv[i] = b1 * wm[i] + (1 - b1) * g, b2 * wv[i] + (1 - b2) * g * g
+            wide[i] = wide[i] * (1 - lr * (wd if i < 2 else 0.0)) - lr * (wm[i] / (1 - b1 ** t)) / (torch.sqrt(wv[i] / (1 - b2 ** t)) + eps)
+            sure[i] &= g.abs() > 0.05 * g.abs().mean()
+    assert int(st["step"]) == 3 and torch.is_tensor(loss)
+    if kind == F32 and bits == 32:
+        for i, p in enumerate(params):
+            off = (p.double() - wide[i]).abs()
+            assert float(sure[i].double().mean()) > 0.5 and float(off[sure[i]].max()) <= 3e-3 * lr + 4 * U * float(wide[i].abs().max())
+    else:   # 8-bit moments and 16-bit gradients: every step still moves by at most a few lr
+        for i, p in enumerate(params):
+            held = p if st["masters"][i] is None else st["masters"][i]
+            assert float((held.double() - wide[i]).abs().max()) <= 12 * lr + (HALF[kind] * float(wide[i].abs().max()) if kind != F32 else 0.0)
+
+
+@pytest.mark.gpu
+def test_more_than_2_to_the_32_logits(ops):
+    """70,001 rows x 70,001 items: rows and items from all over against 64 bits; and a table of over 2^31 values."""
+    n = v = 70001
+    c = _case(n, v, 16, BF16, True, seed=17)
+    loss, dx, ditems, dbias = softmax.softmax_nll_grad(ops, **c)
+    at = torch.tensor([0, 1, 4097, 35000, n - 2, n - 1], device="cuda:0")
+    few = dict(c, x=c["x"][at], target=c["target"][at], weight=c["weight"][at])
+    e = _exact(**few)
+    b = _bounds(e, BF16, c["bias"], c["scale"], 16, 16.0)
+    _close((loss[at], dx[at]), e, b, ("loss", "dx"))
+    g = torch.zeros(len(at), dtype=torch.float64, device="cuda:0")
+    size = torch.zeros_like(g)
+    for i in range(0, n, 5000):
+        e = _exact(**dict(c, x=c["x"][i:i + 5000], target=c["target"][i:i + 5000], weight=c["weight"][i:i + 5000]))
+        g += e["g"][:, at].sum(dim=0)
+        size += e["g"][:, at].abs().sum(dim=0)
+    assert bool(((dbias[at].double() - g).abs() <= size * (64 + 4 * math.sqrt(n)) * U).all())
+    del c, few, e, dx, ditems
+    v = 2 ** 26 + 77
+    items = torch.zeros((v, 33), dtype=BF16, device="cuda:0")
+    gen = torch.Generator(device="cuda:0").manual_seed(1)
+    items[-300:] = torch.randn((300, 33), device="cuda:0", generator=gen)
+    x = torch.randn((2, 33), device="cuda:0", generator=gen).to(BF16)
+    loss, lse = softmax.softmax_nll(ops, x, items, torch.tensor([v - 1, v - 299], device="cuda:0"))
+    z = x.double() @ items[-300:].double().t()
+    want = torch.log(torch.exp(z).sum(dim=1) + (v - 300))
+    assert bool(((lse.double() - want).abs() <= (64 + 4 * math.sqrt(v)) * U).all())
+    assert bool(((loss.double() - (want - z[[0, 1], [299, 1]])).abs() <= (64 + 4 * math.sqrt(v)) * U).all())
