@@ -7,20 +7,24 @@
 // Every product is a matrix instruction (32 x 32 x 16); a row's statistics are kept in base 2 (z log2(e)).
 //
 // PASSES.  A wavefront keeps 32 (or 64) rows of one matrix in registers -- the STATIONARY rows -- and the other matrix streams
-// by in tiles of 32 rows through shared memory, four or eight wavefronts reading each.  A tile's logits come out with the
-// stationary row in the lane and the streamed row in the register, so that what belongs to a stationary row is a lane's own.
+// by in tiles of 32 rows through shared memory, four wavefronts reading each.  A tile's logits come out with the stationary
+// row in the lane and the streamed row in the register, so that what belongs to a stationary row is a lane's own.
 //   rows pass:   x stationary, w streamed: running maximum and sum of a softmax, and the sum of exp(z - max) w over the tiles
 //                -- dx before its normalisation -- in the same pass, rescaled when a maximum grows
-//   items pass:  w stationary, x streamed: G from the finished lse, and its product with x
+//   items pass:  w stationary, x streamed: G from the finished lse, and its product with x, held relative to the item's largest
 // so the logits are computed twice and nothing of their size is written.  An output register's row (8 (i / 4) + 4 (lane / 32) +
 // i % 4) is not an operand's (8 (lane / 32) + j), but a contraction may take its terms in any order: the second product's
 // other operand is laid out in the order in which the first product's output lies in the registers, and the probabilities
 // never leave the lane that made them.
 //
-// 32-BIT MATRICES are split into three bfloat16 parts (8 + 8 + 8 bits of mantissa) and multiplied in six products, all those
-// of at least 2^-16 of the whole: what is left out is below 2^-24 of |a| |b|, the size of one 32-bit rounding.  bfloat16 and
-// half matrices take one product; their probabilities are rounded to the same type (half: times 2^14, so that 2^-28 of a row's
-// largest is still a normal number), everything else stays in 32 bits.
+// 32-BIT MATRICES are split into two half-precision parts (11 + 11 bits of mantissa and the second's sign: a value is held to
+// 2^-23) and multiplied in three products; the fourth, low times low, is below 2^-22 of |a| |b| and of either sign.  For
+// half's range they are scaled by powers of two: 32 rows share one where rows are multiplied with rows (the largest becomes
+// 2^14 .. 2^15), all rows of a column one where the sum is over rows; what is below 2^-17 of the largest is held to 2^-40 of
+// it.  Probabilities are held times 2^14 relative to a running maximum of their row (or item).  bfloat16 and half matrices
+// take one product; their probabilities are rounded to the same type, everything else stays in 32 bits.
+//
+// A running maximum is rounded up to a whole number: rescaling by a power of two changes no digit.
 //
 // THE TARGET's logit is kept out of the sums and joined at the end: 1 - p(target) is then the sum of the others' shares and not a
 // difference of near equals, and the loss of a row that is sure of its target log1p(others / target).
@@ -51,10 +55,13 @@ struct Hf {
     static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 
-// what a user's matrix is, what it is multiplied in, in how many parts, and the power of two its probabilities are held times
-struct F32 { typedef float t; typedef Bf m; static constexpr int S = 3, shift = 0; };
-struct B16 { typedef __bf16 t; typedef Bf m; static constexpr int S = 1, shift = 0; };
-struct H16 { typedef _Float16 t; typedef Hf m; static constexpr int S = 1, shift = 14; };
+// What a user's matrix is, what it is multiplied in, in how many parts, and the power of two its probabilities are held times;
+// ranged: G is held relative to a running maximum (half's range); scaled: the parts are.
+struct F32 { typedef float t; typedef Hf m; static constexpr int S = 2, shift = 14; static constexpr bool ranged = true, scaled = true; };
+struct B16 { typedef __bf16 t; typedef Bf m; static constexpr int S = 1, shift = 0; static constexpr bool ranged = false, scaled = false; };
+struct H16 { typedef _Float16 t; typedef Hf m; static constexpr int S = 1, shift = 14; static constexpr bool ranged = true, scaled = false; };
+// 32-bit rows over 256 wide: three bfloat16 parts, whose range needs neither scales nor maxima, in six products
+struct W32 { typedef float t; typedef Bf m; static constexpr int S = 3, shift = 0; static constexpr bool ranged = false, scaled = false; };
 
 template <class Y> struct Parts { typename Y::m::v8 p[Y::S]; };   // 8 values of an operand
 
@@ -62,10 +69,11 @@ template <class Y> __device__ __forceinline__ void split(float x, Parts<Y> &to, 
 {
     typedef typename Y::m::e e;
     to.p[0][j] = (e)x;
-    if constexpr (Y::S == 3) {
+    if constexpr (Y::S > 1) {
         const float r = x - (float)to.p[0][j];
         to.p[1][j] = (e)r;
-        to.p[2][j] = (e)(r - (float)to.p[1][j]);
+        if constexpr (Y::S > 2)
+            to.p[2][j] = (e)(r - (float)to.p[1][j]);
     }
 }
 
@@ -76,6 +84,8 @@ template <class Y> __device__ __forceinline__ f32x16 product(const Parts<Y> &a, 
         c = Y::m::mfma(a.p[2], b.p[0], c);
         c = Y::m::mfma(a.p[0], b.p[2], c);
         c = Y::m::mfma(a.p[1], b.p[1], c);
+    }
+    if constexpr (Y::S > 1) {
         c = Y::m::mfma(a.p[1], b.p[0], c);
         c = Y::m::mfma(a.p[0], b.p[1], c);
     }
@@ -90,16 +100,173 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32);
 // A UNIT is one operand of a matrix instruction as it lies in memory: 64 lanes x 8 values, 1 KB.
 constexpr int kUnit = 1024;
 
+// the exponent that brings a largest magnitude into [2^14, 2^15) when it is taken away; 0 for nothing but zeros
+__device__ __forceinline__ int half_exponent(float top) { return top > 0.0f ? (int)(__float_as_uint(top) >> 23) - 127 - 14 : 0; }
+__device__ __forceinline__ float finite_size(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }
+
+__device__ __forceinline__ float wave_max(float m)
+{
+    for (int d = 32; d; d >>= 1)
+        m = fmaxf(m, __shfl_xor(m, d));
+    return m;
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
-// packing: rows [R][K] (row stride ld) -> units.  `by_row`: tile of 32 rows after tile, in it K / 16 units (lane: row lane % 32,
+// Preparation.
+// ---------------------------------------------------------------------------------------------------------------------
+struct PrepArgs {
+    const int64_t *target;
+    const float *bias, *weight;
+    int64_t N, V, np, vp;          // np, vp: padded
+    float *bias2;                  // bias in base 2, -inf beyond the catalogue
+    int32_t *meta;                 // targets as 32-bit numbers, kNoTarget where there is none
+    float *wpow;                   // the smallest power of two above every |weight| (1 if there is none): G is held as a share of it
+    uint32_t *col_top;             // largest magnitudes of the columns (bits): zeros before they are looked for
+    int cols;
+};
+
+// block 0: weights and zeros; the others: an item and a row a thread
+__global__ __launch_bounds__(256) void prepare_kernel(PrepArgs A)
+{
+    if (blockIdx.x == 0) {
+        __shared__ float top[4];
+        for (int c = threadIdx.x; c < A.cols; c += 256)
+            A.col_top[c] = 0;
+        if (!A.wpow)
+            return;
+        float m = 0.0f;
+        if (A.weight) {
+            int64_t n = threadIdx.x;
+            for (; n + 768 < A.N; n += 1024)
+                m = fmaxf(fmaxf(m, fmaxf(fabsf(A.weight[n]), fabsf(A.weight[n + 256]))),
+                          fmaxf(fabsf(A.weight[n + 512]), fabsf(A.weight[n + 768])));
+            for (; n < A.N; n += 256)
+                m = fmaxf(m, fabsf(A.weight[n]));
+        }
+        m = wave_max(m);
+        if ((threadIdx.x & 63) == 0)
+            top[threadIdx.x >> 6] = m;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            int e = 0;
+            if (m > 0.0f && m < INFINITY)
+                frexpf(m, &e);                       // m in [2^(e-1), 2^e)
+            A.wpow[0] = ldexpf(1.0f, e > 100 ? 100 : e < -100 ? -100 : e);
+        }
+        return;
+    }
+    const int64_t i = (int64_t)(blockIdx.x - 1) * 256 + threadIdx.x;
+    if (i < A.vp)
+        A.bias2[i] = i >= A.V ? -INFINITY : A.bias ? A.bias[i] * kLog2e : 0.0f;
+    if (i < A.np) {
+        const int64_t t = i < A.N ? A.target[i] : -1;
+        A.meta[i] = t >= 0 && t < A.V ? (int32_t)t : kNoTarget;
+    }
+}
+
+struct Matrix {
+    const void *p;
+    int64_t ld, rows;
+    const int64_t *target;         // of x with its gradients: rows without a target count as zeros (whatever they hold must not
+    int64_t items;                 // reach a sum)
+    float sign;                    // goes into by_row
+    char *by_row, *by_col;
+    int32_t *exps;                 // scaled: of the tiles, and of the columns (as magnitudes' bits)
+    uint32_t *col_top;
+};
+
+__device__ __forceinline__ bool counts(const Matrix &M, int64_t row) { return row < M.rows && !(M.target && (uint64_t)M.target[row] >= (uint64_t)M.items); }
+
+// largest magnitudes of the columns of both matrices (a wavefront reads whole rows)
+__global__ __launch_bounds__(256) void columns_kernel(Matrix W, Matrix X, int K, int w_blocks)
+{
+    __shared__ float top[4][256];
+    const bool second = (int)blockIdx.x >= w_blocks;
+    const Matrix &M = second ? X : W;
+    const int64_t first = (second ? blockIdx.x - w_blocks : blockIdx.x) * 4 + (threadIdx.x >> 6), step = (second ? gridDim.x - w_blocks : w_blocks) * 4;
+    const int lane = threadIdx.x & 63;
+    float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int64_t r = first; r < M.rows; r += step)
+        if (counts(M, r)) {
+            const float *p = (const float *)M.p + r * M.ld;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (lane + 64 * j < K)
+                    m[j] = fmaxf(m[j], finite_size(p[lane + 64 * j]));
+        }
+    for (int j = 0; j < 4; ++j)
+        top[threadIdx.x >> 6][lane + 64 * j] = m[j];
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c < K)
+        atomicMax(&M.col_top[c], __float_as_uint(fmaxf(fmaxf(top[0][c], top[1][c]), fmaxf(top[2][c], top[3][c]))));
+}
+
+// packing: rows -> units, one workgroup 32 rows.  `by_row`: tile of 32 rows after tile, in it K / 16 units (lane: row lane % 32,
 // columns 16 cb + 8 (lane / 32) + j).  `by_col`: tile after tile, in it (K / 32) x 2 units (lane: column 32 ko + lane % 32, rows
 // 16 t + 8 (j / 4) + 4 (lane / 32) + j % 4: the order of a product's output registers).  Columns and rows beyond the matrix
-// are zero, and so are rows whose target is no item (padding: whatever they hold must not reach a sum).  Bound by memory:
-// one workgroup takes 32 rows x 128 columns through shared memory, read once for both forms.
-// ---------------------------------------------------------------------------------------------------------------------
-template <class Y>
-__global__ __launch_bounds__(256) void pack_kernel(const typename Y::t *src, int64_t ld, int64_t R, int K, int CB, int KO, char *by_row,
-                                                   char *by_col, const int64_t *target, int64_t items, float sign)
+// are zero.  Bound by memory: read once for both forms.
+template <class Y, int KO> __global__ __launch_bounds__(256) void pack_kernel(Matrix W, Matrix X, int K, int w_tiles)
+{
+    constexpr int KP = 32 * KO, CB = 2 * KO;
+    __shared__ float tile[32][KP + 1];
+    __shared__ float tops[4];
+    const bool second = (int)blockIdx.x >= w_tiles;
+    const Matrix &M = second ? X : W;
+    const int64_t rb = second ? blockIdx.x - w_tiles : blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, low = lane & 31, h = lane >> 5;
+    float top = 0.0f;
+    for (int i = 0; i < 8; ++i) {
+        const int r = wave * 8 + i;
+        const int64_t row = rb * 32 + r;
+        const bool in = counts(M, row);
+#pragma unroll
+        for (int j = 0; j < (KP + 63) / 64; ++j) {
+            const int c = lane + 64 * j;
+            const float x = in && c < K ? (float)((const typename Y::t *)M.p)[row * M.ld + c] : 0.0f;
+            if (c < KP)
+                tile[r][c] = x;
+            top = fmaxf(top, finite_size(x));
+        }
+    }
+    if constexpr (Y::scaled) {
+        top = wave_max(top);
+        if (lane == 0)
+            tops[wave] = top;
+    }
+    __syncthreads();
+    int e = 0;
+    if constexpr (Y::scaled) {
+        e = half_exponent(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+        if (threadIdx.x == 0)
+            M.exps[rb] = e;
+    }
+    for (int cb = wave; cb < CB; cb += 4) {
+        Parts<Y> q;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            split<Y>(ldexpf(M.sign * tile[low][16 * cb + 8 * h + j], -e), q, j);
+        for (int s = 0; s < Y::S; ++s)
+            *(typename Y::m::v8 *)(M.by_row + (((rb * CB + cb) * Y::S + s) * 64 + lane) * 16) = q.p[s];
+    }
+    if (!M.by_col)
+        return;
+    for (int u = wave; u < 2 * KO; u += 4) {
+        const int ko = u >> 1, t = u & 1, c = 32 * ko + low;
+        const int ce = Y::scaled && c < K ? half_exponent(__uint_as_float(M.col_top[c])) : 0;
+        Parts<Y> q;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            split<Y>(ldexpf(tile[16 * t + 8 * (j >> 2) + 4 * h + (j & 3)][c], -ce), q, j);
+        for (int s = 0; s < Y::S; ++s)
+            *(typename Y::m::v8 *)(M.by_col + ((((rb * KO + ko) * 2 + t) * Y::S + s) * 64 + lane) * 16) = q.p[s];
+    }
+}
+
+// the same for rows of any width, without scales: 32 rows x 128 columns a workgroup
+template <class Y> __global__ __launch_bounds__(256) void pack_wide_kernel(Matrix M, int K, int CB, int KO)
 {
     __shared__ float tile[32][129];
     const int64_t rb = blockIdx.x;
@@ -108,64 +275,30 @@ __global__ __launch_bounds__(256) void pack_kernel(const typename Y::t *src, int
     for (int i = 0; i < 16; ++i) {
         const int at = i * 256 + threadIdx.x, r = at >> 7, c = c0 + (at & 127);
         const int64_t row = rb * 32 + r;
-        float x = 0.0f;
-        if (row < R && c < K && !(target && (uint64_t)target[row] >= (uint64_t)items))
-            x = (float)src[row * ld + c];
-        tile[r][at & 127] = x;
+        tile[r][at & 127] = c < K && counts(M, row) ? (float)((const typename Y::t *)M.p)[row * M.ld + c] : 0.0f;
     }
     __syncthreads();
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int u = i * 4 + (threadIdx.x >> 6), cb = blockIdx.y * 8 + u;
-        if (by_row && cb < CB) {
+        if (cb < CB) {
             Parts<Y> q;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                split<Y>(sign * tile[low][16 * u + 8 * h + j], q, j);
+                split<Y>(M.sign * tile[low][16 * u + 8 * h + j], q, j);
             for (int s = 0; s < Y::S; ++s)
-                *(typename Y::m::v8 *)(by_row + (((rb * CB + cb) * Y::S + s) * 64 + lane) * 16) = q.p[s];
+                *(typename Y::m::v8 *)(M.by_row + (((rb * CB + cb) * Y::S + s) * 64 + lane) * 16) = q.p[s];
         }
         const int ko = blockIdx.y * 4 + (u >> 1), t = u & 1;
-        if (by_col && ko < KO) {
+        if (M.by_col && ko < KO) {
             Parts<Y> q;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 split<Y>(tile[16 * t + 8 * (j >> 2) + 4 * h + (j & 3)][32 * (u >> 1) + low], q, j);
             for (int s = 0; s < Y::S; ++s)
-                *(typename Y::m::v8 *)(by_col + ((((rb * KO + ko) * 2 + t) * Y::S + s) * 64 + lane) * 16) = q.p[s];
+                *(typename Y::m::v8 *)(M.by_col + ((((rb * KO + ko) * 2 + t) * Y::S + s) * 64 + lane) * 16) = q.p[s];
         }
-    }
-}
-
-// bias in base 2, -inf beyond the catalogue (and nothing but that where there is no bias)
-__global__ void bias_kernel(const float *bias, int64_t V, int64_t padded, float *out)
-{
-    const int64_t v = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (v < padded)
-        out[v] = v >= V ? -INFINITY : bias ? bias[v] * kLog2e : 0.0f;
-}
-
-// the smallest power of two that is no less than any |weight| (1 if there is none): G is held as a share of it
-__global__ __launch_bounds__(1024) void weight_kernel(const float *weight, int64_t N, float *out)
-{
-    __shared__ float top[16];
-    float m = 0.0f;
-    if (weight)
-        for (int64_t n = threadIdx.x; n < N; n += 1024)
-            m = fmaxf(m, fabsf(weight[n]));
-    for (int d = 32; d; d >>= 1)
-        m = fmaxf(m, __shfl_xor(m, d));
-    if ((threadIdx.x & 63) == 0)
-        top[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 16; ++i)
-            m = fmaxf(m, top[i]);
-        int e = 0;
-        if (m > 0.0f && m < INFINITY)
-            frexpf(m, &e);                       // m in [2^(e-1), 2^e)
-        out[0] = ldexpf(1.0f, e > 100 ? 100 : e < -100 ? -100 : e);
     }
 }
 
@@ -175,19 +308,26 @@ __global__ __launch_bounds__(1024) void weight_kernel(const float *weight, int64
 enum { kNll, kRows, kItems };
 
 struct PassArgs {
-    const char *still;        // stationary matrix, by_row
-    const char *by_row;       // streamed matrix
-    const char *by_col;
-    const float *reg_bias;    // per streamed row: rows passes: its bias (base 2); items pass: log2 |weight| - lse
-    const float *lane_bias;   // items pass: the stationary item's bias
-    const int32_t *meta;      // items pass: per streamed row its target and flag; rows passes: per stationary row
-    const float *target_g;    // items pass: per streamed row, G at its target
-    float *stats;             // rows passes: [split][3][still rows]: maximum, sum without the target, target's logit
-    float *part;              // [split][still rows][32 KO]
-    float *part_sum;          // items pass: [split][still rows], sums of G
+    const char *still;              // stationary matrix, by_row
+    const char *by_row, *by_col;    // streamed matrix
+    const int32_t *still_exp, *stream_exp;   // scaled: their tiles'
+    const float *reg_bias;          // per streamed row: rows passes: its bias (base 2); items pass: log2(|weight| / wpow) - lse
+    const float *lane_bias;         // items pass: the stationary item's bias
+    const int32_t *meta;            // items pass: per streamed row its target and flag; rows passes: per stationary row
+    const float *target_log;        // items pass: per streamed row, log2 of |G| at its target
+    float *stats;                   // [split][3][still rows]: maximum, sum (rows: without the target), rows: target's logit
+    float *part;                    // [split][still rows][32 KO]
     int64_t still_tiles, still_rows, stream_tiles;   // tiles of 32; still_rows = 32 still_tiles
-    float c;                  // |scale| log2(e)
+    float c;                        // |scale| log2(e)
     int splits, bias;
+    // items pass in one piece: the results themselves
+    void *out;
+    float *dbias;
+    const uint32_t *col_top;
+    const float *wpow;
+    int64_t ld_out, count;
+    int K, quads;                   // quads: rows of `out` allow four values at once
+    float scale;
 };
 
 // every wavefront's staged units are in shared memory (a barrier alone does not wait for them)
@@ -200,11 +340,12 @@ __device__ __forceinline__ void staged_barrier()
 template <class Y, int KO, int MODE> struct Shape {
     static constexpr int S = Y::S, CB = 2 * KO;
     static constexpr int row_units = CB * S, col_units = MODE == kNll ? 0 : 2 * KO * S, units = row_units + col_units;   // per tile
-    static constexpr int NW = S == 3 && KO == 4 ? 8 : 4;                      // wavefronts
-    static constexpr int QB = (S == 1 && KO <= 4) || KO == 1 ? 2 : 1;         // stationary tiles of a wavefront
+    static constexpr int NW = 4;                                              // wavefronts
+    static constexpr int QB = S * KO <= 2 ? 2 : 1;                            // stationary tiles of a wavefront
     static constexpr int RT = units <= 4 ? 4 : units <= 12 ? 2 : 1;           // streamed tiles a stage
-    static constexpr int bufs = 2 * RT * units > 150 ? 1 : 2;
-    static constexpr int waves = S == 3 && KO == 8 ? 1 : 2;                   // per SIMD: 512 or 256 registers
+    static constexpr int waves = S == 2 && KO > 4 && MODE != kNll ? 1 : 2;    // per SIMD: 512 or 256 registers
+    static constexpr int side = RT * 64 * 4 * (MODE == kItems ? 2 : 1);       // reg_bias (and meta) of a stage: 64 values a tile, 32 of them its own
+    static constexpr int stage = RT * units * kUnit + side;
 };
 
 __device__ __forceinline__ void stage_unit(const char *from, char *to)
@@ -212,41 +353,68 @@ __device__ __forceinline__ void stage_unit(const char *from, char *to)
     __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) const void *)(from + (threadIdx.x & 63) * 16),
                                      (__attribute__((address_space(3))) void *)(uintptr_t)to, 16, 0, 0);
 }
-
-// One block of logits (base 2; lane: stationary row, register: item) into a running softmax: the target's own is taken out to `at`, the
-// rest become probabilities relative to the new maximum (times 2^shift); `rescale(f)` is called where the maximum grew.
-template <class Y, class F>
-__device__ __forceinline__ void online(f32x16 &x, int tile, int h, int target, float &top, float &sum, float &at, const F &rescale)
+__device__ __forceinline__ void stage_words(const void *from, char *to)   // 64 of 32 bits
 {
-    if (__any((target >> 5) == tile))
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (target == tile * 32 + 8 * (i >> 2) + 4 * h + (i & 3)) {
-                at = x[i];
-                x[i] = -INFINITY;
-            }
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) const void *)((const char *)from + (threadIdx.x & 63) * 4),
+                                     (__attribute__((address_space(3))) void *)(uintptr_t)to, 4, 0, 0);
+}
+
+// a sum with its own rounding error carried along
+struct Sum {
+    float s, c;
+    __device__ __forceinline__ void add(float x)
+    {
+        const float y = x - c, t = s + y;
+        c = (t - s) - y;
+        s = t;
+    }
+};
+
+__device__ __forceinline__ float sum16(const f32x16 &x)
+{
+    return (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]))) + (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
+}
+
+// One block of base-2 logarithms (lane: stationary row, register: streamed row) becomes its exponentials relative to a running
+// maximum, times 2^shift; `rescale(f)` is called where the maximum grew.
+template <class Y, class F> __device__ __forceinline__ void exponentials(f32x16 &x, float &top, Sum &sum, const F &rescale)
+{
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i)
         m = fmaxf(m, x[i]);
     m = fmaxf(m, other_half(m));
     if (__any(m > top)) {
-        const float grown = fmaxf(m, top), f = __builtin_amdgcn_exp2f(top - grown);
-        sum *= f;
+        const float grown = m > top ? ceilf(m) : top, f = __builtin_amdgcn_exp2f(top - grown);
+        sum.s *= f;
+        sum.c *= f;
         top = grown;
         rescale(f);
     }
     const float down = (float)Y::shift - top;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 16; ++i)
         x[i] = __builtin_amdgcn_exp2f(x[i] + down);
-        sum += x[i];
-    }
 }
 
-__device__ __forceinline__ void store_stats(float *to, int64_t rows, int h, float top, float sum, float at)
+// the register of a block that holds streamed row r (0 .. 31), for the lanes of half h: i with row_of(i, h) = r
+__device__ __forceinline__ constexpr int row_of(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
+// takes the target's logit out of its block
+__device__ __forceinline__ void take_target(f32x16 &x, int tile, int h, int target, float &at)
 {
-    const float both = sum + other_half(sum), hit = larger(at, other_half(at));
+    if (__any((target >> 5) == tile))
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (target == tile * 32 + row_of(i, h)) {
+                at = x[i];
+                x[i] = -INFINITY;
+            }
+}
+
+__device__ __forceinline__ void store_stats(float *to, int64_t rows, int h, float top, const Sum &sum, float at)
+{
+    const float both = sum.s + other_half(sum.s), hit = larger(at, other_half(at));
     if (h == 0) {
         to[0] = top;
         to[rows] = both;
@@ -254,12 +422,15 @@ __device__ __forceinline__ void store_stats(float *to, int64_t rows, int h, floa
     }
 }
 
+// x 2^e for whole numbers held as floats (very low ones: a maximum of nothing)
+__device__ __forceinline__ float times_power(float x, float e) { return ldexpf(x, (int)fmaxf(e, -1000.0f)); }
+
 template <class Y, int KO, int MODE>
 __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>::waves)) void pass_kernel(PassArgs A)
 {
     typedef Shape<Y, KO, MODE> Z;
     constexpr int S = Z::S, CB = Z::CB, QB = Z::QB, RT = Z::RT, NW = Z::NW;
-    __shared__ __attribute__((aligned(1024))) char lds[Z::bufs][RT * Z::units * kUnit];
+    __shared__ __attribute__((aligned(1024))) char lds[2][Z::stage];
 
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -269,7 +440,7 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
     const int64_t g0 = groups * sp / A.splits, g1 = groups * (sp + 1) / A.splits;
 
     Parts<Y> still[QB][CB];
-    int target[QB];
+    int target[QB], still_exp[QB];
     float lane_bias[QB];
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
@@ -282,14 +453,16 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
             }
         target[q] = MODE != kItems && in ? A.meta[(q0 + q) * 32 + low] : kNoTarget;
         lane_bias[q] = MODE == kItems && in && A.bias ? A.lane_bias[(q0 + q) * 32 + low] : 0.0f;
+        still_exp[q] = Y::scaled && in ? A.still_exp[q0 + q] : 0;
     }
 
     f32x16 acc[QB][MODE == kNll ? 1 : KO];
-    float top[QB], sum[QB], at[QB];
+    float top[QB], at[QB];
+    Sum sum[QB];
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
-        top[q] = kNothing;
-        sum[q] = 0.0f;
+        top[q] = MODE == kItems && !Y::ranged ? 0.0f : kNothing;
+        sum[q] = {0.0f, 0.0f};
         at[q] = -INFINITY;
         if constexpr (MODE != kNll)
             for (int ko = 0; ko < KO; ++ko)
@@ -309,6 +482,11 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
                 if (u + wave < RT * Z::col_units)
                     stage_unit(from + (u + wave) * kUnit, &lds[buf][(RT * Z::row_units + u + wave) * kUnit]);
         }
+        if (wave < RT) {
+            stage_words(A.reg_bias + (g * RT + wave) * 32, &lds[buf][RT * Z::units * kUnit + wave * 256]);
+            if constexpr (MODE == kItems)
+                stage_words(A.meta + (g * RT + wave) * 32, &lds[buf][RT * Z::units * kUnit + (RT + wave) * 256]);
+        }
     };
     auto fetch = [&](const char *unit) {
         Parts<Y> x;
@@ -317,88 +495,97 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
         return x;
     };
 
-    if (Z::bufs == 2 && g0 < g1)
+    if (g0 < g1)
         stage(g0, 0);
     for (int64_t g = g0; g < g1; ++g) {
-        int buf = 0;
-        if constexpr (Z::bufs == 2) {
-            buf = (int)(g - g0) & 1;
-            staged_barrier();                     // this group has arrived, and the other buffer has been read
-            if (g + 1 < g1)
-                stage(g + 1, buf ^ 1);
-        } else {
-            __syncthreads();
-            stage(g, 0);
-            staged_barrier();
-        }
+        const int buf = (int)(g - g0) & 1;
+        staged_barrier();                         // this group has arrived, and the other buffer has been read
+        if (g + 1 < g1)
+            stage(g + 1, buf ^ 1);
 #pragma unroll 1
         for (int rt = 0; rt < RT; ++rt) {
             const int64_t tile = g * RT + rt;
             if (tile >= A.stream_tiles)
                 break;
             const char *rows = &lds[buf][rt * Z::row_units * kUnit], *cols = &lds[buf][(RT * Z::row_units + rt * Z::col_units) * kUnit];
+            const char *side = &lds[buf][RT * Z::units * kUnit + rt * 256];
             const bool biased = MODE == kItems || A.bias || tile == A.stream_tiles - 1;
-            f32x4 rb[4];
-            if (biased)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    rb[i] = *(const f32x4 *)(A.reg_bias + tile * 32 + 8 * i + 4 * h);
-            int meta = 0;
-            if constexpr (MODE == kItems)
-                meta = A.meta[tile * 32 + low];
+            const int stream_exp = Y::scaled ? A.stream_exp[tile] : 0;
 
             f32x16 z[QB];
 #pragma unroll
             for (int q = 0; q < QB; ++q)
                 z[q] = (f32x16)(0.0f);
+            Parts<Y> a = fetch(rows);
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) {
-                const Parts<Y> a = fetch(rows + cb * S * kUnit);
+                const Parts<Y> now = a;
+                if (cb + 1 < CB)
+                    a = fetch(rows + (cb + 1) * S * kUnit);
 #pragma unroll
                 for (int q = 0; q < QB; ++q)
-                    z[q] = product<Y>(a, still[q][cb], z[q]);
+                    z[q] = product<Y>(now, still[q][cb], z[q]);
             }
 
             Parts<Y> p[QB][2];
 #pragma unroll
             for (int q = 0; q < QB; ++q) {
                 f32x16 &x = z[q];
-                if constexpr (MODE == kItems) {
+                const float c = Y::scaled ? ldexpf(A.c, stream_exp + still_exp[q]) : A.c;
+                if (biased) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 b = *(const f32x4 *)(side + (8 * i + 4 * h) * 4);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            x[4 * i + j] = fmaf(x[4 * i + j], c, b[j]);
+                    }
+                } else {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], A.c, rb[i >> 2][i & 3] + lane_bias[q]));
-                    if (__any(meta & kNegative))
+                        x[i] *= c;
+                }
+                const auto rescale = [&](float f) {
+                    if constexpr (MODE != kNll)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (__shfl(meta, 8 * (i >> 2) + 4 * h + (i & 3)) & kNegative)
-                                x[i] = -x[i];
-                    if (__any(((meta & ~kNegative) >> 5) == (int)(q0 + q)))
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int r = 8 * (i >> 2) + 4 * h + (i & 3);
-                            if ((__shfl(meta, r) & ~kNegative) == (int)(q0 + q) * 32 + low)
-                                x[i] = A.target_g[tile * 32 + r];
-                        }
+                        for (int ko = 0; ko < KO; ++ko)
+                            acc[q][ko] *= f;
+                };
+                if constexpr (MODE == kItems) {
                     if (A.bias)
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            sum[q] += x[i];
-                } else {
-                    if (biased) {
+                            x[i] += lane_bias[q];
+                    const int meta = ((const int32_t *)(side + RT * 256))[low];
+                    unsigned flip = 0;             // registers of negative G: negative weights, and targets of positive ones
+                    const bool hit = __any(((meta & ~kNegative) >> 5) == (int)(q0 + q)), negative = __any(meta & kNegative);
+                    if (hit || negative) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            x[i] = fmaf(x[i], A.c, rb[i >> 2][i & 3]);
+                        for (int i = 0; i < 16; ++i) {
+                            const int r = row_of(i, h), of = __shfl(meta, r);
+                            const bool mine = (of & ~kNegative) == (int)(q0 + q) * 32 + low;
+                            if (mine)
+                                x[i] = A.target_log[tile * 32 + r];
+                            flip |= (unsigned)(mine != ((of & kNegative) != 0)) << i;
+                        }
+                    }
+                    if constexpr (Y::ranged) {
+                        exponentials<Y>(x, top[q], sum[q], rescale);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            x[i] = x[i] * A.c;
+                            x[i] = __builtin_amdgcn_exp2f(x[i]);
                     }
-                    online<Y>(x, (int)tile, h, target[q], top[q], sum[q], at[q], [&](float f) {
-                        if constexpr (MODE == kRows)
+                    if (hit || negative)
 #pragma unroll
-                            for (int ko = 0; ko < KO; ++ko)
-                                acc[q][ko] *= f;
-                    });
+                        for (int i = 0; i < 16; ++i)
+                            x[i] = flip >> i & 1 ? -x[i] : x[i];
+                    if (A.bias)
+                        sum[q].add(sum16(x));
+                } else {
+                    take_target(x, (int)tile, h, target[q], at[q]);
+                    exponentials<Y>(x, top[q], sum[q], rescale);
+                    sum[q].add(sum16(x));
                 }
                 if constexpr (MODE != kNll)
 #pragma unroll
@@ -406,16 +593,18 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
                         split<Y>(x[i], p[q][i >> 3], i & 7);
             }
 
-            if constexpr (MODE != kNll)
+            if constexpr (MODE != kNll) {
+                a = fetch(cols);
 #pragma unroll
-                for (int ko = 0; ko < KO; ++ko)
+                for (int u = 0; u < 2 * KO; ++u) {
+                    const Parts<Y> now = a;
+                    if (u + 1 < 2 * KO)
+                        a = fetch(cols + (u + 1) * S * kUnit);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const Parts<Y> a = fetch(cols + (ko * 2 + t) * S * kUnit);
-#pragma unroll
-                        for (int q = 0; q < QB; ++q)
-                            acc[q][ko] = product<Y>(a, p[q][t], acc[q][ko]);
-                    }
+                    for (int q = 0; q < QB; ++q)
+                        acc[q][u >> 1] = product<Y>(now, p[q][u & 1], acc[q][u >> 1]);
+                }
+            }
         }
     }
 
@@ -424,13 +613,36 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
         if (q0 + q >= A.still_tiles)
             break;
         const int64_t row = (q0 + q) * 32 + low;
-        if constexpr (MODE == kItems) {
-            const float both = sum[q] + other_half(sum[q]);
-            if (A.bias && h == 0)
-                A.part_sum[sp * A.still_rows + row] = both;
-        } else {
-            store_stats(A.stats + (int64_t)sp * 3 * A.still_rows + row, A.still_rows, h, top[q], sum[q], at[q]);
+        if (MODE == kItems && A.out) {             // the whole sum: the gradients themselves
+            const float both = sum[q].s + other_half(sum[q].s), wpow = *A.wpow, e = top[q] - (float)Y::shift;
+            if (row < A.count) {
+                if (A.dbias && h == 0)
+                    A.dbias[row] = times_power(both * wpow, e);
+                typedef typename Y::t T;
+                T *to = (T *)A.out + row * A.ld_out;
+                if constexpr (MODE != kNll)
+#pragma unroll
+                    for (int ko = 0; ko < KO; ++ko)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int k = 32 * ko + 8 * i + 4 * h;
+                            struct alignas(4 * sizeof(T)) Quad { T v[4]; } o;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int ce = Y::scaled && k + j < A.K ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
+                                o.v[j] = (T)times_power(acc[q][ko][4 * i + j] * (A.scale * wpow), e + (float)ce);
+                            }
+                            if (A.quads && k + 4 <= A.K)
+                                *(Quad *)(to + k) = o;
+                            else
+                                for (int j = 0; j < 4; ++j)
+                                    if (k + j < A.K)
+                                        to[k + j] = o.v[j];
+                        }
+            }
+            continue;
         }
+        store_stats(A.stats + (int64_t)sp * 3 * A.still_rows + row, A.still_rows, h, top[q], sum[q], at[q]);
         if constexpr (MODE != kNll) {
             float *to = A.part + (sp * A.still_rows + row) * (32 * KO) + 4 * h;
 #pragma unroll
@@ -511,7 +723,7 @@ __device__ __forceinline__ void wide_core(char *lds, int64_t groups, int steps, 
 
 struct WideArgs {
     const char *w, *x;              // by_row units
-    const float *bias, *reg_bias, *target_g;
+    const float *bias, *reg_bias, *target_log;
     const int32_t *meta;
     float *stats, *part_sum;
     char *g_rows, *g_items;         // G of a chunk: rows n / contraction v, and rows v / contraction n
@@ -548,13 +760,14 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(W
     const int64_t n0 = (int64_t)(blockIdx.x / A.splits) * 4;
     const int64_t all = (A.v_tiles + 3) / 4, g0 = all * sp / A.splits, g1 = all * (sp + 1) / A.splits;
     int target[2];
-    float top[2], sum[2], at[2];
+    float top[2], at[2];
+    Sum sum[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int64_t tile = n0 + 2 * wb + j;
         target[j] = tile < A.n_tiles ? A.meta[tile * 32 + low] : kNoTarget;
         top[j] = kNothing;
-        sum[j] = 0.0f;
+        sum[j] = {0.0f, 0.0f};
         at[j] = -INFINITY;
     }
     wide_core<Y, Z>(
@@ -571,7 +784,9 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(W
                 for (int j = 0; j < 2; ++j) {
                     f32x16 &x = acc[i][j];
                     wide_bias(x, A, tile, h);
-                    online<Y>(x, (int)tile, h, target[j], top[j], sum[j], at[j], [](float) {});
+                    take_target(x, (int)tile, h, target[j], at[j]);
+                    exponentials<Y>(x, top[j], sum[j], [](float) {});
+                    sum[j].add(sum16(x));
                 }
             }
         });
@@ -603,7 +818,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
         const bool in = tile < A.n_tiles;
         meta[j] = in ? A.meta[tile * 32 + low] : kNoTarget;
         down[j] = in ? A.reg_bias[tile * 32 + low] : -INFINITY;
-        tg[j] = in ? A.target_g[tile * 32 + low] : 0.0f;
+        tg[j] = in ? A.target_log[tile * 32 + low] : 0.0f;
     }
     wide_core<Y, Z>(
         lds, 1, A.CB / Z::KC,
@@ -624,16 +839,22 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
                     f32x16 &x = acc[i][j];
                     wide_bias(x, A, tile, h);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        x[r] = __builtin_amdgcn_exp2f(x[r] + down[j]);
-                        if (meta[j] & kNegative)
-                            x[r] = -x[r];
-                    }
-                    if (__any(((meta[j] & ~kNegative) >> 5) == (int)tile))
+                    for (int r = 0; r < 16; ++r)
+                        x[r] += down[j];
+                    const bool hit = __any(((meta[j] & ~kNegative) >> 5) == (int)tile);
+                    unsigned flip = meta[j] & kNegative ? 0xFFFFu : 0u;
+                    if (hit)
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
-                            if ((meta[j] & ~kNegative) == (int)tile * 32 + 8 * (r >> 2) + 4 * h + (r & 3))
+                            if ((meta[j] & ~kNegative) == (int)tile * 32 + row_of(r, h)) {
                                 x[r] = tg[j];
+                                flip ^= 1u << r;
+                            }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        x[r] = __builtin_amdgcn_exp2f(x[r] + (float)Y::shift);
+                        x[r] = flip >> r & 1 ? -x[r] : x[r];
+                    }
                     total += x;
                     Parts<Y> p[2];
 #pragma unroll
@@ -645,7 +866,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
                             *(typename Y::m::v8 *)(A.g_rows + (((nt * A.v_count + vt) * 2 + t) * S + s) * kUnit + lane * 16) = p[t].p[s];
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
-                            turn[low][8 * (r >> 2) + 4 * h + (r & 3)] = p[r >> 3].p[s][r & 7];
+                            turn[low][row_of(r, h)] = p[r >> 3].p[s][r & 7];
                         // (one wavefront's own block: its accesses to shared memory are served in order)
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -653,7 +874,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
                             typename Y::m::v8 q;
 #pragma unroll
                             for (int r = 0; r < 8; ++r)
-                                q[r] = turn[16 * t + 8 * (r >> 2) + 4 * h + (r & 3)][low];
+                                q[r] = turn[16 * t + row_of(r, h)][low];
                             *(typename Y::m::v8 *)(A.g_items + (((vt * A.n_tiles + nt) * 2 + t) * S + s) * kUnit + lane * 16) = q;
                         }
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -666,7 +887,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
                         for (int d = 16; d; d >>= 1)
                             v += __shfl_xor(v, d);
                         if (low == 0)
-                            A.part_sum[((n0 / 2 + wb) * A.v_count + vt) * 32 + 8 * (r >> 2) + 4 * h + (r & 3)] = v;
+                            A.part_sum[((n0 / 2 + wb) * A.v_count + vt) * 32 + row_of(r, h)] = v;
                     }
                 }
             }
@@ -711,32 +932,23 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_product_kernel
                     float *to = A.part + ((sp * A.a_tiles + mt) * 32) * (int64_t)(32 * A.KO) + 32 * ko + low;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        float *o = to + (8 * (r >> 2) + 4 * h + (r & 3)) * (int64_t)(32 * A.KO);
+                        float *o = to + (row_of(r, h)) * (int64_t)(32 * A.KO);
                         *o = A.more ? *o + acc[i][j][r] : acc[i][j][r];
                     }
                 }
         });
 }
 
-// meta of the rows before their passes: targets as 32-bit numbers
-__global__ void targets_kernel(const int64_t *target, int64_t N, int64_t V, int64_t padded, int32_t *meta)
-{
-    const int64_t n = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (n < padded) {
-        const int64_t t = n < N ? target[n] : -1;
-        meta[n] = t >= 0 && t < V ? (int32_t)t : kNoTarget;
-    }
-}
-
 // ---------------------------------------------------------------------------------------------------------------------
-// Joins a row's splits: loss and lse, what the items pass needs of the row, and dx (a wavefront a row).
+// Joins a row's splits: loss and lse, what the items' side needs of the row, and dx (a workgroup a row).
 // ---------------------------------------------------------------------------------------------------------------------
 struct FinishArgs {
     const float *stats, *part;
     const int64_t *target;
     const float *weight, *wpow;
     const void *w;                 // items, for the target's own row
-    float *loss, *lse, *reg_bias, *target_g;
+    const uint32_t *col_top;
+    float *loss, *lse, *reg_bias, *target_log;
     int32_t *meta;
     void *dx;
     int64_t N, V, rows, ldw, lddx;
@@ -746,29 +958,48 @@ struct FinishArgs {
 
 template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows_kernel(FinishArgs A)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= A.rows)
-        return;
+    __shared__ float join[4][3];
+    __shared__ float pieces[4][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t n = blockIdx.x;
     if (n >= A.N) {                // rows that only fill the last tile: no share of any sum
-        if (GRAD && lane == 0) {
-            A.reg_bias[n] = -INFINITY;
-            A.target_g[n] = 0.0f;
+        if (GRAD && threadIdx.x == 0) {
+            A.reg_bias[n] = A.target_log[n] = -INFINITY;
             A.meta[n] = kNoTarget;
         }
         return;
     }
-    float top = kNothing, others = 0.0f, at = -INFINITY;
-    for (int s = 0; s < A.splits; ++s) {
+    // splits over the threads: maxima first, then sums relative to them
+    float top = kNothing, at = -INFINITY, others = 0.0f;
+    for (int s = threadIdx.x; s < A.splits; s += 256) {
         top = fmaxf(top, A.stats[(3 * s + 0) * A.rows + n]);
         at = larger(at, A.stats[(3 * s + 2) * A.rows + n]);
     }
-    for (int s = 0; s < A.splits; ++s)
-        others += A.stats[(3 * s + 1) * A.rows + n] * __builtin_amdgcn_exp2f(A.stats[3 * s * A.rows + n] - top);
-    others *= __builtin_amdgcn_exp2f(-(float)Y::shift);
+    for (int d = 32; d; d >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, d));
+        at = larger(at, __shfl_xor(at, d));
+    }
+    if (lane == 0) {
+        join[wave][0] = top;
+        join[wave][1] = at;
+    }
+    __syncthreads();
+    for (int i = 0; i < 4; ++i) {
+        top = fmaxf(top, join[i][0]);
+        at = larger(at, join[i][1]);
+    }
+    for (int s = threadIdx.x; s < A.splits; s += 256)
+        others += times_power(A.stats[(3 * s + 1) * A.rows + n], A.stats[3 * s * A.rows + n] - top);
+    for (int d = 32; d; d >>= 1)
+        others += __shfl_xor(others, d);
+    if (lane == 0)
+        join[wave][2] = others;
+    __syncthreads();
+    others = ldexpf((join[0][2] + join[1][2]) + (join[2][2] + join[3][2]), -Y::shift);
+
     // `top` is that of the others; the target's own logit may be far above it
-    const float peak = fmaxf(top, at);
-    const float rest = others * __builtin_amdgcn_exp2f(top - peak), own = __builtin_amdgcn_exp2f(at - peak), all = rest + own;
+    const float peak = fmaxf(top, ceilf(at));
+    const float rest = times_power(others, top - peak), own = __builtin_amdgcn_exp2f(at - peak), all = rest + own;
     const float lse2 = all > 0.0f || all != all ? peak + log2f(all) : -INFINITY;
     const int64_t t = A.target[n];
     float loss = 0.0f;
@@ -786,58 +1017,91 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
             loss = (lse2 - at) * kLn2;
         }
     }
-    if (lane == 0) {
+    if (threadIdx.x == 0) {
         A.loss[n] = loss;
         if (A.lse)
             A.lse[n] = lse2 * kLn2;
     }
     if constexpr (GRAD) {
-        const float weight = alive ? (A.weight ? A.weight[n] : 1.0f) : 0.0f, wpow = *A.wpow;
-        const float gt = -(weight / wpow) * (rest / all);          // G at the target, as a share of wpow
-        if (lane == 0) {
-            A.reg_bias[n] = alive ? (log2f(fabsf(weight) / wpow) - lse2) + (float)Y::shift : -INFINITY;
-            A.target_g[n] = alive ? gt * __builtin_amdgcn_exp2f((float)Y::shift) : 0.0f;
+        const float weight = alive ? (A.weight ? A.weight[n] : 1.0f) : 0.0f, share = fabsf(weight) / *A.wpow;
+        if (threadIdx.x == 0) {
+            A.reg_bias[n] = alive ? log2f(share) - lse2 : -INFINITY;
+            A.target_log[n] = alive ? log2f(share * (rest / all)) : -INFINITY;
             A.meta[n] = alive ? (int32_t)t | (weight < 0.0f ? kNegative : 0) : kNoTarget;
         }
         if (!A.dx)
             return;
-        typedef typename Y::t T;
-        T *dx = (T *)A.dx + n * A.lddx;
-        const T *w = (const T *)A.w + (alive ? t : 0) * A.ldw;
-        const float share = weight / all * __builtin_amdgcn_exp2f(top - peak - (float)Y::shift);
-        for (int k = lane; k < A.K; k += 64) {
-            float sum = 0.0f;
-            if (alive) {
-                for (int s = 0; s < A.splits; ++s)
-                    sum += A.part[(s * A.rows + n) * A.KP + k] * __builtin_amdgcn_exp2f(A.stats[3 * s * A.rows + n] - top);
-                sum = A.scale * (sum * share + gt * wpow * (float)w[k]);
+        // dx: a quarter of the splits a wavefront
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (alive) {
+#pragma unroll 4
+            for (int s = wave; s < A.splits; s += 4) {
+                const float down = A.stats[3 * s * A.rows + n] - top;
+                const float *p = A.part + (s * A.rows + n) * A.KP;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (lane + 64 * j < A.K)
+                        sum[j] += times_power(p[lane + 64 * j], down);
             }
-            dx[k] = (T)sum;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            pieces[wave][lane + 64 * j] = sum[j];
+        __syncthreads();
+        const int k = threadIdx.x;
+        if (k < A.K) {
+            float v = 0.0f;
+            if (alive) {
+                const int ce = Y::scaled ? half_exponent(__uint_as_float(A.col_top[k])) : 0;
+                v = times_power((pieces[0][k] + pieces[1][k]) + (pieces[2][k] + pieces[3][k]), top - peak - (float)Y::shift + (float)ce);
+                v = A.scale * weight * (v / all - rest / all * (float)((const typename Y::t *)A.w)[t * A.ldw + k]);
+            }
+            ((typename Y::t *)A.dx)[n * A.lddx + k] = (typename Y::t)v;
         }
     }
 }
 
 // joins the splits of a product with G: out = scale wpow sum, dbias = wpow sum (a wavefront a row)
-template <class Y>
-__global__ __launch_bounds__(256) void finish_items_kernel(const float *part, const float *part_sum, const float *wpow, int64_t V, int64_t rows,
-                                                           int K, int KP, int splits, int sum_splits, float scale, typename Y::t *dw, int64_t lddw, float *dbias)
+struct JoinArgs {
+    const float *part, *tops, *sums;       // tops (ranged passes): [split][3][rows] with the sums behind, else NULL
+    const float *wpow;
+    const uint32_t *col_top;
+    int64_t count, rows, ld;
+    int K, KP, splits, sum_splits;
+    float scale;
+    void *out;
+    float *dbias;
+};
+
+template <class Y> __global__ __launch_bounds__(256) void join_kernel(JoinArgs A)
 {
     const int lane = threadIdx.x & 63;
     const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (v >= V)
+    if (v >= A.count)
         return;
-    const float f = *wpow * __builtin_amdgcn_exp2f(-(float)Y::shift);
-    for (int k = lane; k < K; k += 64) {
+    float top = A.tops ? kNothing : 0.0f;
+    if (A.tops)
+        for (int s = 0; s < A.splits; ++s)
+            top = fmaxf(top, A.tops[3 * s * A.rows + v]);
+    for (int k = lane; k < A.K; k += 64) {
         float sum = 0.0f;
-        for (int s = 0; s < splits; ++s)
-            sum += part[(s * rows + v) * KP + k];
-        dw[v * lddw + k] = (typename Y::t)(scale * (f * sum));
+#pragma unroll 4
+        for (int s = 0; s < A.splits; ++s) {
+            const float x = A.part[(s * A.rows + v) * A.KP + k];
+            sum += A.tops ? times_power(x, A.tops[3 * s * A.rows + v] - top) : x;
+        }
+        const int ce = Y::scaled ? half_exponent(__uint_as_float(A.col_top[k])) : 0;
+        ((typename Y::t *)A.out)[v * A.ld + k] = (typename Y::t)times_power(sum * (A.scale * *A.wpow), top - (float)Y::shift + (float)ce);
     }
-    if (dbias && lane == 0) {
+    if (A.dbias && lane == 0) {
         float sum = 0.0f;
-        for (int s = 0; s < sum_splits; ++s)
-            sum += part_sum[s * rows + v];
-        dbias[v] = f * sum;
+        if (A.tops)
+            for (int s = 0; s < A.splits; ++s)
+                sum += times_power(A.tops[(3 * s + 1) * A.rows + v], A.tops[3 * s * A.rows + v] - top);
+        else
+            for (int s = 0; s < A.sum_splits; ++s)
+                sum += A.sums[s * A.rows + v];
+        A.dbias[v] = times_power(sum * *A.wpow, top - (float)Y::shift);
     }
 }
 
@@ -851,110 +1115,18 @@ template <class T> __global__ void zero_rows_kernel(T *p, int64_t rows, int K, i
 // host side
 // ---------------------------------------------------------------------------------------------------------------------
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
-
-struct Plan {
-    bool wide;
-    int KO, KP, row_splits, item_splits, stats_splits, sum_splits;
-    int64_t chunk;                                  // wide: tiles of items at a time
-    int64_t n_tiles, v_tiles;                       // of 32, without padding
-    int64_t x_row, x_col, w_row, w_col, bias, reg, tg, meta, wpow, stats, part, part_sum, dx_part, g_rows, g_items, bytes;   // offsets
-};
-
 int64_t tiles_padded(int64_t tiles) { return up(tiles, kPadTiles); }
 
 // how many pieces the streamed side is cut into: enough workgroups for four on each compute unit, each with 8 tiles at least, in eights
 // (one a die) once there are that many
-int64_t pick_splits(int64_t workgroups, int64_t stream_tiles, int cus)
+int pick_splits(int64_t workgroups, int64_t stream_tiles, int cus)
 {
     int64_t s = (4 * cus + workgroups - 1) / workgroups;
     if (s > stream_tiles / 8)
         s = stream_tiles / 8;
     if (s > 8)
         s = s / 8 * 8;
-    return s < 1 ? 1 : s;
-}
-
-// wide: pieces of a chunk's contraction for dx
-int dx_splits(const Plan &P, int cus) { return (int)pick_splits(2 * ((P.n_tiles + 3) / 4) * ((P.KO + 3) / 4), P.chunk, cus); }
-
-template <class Y, int KO, int MODE> int64_t workgroups(int64_t tiles)
-{
-    typedef Shape<Y, KO, MODE> Z;
-    return (tiles + Z::NW * Z::QB - 1) / (Z::NW * Z::QB);
-}
-
-template <class Y> void make_plan(Plan &P, int64_t n, int64_t v, int64_t k, bool grad, int cus)
-{
-    const int need = (int)((k + 31) / 32);
-    P.wide = need > 8;
-    P.KO = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : need <= 8 ? 8 : (need + 1) / 2 * 2;
-    P.KP = 32 * P.KO;
-    P.n_tiles = (n + 31) / 32;
-    P.v_tiles = (v + 31) / 32;
-    int64_t gr = 1, gi = 1;
-    if (!P.wide) switch (P.KO) {
-    case 1: gr = grad ? workgroups<Y, 1, kRows>(P.n_tiles) : workgroups<Y, 1, kNll>(P.n_tiles); gi = workgroups<Y, 1, kItems>(P.v_tiles); break;
-    case 2: gr = grad ? workgroups<Y, 2, kRows>(P.n_tiles) : workgroups<Y, 2, kNll>(P.n_tiles); gi = workgroups<Y, 2, kItems>(P.v_tiles); break;
-    case 4: gr = grad ? workgroups<Y, 4, kRows>(P.n_tiles) : workgroups<Y, 4, kNll>(P.n_tiles); gi = workgroups<Y, 4, kItems>(P.v_tiles); break;
-    default: gr = grad ? workgroups<Y, 8, kRows>(P.n_tiles) : workgroups<Y, 8, kNll>(P.n_tiles); gi = workgroups<Y, 8, kItems>(P.v_tiles);
-    }
-    P.row_splits = (int)pick_splits(gr, P.v_tiles, cus);
-    P.item_splits = (int)pick_splits(gi, P.n_tiles, cus);
-    P.stats_splits = P.row_splits;
-    if (P.wide) {
-        const int64_t ng = (P.n_tiles + 3) / 4;
-        P.row_splits = (int)pick_splits(2 * ng, P.v_tiles, cus);
-        P.stats_splits = 2 * P.row_splits;
-        const int64_t tile_bytes = up(P.n_tiles, 4) * 32 * 32 * 2 * Y::S * 2;
-        P.chunk = kChunkBytes / tile_bytes / 4 * 4;
-        P.chunk = P.chunk < 4 ? 4 : P.chunk > up(P.v_tiles, 4) ? up(P.v_tiles, 4) : P.chunk;
-        const int64_t kg = (P.KO + 3) / 4;
-        P.item_splits = (int)pick_splits(2 * kg * (P.chunk / 4), P.n_tiles, cus);   // dw: contraction over the rows
-        P.sum_splits = (int)(2 * ng);
-    }
-    const int64_t nt = tiles_padded(P.n_tiles), vt = tiles_padded(P.v_tiles), unit = (int64_t)2 * P.KO * Y::S * kUnit;
-    const int64_t nr = P.n_tiles * 32, vr = P.v_tiles * 32;
-    int64_t at = 0;
-    auto take = [&](int64_t bytes) {
-        const int64_t here = at;
-        at += up(bytes, 1024);
-        return here;
-    };
-    P.x_row = take(nt * unit);
-    P.w_row = take(vt * unit);
-    P.bias = take(vt * 32 * 4);
-    P.meta = take(nt * 32 * 4);
-    P.stats = take((int64_t)P.stats_splits * 3 * nr * 4);
-    if (grad) {
-        P.x_col = take(nt * unit);
-        P.w_col = take(vt * unit);
-        P.reg = take(nt * 32 * 4);
-        P.tg = take(nt * 32 * 4);
-        P.wpow = take(4);
-        if (P.wide) {
-            P.part = take(P.item_splits * P.chunk * 32 * P.KP * 4);
-            P.part_sum = take(P.sum_splits * P.chunk * 32 * 4);
-            P.dx_part = take(dx_splits(P, cus) * nr * P.KP * 4);
-            P.g_rows = take(up(P.n_tiles, 4) * P.chunk * 2 * Y::S * kUnit);
-            P.g_items = take(up(P.n_tiles, 4) * P.chunk * 2 * Y::S * kUnit);
-            P.bytes = at;
-            return;
-        }
-        const int64_t rows_part = P.row_splits * nr * P.KP * 4, items_part = P.item_splits * vr * P.KP * 4;
-        P.part = take(rows_part > items_part ? rows_part : items_part);   // (the rows' is read before the items' is written)
-        P.part_sum = take(P.item_splits * vr * 4);
-    }
-    P.bytes = at;
-}
-
-template <class Y, int MODE> void launch_pass(int KO, const PassArgs &A, hipStream_t st)
-{
-    switch (KO) {
-    case 1: pass_kernel<Y, 1, MODE><<<(unsigned)(workgroups<Y, 1, MODE>(A.still_tiles) * A.splits), Shape<Y, 1, MODE>::NW * 64, 0, st>>>(A); break;
-    case 2: pass_kernel<Y, 2, MODE><<<(unsigned)(workgroups<Y, 2, MODE>(A.still_tiles) * A.splits), Shape<Y, 2, MODE>::NW * 64, 0, st>>>(A); break;
-    case 4: pass_kernel<Y, 4, MODE><<<(unsigned)(workgroups<Y, 4, MODE>(A.still_tiles) * A.splits), Shape<Y, 4, MODE>::NW * 64, 0, st>>>(A); break;
-    default: pass_kernel<Y, 8, MODE><<<(unsigned)(workgroups<Y, 8, MODE>(A.still_tiles) * A.splits), Shape<Y, 8, MODE>::NW * 64, 0, st>>>(A);
-    }
+    return s < 1 ? 1 : (int)s;
 }
 
 struct Call {
@@ -967,137 +1139,289 @@ struct Call {
     float scale;
     bool grad;
     int cus;
-    char *ws;
+    char *ws;                 // NULL: only the size is asked for
     int64_t ws_bytes;
     hipStream_t st;
 };
 
-template <class Y> int run(const Call &C)
+// pieces of the workspace, one after the other
+struct Space {
+    char *base;
+    int64_t used;
+    template <class T> T *take(int64_t bytes)
+    {
+        T *const p = (T *)(base + used);
+        used += up(bytes, 1024);
+        return p;
+    }
+};
+
+constexpr int64_t kOneTileMore = 64 * 4;    // staging reads 64 words for a tile's 32
+
+template <class Y, int KO, int MODE> int64_t workgroups(int64_t tiles)
 {
-    typedef typename Y::t T;
-    Plan P = {};
-    make_plan<Y>(P, C.n, C.v, C.k, C.grad, C.cus);
-    if (C.ws_bytes < P.bytes)
-        return HPF_EINVAL;
-    const int K = (int)C.k, CB = 2 * P.KO;
-    const dim3 groups_w((unsigned)P.v_tiles, (unsigned)((P.KP + 127) / 128)), groups_x((unsigned)P.n_tiles, (unsigned)((P.KP + 127) / 128));
-    const float sign = C.scale < 0.0f ? -1.0f : 1.0f;     // goes into the packed x, so that logits rise with the product
-    char *const ws = C.ws;
-    pack_kernel<Y><<<groups_w, 256, 0, C.st>>>((const T *)C.w, C.ldw, C.v, K, CB, P.KO, ws + P.w_row, C.grad ? ws + P.w_col : nullptr, nullptr, 0, 1.0f);
-    pack_kernel<Y><<<groups_x, 256, 0, C.st>>>((const T *)C.x, C.ldx, C.n, K, CB, P.KO, ws + P.x_row, C.grad ? ws + P.x_col : nullptr,
-                                              C.grad ? C.target : nullptr, C.v, sign);
-    const int64_t vp = tiles_padded(P.v_tiles) * 32, np = tiles_padded(P.n_tiles) * 32;
-    bias_kernel<<<(unsigned)((vp + 255) / 256), 256, 0, C.st>>>(C.bias, C.v, vp, (float *)(ws + P.bias));
-    targets_kernel<<<(unsigned)((np + 255) / 256), 256, 0, C.st>>>(C.target, C.n, C.v, np, (int32_t *)(ws + P.meta));
-    if (C.grad)
-        weight_kernel<<<1, 1024, 0, C.st>>>(C.weight, C.n, (float *)(ws + P.wpow));
+    typedef Shape<Y, KO, MODE> Z;
+    return (tiles + Z::NW * Z::QB - 1) / (Z::NW * Z::QB);
+}
 
-    PassArgs A = {};
-    A.still = ws + P.x_row;
-    A.by_row = ws + P.w_row;
-    A.by_col = ws + P.w_col;
-    A.reg_bias = (const float *)(ws + P.bias);
-    A.meta = (const int32_t *)(ws + P.meta);
-    A.stats = (float *)(ws + P.stats);
-    A.part = (float *)(ws + P.part);
-    A.still_tiles = P.n_tiles;
-    A.still_rows = P.n_tiles * 32;
-    A.stream_tiles = P.v_tiles;
-    A.c = fabsf(C.scale) * kLog2e;
-    A.splits = P.row_splits;
-    A.bias = C.bias != nullptr;
-    WideArgs W = {};
-    if (P.wide) {
-        W.w = A.by_row;
-        W.x = A.still;
-        W.bias = A.reg_bias;
-        W.meta = A.meta;
-        W.stats = A.stats;
-        W.n_tiles = P.n_tiles;
-        W.v_tiles = P.v_tiles;
-        W.rows = A.still_rows;
-        W.c = A.c;
-        W.CB = CB;
-        W.splits = P.row_splits;
-        W.has_bias = A.bias;
-        wide_stats_kernel<Y><<<(unsigned)((P.n_tiles + 3) / 4 * P.row_splits), 256, 0, C.st>>>(W);
-    } else if (C.grad)
-        launch_pass<Y, kRows>(P.KO, A, C.st);
-    else
-        launch_pass<Y, kNll>(P.KO, A, C.st);
+void fill_prepare(PrepArgs &P, const Call &C, int64_t np, int64_t vp)
+{
+    P.target = C.target;
+    P.bias = C.bias;
+    P.weight = C.weight;
+    P.N = C.n;
+    P.V = C.v;
+    P.np = np;
+    P.vp = vp;
+}
+unsigned prepare_blocks(int64_t np, int64_t vp) { return (unsigned)((np > vp ? np : vp) + 255) / 256 + 1; }
 
-    FinishArgs F = {};
-    F.stats = A.stats;
-    F.part = A.part;
+void fill_finish(FinishArgs &F, const Call &C)
+{
     F.target = C.target;
     F.weight = C.weight;
-    F.wpow = (const float *)(ws + P.wpow);
     F.w = C.w;
     F.loss = C.loss;
     F.lse = C.lse;
-    F.reg_bias = (float *)(ws + P.reg);
-    F.target_g = (float *)(ws + P.tg);
-    F.meta = (int32_t *)(ws + P.meta);
-    F.dx = P.wide ? nullptr : C.dx;
     F.N = C.n;
     F.V = C.v;
-    F.rows = A.still_rows;
     F.ldw = C.ldw;
     F.lddx = C.lddx;
-    F.K = K;
-    F.KP = P.KP;
-    F.splits = P.stats_splits;
+    F.K = (int)C.k;
     F.scale = C.scale;
-    const unsigned row_blocks = (unsigned)((F.rows + 3) / 4);
-    if (!C.grad) {
-        finish_rows_kernel<Y, false><<<row_blocks, 256, 0, C.st>>>(F);
-        return (int)hipGetLastError();
-    }
-    finish_rows_kernel<Y, true><<<row_blocks, 256, 0, C.st>>>(F);
+}
 
-    if (P.wide) {
-        W.reg_bias = F.reg_bias;
-        W.target_g = F.target_g;
-        W.part_sum = (float *)(ws + P.part_sum);
-        W.g_rows = ws + P.g_rows;
-        W.g_items = ws + P.g_items;
-        const int kg = (P.KO + 3) / 4, zs = dx_splits(P, C.cus);
-        float *const dx_part = (float *)(ws + P.dx_part), *const dw_part = (float *)(ws + P.part);
-        for (int64_t v0 = 0; v0 < P.v_tiles; v0 += P.chunk) {
-            W.v0 = v0;
-            W.v_count = P.v_tiles - v0 < P.chunk ? P.v_tiles - v0 : P.chunk;
-            wide_g_kernel<Y><<<(unsigned)((P.n_tiles + 3) / 4 * ((W.v_count + 3) / 4)), 256, 0, C.st>>>(W);
-            ProductArgs D = {W.g_rows, ws + P.w_col + v0 * 2 * P.KO * Y::S * kUnit, P.n_tiles, W.v_count * 2, W.v_count, P.KO, zs, dx_part, v0 > 0};
-            wide_product_kernel<Y><<<(unsigned)((P.n_tiles + 3) / 4 * kg * zs), 256, 0, C.st>>>(D);
-            D = {W.g_items, ws + P.x_col, W.v_count, P.n_tiles * 2, P.n_tiles, P.KO, P.item_splits, dw_part, 0};
-            wide_product_kernel<Y><<<(unsigned)((W.v_count + 3) / 4 * kg * P.item_splits), 256, 0, C.st>>>(D);
-            const int64_t first = v0 * 32, count = C.v - first < W.v_count * 32 ? C.v - first : W.v_count * 32;
-            finish_items_kernel<Y><<<(unsigned)((count + 3) / 4), 256, 0, C.st>>>(dw_part, W.part_sum, F.wpow, count, W.v_count * 32, K, P.KP,
-                                                                                 P.item_splits, P.sum_splits, C.scale, (T *)C.dw + first * C.lddw,
-                                                                                 C.lddw, C.bias ? C.dbias + first : nullptr);
+// Rows of up to 256 values: returns the workspace's bytes, or a negative code / launch error where there is one to launch in.
+template <class Y, int KO> int64_t run_narrow(const Call &C)
+{
+    typedef typename Y::t T;
+    constexpr int KP = 32 * KO;
+    const int64_t n_tiles = (C.n + 31) / 32, v_tiles = (C.v + 31) / 32, nt = tiles_padded(n_tiles), vt = tiles_padded(v_tiles), unit = (int64_t)2 * KO * Y::S * kUnit;
+    const int64_t nr = n_tiles * 32, vr = v_tiles * 32;
+    const int64_t row_groups = C.grad ? workgroups<Y, KO, kRows>(n_tiles) : workgroups<Y, KO, kNll>(n_tiles), item_groups = workgroups<Y, KO, kItems>(v_tiles);
+    const int row_splits = pick_splits(row_groups, v_tiles, C.cus), item_splits = pick_splits(item_groups, n_tiles, C.cus);
+    Space W = {C.ws, 0};
+    Matrix mw = {C.w, C.ldw, C.v, nullptr, 0, 1.0f, nullptr, nullptr, nullptr, nullptr};
+    // (the sign of the scale goes into the packed x, so that logits rise with the product)
+    Matrix mx = {C.x, C.ldx, C.n, C.grad ? C.target : nullptr, C.v, C.scale < 0.0f ? -1.0f : 1.0f, nullptr, nullptr, nullptr, nullptr};
+    PrepArgs P = {};
+    fill_prepare(P, C, nt * 32, vt * 32);
+    mw.by_row = W.take<char>(vt * unit);
+    mx.by_row = W.take<char>(nt * unit);
+    P.bias2 = W.take<float>(vt * 32 * 4 + kOneTileMore);
+    P.meta = W.take<int32_t>(nt * 32 * 4 + kOneTileMore);
+    if (Y::scaled) {
+        mw.exps = W.take<int32_t>(vt * 4);
+        mx.exps = W.take<int32_t>(nt * 4);
+    }
+    float *const stats = W.take<float>((int64_t)row_splits * 3 * nr * 4), *reg_bias = nullptr, *target_log = nullptr, *item_stats = nullptr, *part = nullptr;
+    if (C.grad) {
+        mw.by_col = W.take<char>(vt * unit);
+        mx.by_col = W.take<char>(nt * unit);
+        if (Y::scaled) {
+            P.cols = 2 * KP;
+            P.col_top = mw.col_top = W.take<uint32_t>(2 * KP * 4);
+            mx.col_top = mw.col_top + KP;
         }
-        finish_items_kernel<Y><<<(unsigned)((C.n + 3) / 4), 256, 0, C.st>>>(dx_part, nullptr, F.wpow, C.n, F.rows, K, P.KP, zs, 0, C.scale,
-                                                                            (T *)C.dx, C.lddx, nullptr);
+        reg_bias = W.take<float>(nt * 32 * 4 + kOneTileMore);
+        target_log = W.take<float>(nt * 32 * 4);
+        P.wpow = W.take<float>(4);
+        const int64_t rows_part = row_splits * nr * KP * 4, items_part = item_splits > 1 ? item_splits * vr * KP * 4 : 0;
+        part = W.take<float>(rows_part > items_part ? rows_part : items_part);   // (the rows' is read before the items' is written)
+        if (item_splits > 1)
+            item_stats = W.take<float>((int64_t)item_splits * 3 * vr * 4);
+    }
+    if (!C.ws)
+        return W.used;
+    if (C.ws_bytes < W.used)
+        return HPF_EINVAL;
+
+    prepare_kernel<<<prepare_blocks(P.np, P.vp), 256, 0, C.st>>>(P);
+    if (Y::scaled && C.grad) {
+        const int wb = (int)(C.v / 64 < 1 ? 1 : C.v / 64 > 4 * C.cus ? 4 * C.cus : C.v / 64), xb = (int)(C.n / 64 < 1 ? 1 : C.n / 64 > 4 * C.cus ? 4 * C.cus : C.n / 64);
+        columns_kernel<<<wb + xb, 256, 0, C.st>>>(mw, mx, (int)C.k, wb);
+    }
+    pack_kernel<Y, KO><<<(unsigned)(v_tiles + n_tiles), 256, 0, C.st>>>(mw, mx, (int)C.k, (int)v_tiles);
+
+    PassArgs A = {};
+    A.still = mx.by_row;
+    A.by_row = mw.by_row;
+    A.by_col = mw.by_col;
+    A.still_exp = mx.exps;
+    A.stream_exp = mw.exps;
+    A.reg_bias = P.bias2;
+    A.meta = P.meta;
+    A.stats = stats;
+    A.part = part;
+    A.still_tiles = n_tiles;
+    A.still_rows = nr;
+    A.stream_tiles = v_tiles;
+    A.c = fabsf(C.scale) * kLog2e;
+    A.splits = row_splits;
+    A.bias = C.bias != nullptr;
+    FinishArgs F = {};
+    fill_finish(F, C);
+    F.stats = stats;
+    F.part = part;
+    F.wpow = P.wpow;
+    F.col_top = mw.col_top;
+    F.reg_bias = reg_bias;
+    F.target_log = target_log;
+    F.meta = P.meta;
+    F.dx = C.dx;
+    F.rows = nr;
+    F.KP = KP;
+    F.splits = row_splits;
+    if (!C.grad) {
+        pass_kernel<Y, KO, kNll><<<(unsigned)(row_groups * row_splits), Shape<Y, KO, kNll>::NW * 64, 0, C.st>>>(A);
+        finish_rows_kernel<Y, false><<<(unsigned)C.n, 256, 0, C.st>>>(F);
         return (int)hipGetLastError();
     }
-    A.still = ws + P.w_row;
-    A.by_row = ws + P.x_row;
-    A.by_col = ws + P.x_col;
-    A.reg_bias = F.reg_bias;
-    A.lane_bias = (const float *)(ws + P.bias);
-    A.target_g = F.target_g;
-    A.part_sum = (float *)(ws + P.part_sum);
-    A.still_tiles = P.v_tiles;
-    A.still_rows = P.v_tiles * 32;
-    A.stream_tiles = P.n_tiles;
-    A.splits = P.item_splits;
-    launch_pass<Y, kItems>(P.KO, A, C.st);
-    finish_items_kernel<Y><<<(unsigned)((C.v + 3) / 4), 256, 0, C.st>>>(A.part, A.part_sum, F.wpow, C.v, A.still_rows, K, P.KP, P.item_splits,
-                                                                        P.item_splits, C.scale, (T *)C.dw, C.lddw, C.bias ? C.dbias : nullptr);
+    pass_kernel<Y, KO, kRows><<<(unsigned)(row_groups * row_splits), Shape<Y, KO, kRows>::NW * 64, 0, C.st>>>(A);
+    finish_rows_kernel<Y, true><<<(unsigned)nr, 256, 0, C.st>>>(F);
+
+    A.still = mw.by_row;
+    A.by_row = mx.by_row;
+    A.by_col = mx.by_col;
+    A.still_exp = mw.exps;
+    A.stream_exp = mx.exps;
+    A.reg_bias = reg_bias;
+    A.lane_bias = P.bias2;
+    A.target_log = target_log;
+    A.stats = item_stats;
+    A.still_tiles = v_tiles;
+    A.still_rows = vr;
+    A.stream_tiles = n_tiles;
+    A.splits = item_splits;
+    if (item_splits == 1) {
+        A.out = C.dw;
+        A.dbias = C.bias ? C.dbias : nullptr;
+        A.col_top = mx.col_top;
+        A.wpow = P.wpow;
+        A.ld_out = C.lddw;
+        A.count = C.v;
+        A.K = (int)C.k;
+        A.quads = C.lddw % 4 == 0 && (uintptr_t)C.dw % (4 * sizeof(T)) == 0;
+        A.scale = C.scale;
+    }
+    pass_kernel<Y, KO, kItems><<<(unsigned)(item_groups * item_splits), Shape<Y, KO, kItems>::NW * 64, 0, C.st>>>(A);
+    if (item_splits > 1) {
+        const JoinArgs J = {part, item_stats, nullptr, P.wpow, mx.col_top, C.v, vr, C.lddw, (int)C.k, KP, item_splits, 0, C.scale, C.dw, C.bias ? C.dbias : nullptr};
+        join_kernel<Y><<<(unsigned)((C.v + 3) / 4), 256, 0, C.st>>>(J);
+    }
     return (int)hipGetLastError();
 }
 
-int run_type(int type, const Call &C) { return type == HPF_F32 ? run<F32>(C) : type == HPF_BF16 ? run<B16>(C) : run<H16>(C); }
+// wider rows
+template <class Y> int64_t run_wide(const Call &C)
+{
+    typedef typename Y::t T;
+    const int KO = (int)((C.k + 31) / 32 + 1) / 2 * 2, KP = 32 * KO, CB = 2 * KO, kg = (KO + 3) / 4;
+    const int64_t n_tiles = (C.n + 31) / 32, v_tiles = (C.v + 31) / 32, nt = tiles_padded(n_tiles), vt = tiles_padded(v_tiles), unit = (int64_t)2 * KO * Y::S * kUnit;
+    const int64_t nr = n_tiles * 32, ng = (n_tiles + 3) / 4;
+    const int row_splits = pick_splits(2 * ng, v_tiles, C.cus);
+    int64_t chunk = kChunkBytes / (ng * 4 * 32 * 32 * 2 * Y::S * 2) / 4 * 4;                 // tiles of items at a time
+    chunk = chunk < 4 ? 4 : chunk > up(v_tiles, 4) ? up(v_tiles, 4) : chunk;
+    const int dw_splits = pick_splits(2 * kg * (chunk / 4), n_tiles, C.cus), dx_splits = pick_splits(2 * kg * ng, chunk, C.cus), sum_splits = (int)(2 * ng);
+    Space S = {C.ws, 0};
+    Matrix mw = {C.w, C.ldw, C.v, nullptr, 0, 1.0f, nullptr, nullptr, nullptr, nullptr};
+    Matrix mx = {C.x, C.ldx, C.n, C.grad ? C.target : nullptr, C.v, C.scale < 0.0f ? -1.0f : 1.0f, nullptr, nullptr, nullptr, nullptr};
+    PrepArgs P = {};
+    fill_prepare(P, C, nt * 32, vt * 32);
+    mw.by_row = S.take<char>(vt * unit);
+    mx.by_row = S.take<char>(nt * unit);
+    P.bias2 = S.take<float>(vt * 32 * 4);
+    P.meta = S.take<int32_t>(nt * 32 * 4);
+    WideArgs A = {};
+    FinishArgs F = {};
+    fill_finish(F, C);
+    float *dw_part = nullptr, *dx_part = nullptr;
+    A.stats = S.take<float>((int64_t)2 * row_splits * 3 * nr * 4);
+    if (C.grad) {
+        mw.by_col = S.take<char>(vt * unit);
+        mx.by_col = S.take<char>(nt * unit);
+        F.reg_bias = S.take<float>(nt * 32 * 4);
+        F.target_log = S.take<float>(nt * 32 * 4);
+        P.wpow = S.take<float>(4);
+        dw_part = S.take<float>(dw_splits * chunk * 32 * KP * 4);
+        dx_part = S.take<float>(dx_splits * nr * KP * 4);
+        A.part_sum = S.take<float>(sum_splits * chunk * 32 * 4);
+        A.g_rows = S.take<char>(ng * 4 * chunk * 2 * Y::S * kUnit);
+        A.g_items = S.take<char>(ng * 4 * chunk * 2 * Y::S * kUnit);
+    }
+    if (!C.ws)
+        return S.used;
+    if (C.ws_bytes < S.used)
+        return HPF_EINVAL;
+
+    prepare_kernel<<<prepare_blocks(P.np, P.vp), 256, 0, C.st>>>(P);
+    pack_wide_kernel<Y><<<dim3((unsigned)v_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mw, (int)C.k, CB, KO);
+    pack_wide_kernel<Y><<<dim3((unsigned)n_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mx, (int)C.k, CB, KO);
+    A.w = mw.by_row;
+    A.x = mx.by_row;
+    A.bias = P.bias2;
+    A.meta = P.meta;
+    A.n_tiles = n_tiles;
+    A.v_tiles = v_tiles;
+    A.rows = nr;
+    A.c = fabsf(C.scale) * kLog2e;
+    A.CB = CB;
+    A.splits = row_splits;
+    A.has_bias = C.bias != nullptr;
+    wide_stats_kernel<Y><<<(unsigned)(ng * row_splits), 256, 0, C.st>>>(A);
+    F.stats = A.stats;
+    F.wpow = P.wpow;
+    F.meta = P.meta;
+    F.rows = nr;
+    F.splits = 2 * row_splits;
+    if (!C.grad) {
+        finish_rows_kernel<Y, false><<<(unsigned)C.n, 256, 0, C.st>>>(F);
+        return (int)hipGetLastError();
+    }
+    finish_rows_kernel<Y, true><<<(unsigned)nr, 256, 0, C.st>>>(F);
+    A.reg_bias = F.reg_bias;
+    A.target_log = F.target_log;
+    for (int64_t v0 = 0; v0 < v_tiles; v0 += chunk) {
+        A.v0 = v0;
+        A.v_count = v_tiles - v0 < chunk ? v_tiles - v0 : chunk;
+        wide_g_kernel<Y><<<(unsigned)(ng * ((A.v_count + 3) / 4)), 256, 0, C.st>>>(A);
+        ProductArgs D = {A.g_rows, mw.by_col + v0 * unit, n_tiles, A.v_count * 2, A.v_count, KO, dx_splits, dx_part, v0 > 0};
+        wide_product_kernel<Y><<<(unsigned)(ng * kg * dx_splits), 256, 0, C.st>>>(D);
+        D = {A.g_items, mx.by_col, A.v_count, n_tiles * 2, n_tiles, KO, dw_splits, dw_part, 0};
+        wide_product_kernel<Y><<<(unsigned)((A.v_count + 3) / 4 * kg * dw_splits), 256, 0, C.st>>>(D);
+        const int64_t first = v0 * 32, count = C.v - first < A.v_count * 32 ? C.v - first : A.v_count * 32;
+        const JoinArgs J = {dw_part, nullptr, A.part_sum, P.wpow, nullptr, count, A.v_count * 32, C.lddw, (int)C.k, KP, dw_splits, sum_splits, C.scale,
+                            (T *)C.dw + first * C.lddw, C.bias ? C.dbias + first : nullptr};
+        join_kernel<Y><<<(unsigned)((count + 3) / 4), 256, 0, C.st>>>(J);
+    }
+    const JoinArgs J = {dx_part, nullptr, nullptr, P.wpow, nullptr, C.n, nr, C.lddx, (int)C.k, KP, dx_splits, 0, C.scale, C.dx, nullptr};
+    join_kernel<Y><<<(unsigned)((C.n + 3) / 4), 256, 0, C.st>>>(J);
+    return (int)hipGetLastError();
+}
+
+template <class Y> int64_t run_any_narrow(const Call &C)
+{
+    switch ((C.k + 31) / 32) {
+    case 1: return run_narrow<Y, 1>(C);
+    case 2: return run_narrow<Y, 2>(C);
+    case 3: return run_narrow<Y, 3>(C);
+    case 4: return run_narrow<Y, 4>(C);
+    case 5: return run_narrow<Y, 5>(C);
+    case 6: return run_narrow<Y, 6>(C);
+    case 7: return run_narrow<Y, 7>(C);
+    default: return run_narrow<Y, 8>(C);
+    }
+}
+
+int64_t run(int type, const Call &C)
+{
+    const bool narrow = C.k <= 256;
+    if (type == HPF_F32)
+        return narrow ? run_any_narrow<F32>(C) : run_wide<W32>(C);
+    if (type == HPF_BF16)
+        return narrow ? run_any_narrow<B16>(C) : run_wide<B16>(C);
+    return narrow ? run_any_narrow<H16>(C) : run_wide<H16>(C);
+}
 
 bool sizes_ok(int64_t n, int64_t v, int64_t k) { return n >= 0 && v > 0 && k > 0 && n < kNoTarget - 31 && v < kNoTarget - 31 && k < (1 << 20); }
 
@@ -1111,14 +1435,13 @@ extern "C" int64_t hpf_hip_softmax_workspace(int64_t n, int64_t v, int64_t k, in
         return HPF_EUNSUPPORTED;
     if (n == 0)
         return 0;
-    Plan P = {};
-    if (type == HPF_F32)
-        make_plan<F32>(P, n, v, k, grad != 0, cu_count);
-    else if (type == HPF_BF16)
-        make_plan<B16>(P, n, v, k, grad != 0, cu_count);
-    else
-        make_plan<H16>(P, n, v, k, grad != 0, cu_count);
-    return P.bytes;
+    Call C = {};
+    C.n = n;
+    C.v = v;
+    C.k = k;
+    C.grad = grad != 0;
+    C.cus = cu_count;
+    return run(type, C);
 }
 
 extern "C" int hpf_hip_softmax_nll(const void *x, int64_t ldx, const void *items, int64_t ld_items, const int64_t *target, const float *bias,
@@ -1150,7 +1473,7 @@ extern "C" int hpf_hip_softmax_nll(const void *x, int64_t ldx, const void *items
     C.ws = (char *)workspace;
     C.ws_bytes = workspace_bytes;
     C.st = (hipStream_t)stream;
-    return run_type(type, C);
+    return (int)run(type, C);
 }
 
 extern "C" int hpf_hip_softmax_nll_grad(const void *x, int64_t ldx, const void *items, int64_t ld_items, const int64_t *target,
@@ -1199,5 +1522,5 @@ extern "C" int hpf_hip_softmax_nll_grad(const void *x, int64_t ldx, const void *
     C.ws = (char *)workspace;
     C.ws_bytes = workspace_bytes;
     C.st = st;
-    return run_type(type, C);
+    return (int)run(type, C);
 }

@@ -155,26 +155,33 @@ def _exact(x, items, target, weight, bias, scale):
 
 
 def _bounds(e, kind, bias, scale, k, wmax=1.0):
-    """A logit: (6 products x) 2 ceil(k / 32) matrix instructions, each rounding its running sum (by a whole unit at most), what
-    six products of three parts leave out (3 U), the conversion to base 2 (constant, product, sum: 4 U of the size).
+    """A logit: up to (6 products x) 2 ceil(k / 32) matrix instructions, each rounding its running sum (by a whole unit at most);
+    what products of parts leave out (each part to 2^-23, low times low 2^-22: 8 U), and 2^-40 of the largest |x| |w|, k times;
+    the conversion to base 2 (constant, product, sum: 4 U of the size).
     A share exp(z - lse): twice that error, 2 U of |z - lse| + |lse| for the argument's rounding, 2 U for the function.
-    Sums of V shares (or V, N products): independent roundings, 4 sqrt(count) U; joining pieces a few U more.
-    16-bit types: shares are rounded to the type once more, results too; half's shares below 2^-14 of 2^-14 absolutely."""
-    steps = (6 if kind == F32 else 1) * 2 * max(1, math.ceil(k / 32)) + 4
-    size = abs(scale) * (e["x"].abs() @ e["w"].abs().t())
+    Sums of V shares (or V, N products): independent roundings, 4 sqrt(count) U; joining pieces a few U more; parts 8 U.
+    16-bit types: shares are rounded to the type once more, results too.  Shares in half precision (float32's parts too) end at
+    2^-39 of the row's, the item's or (rows over 256 wide) the weights' largest, 32-bit matrices at 2^-40 of their column's."""
+    steps = (6 if kind == F32 else 1) * 2 * max(1, math.ceil(k / 32)) + 4 + (4 if kind == F32 else 0)
+    ax, aw = e["x"].abs(), e["w"].abs()
+    size = abs(scale) * (ax @ aw.t())
     b = torch.where(bias > -1e30, bias, torch.zeros_like(bias)).double().abs() if bias is not None else torch.zeros(e["w"].shape[0], dtype=torch.float64, device=e["x"].device)
     ez = (2 * U * steps * size + 4 * U * (size + b)).amax(dim=1)                     # per row
+    if kind == F32:
+        ez = ez + abs(scale) * k * 2.0 ** -39 * float(ax.max()) * float(aw.max())
     n, v = e["z"].shape
     span = torch.where(e["z"] > -1e30, (e["z"] - e["lse"][:, None]).abs(), torch.zeros_like(e["z"]))
     share = e["g"].abs()
     total = ez + (16 + 4 * math.sqrt(v)) * U + 2 * U * (torch.exp(-span) * span).sum(dim=1)
     lse = total + 4 * U * e["lse"].abs()
     rel = (2 * ez + total + 8 * U * (1 + e["lse"].abs()))[:, None] + 4 * U * span   # of a share, per logit
-    coarse = 0.0 if kind == F32 else HALF[kind]
-    least = 0.0 if kind != F16 else 2.0 ** -38 * wmax
+    coarse = 8 * U if kind == F32 else HALF[kind]
+    by_row, by_item = (wmax, wmax) if k > 256 else (share.amax(dim=1, keepdim=True), share.amax(dim=0, keepdim=True))
+    least_row, least_item = (0.0, 0.0) if kind == BF16 else (2.0 ** -38 * by_row, 2.0 ** -38 * by_item)
     long_v, long_n = (32 + 4 * math.sqrt(v)) * U, (32 + 4 * math.sqrt(n)) * U
-    dx = abs(scale) * ((share * (rel + coarse + long_v) + least) @ e["w"].abs()) + HALF[kind] * e["dx"].abs()
-    dw = abs(scale) * ((share * (rel + coarse + long_n) + least).t() @ e["x"].abs()) + HALF[kind] * e["ditems"].abs()
+    end = 2.0 ** -39 if kind == F32 else 0.0
+    dx = abs(scale) * ((share * (rel + coarse + long_v) + least_row) @ aw + end * share.sum(dim=1, keepdim=True) * aw.amax(dim=0)) + HALF[kind] * e["dx"].abs()
+    dw = abs(scale) * ((share * (rel + coarse + long_n) + least_item).t() @ ax + end * share.sum(dim=0)[:, None] * ax.amax(dim=0)) + HALF[kind] * e["ditems"].abs()
     if kind == F16:   # subnormal results
         dx, dw = dx + 2.0 ** -25, dw + 2.0 ** -25
     db = (share * (rel + long_n)).sum(dim=0) + 4 * U * e["dbias"].abs()
@@ -234,7 +241,7 @@ def _check(ops, c):
 
 
 SHAPES = [(1, 1, 1), (1, 7, 3), (2, 33, 31), (31, 31, 32), (33, 1000, 50), (32, 32, 64), (65, 97, 33), (129, 4097, 100), (300, 2000, 128),
-          (200, 1500, 200), (77, 640, 256), (40, 500, 257), (100, 1000, 300), (3, 3000, 520), (150, 900, 1000), (1100, 300, 40), (700, 260, 600)]
+          (200, 1500, 200), (77, 640, 256), (40, 500, 257), (100, 1000, 300), (3, 3000, 520), (150, 900, 1000), (66, 400, 90), (80, 390, 160), (70, 333, 180), (50, 300, 224), (1100, 300, 40), (700, 260, 600)]
 
 
 @pytest.mark.gpu
@@ -255,6 +262,22 @@ def test_scales_strides_and_no_weights(ops, k, scale, kind):
     _check(ops, dict(c, weight=None))
     _check(ops, dict(c, weight=c["weight"] * 1e-6))
     _check(ops, dict(c, weight=torch.zeros_like(c["weight"])))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [40, 300])
+def test_rows_and_columns_of_far_apart_sizes(ops, k):
+    """32-bit matrices: tables of very large, very small, zero and mixed magnitudes; columns from 1e-12 to 1e6 (x the other way
+    round); items whose shares are 1e-9 and less; a row of zeros."""
+    c = _case(90, 700, k, F32, True, seed=21)
+    _check(ops, dict(c, x=c["x"] * 1e-25, items=c["items"] * 1e24))
+    _check(ops, dict(c, x=c["x"] * 1e-30))
+    _check(ops, dict(c, x=torch.zeros_like(c["x"])))
+    size = torch.logspace(-2, 2, k, device="cuda:0")
+    _check(ops, dict(c, x=c["x"] / size, items=c["items"] * size))
+    rows = torch.logspace(-4, 0, 700, device="cuda:0")[torch.randperm(700, device="cuda:0", generator=torch.Generator(device="cuda:0").manual_seed(2))]
+    _check(ops, dict(c, items=c["items"] * rows[:, None]))
+    _check(ops, dict(c, bias=c["bias"] - 30.0 * (torch.arange(700, device="cuda:0") % 3 > 0)))   # two thirds of the items: shares of 1e-13
 
 
 @pytest.mark.gpu
