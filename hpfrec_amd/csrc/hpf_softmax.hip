@@ -77,6 +77,26 @@ template <class Y> __device__ __forceinline__ void split(float x, Parts<Y> &to, 
     }
 }
 
+// two neighbouring values (j even), rounded together; what is left of each by one multiply-add that reads the half in place
+template <class Y> __device__ __forceinline__ void split2(float x0, float x1, Parts<Y> &to, int j)
+{
+    if constexpr (Y::S == 3) {
+        split<Y>(x0, to, j);
+        split<Y>(x1, to, j + 1);
+    } else {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef typename Y::m::e e2 __attribute__((ext_vector_type(2)));
+        const e2 hi = __builtin_convertvector((f2){x0, x1}, e2);
+        to.p[0][j] = hi[0];
+        to.p[0][j + 1] = hi[1];
+        if constexpr (Y::S == 2) {
+            const e2 lo = __builtin_convertvector(((f2){fmaf((float)hi[0], -1.0f, x0), fmaf((float)hi[1], -1.0f, x1)}), e2);
+            to.p[1][j] = lo[0];
+            to.p[1][j + 1] = lo[1];
+        }
+    }
+}
+
 // c += a b, smallest products first
 template <class Y> __device__ __forceinline__ f32x16 product(const Parts<Y> &a, const Parts<Y> &b, f32x16 c)
 {
@@ -95,7 +115,17 @@ template <class Y> __device__ __forceinline__ f32x16 product(const Parts<Y> &a, 
 // the larger of two, NaN if either is
 __device__ __forceinline__ float larger(float a, float b) { return a != a || a >= b ? a : b; }
 
+// a lane's value in the lower half of the wavefront, and in the upper one: both, in every lane
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float halves_max(float x)
+{
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+// a word that earlier launches wrote, the same for all lanes
+__device__ __forceinline__ int uniform_word(const int32_t *p) { return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p; }
 
 // A UNIT is one operand of a matrix instruction as it lies in memory: 64 lanes x 8 values, 1 KB.
 constexpr int kUnit = 1024;
@@ -370,20 +400,35 @@ struct Sum {
     }
 };
 
+// Order for the scheduler, in a block of `steps` (an even number of) x (READS reads of shared memory, then PRODUCTS matrix instructions
+// that use them): two steps' reads behind the first product of the two steps before.  (Left alone it puts each read right
+// ahead of its product, and a wavefront waits for shared memory half of its time.)
+template <int READS, int PRODUCTS> __device__ __forceinline__ void order_reads(int steps)
+{
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * READS, 0);
+#pragma unroll
+    for (int i = 0; i < steps; i += 2) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        if (i + 2 < steps)
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * READS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, 2 * PRODUCTS - 1, 0);
+    }
+}
+
 __device__ __forceinline__ float sum16(const f32x16 &x)
 {
     return (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]))) + (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
 }
 
-// One block of base-2 logarithms (lane: stationary row, register: streamed row) becomes its exponentials relative to a running
-// maximum, times 2^shift; `rescale(f)` is called where the maximum grew.
-template <class Y, class F> __device__ __forceinline__ void exponentials(f32x16 &x, float &top, Sum &sum, const F &rescale)
+// One block of base-2 logarithms times 1 / c (lane: stationary row, register: streamed row) becomes its exponentials relative to a
+// running maximum, times 2^shift; `rescale(f)` is called where the maximum grew.  c > 0.
+template <class Y, class F> __device__ __forceinline__ void exponentials(f32x16 &x, float c, float &top, Sum &sum, const F &rescale)
 {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i)
         m = fmaxf(m, x[i]);
-    m = fmaxf(m, other_half(m));
+    m = halves_max(m) * c;
     if (__any(m > top)) {
         const float grown = m > top ? ceilf(m) : top, f = __builtin_amdgcn_exp2f(top - grown);
         sum.s *= f;
@@ -394,20 +439,20 @@ template <class Y, class F> __device__ __forceinline__ void exponentials(f32x16 
     const float down = (float)Y::shift - top;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-        x[i] = __builtin_amdgcn_exp2f(x[i] + down);
+        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, down));
 }
 
 // the register of a block that holds streamed row r (0 .. 31), for the lanes of half h: i with row_of(i, h) = r
 __device__ __forceinline__ constexpr int row_of(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
 // takes the target's logit out of its block
-__device__ __forceinline__ void take_target(f32x16 &x, int tile, int h, int target, float &at)
+__device__ __forceinline__ void take_target(f32x16 &x, float c, int tile, int h, int target, float &at)
 {
     if (__any((target >> 5) == tile))
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             if (target == tile * 32 + row_of(i, h)) {
-                at = x[i];
+                at = x[i] * c;
                 x[i] = -INFINITY;
             }
 }
@@ -453,7 +498,7 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
             }
         target[q] = MODE != kItems && in ? A.meta[(q0 + q) * 32 + low] : kNoTarget;
         lane_bias[q] = MODE == kItems && in && A.bias ? A.lane_bias[(q0 + q) * 32 + low] : 0.0f;
-        still_exp[q] = Y::scaled && in ? A.still_exp[q0 + q] : 0;
+        still_exp[q] = Y::scaled && in ? uniform_word(A.still_exp + q0 + q) : 0;
     }
 
     f32x16 acc[QB][MODE == kNll ? 1 : KO];
@@ -510,29 +555,27 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
             const char *rows = &lds[buf][rt * Z::row_units * kUnit], *cols = &lds[buf][(RT * Z::row_units + rt * Z::col_units) * kUnit];
             const char *side = &lds[buf][RT * Z::units * kUnit + rt * 256];
             const bool biased = MODE == kItems || A.bias || tile == A.stream_tiles - 1;
-            const int stream_exp = Y::scaled ? A.stream_exp[tile] : 0;
+            const int stream_exp = Y::scaled ? uniform_word(A.stream_exp + tile) : 0;
 
             f32x16 z[QB];
 #pragma unroll
             for (int q = 0; q < QB; ++q)
                 z[q] = (f32x16)(0.0f);
-            Parts<Y> a = fetch(rows);
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) {
-                const Parts<Y> now = a;
-                if (cb + 1 < CB)
-                    a = fetch(rows + (cb + 1) * S * kUnit);
+                const Parts<Y> a = fetch(rows + cb * S * kUnit);
 #pragma unroll
                 for (int q = 0; q < QB; ++q)
-                    z[q] = product<Y>(now, still[q][cb], z[q]);
+                    z[q] = product<Y>(a, still[q][cb], z[q]);
             }
+            order_reads<S, QB * (2 * S - 1)>(CB);
 
             Parts<Y> p[QB][2];
 #pragma unroll
             for (int q = 0; q < QB; ++q) {
                 f32x16 &x = z[q];
-                const float c = Y::scaled ? ldexpf(A.c, stream_exp + still_exp[q]) : A.c;
-                if (biased) {
+                float c = Y::scaled ? ldexpf(A.c, stream_exp + still_exp[q]) : A.c;
+                if (biased || c == 0.0f) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const f32x4 b = *(const f32x4 *)(side + (8 * i + 4 * h) * 4);
@@ -540,10 +583,7 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
                         for (int j = 0; j < 4; ++j)
                             x[4 * i + j] = fmaf(x[4 * i + j], c, b[j]);
                     }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        x[i] *= c;
+                    c = 1.0f;
                 }
                 const auto rescale = [&](float f) {
                     if constexpr (MODE != kNll)
@@ -570,7 +610,7 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
                         }
                     }
                     if constexpr (Y::ranged) {
-                        exponentials<Y>(x, top[q], sum[q], rescale);
+                        exponentials<Y>(x, c, top[q], sum[q], rescale);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
@@ -583,27 +623,25 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
                     if (A.bias)
                         sum[q].add(sum16(x));
                 } else {
-                    take_target(x, (int)tile, h, target[q], at[q]);
-                    exponentials<Y>(x, top[q], sum[q], rescale);
+                    take_target(x, c, (int)tile, h, target[q], at[q]);
+                    exponentials<Y>(x, c, top[q], sum[q], rescale);
                     sum[q].add(sum16(x));
                 }
                 if constexpr (MODE != kNll)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        split<Y>(x[i], p[q][i >> 3], i & 7);
+                    for (int i = 0; i < 16; i += 2)
+                        split2<Y>(x[i], x[i + 1], p[q][i >> 3], i & 7);
             }
 
             if constexpr (MODE != kNll) {
-                a = fetch(cols);
 #pragma unroll
                 for (int u = 0; u < 2 * KO; ++u) {
-                    const Parts<Y> now = a;
-                    if (u + 1 < 2 * KO)
-                        a = fetch(cols + (u + 1) * S * kUnit);
+                    const Parts<Y> a = fetch(cols + u * S * kUnit);
 #pragma unroll
                     for (int q = 0; q < QB; ++q)
-                        acc[q][u >> 1] = product<Y>(now, p[q][u & 1], acc[q][u >> 1]);
+                        acc[q][u >> 1] = product<Y>(a, p[q][u & 1], acc[q][u >> 1]);
                 }
+                order_reads<S, QB * (2 * S - 1)>(2 * KO);
             }
         }
     }
@@ -784,8 +822,8 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(W
                 for (int j = 0; j < 2; ++j) {
                     f32x16 &x = acc[i][j];
                     wide_bias(x, A, tile, h);
-                    take_target(x, (int)tile, h, target[j], at[j]);
-                    exponentials<Y>(x, top[j], sum[j], [](float) {});
+                    take_target(x, 1.0f, (int)tile, h, target[j], at[j]);
+                    exponentials<Y>(x, 1.0f, top[j], sum[j], [](float) {});
                     sum[j].add(sum16(x));
                 }
             }
@@ -858,8 +896,8 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
                     total += x;
                     Parts<Y> p[2];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        split<Y>(x[r], p[r >> 3], r & 7);
+                    for (int r = 0; r < 16; r += 2)
+                        split2<Y>(x[r], x[r + 1], p[r >> 3], r & 7);
                     for (int s = 0; s < S; ++s) {
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
