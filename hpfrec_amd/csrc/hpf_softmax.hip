@@ -217,15 +217,20 @@ __global__ __launch_bounds__(256) void columns_kernel(Matrix W, Matrix X, int K,
     const int64_t first = (second ? blockIdx.x - w_blocks : blockIdx.x) * 4 + (threadIdx.x >> 6), step = (second ? gridDim.x - w_blocks : w_blocks) * 4;
     const int lane = threadIdx.x & 63;
     float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int64_t r = first; r < M.rows; r += step)
-        if (counts(M, r)) {
-            const float *p = (const float *)M.p + r * M.ld;
+    for (int64_t r = first; r < M.rows; r += 8 * step) {
+        float x[8][4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (lane + 64 * j < K)
-                    m[j] = fmaxf(m[j], finite_size(p[lane + 64 * j]));
-        }
+                x[i][j] = r + i * step < M.rows && lane + 64 * j < K ? ((const float *)M.p)[(r + i * step) * M.ld + lane + 64 * j] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (!M.target || counts(M, r + i * step))
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    m[j] = fmaxf(m[j], finite_size(x[i][j]));
+    }
     for (int j = 0; j < 4; ++j)
         top[threadIdx.x >> 6][lane + 64 * j] = m[j];
     __syncthreads();
@@ -349,7 +354,7 @@ struct PassArgs {
     float *part;                    // [split][still rows][32 KO]
     int64_t still_tiles, still_rows, stream_tiles;   // tiles of 32; still_rows = 32 still_tiles
     float c;                        // |scale| log2(e)
-    int splits, bias;
+    int splits, bias, base, more;   // pieces of the streamed groups: `more` of base + 1, the rest of base
     // items pass in one piece: the results themselves
     void *out;
     float *dbias;
@@ -359,6 +364,8 @@ struct PassArgs {
     int K, quads;                   // quads: rows of `out` allow four values at once
     float scale;
 };
+
+constexpr int kGridY = 32768;
 
 // every wavefront's staged units are in shared memory (a barrier alone does not wait for them)
 __device__ __forceinline__ void staged_barrier()
@@ -479,10 +486,11 @@ __global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>:
 
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int sp = blockIdx.x % A.splits;                                  // equal splits stream the same tiles: ids a multiple of 8 apart
-    const int64_t q0 = ((int64_t)(blockIdx.x / A.splits) * NW + wave) * QB;   // meet on one die and its cache
-    const int64_t groups = (A.stream_tiles + RT - 1) / RT;
-    const int64_t g0 = groups * sp / A.splits, g1 = groups * (sp + 1) / A.splits;
+    const int sp = blockIdx.x;      // equal splits stream the same tiles: where there are eight, they meet on one die and its cache
+    const int64_t q0 = (((int64_t)blockIdx.z * kGridY + blockIdx.y) * NW + wave) * QB;
+    if (q0 - wave * QB >= A.still_tiles)
+        return;
+    const int64_t g0 = (int64_t)A.base * sp + (sp < A.more ? sp : A.more), g1 = g0 + A.base + (sp < A.more);
 
     Parts<Y> still[QB][CB];
     int target[QB], still_exp[QB];
@@ -978,7 +986,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_product_kernel
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Joins a row's splits: loss and lse, what the items' side needs of the row, and dx (a workgroup a row).
+// Joins a row's splits: loss and lse, what the items' side needs of the row, and dx (a wavefront a row).
 // ---------------------------------------------------------------------------------------------------------------------
 struct FinishArgs {
     const float *stats, *part;
@@ -996,20 +1004,20 @@ struct FinishArgs {
 
 template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows_kernel(FinishArgs A)
 {
-    __shared__ float join[4][3];
-    __shared__ float pieces[4][256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t n = blockIdx.x;
+    const int lane = threadIdx.x & 63;
+    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (n >= A.rows)
+        return;
     if (n >= A.N) {                // rows that only fill the last tile: no share of any sum
-        if (GRAD && threadIdx.x == 0) {
+        if (GRAD && lane == 0) {
             A.reg_bias[n] = A.target_log[n] = -INFINITY;
             A.meta[n] = kNoTarget;
         }
         return;
     }
-    // splits over the threads: maxima first, then sums relative to them
+    // splits over the lanes: maxima first, then sums relative to them
     float top = kNothing, at = -INFINITY, others = 0.0f;
-    for (int s = threadIdx.x; s < A.splits; s += 256) {
+    for (int s = lane; s < A.splits; s += 64) {
         top = fmaxf(top, A.stats[(3 * s + 0) * A.rows + n]);
         at = larger(at, A.stats[(3 * s + 2) * A.rows + n]);
     }
@@ -1017,23 +1025,11 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
         top = fmaxf(top, __shfl_xor(top, d));
         at = larger(at, __shfl_xor(at, d));
     }
-    if (lane == 0) {
-        join[wave][0] = top;
-        join[wave][1] = at;
-    }
-    __syncthreads();
-    for (int i = 0; i < 4; ++i) {
-        top = fmaxf(top, join[i][0]);
-        at = larger(at, join[i][1]);
-    }
-    for (int s = threadIdx.x; s < A.splits; s += 256)
+    for (int s = lane; s < A.splits; s += 64)
         others += times_power(A.stats[(3 * s + 1) * A.rows + n], A.stats[3 * s * A.rows + n] - top);
     for (int d = 32; d; d >>= 1)
         others += __shfl_xor(others, d);
-    if (lane == 0)
-        join[wave][2] = others;
-    __syncthreads();
-    others = ldexpf((join[0][2] + join[1][2]) + (join[2][2] + join[3][2]), -Y::shift);
+    others = ldexpf(others, -Y::shift);
 
     // `top` is that of the others; the target's own logit may be far above it
     const float peak = fmaxf(top, ceilf(at));
@@ -1055,51 +1051,235 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
             loss = (lse2 - at) * kLn2;
         }
     }
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
         A.loss[n] = loss;
         if (A.lse)
             A.lse[n] = lse2 * kLn2;
     }
     if constexpr (GRAD) {
         const float weight = alive ? (A.weight ? A.weight[n] : 1.0f) : 0.0f, share = fabsf(weight) / *A.wpow;
-        if (threadIdx.x == 0) {
+        if (lane == 0) {
             A.reg_bias[n] = alive ? log2f(share) - lse2 : -INFINITY;
             A.target_log[n] = alive ? log2f(share * (rest / all)) : -INFINITY;
             A.meta[n] = alive ? (int32_t)t | (weight < 0.0f ? kNegative : 0) : kNoTarget;
         }
         if (!A.dx)
             return;
-        // dx: a quarter of the splits a wavefront
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (alive) {
+        // dx: four columns a lane, the splits over as many lanes as that leaves (KP / 4 = 8 KO lanes for a split, a power of two above)
+        typedef typename Y::t T;
+        T *dx = (T *)A.dx + n * A.lddx;
+        const T *w = (const T *)A.w + (alive ? t : 0) * A.ldw;
+        const int span = A.KP <= 32 ? 8 : A.KP <= 64 ? 16 : A.KP <= 128 ? 32 : 64, k = 4 * (lane & (span - 1)), step = 64 / span;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (alive && k < A.KP)
 #pragma unroll 4
-            for (int s = wave; s < A.splits; s += 4) {
+            for (int s = lane / span; s < A.splits; s += step) {
                 const float down = A.stats[3 * s * A.rows + n] - top;
-                const float *p = A.part + (s * A.rows + n) * A.KP;
+                const f32x4 p = *(const f32x4 *)(A.part + (s * A.rows + n) * A.KP + k);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (lane + 64 * j < A.K)
-                        sum[j] += times_power(p[lane + 64 * j], down);
+                    sum[j] += times_power(p[j], down);
             }
-        }
+        for (int d = 32; d >= span; d >>= 1)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            pieces[wave][lane + 64 * j] = sum[j];
-        __syncthreads();
-        const int k = threadIdx.x;
-        if (k < A.K) {
-            float v = 0.0f;
-            if (alive) {
-                const int ce = Y::scaled ? half_exponent(__uint_as_float(A.col_top[k])) : 0;
-                v = times_power((pieces[0][k] + pieces[1][k]) + (pieces[2][k] + pieces[3][k]), top - peak - (float)Y::shift + (float)ce);
-                v = A.scale * weight * (v / all - rest / all * (float)((const typename Y::t *)A.w)[t * A.ldw + k]);
-            }
-            ((typename Y::t *)A.dx)[n * A.lddx + k] = (typename Y::t)v;
-        }
+            for (int j = 0; j < 4; ++j)
+                sum[j] += __shfl_xor(sum[j], d);
+        if (lane < span)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (k + j < A.K) {
+                    const int ce = Y::scaled ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
+                    const float v = times_power(sum[j], top - peak - (float)Y::shift + (float)ce);
+                    dx[k + j] = (T)(alive ? A.scale * weight * (v / all - rest / all * (float)w[k + j]) : 0.0f);
+                }
     }
 }
 
-// joins the splits of a product with G: out = scale wpow sum, dbias = wpow sum (a wavefront a row)
+// ---------------------------------------------------------------------------------------------------------------------
+// A few rows (up to 64) without gradients: what serving asks for.  Bound by reading the items once, so nothing is packed: a
+// wavefront takes a tile of 32 items straight from the table, two operands' halves of a row a lane, and splits them as it
+// goes; the rows lie in shared memory as operands.  (Three bfloat16 parts for 32-bit matrices: they need no scale, and the
+// matrix instructions have time to spare.)
+// ---------------------------------------------------------------------------------------------------------------------
+struct FewArgs {
+    const void *x, *w;
+    const int64_t *target;
+    const float *bias;
+    float *stats;                  // [workgroup][3][rows]
+    int64_t N, V, ldx, ldw, rows, v_tiles;
+    int K;
+    float c, sign;
+};
+
+// 8 values as words, from any address that suits their type
+template <class T> struct Raw { uint32_t v[2 * sizeof(T)]; };
+template <class T> __device__ __forceinline__ Raw<T> load8(const T *p)
+{
+    Raw<T> r;
+    __builtin_memcpy(&r, p, sizeof(r));
+    return r;
+}
+template <class T> __device__ __forceinline__ void zeros_from(Raw<T> &r, int left)   // `left` of the 8 are values (fewer than none: none)
+{
+#pragma unroll
+    for (int j = 0; j < (int)(2 * sizeof(T)); ++j) {
+        if (sizeof(T) == 4)
+            r.v[j] = j < left ? r.v[j] : 0u;
+        else
+            r.v[j] &= 2 * j + 1 < left ? 0xFFFFFFFFu : 2 * j < left ? 0xFFFFu : 0u;
+    }
+}
+template <class Y> __device__ __forceinline__ Parts<Y> parts_of(const Raw<typename Y::t> &r)
+{
+    Parts<Y> q;
+    if constexpr (Y::S == 1) {     // as they are
+        __builtin_memcpy(&q, &r, sizeof(q));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            split<Y>(__uint_as_float(r.v[j]), q, j);
+    }
+    return q;
+}
+
+// QB: tiles of 32 rows; CB: operands of a row, K / 16 or more
+template <class Y, int QB, int CB> __global__ __launch_bounds__(256, 2) void few_kernel(FewArgs A)
+{
+    constexpr int S = Y::S;
+    typedef typename Y::t T;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    __shared__ float join[4][QB][3][32];
+    const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int u = wave; u < QB * CB; u += 4) {
+        const int q = u / CB, cb = u % CB;
+        const int64_t n = q * 32 + low;
+        Parts<Y> p;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int k = 16 * cb + 8 * h + j;
+            split<Y>(n < A.N && k < A.K ? A.sign * (float)((const T *)A.x)[n * A.ldx + k] : 0.0f, p, j);
+        }
+        for (int s = 0; s < S; ++s)
+            *(typename Y::m::v8 *)(lds + (u * S + s) * kUnit + lane * 16) = p.p[s];
+    }
+    int target[QB];
+    float top[QB], at[QB];
+    Sum sum[QB];
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int64_t n = q * 32 + low, t = n < A.N ? A.target[n] : -1;
+        target[q] = t >= 0 && t < A.V ? (int)t : kNoTarget;
+        top[q] = kNothing;
+        at[q] = -INFINITY;
+        sum[q] = {0.0f, 0.0f};
+    }
+    __syncthreads();
+    const int64_t step = (int64_t)gridDim.x * 4, fast = A.V >= 64 ? (A.V - 32) / 32 : 0;
+    Raw<T> next[CB];
+    // A tile's rows are read in whole operands, beyond their own end, where 32 rows or more follow (K > 8 CB or CB is 2: no further than
+    // that); the last one or two tiles go through shared memory, which holds zeros there.
+    auto load = [&](int64_t tile) {
+        const int64_t v = tile * 32 + low;
+        if (tile < fast) {
+            const T *row = (const T *)A.w + v * A.ldw + 8 * h;
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+                next[cb] = load8(row + 16 * cb);
+        } else {
+            T *const copy = (T *)(lds + QB * CB * S * kUnit) + (tile - fast) * 32 * 16 * CB;
+            for (int i = lane; i < 32 * 16 * CB; i += 64) {
+                const int r = i / (16 * CB), k = i % (16 * CB);
+                copy[i] = tile * 32 + r < A.V && k < A.K ? ((const T *)A.w)[(tile * 32 + r) * A.ldw + k] : (T)0.0f;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+                next[cb] = load8(copy + low * 16 * CB + 16 * cb + 8 * h);
+        }
+    };
+    int64_t tile = (int64_t)blockIdx.x * 4 + wave;
+    if (tile < A.v_tiles)
+        load(tile);
+    for (; tile < A.v_tiles; tile += step) {
+        Raw<T> cur[CB];
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+            cur[cb] = next[cb];
+        f32x4 b[4];
+        const bool whole = tile < fast;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            b[i] = (f32x4)(0.0f);
+            if (whole && A.bias) {
+                __builtin_memcpy(&b[i], A.bias + tile * 32 + row_of(4 * i, h), 16);
+                b[i] *= kLog2e;
+            } else if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t v = tile * 32 + row_of(4 * i + j, h);
+                    b[i][j] = v >= A.V ? -INFINITY : A.bias ? A.bias[v] * kLog2e : 0.0f;
+                }
+            }
+        }
+        if (tile + step < A.v_tiles)
+            load(tile + step);
+        f32x16 z[QB];
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+            z[q] = (f32x16)(0.0f);
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            if (16 * cb + 16 > A.K)
+                zeros_from(cur[cb], A.K - 16 * cb - 8 * h);
+            const Parts<Y> a = parts_of<Y>(cur[cb]);
+#pragma unroll
+            for (int q = 0; q < QB; ++q) {
+                Parts<Y> y;
+                for (int s = 0; s < S; ++s)
+                    y.p[s] = *(const typename Y::m::v8 *)(lds + ((q * CB + cb) * S + s) * kUnit + lane * 16);
+                z[q] = product<Y>(a, y, z[q]);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < QB; ++q) {
+            f32x16 &x = z[q];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                x[i] = fmaf(x[i], A.c, b[i >> 2][i & 3]);
+            take_target(x, 1.0f, (int)tile, h, target[q], at[q]);
+            exponentials<Y>(x, 1.0f, top[q], sum[q], [](float) {});
+            sum[q].add(sum16(x));
+        }
+    }
+    // the four wavefronts' pieces become the workgroup's
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const float both = sum[q].s + other_half(sum[q].s), hit = larger(at[q], other_half(at[q]));
+        if (h == 0) {
+            join[wave][q][0][low] = top[q];
+            join[wave][q][1][low] = both;
+            join[wave][q][2][low] = hit;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 32 * QB) {
+        const int q = threadIdx.x >> 5;
+        float m = kNothing, all = 0.0f, hit = -INFINITY;
+        for (int i = 0; i < 4; ++i) {
+            m = fmaxf(m, join[i][q][0][low]);
+            hit = larger(hit, join[i][q][2][low]);
+        }
+        for (int i = 0; i < 4; ++i)
+            all += times_power(join[i][q][1][low], join[i][q][0][low] - m);
+        float *to = A.stats + (int64_t)blockIdx.x * 3 * A.rows + threadIdx.x;
+        to[0] = m;
+        to[A.rows] = all;
+        to[2 * A.rows] = hit;
+    }
+}
+
+// joins the splits of a product with G: out = scale wpow sum, dbias = wpow sum (four columns a thread)
 struct JoinArgs {
     const float *part, *tops, *sums;       // tops (ranged passes): [split][3][rows] with the sums behind, else NULL
     const float *wpow;
@@ -1113,33 +1293,39 @@ struct JoinArgs {
 
 template <class Y> __global__ __launch_bounds__(256) void join_kernel(JoinArgs A)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int quads = A.KP / 4;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, v = id / quads;
+    const int k = (int)(id - v * quads) * 4;
     if (v >= A.count)
         return;
     float top = A.tops ? kNothing : 0.0f;
     if (A.tops)
         for (int s = 0; s < A.splits; ++s)
             top = fmaxf(top, A.tops[3 * s * A.rows + v]);
-    for (int k = lane; k < A.K; k += 64) {
-        float sum = 0.0f;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-        for (int s = 0; s < A.splits; ++s) {
-            const float x = A.part[(s * A.rows + v) * A.KP + k];
-            sum += A.tops ? times_power(x, A.tops[3 * s * A.rows + v] - top) : x;
-        }
-        const int ce = Y::scaled ? half_exponent(__uint_as_float(A.col_top[k])) : 0;
-        ((typename Y::t *)A.out)[v * A.ld + k] = (typename Y::t)times_power(sum * (A.scale * *A.wpow), top - (float)Y::shift + (float)ce);
+    for (int s = 0; s < A.splits; ++s) {
+        const f32x4 p = *(const f32x4 *)(A.part + (s * A.rows + v) * A.KP + k);
+        const float down = A.tops ? A.tops[3 * s * A.rows + v] - top : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            sum[j] += times_power(p[j], down);
     }
-    if (A.dbias && lane == 0) {
-        float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (k + j < A.K) {
+            const int ce = Y::scaled ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
+            ((typename Y::t *)A.out)[v * A.ld + k + j] = (typename Y::t)times_power(sum[j] * (A.scale * *A.wpow), top - (float)Y::shift + (float)ce);
+        }
+    if (A.dbias && k == 0) {
+        float all = 0.0f;
         if (A.tops)
             for (int s = 0; s < A.splits; ++s)
-                sum += times_power(A.tops[(3 * s + 1) * A.rows + v], A.tops[3 * s * A.rows + v] - top);
+                all += times_power(A.tops[(3 * s + 1) * A.rows + v], A.tops[3 * s * A.rows + v] - top);
         else
             for (int s = 0; s < A.sum_splits; ++s)
-                sum += A.sums[s * A.rows + v];
-        A.dbias[v] = times_power(sum * *A.wpow, top - (float)Y::shift);
+                all += A.sums[s * A.rows + v];
+        A.dbias[v] = times_power(all * *A.wpow, top - (float)Y::shift);
     }
 }
 
@@ -1153,18 +1339,24 @@ template <class T> __global__ void zero_rows_kernel(T *p, int64_t rows, int K, i
 // host side
 // ---------------------------------------------------------------------------------------------------------------------
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+constexpr int kMostSplits = 256;      // a row's pieces are joined by one wavefront
 int64_t tiles_padded(int64_t tiles) { return up(tiles, kPadTiles); }
 
-// how many pieces the streamed side is cut into: enough workgroups for four on each compute unit, each with 8 tiles at least, in eights
-// (one a die) once there are that many
+// How many pieces the streamed side is cut into: enough workgroups for four on each compute unit with 8 tiles or more each, in eights (one
+// a die) once there are that many; where that leaves compute units idle, down to 2 tiles each.
 int pick_splits(int64_t workgroups, int64_t stream_tiles, int cus)
 {
     int64_t s = (4 * cus + workgroups - 1) / workgroups;
     if (s > stream_tiles / 8)
         s = stream_tiles / 8;
+    if (s * workgroups < cus) {
+        s = (cus + workgroups - 1) / workgroups;
+        if (s > stream_tiles / 2)
+            s = stream_tiles / 2;
+    }
     if (s > 8)
         s = s / 8 * 8;
-    return s < 1 ? 1 : (int)s;
+    return s < 1 ? 1 : s > kMostSplits ? kMostSplits : (int)s;
 }
 
 struct Call {
@@ -1202,6 +1394,15 @@ template <class Y, int KO, int MODE> int64_t workgroups(int64_t tiles)
     return (tiles + Z::NW * Z::QB - 1) / (Z::NW * Z::QB);
 }
 
+template <class Y, int KO, int MODE> void launch_pass(PassArgs &A, int64_t groups, hipStream_t st)
+{
+    typedef Shape<Y, KO, MODE> Z;
+    const int64_t stages = (A.stream_tiles + Z::RT - 1) / Z::RT;
+    A.base = (int)(stages / A.splits);
+    A.more = (int)(stages % A.splits);
+    pass_kernel<Y, KO, MODE><<<dim3((unsigned)A.splits, (unsigned)(groups < kGridY ? groups : kGridY), (unsigned)((groups + kGridY - 1) / kGridY)), Z::NW * 64, 0, st>>>(A);
+}
+
 void fill_prepare(PrepArgs &P, const Call &C, int64_t np, int64_t vp)
 {
     P.target = C.target;
@@ -1212,6 +1413,7 @@ void fill_prepare(PrepArgs &P, const Call &C, int64_t np, int64_t vp)
     P.np = np;
     P.vp = vp;
 }
+unsigned join_blocks(int64_t rows, int KP) { return (unsigned)((rows * (KP / 4) + 255) / 256); }
 unsigned prepare_blocks(int64_t np, int64_t vp) { return (unsigned)((np > vp ? np : vp) + 255) / 256 + 1; }
 
 void fill_finish(FinishArgs &F, const Call &C)
@@ -1276,7 +1478,7 @@ template <class Y, int KO> int64_t run_narrow(const Call &C)
 
     prepare_kernel<<<prepare_blocks(P.np, P.vp), 256, 0, C.st>>>(P);
     if (Y::scaled && C.grad) {
-        const int wb = (int)(C.v / 64 < 1 ? 1 : C.v / 64 > 4 * C.cus ? 4 * C.cus : C.v / 64), xb = (int)(C.n / 64 < 1 ? 1 : C.n / 64 > 4 * C.cus ? 4 * C.cus : C.n / 64);
+        const int most = 4 * C.cus, wb = (int)(C.v / 32 < 1 ? 1 : C.v / 32 > most ? most : C.v / 32), xb = (int)(C.n / 32 < 1 ? 1 : C.n / 32 > most ? most : C.n / 32);
         columns_kernel<<<wb + xb, 256, 0, C.st>>>(mw, mx, (int)C.k, wb);
     }
     pack_kernel<Y, KO><<<(unsigned)(v_tiles + n_tiles), 256, 0, C.st>>>(mw, mx, (int)C.k, (int)v_tiles);
@@ -1311,12 +1513,12 @@ template <class Y, int KO> int64_t run_narrow(const Call &C)
     F.KP = KP;
     F.splits = row_splits;
     if (!C.grad) {
-        pass_kernel<Y, KO, kNll><<<(unsigned)(row_groups * row_splits), Shape<Y, KO, kNll>::NW * 64, 0, C.st>>>(A);
-        finish_rows_kernel<Y, false><<<(unsigned)C.n, 256, 0, C.st>>>(F);
+        launch_pass<Y, KO, kNll>(A, row_groups, C.st);
+        finish_rows_kernel<Y, false><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
         return (int)hipGetLastError();
     }
-    pass_kernel<Y, KO, kRows><<<(unsigned)(row_groups * row_splits), Shape<Y, KO, kRows>::NW * 64, 0, C.st>>>(A);
-    finish_rows_kernel<Y, true><<<(unsigned)nr, 256, 0, C.st>>>(F);
+    launch_pass<Y, KO, kRows>(A, row_groups, C.st);
+    finish_rows_kernel<Y, true><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
 
     A.still = mw.by_row;
     A.by_row = mx.by_row;
@@ -1342,10 +1544,10 @@ template <class Y, int KO> int64_t run_narrow(const Call &C)
         A.quads = C.lddw % 4 == 0 && (uintptr_t)C.dw % (4 * sizeof(T)) == 0;
         A.scale = C.scale;
     }
-    pass_kernel<Y, KO, kItems><<<(unsigned)(item_groups * item_splits), Shape<Y, KO, kItems>::NW * 64, 0, C.st>>>(A);
+    launch_pass<Y, KO, kItems>(A, item_groups, C.st);
     if (item_splits > 1) {
         const JoinArgs J = {part, item_stats, nullptr, P.wpow, mx.col_top, C.v, vr, C.lddw, (int)C.k, KP, item_splits, 0, C.scale, C.dw, C.bias ? C.dbias : nullptr};
-        join_kernel<Y><<<(unsigned)((C.v + 3) / 4), 256, 0, C.st>>>(J);
+        join_kernel<Y><<<join_blocks(C.v, KP), 256, 0, C.st>>>(J);
     }
     return (int)hipGetLastError();
 }
@@ -1413,10 +1615,10 @@ template <class Y> int64_t run_wide(const Call &C)
     F.rows = nr;
     F.splits = 2 * row_splits;
     if (!C.grad) {
-        finish_rows_kernel<Y, false><<<(unsigned)C.n, 256, 0, C.st>>>(F);
+        finish_rows_kernel<Y, false><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
         return (int)hipGetLastError();
     }
-    finish_rows_kernel<Y, true><<<(unsigned)nr, 256, 0, C.st>>>(F);
+    finish_rows_kernel<Y, true><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
     A.reg_bias = F.reg_bias;
     A.target_log = F.target_log;
     for (int64_t v0 = 0; v0 < v_tiles; v0 += chunk) {
@@ -1430,10 +1632,74 @@ template <class Y> int64_t run_wide(const Call &C)
         const int64_t first = v0 * 32, count = C.v - first < A.v_count * 32 ? C.v - first : A.v_count * 32;
         const JoinArgs J = {dw_part, nullptr, A.part_sum, P.wpow, nullptr, count, A.v_count * 32, C.lddw, (int)C.k, KP, dw_splits, sum_splits, C.scale,
                             (T *)C.dw + first * C.lddw, C.bias ? C.dbias + first : nullptr};
-        join_kernel<Y><<<(unsigned)((count + 3) / 4), 256, 0, C.st>>>(J);
+        join_kernel<Y><<<join_blocks(count, KP), 256, 0, C.st>>>(J);
     }
     const JoinArgs J = {dx_part, nullptr, nullptr, P.wpow, nullptr, C.n, nr, C.lddx, (int)C.k, KP, dx_splits, 0, C.scale, C.dx, nullptr};
-    join_kernel<Y><<<(unsigned)((C.n + 3) / 4), 256, 0, C.st>>>(J);
+    join_kernel<Y><<<join_blocks(C.n, KP), 256, 0, C.st>>>(J);
+    return (int)hipGetLastError();
+}
+
+// a few rows, no gradients (Y as the products take it: W32 for 32 bits).  A wavefront holds two tiles' rows as they are: 256 registers
+// have room for 2 x 128 values of 32 bits, or 2 x 256 of 16, a row.
+template <class Y> bool is_few(const Call &C) { return !C.grad && C.n <= 64 && C.k <= (Y::S == 1 ? 256 : 128); }
+
+template <class Y, int QB, int CB> void launch_few(const FewArgs &A, unsigned grid, hipStream_t st)
+{
+    const int bytes = QB * CB * Y::S * kUnit + 2 * 32 * 16 * CB * (int)sizeof(typename Y::t);   // at most 48 + 32 KB
+    few_kernel<Y, QB, CB><<<grid, 256, bytes, st>>>(A);
+}
+template <class Y, int QB> void launch_few_rows(const FewArgs &A, unsigned grid, hipStream_t st)
+{
+    if (A.K <= 32)
+        launch_few<Y, QB, 2>(A, grid, st);
+    else if (A.K <= 64)
+        launch_few<Y, QB, 4>(A, grid, st);
+    else if (A.K <= 112)
+        launch_few<Y, QB, 7>(A, grid, st);
+    else if (A.K <= 128)
+        launch_few<Y, QB, 8>(A, grid, st);
+    else if constexpr (Y::S == 1) {
+        if (A.K <= 208)
+            launch_few<Y, QB, 13>(A, grid, st);
+        else
+            launch_few<Y, QB, 16>(A, grid, st);
+    }
+}
+
+template <class Y> int64_t run_few(const Call &C)
+{
+    FewArgs A = {};
+    A.rows = up(C.n, 32);
+    A.v_tiles = (C.v + 31) / 32;
+    A.K = (int)C.k;
+    int64_t grid = (A.v_tiles + 7) / 8;            // two tiles a wavefront at least
+    grid = grid > 2 * C.cus ? 2 * C.cus : grid;
+    Space S = {C.ws, 0};
+    A.stats = S.take<float>(grid * 3 * A.rows * 4);
+    if (!C.ws)
+        return S.used;
+    if (C.ws_bytes < S.used)
+        return HPF_EINVAL;
+    A.x = C.x;
+    A.w = C.w;
+    A.target = C.target;
+    A.bias = C.bias;
+    A.N = C.n;
+    A.V = C.v;
+    A.ldx = C.ldx;
+    A.ldw = C.ldw;
+    A.c = fabsf(C.scale) * kLog2e;
+    A.sign = C.scale < 0.0f ? -1.0f : 1.0f;
+    if (C.n <= 32)
+        launch_few_rows<Y, 1>(A, (unsigned)grid, C.st);
+    else
+        launch_few_rows<Y, 2>(A, (unsigned)grid, C.st);
+    FinishArgs F = {};
+    fill_finish(F, C);
+    F.stats = A.stats;
+    F.rows = A.rows;
+    F.splits = (int)grid;
+    finish_rows_kernel<Y, false><<<(unsigned)(A.rows / 4), 256, 0, C.st>>>(F);
     return (int)hipGetLastError();
 }
 
@@ -1455,10 +1721,10 @@ int64_t run(int type, const Call &C)
 {
     const bool narrow = C.k <= 256;
     if (type == HPF_F32)
-        return narrow ? run_any_narrow<F32>(C) : run_wide<W32>(C);
+        return is_few<W32>(C) ? run_few<W32>(C) : narrow ? run_any_narrow<F32>(C) : run_wide<W32>(C);
     if (type == HPF_BF16)
-        return narrow ? run_any_narrow<B16>(C) : run_wide<B16>(C);
-    return narrow ? run_any_narrow<H16>(C) : run_wide<H16>(C);
+        return is_few<B16>(C) ? run_few<B16>(C) : narrow ? run_any_narrow<B16>(C) : run_wide<B16>(C);
+    return is_few<H16>(C) ? run_few<H16>(C) : narrow ? run_any_narrow<H16>(C) : run_wide<H16>(C);
 }
 
 bool sizes_ok(int64_t n, int64_t v, int64_t k) { return n >= 0 && v > 0 && k > 0 && n < kNoTarget - 31 && v < kNoTarget - 31 && k < (1 << 20); }
