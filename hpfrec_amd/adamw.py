@@ -39,15 +39,15 @@ def adamw_state(params, state_bits=32):
 
 
 def _held(t, name, i, shape, dtypes, device):
-    if not torch.is_tensor(t) or t.dtype not in dtypes:
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.shape == shape and t.device == device and t.is_contiguous():
+        return t.data_ptr()
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         raise ValueError("%s[%d] must be a tensor of %s" % (name, i, " or ".join(str(d) for d in dtypes)))
     if t.shape != shape:
         raise ValueError("%s[%d] has shape %s, expected %s" % (name, i, tuple(t.shape), tuple(shape)))
     if not t.is_contiguous():
         raise ValueError("%s[%d] must be contiguous" % (name, i))
-    if t.device != device:
-        raise ValueError("%s[%d] is on %s, expected %s" % (name, i, t.device, device))
-    return t.data_ptr()
+    raise ValueError("%s[%d] is on %s, expected %s" % (name, i, t.device, device))
 
 
 _PARAM_TYPES = tuple(TYPE_CODES)
@@ -84,15 +84,16 @@ def adamw_step(ops, params, grads, m, v, step, masters=None, m_scale=None, v_sca
     device = step.device if torch.is_tensor(step) else None
     if device is None or step.dtype != torch.int64 or step.numel() != 1:
         raise ValueError("step must be an int64 tensor of one element")
-    if device.type != ops.device.type or ops.device.index not in (None, device.index):
+    if device != ops.device and (ops.device.index is not None or device.type != ops.device.type):
         raise ValueError("step is on %s, expected %s" % (device, ops.device))
     if torch.is_tensor(lr):
         if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
             raise ValueError("lr must be a number or a float32 tensor of one element on %s" % device)
     elif not (math.isfinite(lr) and lr >= 0.0):
         raise ValueError("lr must be finite and not negative")
-    decay = [float(weight_decay)] * count if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
-    if len(decay) != count or not all(math.isfinite(w) and w >= 0.0 for w in decay):
+    one = isinstance(weight_decay, (int, float))
+    decay = [float(weight_decay)] * count if one else [float(w) for w in weight_decay]
+    if len(decay) != count or not all(math.isfinite(w) and w >= 0.0 for w in (decay[:1] if one else decay)):
         raise ValueError("weight_decay must be a finite number that is not negative, or one for each of params")
     groups, written, read = {}, [(step.data_ptr(), 8)], []
     for i in range(count):
@@ -118,13 +119,13 @@ def adamw_step(ops, params, grads, m, v, step, masters=None, m_scale=None, v_sca
             raise ValueError("m_scale[%d], v_scale[%d]: 32-bit moments have no scales" % (i, i))
         if n == 0:
             continue
-        size, moment = p.element_size() * n, m[i].element_size() * n
+        size, moment = (4 if at_w is None else 2) * n, (1 if eight else 4) * n
         written += [(at, size), (at_m, moment), (at_v, moment)]
         if at_w is not None:
             written.append((at_w, 4 * n))
         if eight:
             written += [(at_ms, 4 * scales[0]), (at_vs, 4 * scales[0])]
-        read.append((g, grads[i].element_size() * n))
+        read.append((g, (4 if grads[i].dtype == torch.float32 else 2) * n))
         groups.setdefault((p.dtype, grads[i].dtype, 8 if eight else 32), []).append((at, g, at_m, at_v, at_w, at_ms, at_vs, n, decay[i], i, 0))
     written.sort()
     if any(a + size > b for (a, size), (b, _) in zip(written, written[1:])):

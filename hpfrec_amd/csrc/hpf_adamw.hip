@@ -26,7 +26,7 @@
 namespace {
 
 constexpr int kBlock = 256;              // values per wavefront pass = values per scale of an 8-bit moment
-constexpr int kChunkBlocks = 16;         // blocks per workgroup pass: 4 wavefronts x 4
+constexpr int kAtOnce = 2;               // blocks of a wavefront in flight
 constexpr int kMaxTensors = 40;          // per launch: their descriptors travel in the kernel's arguments
 constexpr int kTicketShift = 40;         // the step counter's upper bits count the workgroups that are done
 
@@ -37,7 +37,7 @@ struct Tensor {
     float *master, *m_scale, *v_scale;
     int64_t n;
     double wd;
-    int32_t chunk0;                      // first chunk of this tensor in the launch
+    int32_t block0;                      // its first block in the launch
     int32_t number;                      // its number in the caller's list (part of the random bits' key)
     int32_t wide;                        // every pointer allows the wide accesses
 };
@@ -48,7 +48,7 @@ struct Args {
     const float *lr_dev;
     double lr, b1, b2, eps;
     uint64_t seed;
-    int32_t ntensors, nchunks, advance;
+    int32_t ntensors, nblocks, advance;
 };
 static_assert(sizeof(Args) <= 4096, "kernel arguments");
 
@@ -125,133 +125,178 @@ __device__ inline uint32_t mix(uint32_t x)
 // the power of two that puts `top` (finite, >= 0) into [128, 256); 1 for an empty block
 __device__ inline float block_scale(float top)
 {
-    int e = 127 - 126;                                          // a subnormal's scale: 2^-126
-    const int b = (int)(__float_as_uint(top) >> 23);            // biased exponent
-    if (b - 7 > 1)
-        e = b - 7;
-    return top > 0.0f ? __uint_as_float((uint32_t)e << 23) : 1.0f;
+    const int e = (int)(__float_as_uint(top) >> 23) - 7;        // biased; a subnormal's scale: 2^-126
+    return top > 0.0f ? __uint_as_float((uint32_t)(e > 1 ? e : 1) << 23) : 1.0f;
 }
 
 // four values' codes; inv is the scale's reciprocal (exact: a power of two)
-__device__ inline uint32_t encode4(const float x[4], float inv, const uint32_t bits16[4], bool least)
+template <bool ROOT> __device__ inline uint32_t encode4(const float x[4], float inv, const uint32_t bits16[4])
 {
     float q[4];
-    uint32_t lost = 0;
+    bool lost = false;
     for (int i = 0; i < 4; ++i) {
         const float y = x[i] * inv, a = fabsf(y);
         const float low = a < 0x1p-6f ? 0x1p-6f : 0.0f;         // e4m3's subnormals: a fixed step, at the end of this sum's mantissa
         const uint32_t b = (__float_as_uint(a + low) + (bits16[i] << 4)) & 0xFFF00000u;
         float r = __uint_as_float(b) - low;
-        if (least && r == 0.0f && x[i] > 0.0f)
-            r = 0x1p-9f;
-        q[i] = copysignf(r, y);
-        if (!(a < 0x1p127f))                                    // infinite or NaN: the one code that says so
-            lost |= 0x7Fu << (8 * i);
+        if (ROOT)
+            r = fmaxf(r, x[i] > 0.0f ? 0x1p-9f : 0.0f);         // a root above zero keeps the smallest code
+        q[i] = ROOT ? r : copysignf(r, y);
+        lost |= !(a < 0x1p127f);
     }
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
     w = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
-    uint32_t keep = (uint32_t)w;
-    for (int i = 0; i < 4; ++i)
-        if (lost >> (8 * i) & 0xFF)
-            keep = (keep & ~(0xFFu << (8 * i))) | 0x7Fu << (8 * i);
-    return keep;
+    if (__any(lost))                                            // infinite or NaN: the one code that says so
+        for (int i = 0; i < 4; ++i)
+            if (!(fabsf(x[i]) < INFINITY))
+                w = (int)(((uint32_t)w & ~(0xFFu << (8 * i))) | 0x7Fu << (8 * i));
+    return (uint32_t)w;
 }
 
+// the wavefront's largest, by exchanges within registers (lanes' neighbours, rows of 16, halves)
+template <int CTRL> __device__ inline float max_dpp(float x)
+{
+    return fmaxf(x, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)__float_as_uint(x), (int)__float_as_uint(x), CTRL, 0xF, 0xF, true)));
+}
 __device__ inline float wave_max(float x)
 {
-    for (int d = 32; d; d >>= 1)
-        x = fmaxf(x, __shfl_xor(x, d));
-    return x;
+    x = max_dpp<0xB1>(x);     // lanes 1 0 3 2
+    x = max_dpp<0x4E>(x);     // lanes 2 3 0 1
+    x = max_dpp<0x141>(x);    // mirrored within 8
+    x = max_dpp<0x140>(x);    // mirrored within 16
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-__device__ inline float finite_or_zero(float x) { return x < INFINITY ? x : 0.0f; }   // x >= 0 or NaN
+// the largest finite magnitude of the block
+__device__ inline float block_top(const float x[4])
+{
+    float top = wave_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));   // (of NaN and a number: the number)
+    if (!(top < INFINITY)) {
+        top = 0.0f;
+        for (int i = 0; i < 4; ++i)
+            top = fmaxf(top, fabsf(x[i]) < INFINITY ? fabsf(x[i]) : 0.0f);
+        top = wave_max(top);
+    }
+    return top;
+}
+
+// the square root of x >= 2^-96, rounded to nearest: the hardware's, good to one unit, against its two neighbours
+__device__ inline float root_of(float x)
+{
+    const float s = __builtin_amdgcn_sqrtf(x), down = __uint_as_float(__float_as_uint(s) - 1), up = __uint_as_float(__float_as_uint(s) + 1);
+    const float r = fmaf(-down, s, x) <= 0.0f ? down : s;
+    return fmaf(-up, s, x) > 0.0f ? up : r;
+}
+
+// b^n
+__device__ inline double power(double b, unsigned long long n)
+{
+    double r = 1.0;
+    for (; n; n >>= 1, b *= b)
+        r = n & 1 ? r * b : r;
+    return r;
+}
 
 template <class P, class G, int BITS> __global__ __launch_bounds__(256) void adamw_kernel(Args A)
 {
-    __shared__ double corr[2];
-    __shared__ float lr_s;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
     const unsigned long long at = __hip_atomic_load(A.step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & ((1ull << kTicketShift) - 1);
     const unsigned long long now = at + 1;
-    if (threadIdx.x == 0) {
-        corr[0] = 1.0 - pow(A.b1, (double)now);
-        corr[1] = sqrt(1.0 - pow(A.b2, (double)now));
-        lr_s = A.lr_dev ? *A.lr_dev : 0.0f;
-    }
-    __syncthreads();
-    const double lr = A.lr_dev ? (double)lr_s : A.lr;
-    const float rate = (float)(lr / corr[0]), root = (float)corr[1], eps = (float)A.eps;
+    const double lr = A.lr_dev ? (double)*A.lr_dev : A.lr;
+    const float rate = (float)(lr / (1.0 - power(A.b1, now))), over_root = (float)(1.0 / sqrt(1.0 - power(A.b2, now))), eps = (float)A.eps;
     const float b1 = (float)A.b1, b2 = (float)A.b2, c1 = (float)(1.0 - A.b1), c2 = (float)(1.0 - A.b2);
     const uint32_t key0 = mix(mix(mix((uint32_t)A.seed) ^ (uint32_t)(A.seed >> 32)) + (uint32_t)now);
 
-    int ti = 0;
-    for (int chunk = blockIdx.x; chunk < A.nchunks; chunk += gridDim.x) {
-        while (ti + 1 < A.ntensors && A.t[ti + 1].chunk0 <= chunk)
-            ++ti;
+    // an equal share of consecutive blocks for each wavefront, from the tensor that holds the first one on
+    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6))), waves = gridDim.x * 4;
+    const int share = A.nblocks / waves, more = A.nblocks % waves;
+    int done = share * wave + (wave < more ? wave : more);
+    const int stop = done + share + (wave < more);
+    for (int ti = 0; done < stop; ++ti) {
+        const int last = ti + 1 < A.ntensors ? A.t[ti + 1].block0 : A.nblocks;     // beyond the tensor's
+        if (last <= done)
+            continue;
         const Tensor &t = A.t[ti];
         const float keep = (float)(1.0 - lr * t.wd);
         const bool wide = t.wide != 0;
         const uint32_t key = mix(key0 + (uint32_t)t.number);
         P *const pp = (P *)t.p;
         const G *const gp = (const G *)t.g;
-        const int64_t block0 = (int64_t)(chunk - t.chunk0) * kChunkBlocks + wave;
+        const int end = last < stop ? last : stop;
+        for (; done < end; done += kAtOnce) {      // kAtOnce blocks' loads are on their way together
+            float p[kAtOnce][4], g[kAtOnce][4], m[kAtOnce][4], v[kAtOnce][4];
+            int valid[kAtOnce];
 #pragma unroll
-        for (int k = 0; k < kChunkBlocks / 4; ++k) {
-            const int64_t block = block0 + 4 * k, i0 = block * kBlock + 4 * lane, left = t.n - i0;
-            if (block * kBlock >= t.n)
-                break;
-            const int valid = left >= 4 ? 4 : left > 0 ? (int)left : 0;
-            float p[4], g[4], m[4], v[4];
-            load4(gp + i0, wide, valid, g);
-            if constexpr (sizeof(P) == 4)
-                load4((const float *)pp + i0, wide, valid, p);
-            else
-                load4(t.master + i0, wide, valid, p);
-            if constexpr (BITS == 8) {
-                decode4(load_codes((const uint8_t *)t.m + i0, wide, valid), t.m_scale[block], m);
-                decode4(load_codes((const uint8_t *)t.v + i0, wide, valid), t.v_scale[block], v);
-                for (int i = 0; i < 4; ++i)
-                    v[i] = v[i] * v[i];
-            } else {
-                load4((const float *)t.m + i0, wide, valid, m);
-                load4((const float *)t.v + i0, wide, valid, v);
-            }
-            float r[4], top_m = 0.0f, top_r = 0.0f;
-            for (int i = 0; i < 4; ++i) {
-                m[i] = m[i] * b1 + g[i] * c1;
-                v[i] = v[i] * b2 + (g[i] * g[i]) * c2;
-                r[i] = sqrtf(v[i]);
-                p[i] = p[i] * keep - rate * m[i] / (r[i] / root + eps);
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int64_t block = done + u - t.block0, i0 = block * kBlock + 4 * lane, left = done + u < end ? t.n - i0 : 0;
+                valid[u] = left >= 4 ? 4 : left > 0 ? (int)left : 0;
+                load4(gp + i0, wide, valid[u], g[u]);
+                if constexpr (sizeof(P) == 4)
+                    load4((const float *)pp + i0, wide, valid[u], p[u]);
+                else
+                    load4(t.master + i0, wide, valid[u], p[u]);
                 if constexpr (BITS == 8) {
-                    top_m = fmaxf(top_m, finite_or_zero(fabsf(m[i])));
-                    top_r = fmaxf(top_r, finite_or_zero(r[i]));
+                    const bool in = done + u < end;
+                    decode4(load_codes((const uint8_t *)t.m + i0, wide, valid[u]), in ? t.m_scale[block] : 0.0f, m[u]);
+                    decode4(load_codes((const uint8_t *)t.v + i0, wide, valid[u]), in ? t.v_scale[block] : 0.0f, v[u]);
+                    for (int i = 0; i < 4; ++i)
+                        v[u][i] = v[u][i] * v[u][i];
+                } else {
+                    load4((const float *)t.m + i0, wide, valid[u], m[u]);
+                    load4((const float *)t.v + i0, wide, valid[u], v[u]);
                 }
             }
-            if constexpr (sizeof(P) == 4) {
-                store4((float *)pp + i0, wide, valid, p);
-            } else {
-                store4(t.master + i0, wide, valid, p);
-                store4(pp + i0, wide, valid, p);
-            }
-            if constexpr (BITS == 8) {
-                const float ms = block_scale(wave_max(top_m)), rs = block_scale(wave_max(top_r));
-                uint32_t bm[4], br[4];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int64_t block = done + u - t.block0, i0 = block * kBlock + 4 * lane;
+                float r[4];
+                bool tiny = false;
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t w = mix((uint32_t)(i0 + i) + key + (uint32_t)((i0 + i) >> 32) * kMulA);
-                    bm[i] = w & 0xFFFFu;
-                    br[i] = w >> 16;
+                    m[u][i] = m[u][i] * b1 + g[u][i] * c1;
+                    v[u][i] = v[u][i] * b2 + (g[u][i] * g[u][i]) * c2;
+                    tiny |= v[u][i] < 0x1p-96f;
                 }
-                store_codes((uint8_t *)t.m + i0, wide, valid, encode4(m, 1.0f / ms, bm, false));
-                store_codes((uint8_t *)t.v + i0, wide, valid, encode4(r, 1.0f / rs, br, true));
-                if (lane == 0) {
-                    t.m_scale[block] = ms;
-                    t.v_scale[block] = rs;
+                if (__any(tiny)) {             // whatever the size
+                    for (int i = 0; i < 4; ++i) {
+                        r[i] = sqrtf(v[u][i]);
+                        p[u][i] = p[u][i] * keep - rate * m[u][i] / (r[i] * over_root + eps);
+                    }
+                } else {                       // (the hardware's reciprocal is good to one unit, which is what p needs of it)
+                    for (int i = 0; i < 4; ++i) {
+                        r[i] = root_of(v[u][i]);
+                        p[u][i] = p[u][i] * keep - (rate * m[u][i]) * __builtin_amdgcn_rcpf(r[i] * over_root + eps);
+                    }
                 }
-            } else {
-                store4((float *)t.m + i0, wide, valid, m);
-                store4((float *)t.v + i0, wide, valid, v);
+                if constexpr (sizeof(P) == 4) {
+                    store4((float *)pp + i0, wide, valid[u], p[u]);
+                } else {
+                    store4(t.master + i0, wide, valid[u], p[u]);
+                    store4(pp + i0, wide, valid[u], p[u]);
+                }
+                if constexpr (BITS == 8) {
+                    const float ms = block_scale(block_top(m[u])), rs = block_scale(block_top(r));
+                    uint32_t bm[4], br[4];
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t w = mix((uint32_t)(i0 + i) + key + (uint32_t)((i0 + i) >> 32) * kMulA);
+                        bm[i] = w & 0xFFFFu;
+                        br[i] = w >> 16;
+                    }
+                    store_codes((uint8_t *)t.m + i0, wide, valid[u], encode4<false>(m[u], 1.0f / ms, bm));
+                    store_codes((uint8_t *)t.v + i0, wide, valid[u], encode4<true>(r, 1.0f / rs, br));
+                    if (lane == 0 && done + u < end) {
+                        t.m_scale[block] = ms;
+                        t.v_scale[block] = rs;
+                    }
+                } else {
+                    store4((float *)t.m + i0, wide, valid[u], m[u]);
+                    store4((float *)t.v + i0, wide, valid[u], v[u]);
+                }
             }
         }
+        done = end;
     }
     // The counter moves on once every workgroup has read it: the last to arrive adds the one and takes the arrivals away.
     if (A.advance) {
@@ -324,15 +369,15 @@ extern "C" int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors,
         A.eps = eps;
         A.seed = seed;
         A.ntensors = 0;
-        int64_t chunks = 0;
+        int64_t blocks = 0;
         for (; i < ntensors && A.ntensors < kMaxTensors; ++i) {
             const hpf_adamw_tensor &t = tensors[i];
             if (t.n == 0)
                 continue;
-            const int64_t mine = (t.n + (int64_t)kBlock * kChunkBlocks - 1) / ((int64_t)kBlock * kChunkBlocks);
-            if (chunks + mine > 0x7FFFFFFF) {
-                if (chunks == 0)
-                    return HPF_EUNSUPPORTED;   // one tensor of over 2^43 values
+            const int64_t mine = (t.n + kBlock - 1) / kBlock;
+            if (blocks + mine > 0x7FFFFF00) {
+                if (blocks == 0)
+                    return HPF_EUNSUPPORTED;   // one tensor of over 2^38 values
                 break;
             }
             Tensor &d = A.t[A.ntensors++];
@@ -345,17 +390,18 @@ extern "C" int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors,
             d.v_scale = t.v_scale;
             d.n = t.n;
             d.wd = t.weight_decay;
-            d.chunk0 = (int32_t)chunks;
+            d.block0 = (int32_t)blocks;
             d.number = t.number;
             d.wide = aligned(t.param, 4 * psize) && aligned(t.grad, 4 * gsize) && aligned(t.m, 4 * ssize) &&
                      aligned(t.v, 4 * ssize) && aligned(t.master, 16);
-            chunks += mine;
+            blocks += mine;
         }
-        A.nchunks = (int32_t)chunks;
+        A.nblocks = (int32_t)blocks;
         A.advance = i >= ntensors ? advance != 0 : 0;
-        if (chunks == 0 && !A.advance)
+        if (blocks == 0 && !A.advance)
             break;
-        const int grid = (int)(chunks < 1 ? 1 : chunks < grid_blocks ? chunks : grid_blocks);
+        const int64_t want = (blocks + 7) / 8;       // four wavefronts of kAtOnce blocks
+        const int grid = (int)(want < 1 ? 1 : want < grid_blocks ? want : grid_blocks);
         const hipStream_t st = (hipStream_t)stream;
         const int rc = param_type == HPF_F32    ? launch_g<float>(A, grad_type, state_bits, grid, st)
                        : param_type == HPF_BF16 ? launch_g<__bf16>(A, grad_type, state_bits, grid, st)

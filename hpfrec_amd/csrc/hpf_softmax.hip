@@ -208,35 +208,45 @@ struct Matrix {
 
 __device__ __forceinline__ bool counts(const Matrix &M, int64_t row) { return row < M.rows && !(M.target && (uint64_t)M.target[row] >= (uint64_t)M.items); }
 
-// largest magnitudes of the columns of both matrices (a wavefront reads whole rows)
-__global__ __launch_bounds__(256) void columns_kernel(Matrix W, Matrix X, int K, int w_blocks)
+// Largest magnitudes of the columns of both matrices; a wavefront reads whole rows, 8 at a time.  One workgroup of 16 wavefronts a compute
+// unit: each ends in an atomic maximum a column, and those of one column are served one after the other (about 60 ns each).
+__global__ __launch_bounds__(1024) void columns_kernel(Matrix W, Matrix X, int K, int w_blocks)
 {
-    __shared__ float top[4][256];
+    __shared__ float top[16][256];
     const bool second = (int)blockIdx.x >= w_blocks;
     const Matrix &M = second ? X : W;
-    const int64_t first = (second ? blockIdx.x - w_blocks : blockIdx.x) * 4 + (threadIdx.x >> 6), step = (second ? gridDim.x - w_blocks : w_blocks) * 4;
-    const int lane = threadIdx.x & 63;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t first = (second ? blockIdx.x - w_blocks : blockIdx.x) * 16 + wave, step = (second ? gridDim.x - w_blocks : w_blocks) * 16;
     float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int64_t r = first; r < M.rows; r += 8 * step) {
         float x[8][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int j = 0; j < 4; ++j)
+            if (64 * j < K)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                x[i][j] = r + i * step < M.rows && lane + 64 * j < K ? ((const float *)M.p)[(r + i * step) * M.ld + lane + 64 * j] : 0.0f;
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t row = r + i * step < M.rows ? r + i * step : r;      // (a row twice changes no maximum)
+                    x[i][j] = ((const float *)M.p)[row * M.ld + (lane + 64 * j < K ? lane + 64 * j : K - 1)];
+                }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (!M.target || counts(M, r + i * step))
+            if (!M.target || counts(M, r + i * step < M.rows ? r + i * step : r))
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    m[j] = fmaxf(m[j], finite_size(x[i][j]));
+                    if (64 * j < K)
+                        m[j] = fmaxf(m[j], finite_size(x[i][j]));
     }
     for (int j = 0; j < 4; ++j)
-        top[threadIdx.x >> 6][lane + 64 * j] = m[j];
+        top[wave][lane + 64 * j] = m[j];
     __syncthreads();
     const int c = threadIdx.x;
-    if (c < K)
-        atomicMax(&M.col_top[c], __float_as_uint(fmaxf(fmaxf(top[0][c], top[1][c]), fmaxf(top[2][c], top[3][c]))));
+    if (c < K) {
+        float all = top[0][c];
+        for (int i = 1; i < 16; ++i)
+            all = fmaxf(all, top[i][c]);
+        if (__float_as_uint(all) > __hip_atomic_load(&M.col_top[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+            atomicMax(&M.col_top[c], __float_as_uint(all));
+    }
 }
 
 // packing: rows -> units, one workgroup 32 rows.  `by_row`: tile of 32 rows after tile, in it K / 16 units (lane: row lane % 32,
@@ -1017,6 +1027,7 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
     }
     // splits over the lanes: maxima first, then sums relative to them
     float top = kNothing, at = -INFINITY, others = 0.0f;
+#pragma unroll 4
     for (int s = lane; s < A.splits; s += 64) {
         top = fmaxf(top, A.stats[(3 * s + 0) * A.rows + n]);
         at = larger(at, A.stats[(3 * s + 2) * A.rows + n]);
@@ -1025,6 +1036,7 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
         top = fmaxf(top, __shfl_xor(top, d));
         at = larger(at, __shfl_xor(at, d));
     }
+#pragma unroll 4
     for (int s = lane; s < A.splits; s += 64)
         others += times_power(A.stats[(3 * s + 1) * A.rows + n], A.stats[3 * s * A.rows + n] - top);
     for (int d = 32; d; d >>= 1)
@@ -1111,6 +1123,8 @@ struct FewArgs {
     float c, sign;
 };
 
+constexpr int kFewWaves = 8;
+
 // 8 values as words, from any address that suits their type
 template <class T> struct Raw { uint32_t v[2 * sizeof(T)]; };
 template <class T> __device__ __forceinline__ Raw<T> load8(const T *p)
@@ -1143,15 +1157,41 @@ template <class Y> __device__ __forceinline__ Parts<Y> parts_of(const Raw<typena
 }
 
 // QB: tiles of 32 rows; CB: operands of a row, K / 16 or more
-template <class Y, int QB, int CB> __global__ __launch_bounds__(256, 2) void few_kernel(FewArgs A)
+template <class Y, int QB, int CB> __global__ __launch_bounds__(kFewWaves * 64, 2) void few_kernel(FewArgs A)
 {
     constexpr int S = Y::S;
     typedef typename Y::t T;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
-    __shared__ float join[4][QB][3][32];
+    __shared__ float join[kFewWaves][QB][3][32];
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int u = wave; u < QB * CB; u += 4) {
+    const int64_t step = (int64_t)gridDim.x * kFewWaves, fast = A.V >= 64 ? (A.V - 32) / 32 : 0;
+    Raw<T> next[CB];
+    // A tile's rows are read in whole operands, beyond their own end, where 32 rows or more follow (K > 8 CB or CB is 2: no further than
+    // that); the last one or two tiles go through shared memory, which holds zeros there.
+    auto load = [&](int64_t tile) {
+        const int64_t v = tile * 32 + low;
+        if (tile < fast) {
+            const T *row = (const T *)A.w + v * A.ldw + 8 * h;
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+                next[cb] = load8(row + 16 * cb);
+        } else {
+            T *const copy = (T *)(lds + QB * CB * S * kUnit) + (tile - fast) * 32 * 16 * CB;
+            for (int i = lane; i < 32 * 16 * CB; i += 64) {
+                const int r = i / (16 * CB), k = i % (16 * CB);
+                copy[i] = tile * 32 + r < A.V && k < A.K ? ((const T *)A.w)[(tile * 32 + r) * A.ldw + k] : (T)0.0f;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb)
+                next[cb] = load8(copy + low * 16 * CB + 16 * cb + 8 * h);
+        }
+    };
+    int64_t tile = (int64_t)blockIdx.x * kFewWaves + wave;
+    if (tile < A.v_tiles)
+        load(tile);
+    for (int u = wave; u < QB * CB; u += kFewWaves) {
         const int q = u / CB, cb = u % CB;
         const int64_t n = q * 32 + low;
         Parts<Y> p;
@@ -1175,32 +1215,6 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__(256, 2) void few
         sum[q] = {0.0f, 0.0f};
     }
     __syncthreads();
-    const int64_t step = (int64_t)gridDim.x * 4, fast = A.V >= 64 ? (A.V - 32) / 32 : 0;
-    Raw<T> next[CB];
-    // A tile's rows are read in whole operands, beyond their own end, where 32 rows or more follow (K > 8 CB or CB is 2: no further than
-    // that); the last one or two tiles go through shared memory, which holds zeros there.
-    auto load = [&](int64_t tile) {
-        const int64_t v = tile * 32 + low;
-        if (tile < fast) {
-            const T *row = (const T *)A.w + v * A.ldw + 8 * h;
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
-                next[cb] = load8(row + 16 * cb);
-        } else {
-            T *const copy = (T *)(lds + QB * CB * S * kUnit) + (tile - fast) * 32 * 16 * CB;
-            for (int i = lane; i < 32 * 16 * CB; i += 64) {
-                const int r = i / (16 * CB), k = i % (16 * CB);
-                copy[i] = tile * 32 + r < A.V && k < A.K ? ((const T *)A.w)[(tile * 32 + r) * A.ldw + k] : (T)0.0f;
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
-                next[cb] = load8(copy + low * 16 * CB + 16 * cb + 8 * h);
-        }
-    };
-    int64_t tile = (int64_t)blockIdx.x * 4 + wave;
-    if (tile < A.v_tiles)
-        load(tile);
     for (; tile < A.v_tiles; tile += step) {
         Raw<T> cur[CB];
 #pragma unroll
@@ -1252,7 +1266,7 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__(256, 2) void few
             sum[q].add(sum16(x));
         }
     }
-    // the four wavefronts' pieces become the workgroup's
+    // the wavefronts' pieces become the workgroup's
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const float both = sum[q].s + other_half(sum[q].s), hit = larger(at[q], other_half(at[q]));
@@ -1266,11 +1280,11 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__(256, 2) void few
     if (threadIdx.x < 32 * QB) {
         const int q = threadIdx.x >> 5;
         float m = kNothing, all = 0.0f, hit = -INFINITY;
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kFewWaves; ++i) {
             m = fmaxf(m, join[i][q][0][low]);
             hit = larger(hit, join[i][q][2][low]);
         }
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kFewWaves; ++i)
             all += times_power(join[i][q][1][low], join[i][q][0][low] - m);
         float *to = A.stats + (int64_t)blockIdx.x * 3 * A.rows + threadIdx.x;
         to[0] = m;
@@ -1478,8 +1492,8 @@ template <class Y, int KO> int64_t run_narrow(const Call &C)
 
     prepare_kernel<<<prepare_blocks(P.np, P.vp), 256, 0, C.st>>>(P);
     if (Y::scaled && C.grad) {
-        const int most = 4 * C.cus, wb = (int)(C.v / 32 < 1 ? 1 : C.v / 32 > most ? most : C.v / 32), xb = (int)(C.n / 32 < 1 ? 1 : C.n / 32 > most ? most : C.n / 32);
-        columns_kernel<<<wb + xb, 256, 0, C.st>>>(mw, mx, (int)C.k, wb);
+        const int most = C.cus, wb = (int)(C.v / 128 < 1 ? 1 : C.v / 128 > most ? most : C.v / 128), xb = (int)(C.n / 128 < 1 ? 1 : C.n / 128 > most ? most : C.n / 128);
+        columns_kernel<<<wb + xb, 1024, 0, C.st>>>(mw, mx, (int)C.k, wb);
     }
     pack_kernel<Y, KO><<<(unsigned)(v_tiles + n_tiles), 256, 0, C.st>>>(mw, mx, (int)C.k, (int)v_tiles);
 
@@ -1646,7 +1660,7 @@ template <class Y> bool is_few(const Call &C) { return !C.grad && C.n <= 64 && C
 template <class Y, int QB, int CB> void launch_few(const FewArgs &A, unsigned grid, hipStream_t st)
 {
     const int bytes = QB * CB * Y::S * kUnit + 2 * 32 * 16 * CB * (int)sizeof(typename Y::t);   // at most 48 + 32 KB
-    few_kernel<Y, QB, CB><<<grid, 256, bytes, st>>>(A);
+    few_kernel<Y, QB, CB><<<grid, kFewWaves * 64, bytes, st>>>(A);
 }
 template <class Y, int QB> void launch_few_rows(const FewArgs &A, unsigned grid, hipStream_t st)
 {
@@ -1672,8 +1686,8 @@ template <class Y> int64_t run_few(const Call &C)
     A.rows = up(C.n, 32);
     A.v_tiles = (C.v + 31) / 32;
     A.K = (int)C.k;
-    int64_t grid = (A.v_tiles + 7) / 8;            // two tiles a wavefront at least
-    grid = grid > 2 * C.cus ? 2 * C.cus : grid;
+    int64_t grid = (A.v_tiles + kFewWaves - 1) / kFewWaves;   // two wavefronts a SIMD at most: what its registers have room for
+    grid = grid > C.cus ? C.cus : grid;
     Space S = {C.ws, 0};
     A.stats = S.take<float>(grid * 3 * A.rows * 4);
     if (!C.ws)

@@ -5,11 +5,14 @@ numpy stand-in with the same method names so that host logic -- layouts, shardin
 driver loop, the HPF class -- can be exercised on machines without a GPU; it is never
 importable from this package.)
 """
+import contextlib
 import os
 
 import torch
 
 from . import _lib
+
+_NOTHING = contextlib.nullcontext()
 
 
 def _ptr(t):
@@ -103,8 +106,13 @@ class HipOps:
         # guideline 11); 16 rather than 8 evens out the tail: +0.8 % at C3 (6 -- not a multiple -- costs 6 %)
         self.sweep_blocks = max(1, self.cu_count) * int(os.environ.get("HPF_SWEEP_BPC", "16"))
         self.finalize_blocks = max(1, self.cu_count) * int(os.environ.get("HPF_FIN_BPC", "4"))
-        self.adamw_blocks = max(1, self.cu_count) * 8
+        self.adamw_blocks = max(1, self.cu_count) * int(os.environ.get("HPF_ADAMW_BPC", "4"))
         self.refresh_blocks = max(1, self.cu_count) * int(os.environ.get("HPF_REFRESH_BPC", "8"))
+
+    def _on_device(self):
+        """A context in which launches go to this object's device (nothing to do where it is the current one)."""
+        index = self.device.index
+        return _NOTHING if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
 
     def _stream(self):
         return torch.cuda.current_stream(self.device).cuda_stream
@@ -427,7 +435,7 @@ class HipOps:
     def softmax_nll(self, x, ldx, items, ld_items, target, bias, scale, n, v, k, loss, lse):
         """Loss and log-sum-exp of n rows against a catalogue of v items (hpf_hip_softmax_nll); hpfrec_amd.softmax checks
         the arguments."""
-        with torch.cuda.device(self.device):
+        with self._on_device():
             ws = self._softmax_scratch(n, v, k, x.dtype, False)
             _lib.check(self.L.hpf_hip_softmax_nll(_ptr(x), ldx, _ptr(items), ld_items, _ptr(target), _ptr(bias), scale, n, v, k,
                                                   TYPE_CODES[x.dtype], _ptr(loss), _ptr(lse), _ptr(ws), ws.numel(), self.cu_count,
@@ -437,7 +445,7 @@ class HipOps:
                          dbias):
         """softmax_nll with the gradients of sum weight * loss (hpf_hip_softmax_nll_grad); hpfrec_amd.softmax checks the
         arguments."""
-        with torch.cuda.device(self.device):
+        with self._on_device():
             ws = self._softmax_scratch(n, v, k, x.dtype, True)
             _lib.check(self.L.hpf_hip_softmax_nll_grad(_ptr(x), ldx, _ptr(items), ld_items, _ptr(target), _ptr(weight), _ptr(bias),
                                                        scale, n, v, k, TYPE_CODES[x.dtype], _ptr(loss), _ptr(dx), ld_dx, _ptr(ditems),
@@ -450,7 +458,7 @@ class HipOps:
         n = len(tensors)
         desc = (AdamwTensor * max(1, n))(*tensors)
         lr_dev = lr if torch.is_tensor(lr) else None
-        with torch.cuda.device(self.device):
+        with self._on_device():
             _lib.check(self.L.hpf_hip_adamw_step(desc, n, TYPE_CODES[param_type], TYPE_CODES[grad_type], int(state_bits),
                                                  _ptr(step), int(bool(advance)), _ptr(lr_dev), 0.0 if lr_dev is not None else float(lr),
                                                  float(beta1), float(beta2), float(eps), int(seed) & (2 ** 64 - 1),

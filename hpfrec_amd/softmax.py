@@ -15,37 +15,42 @@ from .ops_hip import TYPE_CODES
 
 def _matrix(t, name, ops, dtype=None, shape=None):
     """Row stride of a matrix whose rows are contiguous."""
-    if not torch.is_tensor(t) or t.dim() != 2:
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise ValueError("%s must be a matrix" % name)
     if t.dtype not in TYPE_CODES if dtype is None else t.dtype != dtype:
         raise ValueError("%s must be of %s" % (name, " or ".join(str(d) for d in TYPE_CODES) if dtype is None else dtype))
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), shape))
-    _on(t, name, ops)
     rows, k = t.shape
-    if k > 1 and t.stride(1) != 1:
+    if shape is not None and (rows, k) != shape:
+        raise ValueError("%s has shape %s, expected %s" % (name, (rows, k), shape))
+    _on(t, name, ops)
+    ld, inner = t.stride()
+    if inner != 1 and k > 1:
         raise ValueError("%s must have contiguous rows" % name)
-    if rows > 1 and t.stride(0) < k:
+    if ld >= k:
+        return ld
+    if rows > 1:
         raise ValueError("%s must have rows that do not overlap" % name)
-    return t.stride(0) if rows > 1 else max(k, t.stride(0))
+    return k
 
 
 def _vector(t, name, ops, dtype, n):
-    if not torch.is_tensor(t) or t.dtype != dtype or tuple(t.shape) != (n,) or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != 1 or len(t) != n or not t.is_contiguous():
         raise ValueError("%s must be a contiguous %s vector of %d" % (name, dtype, n))
     _on(t, name, ops)
 
 
 def _on(t, name, ops):
-    if t.device.type != ops.device.type or ops.device.index not in (None, t.device.index):
+    if t.device != ops.device and (ops.device.index is not None or t.device.type != ops.device.type):
         raise ValueError("%s is on %s, expected %s" % (name, t.device, ops.device))
 
 
 def _inputs(ops, x, items, target, bias, scale):
     ldx = _matrix(x, "x", ops)
     n, k = x.shape
-    ldi = _matrix(items, "items", ops, x.dtype, (items.shape[0], k) if torch.is_tensor(items) and items.dim() == 2 else None)
+    ldi = _matrix(items, "items", ops, x.dtype)
     v = items.shape[0]
+    if items.shape[1] != k:
+        raise ValueError("items has shape %s, expected (%d, %d)" % (tuple(items.shape), v, k))
     if v == 0 or k == 0:
         raise ValueError("items is empty")
     if max(n, v) >= 2 ** 30 - 32:
@@ -93,16 +98,24 @@ def softmax_nll_grad(ops, x, items, target, weight=None, bias=None, scale=1.0, d
         _vector(weight, "weight", ops, torch.float32, n)
     if bias is None and dbias is not None:
         raise ValueError("dbias without a bias")
-    dx = torch.empty((n, k), dtype=x.dtype, device=x.device) if dx is None else dx
-    ditems = torch.empty((v, k), dtype=x.dtype, device=x.device) if ditems is None else ditems
-    lddx, lddi = _matrix(dx, "dx", ops, x.dtype, (n, k)), _matrix(ditems, "ditems", ops, x.dtype, (v, k))
-    if bias is not None:
-        dbias = torch.empty(v, dtype=torch.float32, device=x.device) if dbias is None else dbias
+    given = [t for t in (dx, ditems, dbias) if t is not None]
+    if dx is None:
+        dx, lddx = torch.empty((n, k), dtype=x.dtype, device=x.device), k
+    else:
+        lddx = _matrix(dx, "dx", ops, x.dtype, (n, k))
+    if ditems is None:
+        ditems, lddi = torch.empty((v, k), dtype=x.dtype, device=x.device), k
+    else:
+        lddi = _matrix(ditems, "ditems", ops, x.dtype, (v, k))
+    if dbias is not None:
         _vector(dbias, "dbias", ops, torch.float32, v)
-    outs, ins = [[s for s in map(_span, ts) if s] for ts in ((dx, ditems, dbias), (x, items, target, bias, weight))]
-    for i, (a, b) in enumerate(outs):
-        if any(a < d and c < b for c, d in outs[:i] + ins):
-            raise ValueError("dx, ditems or dbias overlaps another tensor of the call")
+    elif bias is not None:
+        dbias = torch.empty(v, dtype=torch.float32, device=x.device)
+    if given:
+        outs, ins = [[s for s in map(_span, ts) if s] for ts in (given, (x, items, target, bias, weight))]
+        for i, (a, b) in enumerate(outs):
+            if any(a < d and c < b for c, d in outs[:i] + ins):
+                raise ValueError("dx, ditems or dbias overlaps another tensor of the call")
     loss = torch.empty(n, dtype=torch.float32, device=x.device)
     ops.softmax_nll_grad(x, ldx, items, ldi, target, weight, bias, float(scale), n, v, k, loss, dx, lddx, ditems, lddi, dbias)
     return loss, dx, ditems, dbias
