@@ -26,9 +26,10 @@ MT_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_mt19937.hip")   # the MT19937 stre
 SVI_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_svi_prep.hip") # index structures of a stochastic batch, on the device
 P2P_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_p2p.hip")      # peer-mapped exchange regions (hipIpc*) + their primitives
 ADAMW_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_adamw.hip")  # the first-order step over many tensors
-SOFTMAX_SRC_PATH = os.path.join(_PKG, "csrc", "hpf_softmax.hip")  # the full-catalogue softmax loss and its gradients
-SOURCES = (SRC_PATH, SHARD_SRC_PATH, MT_SRC_PATH, SVI_SRC_PATH, P2P_SRC_PATH, ADAMW_SRC_PATH, SOFTMAX_SRC_PATH)
-HEADERS = (os.path.join(_PKG, "csrc", "hpf_p2p_dev.h"),)
+# the full-catalogue softmax loss and its gradients: the entries, and the kernels of one type each
+SOFTMAX_SRC_PATHS = tuple(os.path.join(_PKG, "csrc", "hpf_softmax%s.hip" % s) for s in ("", "_f32", "_bf16", "_f16"))
+SOURCES = (SRC_PATH, SHARD_SRC_PATH, MT_SRC_PATH, SVI_SRC_PATH, P2P_SRC_PATH, ADAMW_SRC_PATH) + SOFTMAX_SRC_PATHS
+HEADERS = tuple(os.path.join(_PKG, "csrc", h) for h in ("hpf_p2p_dev.h", "hpf_internal.h", "hpf_softmax_dev.h"))
 INC_PATH = os.path.join(_ROOT, "include")
 
 HPF_HIP_ABI_VERSION = 25

@@ -1,1747 +1,13 @@
-// hpf_softmax.hip -- softmax cross entropy of rows against a whole catalogue, with its gradients, without keeping the logits.
-//
-//   z[n, v] = scale <x[n], w[v]> + bias[v];   lse[n] = log sum_v exp z[n, v];   loss[n] = lse[n] - z[n, t[n]]
-//   G[n, v] = weight[n] (exp(z[n, v] - lse[n]) - [v = t[n]])
-//   dx = scale G w;   dw = scale G^T x;   dbias[v] = sum_n G[n, v]
-//
-// Every product is a matrix instruction (32 x 32 x 16); a row's statistics are kept in base 2 (z log2(e)).
-//
-// PASSES.  A wavefront keeps 32 (or 64) rows of one matrix in registers -- the STATIONARY rows -- and the other matrix streams
-// by in tiles of 32 rows through shared memory, four wavefronts reading each.  A tile's logits come out with the stationary
-// row in the lane and the streamed row in the register, so that what belongs to a stationary row is a lane's own.
-//   rows pass:   x stationary, w streamed: running maximum and sum of a softmax, and the sum of exp(z - max) w over the tiles
-//                -- dx before its normalisation -- in the same pass, rescaled when a maximum grows
-//   items pass:  w stationary, x streamed: G from the finished lse, and its product with x, held relative to the item's largest
-// so the logits are computed twice and nothing of their size is written.  An output register's row (8 (i / 4) + 4 (lane / 32) +
-// i % 4) is not an operand's (8 (lane / 32) + j), but a contraction may take its terms in any order: the second product's
-// other operand is laid out in the order in which the first product's output lies in the registers, and the probabilities
-// never leave the lane that made them.
-//
-// 32-BIT MATRICES are split into two half-precision parts (11 + 11 bits of mantissa and the second's sign: a value is held to
-// 2^-23) and multiplied in three products; the fourth, low times low, is below 2^-22 of |a| |b| and of either sign.  For
-// half's range they are scaled by powers of two: 32 rows share one where rows are multiplied with rows (the largest becomes
-// 2^14 .. 2^15), all rows of a column one where the sum is over rows; what is below 2^-17 of the largest is held to 2^-40 of
-// it.  Probabilities are held times 2^14 relative to a running maximum of their row (or item).  bfloat16 and half matrices
-// take one product; their probabilities are rounded to the same type, everything else stays in 32 bits.
-//
-// A running maximum is rounded up to a whole number: rescaling by a power of two changes no digit.
-//
-// THE TARGET's logit is kept out of the sums and joined at the end: 1 - p(target) is then the sum of the others' shares and not a
-// difference of near equals, and the loss of a row that is sure of its target log1p(others / target).
-#include <hip/hip_runtime.h>
-#include <stdint.h>
-
-#include "hpf_hip.h"
+// hpf_softmax.hip -- the C entries of the full-catalogue softmax loss (kernels and formulas: hpf_softmax_dev.h).
+#include "hpf_softmax_dev.h"
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
-constexpr float kNothing = -0x1p126f;     // a running maximum before anything: logits (base 2) at or below it are masked
-constexpr int kNoTarget = 0x3FFFFFFF;     // block 2^25 of 32 items: beyond every catalogue
-constexpr int kNegative = 0x40000000;     // flag beside a row's target: its weight is negative
-constexpr int kPadTiles = 8;              // packed matrices end on a multiple of so many tiles: staging reads whole groups
+using hpf_softmax::Call;
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+int64_t run(int type, const Call &C) { return type == HPF_F32 ? hpf_softmax::run_f32(C) : type == HPF_BF16 ? hpf_softmax::run_bf16(C) : hpf_softmax::run_f16(C); }
 
-struct Bf {
-    typedef __bf16 e;
-    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
-    static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-};
-struct Hf {
-    typedef _Float16 e;
-    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
-    static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-};
-
-// What a user's matrix is, what it is multiplied in, in how many parts, and the power of two its probabilities are held times;
-// ranged: G is held relative to a running maximum (half's range); scaled: the parts are.
-struct F32 { typedef float t; typedef Hf m; static constexpr int S = 2, shift = 14; static constexpr bool ranged = true, scaled = true; };
-struct B16 { typedef __bf16 t; typedef Bf m; static constexpr int S = 1, shift = 0; static constexpr bool ranged = false, scaled = false; };
-struct H16 { typedef _Float16 t; typedef Hf m; static constexpr int S = 1, shift = 14; static constexpr bool ranged = true, scaled = false; };
-// 32-bit rows over 256 wide: three bfloat16 parts, whose range needs neither scales nor maxima, in six products
-struct W32 { typedef float t; typedef Bf m; static constexpr int S = 3, shift = 0; static constexpr bool ranged = false, scaled = false; };
-
-template <class Y> struct Parts { typename Y::m::v8 p[Y::S]; };   // 8 values of an operand
-
-template <class Y> __device__ __forceinline__ void split(float x, Parts<Y> &to, int j)
-{
-    typedef typename Y::m::e e;
-    to.p[0][j] = (e)x;
-    if constexpr (Y::S > 1) {
-        const float r = x - (float)to.p[0][j];
-        to.p[1][j] = (e)r;
-        if constexpr (Y::S > 2)
-            to.p[2][j] = (e)(r - (float)to.p[1][j]);
-    }
-}
-
-// two neighbouring values (j even), rounded together; what is left of each by one multiply-add that reads the half in place
-template <class Y> __device__ __forceinline__ void split2(float x0, float x1, Parts<Y> &to, int j)
-{
-    if constexpr (Y::S == 3) {
-        split<Y>(x0, to, j);
-        split<Y>(x1, to, j + 1);
-    } else {
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        typedef typename Y::m::e e2 __attribute__((ext_vector_type(2)));
-        const e2 hi = __builtin_convertvector((f2){x0, x1}, e2);
-        to.p[0][j] = hi[0];
-        to.p[0][j + 1] = hi[1];
-        if constexpr (Y::S == 2) {
-            const e2 lo = __builtin_convertvector(((f2){fmaf((float)hi[0], -1.0f, x0), fmaf((float)hi[1], -1.0f, x1)}), e2);
-            to.p[1][j] = lo[0];
-            to.p[1][j + 1] = lo[1];
-        }
-    }
-}
-
-// c += a b, smallest products first
-template <class Y> __device__ __forceinline__ f32x16 product(const Parts<Y> &a, const Parts<Y> &b, f32x16 c)
-{
-    if constexpr (Y::S == 3) {
-        c = Y::m::mfma(a.p[2], b.p[0], c);
-        c = Y::m::mfma(a.p[0], b.p[2], c);
-        c = Y::m::mfma(a.p[1], b.p[1], c);
-    }
-    if constexpr (Y::S > 1) {
-        c = Y::m::mfma(a.p[1], b.p[0], c);
-        c = Y::m::mfma(a.p[0], b.p[1], c);
-    }
-    return Y::m::mfma(a.p[0], b.p[0], c);
-}
-
-// the larger of two, NaN if either is
-__device__ __forceinline__ float larger(float a, float b) { return a != a || a >= b ? a : b; }
-
-// a lane's value in the lower half of the wavefront, and in the upper one: both, in every lane
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ float halves_max(float x)
-{
-    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
-
-// a word that earlier launches wrote, the same for all lanes
-__device__ __forceinline__ int uniform_word(const int32_t *p) { return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p; }
-
-// A UNIT is one operand of a matrix instruction as it lies in memory: 64 lanes x 8 values, 1 KB.
-constexpr int kUnit = 1024;
-
-// the exponent that brings a largest magnitude into [2^14, 2^15) when it is taken away; 0 for nothing but zeros
-__device__ __forceinline__ int half_exponent(float top) { return top > 0.0f ? (int)(__float_as_uint(top) >> 23) - 127 - 14 : 0; }
-__device__ __forceinline__ float finite_size(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }
-
-__device__ __forceinline__ float wave_max(float m)
-{
-    for (int d = 32; d; d >>= 1)
-        m = fmaxf(m, __shfl_xor(m, d));
-    return m;
-}
-
-// ---------------------------------------------------------------------------------------------------------------------
-// Preparation.
-// ---------------------------------------------------------------------------------------------------------------------
-struct PrepArgs {
-    const int64_t *target;
-    const float *bias, *weight;
-    int64_t N, V, np, vp;          // np, vp: padded
-    float *bias2;                  // bias in base 2, -inf beyond the catalogue
-    int32_t *meta;                 // targets as 32-bit numbers, kNoTarget where there is none
-    float *wpow;                   // the smallest power of two above every |weight| (1 if there is none): G is held as a share of it
-    uint32_t *col_top;             // largest magnitudes of the columns (bits): zeros before they are looked for
-    int cols;
-};
-
-// block 0: weights and zeros; the others: an item and a row a thread
-__global__ __launch_bounds__(256) void prepare_kernel(PrepArgs A)
-{
-    if (blockIdx.x == 0) {
-        __shared__ float top[4];
-        for (int c = threadIdx.x; c < A.cols; c += 256)
-            A.col_top[c] = 0;
-        if (!A.wpow)
-            return;
-        float m = 0.0f;
-        if (A.weight) {
-            int64_t n = threadIdx.x;
-            for (; n + 768 < A.N; n += 1024)
-                m = fmaxf(fmaxf(m, fmaxf(fabsf(A.weight[n]), fabsf(A.weight[n + 256]))),
-                          fmaxf(fabsf(A.weight[n + 512]), fabsf(A.weight[n + 768])));
-            for (; n < A.N; n += 256)
-                m = fmaxf(m, fabsf(A.weight[n]));
-        }
-        m = wave_max(m);
-        if ((threadIdx.x & 63) == 0)
-            top[threadIdx.x >> 6] = m;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            int e = 0;
-            if (m > 0.0f && m < INFINITY)
-                frexpf(m, &e);                       // m in [2^(e-1), 2^e)
-            A.wpow[0] = ldexpf(1.0f, e > 100 ? 100 : e < -100 ? -100 : e);
-        }
-        return;
-    }
-    const int64_t i = (int64_t)(blockIdx.x - 1) * 256 + threadIdx.x;
-    if (i < A.vp)
-        A.bias2[i] = i >= A.V ? -INFINITY : A.bias ? A.bias[i] * kLog2e : 0.0f;
-    if (i < A.np) {
-        const int64_t t = i < A.N ? A.target[i] : -1;
-        A.meta[i] = t >= 0 && t < A.V ? (int32_t)t : kNoTarget;
-    }
-}
-
-struct Matrix {
-    const void *p;
-    int64_t ld, rows;
-    const int64_t *target;         // of x with its gradients: rows without a target count as zeros (whatever they hold must not
-    int64_t items;                 // reach a sum)
-    float sign;                    // goes into by_row
-    char *by_row, *by_col;
-    int32_t *exps;                 // scaled: of the tiles, and of the columns (as magnitudes' bits)
-    uint32_t *col_top;
-};
-
-__device__ __forceinline__ bool counts(const Matrix &M, int64_t row) { return row < M.rows && !(M.target && (uint64_t)M.target[row] >= (uint64_t)M.items); }
-
-// Largest magnitudes of the columns of both matrices; a wavefront reads whole rows, 8 at a time.  One workgroup of 16 wavefronts a compute
-// unit: each ends in an atomic maximum a column, and those of one column are served one after the other (about 60 ns each).
-__global__ __launch_bounds__(1024) void columns_kernel(Matrix W, Matrix X, int K, int w_blocks)
-{
-    __shared__ float top[16][256];
-    const bool second = (int)blockIdx.x >= w_blocks;
-    const Matrix &M = second ? X : W;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t first = (second ? blockIdx.x - w_blocks : blockIdx.x) * 16 + wave, step = (second ? gridDim.x - w_blocks : w_blocks) * 16;
-    float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t r = first; r < M.rows; r += 8 * step) {
-        float x[8][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (64 * j < K)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int64_t row = r + i * step < M.rows ? r + i * step : r;      // (a row twice changes no maximum)
-                    x[i][j] = ((const float *)M.p)[row * M.ld + (lane + 64 * j < K ? lane + 64 * j : K - 1)];
-                }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (!M.target || counts(M, r + i * step < M.rows ? r + i * step : r))
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (64 * j < K)
-                        m[j] = fmaxf(m[j], finite_size(x[i][j]));
-    }
-    for (int j = 0; j < 4; ++j)
-        top[wave][lane + 64 * j] = m[j];
-    __syncthreads();
-    const int c = threadIdx.x;
-    if (c < K) {
-        float all = top[0][c];
-        for (int i = 1; i < 16; ++i)
-            all = fmaxf(all, top[i][c]);
-        if (__float_as_uint(all) > __hip_atomic_load(&M.col_top[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-            atomicMax(&M.col_top[c], __float_as_uint(all));
-    }
-}
-
-// packing: rows -> units, one workgroup 32 rows.  `by_row`: tile of 32 rows after tile, in it K / 16 units (lane: row lane % 32,
-// columns 16 cb + 8 (lane / 32) + j).  `by_col`: tile after tile, in it (K / 32) x 2 units (lane: column 32 ko + lane % 32, rows
-// 16 t + 8 (j / 4) + 4 (lane / 32) + j % 4: the order of a product's output registers).  Columns and rows beyond the matrix
-// are zero.  Bound by memory: read once for both forms.
-template <class Y, int KO> __global__ __launch_bounds__(256) void pack_kernel(Matrix W, Matrix X, int K, int w_tiles)
-{
-    constexpr int KP = 32 * KO, CB = 2 * KO;
-    __shared__ float tile[32][KP + 1];
-    __shared__ float tops[4];
-    const bool second = (int)blockIdx.x >= w_tiles;
-    const Matrix &M = second ? X : W;
-    const int64_t rb = second ? blockIdx.x - w_tiles : blockIdx.x;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, low = lane & 31, h = lane >> 5;
-    float top = 0.0f;
-    for (int i = 0; i < 8; ++i) {
-        const int r = wave * 8 + i;
-        const int64_t row = rb * 32 + r;
-        const bool in = counts(M, row);
-#pragma unroll
-        for (int j = 0; j < (KP + 63) / 64; ++j) {
-            const int c = lane + 64 * j;
-            const float x = in && c < K ? (float)((const typename Y::t *)M.p)[row * M.ld + c] : 0.0f;
-            if (c < KP)
-                tile[r][c] = x;
-            top = fmaxf(top, finite_size(x));
-        }
-    }
-    if constexpr (Y::scaled) {
-        top = wave_max(top);
-        if (lane == 0)
-            tops[wave] = top;
-    }
-    __syncthreads();
-    int e = 0;
-    if constexpr (Y::scaled) {
-        e = half_exponent(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-        if (threadIdx.x == 0)
-            M.exps[rb] = e;
-    }
-    for (int cb = wave; cb < CB; cb += 4) {
-        Parts<Y> q;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            split<Y>(ldexpf(M.sign * tile[low][16 * cb + 8 * h + j], -e), q, j);
-        for (int s = 0; s < Y::S; ++s)
-            *(typename Y::m::v8 *)(M.by_row + (((rb * CB + cb) * Y::S + s) * 64 + lane) * 16) = q.p[s];
-    }
-    if (!M.by_col)
-        return;
-    for (int u = wave; u < 2 * KO; u += 4) {
-        const int ko = u >> 1, t = u & 1, c = 32 * ko + low;
-        const int ce = Y::scaled && c < K ? half_exponent(__uint_as_float(M.col_top[c])) : 0;
-        Parts<Y> q;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            split<Y>(ldexpf(tile[16 * t + 8 * (j >> 2) + 4 * h + (j & 3)][c], -ce), q, j);
-        for (int s = 0; s < Y::S; ++s)
-            *(typename Y::m::v8 *)(M.by_col + ((((rb * KO + ko) * 2 + t) * Y::S + s) * 64 + lane) * 16) = q.p[s];
-    }
-}
-
-// the same for rows of any width, without scales: 32 rows x 128 columns a workgroup
-template <class Y> __global__ __launch_bounds__(256) void pack_wide_kernel(Matrix M, int K, int CB, int KO)
-{
-    __shared__ float tile[32][129];
-    const int64_t rb = blockIdx.x;
-    const int c0 = blockIdx.y * 128;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int at = i * 256 + threadIdx.x, r = at >> 7, c = c0 + (at & 127);
-        const int64_t row = rb * 32 + r;
-        tile[r][at & 127] = c < K && counts(M, row) ? (float)((const typename Y::t *)M.p)[row * M.ld + c] : 0.0f;
-    }
-    __syncthreads();
-    const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int u = i * 4 + (threadIdx.x >> 6), cb = blockIdx.y * 8 + u;
-        if (cb < CB) {
-            Parts<Y> q;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                split<Y>(M.sign * tile[low][16 * u + 8 * h + j], q, j);
-            for (int s = 0; s < Y::S; ++s)
-                *(typename Y::m::v8 *)(M.by_row + (((rb * CB + cb) * Y::S + s) * 64 + lane) * 16) = q.p[s];
-        }
-        const int ko = blockIdx.y * 4 + (u >> 1), t = u & 1;
-        if (M.by_col && ko < KO) {
-            Parts<Y> q;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                split<Y>(tile[16 * t + 8 * (j >> 2) + 4 * h + (j & 3)][32 * (u >> 1) + low], q, j);
-            for (int s = 0; s < Y::S; ++s)
-                *(typename Y::m::v8 *)(M.by_col + ((((rb * KO + ko) * 2 + t) * Y::S + s) * 64 + lane) * 16) = q.p[s];
-        }
-    }
-}
-
-// ---------------------------------------------------------------------------------------------------------------------
-// the passes
-// ---------------------------------------------------------------------------------------------------------------------
-enum { kNll, kRows, kItems };
-
-struct PassArgs {
-    const char *still;              // stationary matrix, by_row
-    const char *by_row, *by_col;    // streamed matrix
-    const int32_t *still_exp, *stream_exp;   // scaled: their tiles'
-    const float *reg_bias;          // per streamed row: rows passes: its bias (base 2); items pass: log2(|weight| / wpow) - lse
-    const float *lane_bias;         // items pass: the stationary item's bias
-    const int32_t *meta;            // items pass: per streamed row its target and flag; rows passes: per stationary row
-    const float *target_log;        // items pass: per streamed row, log2 of |G| at its target
-    float *stats;                   // [split][3][still rows]: maximum, sum (rows: without the target), rows: target's logit
-    float *part;                    // [split][still rows][32 KO]
-    int64_t still_tiles, still_rows, stream_tiles;   // tiles of 32; still_rows = 32 still_tiles
-    float c;                        // |scale| log2(e)
-    int splits, bias, base, more;   // pieces of the streamed groups: `more` of base + 1, the rest of base
-    // items pass in one piece: the results themselves
-    void *out;
-    float *dbias;
-    const uint32_t *col_top;
-    const float *wpow;
-    int64_t ld_out, count;
-    int K, quads;                   // quads: rows of `out` allow four values at once
-    float scale;
-};
-
-constexpr int kGridY = 32768;
-
-// every wavefront's staged units are in shared memory (a barrier alone does not wait for them)
-__device__ __forceinline__ void staged_barrier()
-{
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-}
-
-template <class Y, int KO, int MODE> struct Shape {
-    static constexpr int S = Y::S, CB = 2 * KO;
-    static constexpr int row_units = CB * S, col_units = MODE == kNll ? 0 : 2 * KO * S, units = row_units + col_units;   // per tile
-    static constexpr int NW = 4;                                              // wavefronts
-    static constexpr int QB = S * KO <= 2 ? 2 : 1;                            // stationary tiles of a wavefront
-    static constexpr int RT = units <= 4 ? 4 : units <= 12 ? 2 : 1;           // streamed tiles a stage
-    static constexpr int waves = S == 2 && KO > 4 && MODE != kNll ? 1 : 2;    // per SIMD: 512 or 256 registers
-    static constexpr int side = RT * 64 * 4 * (MODE == kItems ? 2 : 1);       // reg_bias (and meta) of a stage: 64 values a tile, 32 of them its own
-    static constexpr int stage = RT * units * kUnit + side;
-};
-
-__device__ __forceinline__ void stage_unit(const char *from, char *to)
-{
-    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) const void *)(from + (threadIdx.x & 63) * 16),
-                                     (__attribute__((address_space(3))) void *)(uintptr_t)to, 16, 0, 0);
-}
-__device__ __forceinline__ void stage_words(const void *from, char *to)   // 64 of 32 bits
-{
-    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) const void *)((const char *)from + (threadIdx.x & 63) * 4),
-                                     (__attribute__((address_space(3))) void *)(uintptr_t)to, 4, 0, 0);
-}
-
-// a sum with its own rounding error carried along
-struct Sum {
-    float s, c;
-    __device__ __forceinline__ void add(float x)
-    {
-        const float y = x - c, t = s + y;
-        c = (t - s) - y;
-        s = t;
-    }
-};
-
-// Order for the scheduler, in a block of `steps` (an even number of) x (READS reads of shared memory, then PRODUCTS matrix instructions
-// that use them): two steps' reads behind the first product of the two steps before.  (Left alone it puts each read right
-// ahead of its product, and a wavefront waits for shared memory half of its time.)
-template <int READS, int PRODUCTS> __device__ __forceinline__ void order_reads(int steps)
-{
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * READS, 0);
-#pragma unroll
-    for (int i = 0; i < steps; i += 2) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        if (i + 2 < steps)
-            __builtin_amdgcn_sched_group_barrier(0x100, 2 * READS, 0);
-        __builtin_amdgcn_sched_group_barrier(0x8, 2 * PRODUCTS - 1, 0);
-    }
-}
-
-__device__ __forceinline__ float sum16(const f32x16 &x)
-{
-    return (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]))) + (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
-}
-
-// One block of base-2 logarithms times 1 / c (lane: stationary row, register: streamed row) becomes its exponentials relative to a
-// running maximum, times 2^shift; `rescale(f)` is called where the maximum grew.  c > 0.
-template <class Y, class F> __device__ __forceinline__ void exponentials(f32x16 &x, float c, float &top, Sum &sum, const F &rescale)
-{
-    float m = x[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i)
-        m = fmaxf(m, x[i]);
-    m = halves_max(m) * c;
-    if (__any(m > top)) {
-        const float grown = m > top ? ceilf(m) : top, f = __builtin_amdgcn_exp2f(top - grown);
-        sum.s *= f;
-        sum.c *= f;
-        top = grown;
-        rescale(f);
-    }
-    const float down = (float)Y::shift - top;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, down));
-}
-
-// the register of a block that holds streamed row r (0 .. 31), for the lanes of half h: i with row_of(i, h) = r
-__device__ __forceinline__ constexpr int row_of(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
-
-// takes the target's logit out of its block
-__device__ __forceinline__ void take_target(f32x16 &x, float c, int tile, int h, int target, float &at)
-{
-    if (__any((target >> 5) == tile))
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (target == tile * 32 + row_of(i, h)) {
-                at = x[i] * c;
-                x[i] = -INFINITY;
-            }
-}
-
-__device__ __forceinline__ void store_stats(float *to, int64_t rows, int h, float top, const Sum &sum, float at)
-{
-    const float both = sum.s + other_half(sum.s), hit = larger(at, other_half(at));
-    if (h == 0) {
-        to[0] = top;
-        to[rows] = both;
-        to[2 * rows] = hit;
-    }
-}
-
-// x 2^e for whole numbers held as floats (very low ones: a maximum of nothing)
-__device__ __forceinline__ float times_power(float x, float e) { return ldexpf(x, (int)fmaxf(e, -1000.0f)); }
-
-template <class Y, int KO, int MODE>
-__global__ __launch_bounds__((Shape<Y, KO, MODE>::NW * 64), (Shape<Y, KO, MODE>::waves)) void pass_kernel(PassArgs A)
-{
-    typedef Shape<Y, KO, MODE> Z;
-    constexpr int S = Z::S, CB = Z::CB, QB = Z::QB, RT = Z::RT, NW = Z::NW;
-    __shared__ __attribute__((aligned(1024))) char lds[2][Z::stage];
-
-    const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int sp = blockIdx.x;      // equal splits stream the same tiles: where there are eight, they meet on one die and its cache
-    const int64_t q0 = (((int64_t)blockIdx.z * kGridY + blockIdx.y) * NW + wave) * QB;
-    if (q0 - wave * QB >= A.still_tiles)
-        return;
-    const int64_t g0 = (int64_t)A.base * sp + (sp < A.more ? sp : A.more), g1 = g0 + A.base + (sp < A.more);
-
-    Parts<Y> still[QB][CB];
-    int target[QB], still_exp[QB];
-    float lane_bias[QB];
-#pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        const bool in = q0 + q < A.still_tiles;
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
-            for (int s = 0; s < S; ++s) {
-                typename Y::m::v8 z = {};
-                still[q][cb].p[s] = in ? *(const typename Y::m::v8 *)(A.still + (((q0 + q) * CB + cb) * S + s) * kUnit + lane * 16) : z;
-            }
-        target[q] = MODE != kItems && in ? A.meta[(q0 + q) * 32 + low] : kNoTarget;
-        lane_bias[q] = MODE == kItems && in && A.bias ? A.lane_bias[(q0 + q) * 32 + low] : 0.0f;
-        still_exp[q] = Y::scaled && in ? uniform_word(A.still_exp + q0 + q) : 0;
-    }
-
-    f32x16 acc[QB][MODE == kNll ? 1 : KO];
-    float top[QB], at[QB];
-    Sum sum[QB];
-#pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        top[q] = MODE == kItems && !Y::ranged ? 0.0f : kNothing;
-        sum[q] = {0.0f, 0.0f};
-        at[q] = -INFINITY;
-        if constexpr (MODE != kNll)
-            for (int ko = 0; ko < KO; ++ko)
-                acc[q][ko] = (f32x16)(0.0f);
-    }
-
-    auto stage = [&](int64_t g, int buf) {
-        const char *from = A.by_row + g * RT * Z::row_units * kUnit;
-#pragma unroll
-        for (int u = 0; u < RT * Z::row_units; u += NW)
-            if (u + wave < RT * Z::row_units)
-                stage_unit(from + (u + wave) * kUnit, &lds[buf][(u + wave) * kUnit]);
-        if constexpr (MODE != kNll) {
-            from = A.by_col + g * RT * Z::col_units * kUnit;
-#pragma unroll
-            for (int u = 0; u < RT * Z::col_units; u += NW)
-                if (u + wave < RT * Z::col_units)
-                    stage_unit(from + (u + wave) * kUnit, &lds[buf][(RT * Z::row_units + u + wave) * kUnit]);
-        }
-        if (wave < RT) {
-            stage_words(A.reg_bias + (g * RT + wave) * 32, &lds[buf][RT * Z::units * kUnit + wave * 256]);
-            if constexpr (MODE == kItems)
-                stage_words(A.meta + (g * RT + wave) * 32, &lds[buf][RT * Z::units * kUnit + (RT + wave) * 256]);
-        }
-    };
-    auto fetch = [&](const char *unit) {
-        Parts<Y> x;
-        for (int s = 0; s < S; ++s)
-            x.p[s] = *(const typename Y::m::v8 *)(unit + s * kUnit + lane * 16);
-        return x;
-    };
-
-    if (g0 < g1)
-        stage(g0, 0);
-    for (int64_t g = g0; g < g1; ++g) {
-        const int buf = (int)(g - g0) & 1;
-        staged_barrier();                         // this group has arrived, and the other buffer has been read
-        if (g + 1 < g1)
-            stage(g + 1, buf ^ 1);
-#pragma unroll 1
-        for (int rt = 0; rt < RT; ++rt) {
-            const int64_t tile = g * RT + rt;
-            if (tile >= A.stream_tiles)
-                break;
-            const char *rows = &lds[buf][rt * Z::row_units * kUnit], *cols = &lds[buf][(RT * Z::row_units + rt * Z::col_units) * kUnit];
-            const char *side = &lds[buf][RT * Z::units * kUnit + rt * 256];
-            const bool biased = MODE == kItems || A.bias || tile == A.stream_tiles - 1;
-            const int stream_exp = Y::scaled ? uniform_word(A.stream_exp + tile) : 0;
-
-            f32x16 z[QB];
-#pragma unroll
-            for (int q = 0; q < QB; ++q)
-                z[q] = (f32x16)(0.0f);
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
-                const Parts<Y> a = fetch(rows + cb * S * kUnit);
-#pragma unroll
-                for (int q = 0; q < QB; ++q)
-                    z[q] = product<Y>(a, still[q][cb], z[q]);
-            }
-            order_reads<S, QB * (2 * S - 1)>(CB);
-
-            Parts<Y> p[QB][2];
-#pragma unroll
-            for (int q = 0; q < QB; ++q) {
-                f32x16 &x = z[q];
-                float c = Y::scaled ? ldexpf(A.c, stream_exp + still_exp[q]) : A.c;
-                if (biased || c == 0.0f) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 b = *(const f32x4 *)(side + (8 * i + 4 * h) * 4);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            x[4 * i + j] = fmaf(x[4 * i + j], c, b[j]);
-                    }
-                    c = 1.0f;
-                }
-                const auto rescale = [&](float f) {
-                    if constexpr (MODE != kNll)
-#pragma unroll
-                        for (int ko = 0; ko < KO; ++ko)
-                            acc[q][ko] *= f;
-                };
-                if constexpr (MODE == kItems) {
-                    if (A.bias)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            x[i] += lane_bias[q];
-                    const int meta = ((const int32_t *)(side + RT * 256))[low];
-                    unsigned flip = 0;             // registers of negative G: negative weights, and targets of positive ones
-                    const bool hit = __any(((meta & ~kNegative) >> 5) == (int)(q0 + q)), negative = __any(meta & kNegative);
-                    if (hit || negative) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int r = row_of(i, h), of = __shfl(meta, r);
-                            const bool mine = (of & ~kNegative) == (int)(q0 + q) * 32 + low;
-                            if (mine)
-                                x[i] = A.target_log[tile * 32 + r];
-                            flip |= (unsigned)(mine != ((of & kNegative) != 0)) << i;
-                        }
-                    }
-                    if constexpr (Y::ranged) {
-                        exponentials<Y>(x, c, top[q], sum[q], rescale);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            x[i] = __builtin_amdgcn_exp2f(x[i]);
-                    }
-                    if (hit || negative)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            x[i] = flip >> i & 1 ? -x[i] : x[i];
-                    if (A.bias)
-                        sum[q].add(sum16(x));
-                } else {
-                    take_target(x, c, (int)tile, h, target[q], at[q]);
-                    exponentials<Y>(x, c, top[q], sum[q], rescale);
-                    sum[q].add(sum16(x));
-                }
-                if constexpr (MODE != kNll)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2)
-                        split2<Y>(x[i], x[i + 1], p[q][i >> 3], i & 7);
-            }
-
-            if constexpr (MODE != kNll) {
-#pragma unroll
-                for (int u = 0; u < 2 * KO; ++u) {
-                    const Parts<Y> a = fetch(cols + u * S * kUnit);
-#pragma unroll
-                    for (int q = 0; q < QB; ++q)
-                        acc[q][u >> 1] = product<Y>(a, p[q][u & 1], acc[q][u >> 1]);
-                }
-                order_reads<S, QB * (2 * S - 1)>(2 * KO);
-            }
-        }
-    }
-
-#pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        if (q0 + q >= A.still_tiles)
-            break;
-        const int64_t row = (q0 + q) * 32 + low;
-        if (MODE == kItems && A.out) {             // the whole sum: the gradients themselves
-            const float both = sum[q].s + other_half(sum[q].s), wpow = *A.wpow, e = top[q] - (float)Y::shift;
-            if (row < A.count) {
-                if (A.dbias && h == 0)
-                    A.dbias[row] = times_power(both * wpow, e);
-                typedef typename Y::t T;
-                T *to = (T *)A.out + row * A.ld_out;
-                if constexpr (MODE != kNll)
-#pragma unroll
-                    for (int ko = 0; ko < KO; ++ko)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int k = 32 * ko + 8 * i + 4 * h;
-                            struct alignas(4 * sizeof(T)) Quad { T v[4]; } o;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int ce = Y::scaled && k + j < A.K ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
-                                o.v[j] = (T)times_power(acc[q][ko][4 * i + j] * (A.scale * wpow), e + (float)ce);
-                            }
-                            if (A.quads && k + 4 <= A.K)
-                                *(Quad *)(to + k) = o;
-                            else
-                                for (int j = 0; j < 4; ++j)
-                                    if (k + j < A.K)
-                                        to[k + j] = o.v[j];
-                        }
-            }
-            continue;
-        }
-        store_stats(A.stats + (int64_t)sp * 3 * A.still_rows + row, A.still_rows, h, top[q], sum[q], at[q]);
-        if constexpr (MODE != kNll) {
-            float *to = A.part + (sp * A.still_rows + row) * (32 * KO) + 4 * h;
-#pragma unroll
-            for (int ko = 0; ko < KO; ++ko)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f32x4 o = {acc[q][ko][4 * i], acc[q][ko][4 * i + 1], acc[q][ko][4 * i + 2], acc[q][ko][4 * i + 3]};
-                    *(f32x4 *)(to + 32 * ko + 8 * i) = o;
-                }
-        }
-    }
-}
-
-// ---------------------------------------------------------------------------------------------------------------------
-// Rows too wide for a wavefront's registers (k > 256): plain tiled products of packed matrices, the catalogue in chunks.  The
-// statistics come from a first run over all logits; then, chunk by chunk, G is written in both operand layouts (16-bit parts,
-// a chunk at a time: at most kChunkBytes) and multiplied with the items (dx, summed over the chunks) and with x (dw).
-// Bound by the matrix instructions: 8 N V K operations, 128 x 128 outputs a workgroup, 64 x 64 a wavefront.
-// ---------------------------------------------------------------------------------------------------------------------
-constexpr int64_t kChunkBytes = 192ll << 20;
-
-template <class Y, int KC_> struct Wide {
-    static constexpr int S = Y::S, KC = KC_;                // units of the contraction a stage
-    static constexpr int stage = 8 * KC * S * kUnit;        // 4 tiles of each matrix
-};
-template <class Y> struct Logits : Wide<Y, Y::S == 1 ? 4 : 2> {};
-
-// For each group: the 128 x 128 product of 4 + 4 tiles over `steps` stages, handed to `done(group, acc)`.  a(group, step, tile) and
-// b(group, step, tile) are a tile's KC S consecutive units.
-template <class Y, class Z, class A, class B, class D>
-__device__ __forceinline__ void wide_core(char *lds, int64_t groups, int steps, const A &a, const B &b, const D &done)
-{
-    constexpr int S = Z::S, KC = Z::KC, per = KC * S;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
-    auto stage = [&](int64_t g, int step, int buf) {
-        const char *pa = a(g, step, wave), *pb = b(g, step, wave);       // wavefront w brings tile w of each matrix
-#pragma unroll
-        for (int u = 0; u < per; ++u) {
-            stage_unit(pa + u * kUnit, lds + buf * Z::stage + (wave * per + u) * kUnit);
-            stage_unit(pb + u * kUnit, lds + buf * Z::stage + ((4 + wave) * per + u) * kUnit);
-        }
-    };
-    f32x16 acc[2][2];
-    int buf = 0;
-    if (groups > 0 && steps > 0)
-        stage(0, 0, 0);
-    for (int64_t g = 0; g < groups; ++g) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            for (int j = 0; j < 2; ++j)
-                acc[i][j] = (f32x16)(0.0f);
-        for (int step = 0; step < steps; ++step, buf ^= 1) {
-            staged_barrier();                      // this stage has arrived, the other has been read
-            if (step + 1 < steps)
-                stage(g, step + 1, buf ^ 1);
-            else if (g + 1 < groups)   // (groups of one length: steps > 0 here)
-                stage(g + 1, 0, buf ^ 1);
-            const char *at = lds + buf * Z::stage + lane * 16;
-#pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                Parts<Y> x[2], y[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    for (int s = 0; s < S; ++s) {
-                        x[i].p[s] = *(const typename Y::m::v8 *)(at + ((2 * wa + i) * per + c * S + s) * kUnit);
-                        y[i].p[s] = *(const typename Y::m::v8 *)(at + ((4 + 2 * wb + i) * per + c * S + s) * kUnit);
-                    }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        acc[i][j] = product<Y>(x[i], y[j], acc[i][j]);
-            }
-        }
-        done(g, acc);
-    }
-}
-
-struct WideArgs {
-    const char *w, *x;              // by_row units
-    const float *bias, *reg_bias, *target_log;
-    const int32_t *meta;
-    float *stats, *part_sum;
-    char *g_rows, *g_items;         // G of a chunk: rows n / contraction v, and rows v / contraction n
-    int64_t n_tiles, v_tiles, rows, v0, v_count;   // tiles; v0, v_count: the chunk
-    float c;
-    int CB, splits, has_bias;
-};
-
-// logits in base 2 of one 32 x 32 block: lane: row n, register: item
-__device__ __forceinline__ void wide_bias(f32x16 &x, const WideArgs &A, int64_t tile, int h)
-{
-    if (A.has_bias || tile == A.v_tiles - 1) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x4 b = *(const f32x4 *)(A.bias + tile * 32 + 8 * i + 4 * h);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                x[4 * i + j] = fmaf(x[4 * i + j], A.c, b[j]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            x[i] *= A.c;
-    }
-}
-
-template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(WideArgs A)
-{
-    typedef Logits<Y> Z;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * Z::stage];
-    const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
-    const int sp = blockIdx.x % A.splits;
-    const int64_t n0 = (int64_t)(blockIdx.x / A.splits) * 4;
-    const int64_t all = (A.v_tiles + 3) / 4, g0 = all * sp / A.splits, g1 = all * (sp + 1) / A.splits;
-    int target[2];
-    float top[2], at[2];
-    Sum sum[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int64_t tile = n0 + 2 * wb + j;
-        target[j] = tile < A.n_tiles ? A.meta[tile * 32 + low] : kNoTarget;
-        top[j] = kNothing;
-        sum[j] = {0.0f, 0.0f};
-        at[j] = -INFINITY;
-    }
-    wide_core<Y, Z>(
-        lds, g1 - g0, A.CB / Z::KC,
-        [&](int64_t g, int step, int tile) { return A.w + (((g0 + g) * 4 + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
-        [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
-        [&](int64_t g, f32x16 (&acc)[2][2]) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t tile = (g0 + g) * 4 + 2 * wa + i;
-                if (tile >= A.v_tiles)
-                    break;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    f32x16 &x = acc[i][j];
-                    wide_bias(x, A, tile, h);
-                    take_target(x, 1.0f, (int)tile, h, target[j], at[j]);
-                    exponentials<Y>(x, 1.0f, top[j], sum[j], [](float) {});
-                    sum[j].add(sum16(x));
-                }
-            }
-        });
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int64_t tile = n0 + 2 * wb + j;
-        if (tile < A.n_tiles)
-            store_stats(A.stats + (int64_t)(2 * sp + wa) * 3 * A.rows + tile * 32 + low, A.rows, h, top[j], sum[j], at[j]);
-    }
-}
-
-// G of 4 tiles of rows against 4 tiles of items of the chunk, in both layouts, and the sums over its rows
-template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideArgs A)
-{
-    typedef Logits<Y> Z;
-    typedef typename Y::m::e e;
-    constexpr int S = Y::S;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * Z::stage];
-    __shared__ __attribute__((aligned(16))) e turn_all[4][32][36];      // a block a wavefront, to exchange its lanes and registers
-    const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
-    e(*turn)[36] = turn_all[wave];
-    const int64_t ngroups = (A.n_tiles + 3) / 4, n0 = blockIdx.x % ngroups * 4, vg = blockIdx.x / ngroups * 4;   // vg: within the chunk
-    int meta[2];
-    float down[2], tg[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int64_t tile = n0 + 2 * wb + j;
-        const bool in = tile < A.n_tiles;
-        meta[j] = in ? A.meta[tile * 32 + low] : kNoTarget;
-        down[j] = in ? A.reg_bias[tile * 32 + low] : -INFINITY;
-        tg[j] = in ? A.target_log[tile * 32 + low] : 0.0f;
-    }
-    wide_core<Y, Z>(
-        lds, 1, A.CB / Z::KC,
-        [&](int64_t, int step, int tile) { return A.w + ((A.v0 + vg + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
-        [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
-        [&](int64_t, f32x16 (&acc)[2][2]) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t vt = vg + 2 * wa + i, tile = A.v0 + vt;
-                if (vt >= A.v_count)
-                    break;
-                f32x16 total = (f32x16)(0.0f);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int64_t nt = n0 + 2 * wb + j;
-                    if (nt >= A.n_tiles)
-                        break;
-                    f32x16 &x = acc[i][j];
-                    wide_bias(x, A, tile, h);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        x[r] += down[j];
-                    const bool hit = __any(((meta[j] & ~kNegative) >> 5) == (int)tile);
-                    unsigned flip = meta[j] & kNegative ? 0xFFFFu : 0u;
-                    if (hit)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if ((meta[j] & ~kNegative) == (int)tile * 32 + row_of(r, h)) {
-                                x[r] = tg[j];
-                                flip ^= 1u << r;
-                            }
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        x[r] = __builtin_amdgcn_exp2f(x[r] + (float)Y::shift);
-                        x[r] = flip >> r & 1 ? -x[r] : x[r];
-                    }
-                    total += x;
-                    Parts<Y> p[2];
-#pragma unroll
-                    for (int r = 0; r < 16; r += 2)
-                        split2<Y>(x[r], x[r + 1], p[r >> 3], r & 7);
-                    for (int s = 0; s < S; ++s) {
-#pragma unroll
-                        for (int t = 0; t < 2; ++t)
-                            *(typename Y::m::v8 *)(A.g_rows + (((nt * A.v_count + vt) * 2 + t) * S + s) * kUnit + lane * 16) = p[t].p[s];
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            turn[low][row_of(r, h)] = p[r >> 3].p[s][r & 7];
-                        // (one wavefront's own block: its accesses to shared memory are served in order)
-                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            typename Y::m::v8 q;
-#pragma unroll
-                            for (int r = 0; r < 8; ++r)
-                                q[r] = turn[16 * t + row_of(r, h)][low];
-                            *(typename Y::m::v8 *)(A.g_items + (((vt * A.n_tiles + nt) * 2 + t) * S + s) * kUnit + lane * 16) = q;
-                        }
-                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    }
-                }
-                if (A.has_bias) {   // over the lanes of each half: [64 rows][chunk's items]
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float v = total[r];
-                        for (int d = 16; d; d >>= 1)
-                            v += __shfl_xor(v, d);
-                        if (low == 0)
-                            A.part_sum[((n0 / 2 + wb) * A.v_count + vt) * 32 + row_of(r, h)] = v;
-                    }
-                }
-            }
-        });
-}
-
-// c[m][k] = sum over the contraction's tiles of a (by_row units, U of them a tile) times b (by_col units)
-struct ProductArgs {
-    const char *a, *b;
-    int64_t a_tiles, a_units, tiles;      // output tiles, units of one, contraction tiles (32 each)
-    int KO, splits;
-    float *part;                          // [split][32 a_tiles][32 KO] sums; `more`: added to what is there
-    int more;
-};
-
-template <class Y> __global__ __launch_bounds__(256, 2) void wide_product_kernel(ProductArgs A)
-{
-    typedef Wide<Y, 2> Z;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * Z::stage];
-    const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
-    const int kgroups = (A.KO + 3) / 4;
-    int64_t id = blockIdx.x;
-    const int kg = (int)(id % kgroups) * 4;
-    id /= kgroups;
-    const int sp = (int)(id % A.splits);
-    const int64_t m0 = id / A.splits * 4;
-    const int64_t s0 = A.tiles * sp / A.splits, s1 = A.tiles * (sp + 1) / A.splits;   // a contraction tile a stage
-    wide_core<Y, Z>(
-        lds, 1, (int)(s1 - s0),
-        [&](int64_t, int step, int tile) { return A.a + ((m0 + tile) * A.a_units + (s0 + step) * Z::KC) * Z::S * kUnit; },
-        [&](int64_t, int step, int tile) { return A.b + ((s0 + step) * A.KO + (kg + tile < A.KO ? kg + tile : A.KO - 1)) * Z::KC * Z::S * kUnit; },
-        [&](int64_t, f32x16 (&acc)[2][2]) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int64_t mt = m0 + 2 * wa + i;
-                    const int ko = kg + 2 * wb + j;
-                    if (mt >= A.a_tiles || ko >= A.KO)
-                        continue;
-                    float *to = A.part + ((sp * A.a_tiles + mt) * 32) * (int64_t)(32 * A.KO) + 32 * ko + low;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float *o = to + (row_of(r, h)) * (int64_t)(32 * A.KO);
-                        *o = A.more ? *o + acc[i][j][r] : acc[i][j][r];
-                    }
-                }
-        });
-}
-
-// ---------------------------------------------------------------------------------------------------------------------
-// Joins a row's splits: loss and lse, what the items' side needs of the row, and dx (a wavefront a row).
-// ---------------------------------------------------------------------------------------------------------------------
-struct FinishArgs {
-    const float *stats, *part;
-    const int64_t *target;
-    const float *weight, *wpow;
-    const void *w;                 // items, for the target's own row
-    const uint32_t *col_top;
-    float *loss, *lse, *reg_bias, *target_log;
-    int32_t *meta;
-    void *dx;
-    int64_t N, V, rows, ldw, lddx;
-    int K, KP, splits;
-    float scale;
-};
-
-template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows_kernel(FinishArgs A)
-{
-    const int lane = threadIdx.x & 63;
-    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= A.rows)
-        return;
-    if (n >= A.N) {                // rows that only fill the last tile: no share of any sum
-        if (GRAD && lane == 0) {
-            A.reg_bias[n] = A.target_log[n] = -INFINITY;
-            A.meta[n] = kNoTarget;
-        }
-        return;
-    }
-    // splits over the lanes: maxima first, then sums relative to them
-    float top = kNothing, at = -INFINITY, others = 0.0f;
-#pragma unroll 4
-    for (int s = lane; s < A.splits; s += 64) {
-        top = fmaxf(top, A.stats[(3 * s + 0) * A.rows + n]);
-        at = larger(at, A.stats[(3 * s + 2) * A.rows + n]);
-    }
-    for (int d = 32; d; d >>= 1) {
-        top = fmaxf(top, __shfl_xor(top, d));
-        at = larger(at, __shfl_xor(at, d));
-    }
-#pragma unroll 4
-    for (int s = lane; s < A.splits; s += 64)
-        others += times_power(A.stats[(3 * s + 1) * A.rows + n], A.stats[3 * s * A.rows + n] - top);
-    for (int d = 32; d; d >>= 1)
-        others += __shfl_xor(others, d);
-    others = ldexpf(others, -Y::shift);
-
-    // `top` is that of the others; the target's own logit may be far above it
-    const float peak = fmaxf(top, ceilf(at));
-    const float rest = times_power(others, top - peak), own = __builtin_amdgcn_exp2f(at - peak), all = rest + own;
-    const float lse2 = all > 0.0f || all != all ? peak + log2f(all) : -INFINITY;
-    const int64_t t = A.target[n];
-    float loss = 0.0f;
-    bool alive = t >= 0;
-    if (t >= A.V) {                // no such item: said in the loss, and kept out of the gradients
-        loss = __builtin_nanf("");
-        alive = false;
-    } else if (t >= 0) {
-        if (!(at > kNothing) && at == at && all == all) {   // a masked target
-            loss = INFINITY;
-            alive = false;
-        } else if (own > 0.0f && rest < 0x1p20f * own) {
-            loss = log1pf(rest / own);
-        } else {
-            loss = (lse2 - at) * kLn2;
-        }
-    }
-    if (lane == 0) {
-        A.loss[n] = loss;
-        if (A.lse)
-            A.lse[n] = lse2 * kLn2;
-    }
-    if constexpr (GRAD) {
-        const float weight = alive ? (A.weight ? A.weight[n] : 1.0f) : 0.0f, share = fabsf(weight) / *A.wpow;
-        if (lane == 0) {
-            A.reg_bias[n] = alive ? log2f(share) - lse2 : -INFINITY;
-            A.target_log[n] = alive ? log2f(share * (rest / all)) : -INFINITY;
-            A.meta[n] = alive ? (int32_t)t | (weight < 0.0f ? kNegative : 0) : kNoTarget;
-        }
-        if (!A.dx)
-            return;
-        // dx: four columns a lane, the splits over as many lanes as that leaves (KP / 4 = 8 KO lanes for a split, a power of two above)
-        typedef typename Y::t T;
-        T *dx = (T *)A.dx + n * A.lddx;
-        const T *w = (const T *)A.w + (alive ? t : 0) * A.ldw;
-        const int span = A.KP <= 32 ? 8 : A.KP <= 64 ? 16 : A.KP <= 128 ? 32 : 64, k = 4 * (lane & (span - 1)), step = 64 / span;
-        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (alive && k < A.KP)
-#pragma unroll 4
-            for (int s = lane / span; s < A.splits; s += step) {
-                const float down = A.stats[3 * s * A.rows + n] - top;
-                const f32x4 p = *(const f32x4 *)(A.part + (s * A.rows + n) * A.KP + k);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    sum[j] += times_power(p[j], down);
-            }
-        for (int d = 32; d >= span; d >>= 1)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                sum[j] += __shfl_xor(sum[j], d);
-        if (lane < span)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (k + j < A.K) {
-                    const int ce = Y::scaled ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
-                    const float v = times_power(sum[j], top - peak - (float)Y::shift + (float)ce);
-                    dx[k + j] = (T)(alive ? A.scale * weight * (v / all - rest / all * (float)w[k + j]) : 0.0f);
-                }
-    }
-}
-
-// ---------------------------------------------------------------------------------------------------------------------
-// A few rows (up to 64) without gradients: what serving asks for.  Bound by reading the items once, so nothing is packed: a
-// wavefront takes a tile of 32 items straight from the table, two operands' halves of a row a lane, and splits them as it
-// goes; the rows lie in shared memory as operands.  (Three bfloat16 parts for 32-bit matrices: they need no scale, and the
-// matrix instructions have time to spare.)
-// ---------------------------------------------------------------------------------------------------------------------
-struct FewArgs {
-    const void *x, *w;
-    const int64_t *target;
-    const float *bias;
-    float *stats;                  // [workgroup][3][rows]
-    int64_t N, V, ldx, ldw, rows, v_tiles;
-    int K;
-    float c, sign;
-};
-
-constexpr int kFewWaves = 8;
-
-// 8 values as words, from any address that suits their type
-template <class T> struct Raw { uint32_t v[2 * sizeof(T)]; };
-template <class T> __device__ __forceinline__ Raw<T> load8(const T *p)
-{
-    Raw<T> r;
-    __builtin_memcpy(&r, p, sizeof(r));
-    return r;
-}
-template <class T> __device__ __forceinline__ void zeros_from(Raw<T> &r, int left)   // `left` of the 8 are values (fewer than none: none)
-{
-#pragma unroll
-    for (int j = 0; j < (int)(2 * sizeof(T)); ++j) {
-        if (sizeof(T) == 4)
-            r.v[j] = j < left ? r.v[j] : 0u;
-        else
-            r.v[j] &= 2 * j + 1 < left ? 0xFFFFFFFFu : 2 * j < left ? 0xFFFFu : 0u;
-    }
-}
-template <class Y> __device__ __forceinline__ Parts<Y> parts_of(const Raw<typename Y::t> &r)
-{
-    Parts<Y> q;
-    if constexpr (Y::S == 1) {     // as they are
-        __builtin_memcpy(&q, &r, sizeof(q));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            split<Y>(__uint_as_float(r.v[j]), q, j);
-    }
-    return q;
-}
-
-// QB: tiles of 32 rows; CB: operands of a row, K / 16 or more
-template <class Y, int QB, int CB> __global__ __launch_bounds__(kFewWaves * 64, 2) void few_kernel(FewArgs A)
-{
-    constexpr int S = Y::S;
-    typedef typename Y::t T;
-    extern __shared__ __attribute__((aligned(1024))) char lds[];
-    __shared__ float join[kFewWaves][QB][3][32];
-    const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t step = (int64_t)gridDim.x * kFewWaves, fast = A.V >= 64 ? (A.V - 32) / 32 : 0;
-    Raw<T> next[CB];
-    // A tile's rows are read in whole operands, beyond their own end, where 32 rows or more follow (K > 8 CB or CB is 2: no further than
-    // that); the last one or two tiles go through shared memory, which holds zeros there.
-    auto load = [&](int64_t tile) {
-        const int64_t v = tile * 32 + low;
-        if (tile < fast) {
-            const T *row = (const T *)A.w + v * A.ldw + 8 * h;
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
-                next[cb] = load8(row + 16 * cb);
-        } else {
-            T *const copy = (T *)(lds + QB * CB * S * kUnit) + (tile - fast) * 32 * 16 * CB;
-            for (int i = lane; i < 32 * 16 * CB; i += 64) {
-                const int r = i / (16 * CB), k = i % (16 * CB);
-                copy[i] = tile * 32 + r < A.V && k < A.K ? ((const T *)A.w)[(tile * 32 + r) * A.ldw + k] : (T)0.0f;
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
-                next[cb] = load8(copy + low * 16 * CB + 16 * cb + 8 * h);
-        }
-    };
-    int64_t tile = (int64_t)blockIdx.x * kFewWaves + wave;
-    if (tile < A.v_tiles)
-        load(tile);
-    for (int u = wave; u < QB * CB; u += kFewWaves) {
-        const int q = u / CB, cb = u % CB;
-        const int64_t n = q * 32 + low;
-        Parts<Y> p;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int k = 16 * cb + 8 * h + j;
-            split<Y>(n < A.N && k < A.K ? A.sign * (float)((const T *)A.x)[n * A.ldx + k] : 0.0f, p, j);
-        }
-        for (int s = 0; s < S; ++s)
-            *(typename Y::m::v8 *)(lds + (u * S + s) * kUnit + lane * 16) = p.p[s];
-    }
-    int target[QB];
-    float top[QB], at[QB];
-    Sum sum[QB];
-#pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        const int64_t n = q * 32 + low, t = n < A.N ? A.target[n] : -1;
-        target[q] = t >= 0 && t < A.V ? (int)t : kNoTarget;
-        top[q] = kNothing;
-        at[q] = -INFINITY;
-        sum[q] = {0.0f, 0.0f};
-    }
-    __syncthreads();
-    for (; tile < A.v_tiles; tile += step) {
-        Raw<T> cur[CB];
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
-            cur[cb] = next[cb];
-        f32x4 b[4];
-        const bool whole = tile < fast;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            b[i] = (f32x4)(0.0f);
-            if (whole && A.bias) {
-                __builtin_memcpy(&b[i], A.bias + tile * 32 + row_of(4 * i, h), 16);
-                b[i] *= kLog2e;
-            } else if (!whole) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int64_t v = tile * 32 + row_of(4 * i + j, h);
-                    b[i][j] = v >= A.V ? -INFINITY : A.bias ? A.bias[v] * kLog2e : 0.0f;
-                }
-            }
-        }
-        if (tile + step < A.v_tiles)
-            load(tile + step);
-        f32x16 z[QB];
-#pragma unroll
-        for (int q = 0; q < QB; ++q)
-            z[q] = (f32x16)(0.0f);
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
-            if (16 * cb + 16 > A.K)
-                zeros_from(cur[cb], A.K - 16 * cb - 8 * h);
-            const Parts<Y> a = parts_of<Y>(cur[cb]);
-#pragma unroll
-            for (int q = 0; q < QB; ++q) {
-                Parts<Y> y;
-                for (int s = 0; s < S; ++s)
-                    y.p[s] = *(const typename Y::m::v8 *)(lds + ((q * CB + cb) * S + s) * kUnit + lane * 16);
-                z[q] = product<Y>(a, y, z[q]);
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < QB; ++q) {
-            f32x16 &x = z[q];
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                x[i] = fmaf(x[i], A.c, b[i >> 2][i & 3]);
-            take_target(x, 1.0f, (int)tile, h, target[q], at[q]);
-            exponentials<Y>(x, 1.0f, top[q], sum[q], [](float) {});
-            sum[q].add(sum16(x));
-        }
-    }
-    // the wavefronts' pieces become the workgroup's
-#pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        const float both = sum[q].s + other_half(sum[q].s), hit = larger(at[q], other_half(at[q]));
-        if (h == 0) {
-            join[wave][q][0][low] = top[q];
-            join[wave][q][1][low] = both;
-            join[wave][q][2][low] = hit;
-        }
-    }
-    __syncthreads();
-    if (threadIdx.x < 32 * QB) {
-        const int q = threadIdx.x >> 5;
-        float m = kNothing, all = 0.0f, hit = -INFINITY;
-        for (int i = 0; i < kFewWaves; ++i) {
-            m = fmaxf(m, join[i][q][0][low]);
-            hit = larger(hit, join[i][q][2][low]);
-        }
-        for (int i = 0; i < kFewWaves; ++i)
-            all += times_power(join[i][q][1][low], join[i][q][0][low] - m);
-        float *to = A.stats + (int64_t)blockIdx.x * 3 * A.rows + threadIdx.x;
-        to[0] = m;
-        to[A.rows] = all;
-        to[2 * A.rows] = hit;
-    }
-}
-
-// joins the splits of a product with G: out = scale wpow sum, dbias = wpow sum (four columns a thread)
-struct JoinArgs {
-    const float *part, *tops, *sums;       // tops (ranged passes): [split][3][rows] with the sums behind, else NULL
-    const float *wpow;
-    const uint32_t *col_top;
-    int64_t count, rows, ld;
-    int K, KP, splits, sum_splits;
-    float scale;
-    void *out;
-    float *dbias;
-};
-
-template <class Y> __global__ __launch_bounds__(256) void join_kernel(JoinArgs A)
-{
-    const int quads = A.KP / 4;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, v = id / quads;
-    const int k = (int)(id - v * quads) * 4;
-    if (v >= A.count)
-        return;
-    float top = A.tops ? kNothing : 0.0f;
-    if (A.tops)
-        for (int s = 0; s < A.splits; ++s)
-            top = fmaxf(top, A.tops[3 * s * A.rows + v]);
-    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int s = 0; s < A.splits; ++s) {
-        const f32x4 p = *(const f32x4 *)(A.part + (s * A.rows + v) * A.KP + k);
-        const float down = A.tops ? A.tops[3 * s * A.rows + v] - top : 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            sum[j] += times_power(p[j], down);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (k + j < A.K) {
-            const int ce = Y::scaled ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
-            ((typename Y::t *)A.out)[v * A.ld + k + j] = (typename Y::t)times_power(sum[j] * (A.scale * *A.wpow), top - (float)Y::shift + (float)ce);
-        }
-    if (A.dbias && k == 0) {
-        float all = 0.0f;
-        if (A.tops)
-            for (int s = 0; s < A.splits; ++s)
-                all += times_power(A.tops[(3 * s + 1) * A.rows + v], A.tops[3 * s * A.rows + v] - top);
-        else
-            for (int s = 0; s < A.sum_splits; ++s)
-                all += A.sums[s * A.rows + v];
-        A.dbias[v] = times_power(all * *A.wpow, top - (float)Y::shift);
-    }
-}
-
-template <class T> __global__ void zero_rows_kernel(T *p, int64_t rows, int K, int64_t ld)
-{
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < rows * K; i += (int64_t)gridDim.x * blockDim.x)
-        p[i / K * ld + i % K] = (T)0.0f;
-}
-
-// ---------------------------------------------------------------------------------------------------------------------
-// host side
-// ---------------------------------------------------------------------------------------------------------------------
-int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
-constexpr int kMostSplits = 256;      // a row's pieces are joined by one wavefront
-int64_t tiles_padded(int64_t tiles) { return up(tiles, kPadTiles); }
-
-// How many pieces the streamed side is cut into: enough workgroups for four on each compute unit with 8 tiles or more each, in eights (one
-// a die) once there are that many; where that leaves compute units idle, down to 2 tiles each.
-int pick_splits(int64_t workgroups, int64_t stream_tiles, int cus)
-{
-    int64_t s = (4 * cus + workgroups - 1) / workgroups;
-    if (s > stream_tiles / 8)
-        s = stream_tiles / 8;
-    if (s * workgroups < cus) {
-        s = (cus + workgroups - 1) / workgroups;
-        if (s > stream_tiles / 2)
-            s = stream_tiles / 2;
-    }
-    if (s > 8)
-        s = s / 8 * 8;
-    return s < 1 ? 1 : s > kMostSplits ? kMostSplits : (int)s;
-}
-
-struct Call {
-    const void *x, *w;
-    const int64_t *target;
-    const float *weight, *bias;
-    float *loss, *lse, *dbias;
-    void *dx, *dw;
-    int64_t n, v, k, ldx, ldw, lddx, lddw;
-    float scale;
-    bool grad;
-    int cus;
-    char *ws;                 // NULL: only the size is asked for
-    int64_t ws_bytes;
-    hipStream_t st;
-};
-
-// pieces of the workspace, one after the other
-struct Space {
-    char *base;
-    int64_t used;
-    template <class T> T *take(int64_t bytes)
-    {
-        T *const p = (T *)(base + used);
-        used += up(bytes, 1024);
-        return p;
-    }
-};
-
-constexpr int64_t kOneTileMore = 64 * 4;    // staging reads 64 words for a tile's 32
-
-template <class Y, int KO, int MODE> int64_t workgroups(int64_t tiles)
-{
-    typedef Shape<Y, KO, MODE> Z;
-    return (tiles + Z::NW * Z::QB - 1) / (Z::NW * Z::QB);
-}
-
-template <class Y, int KO, int MODE> void launch_pass(PassArgs &A, int64_t groups, hipStream_t st)
-{
-    typedef Shape<Y, KO, MODE> Z;
-    const int64_t stages = (A.stream_tiles + Z::RT - 1) / Z::RT;
-    A.base = (int)(stages / A.splits);
-    A.more = (int)(stages % A.splits);
-    pass_kernel<Y, KO, MODE><<<dim3((unsigned)A.splits, (unsigned)(groups < kGridY ? groups : kGridY), (unsigned)((groups + kGridY - 1) / kGridY)), Z::NW * 64, 0, st>>>(A);
-}
-
-void fill_prepare(PrepArgs &P, const Call &C, int64_t np, int64_t vp)
-{
-    P.target = C.target;
-    P.bias = C.bias;
-    P.weight = C.weight;
-    P.N = C.n;
-    P.V = C.v;
-    P.np = np;
-    P.vp = vp;
-}
-unsigned join_blocks(int64_t rows, int KP) { return (unsigned)((rows * (KP / 4) + 255) / 256); }
-unsigned prepare_blocks(int64_t np, int64_t vp) { return (unsigned)((np > vp ? np : vp) + 255) / 256 + 1; }
-
-void fill_finish(FinishArgs &F, const Call &C)
-{
-    F.target = C.target;
-    F.weight = C.weight;
-    F.w = C.w;
-    F.loss = C.loss;
-    F.lse = C.lse;
-    F.N = C.n;
-    F.V = C.v;
-    F.ldw = C.ldw;
-    F.lddx = C.lddx;
-    F.K = (int)C.k;
-    F.scale = C.scale;
-}
-
-// Rows of up to 256 values: returns the workspace's bytes, or a negative code / launch error where there is one to launch in.
-template <class Y, int KO> int64_t run_narrow(const Call &C)
-{
-    typedef typename Y::t T;
-    constexpr int KP = 32 * KO;
-    const int64_t n_tiles = (C.n + 31) / 32, v_tiles = (C.v + 31) / 32, nt = tiles_padded(n_tiles), vt = tiles_padded(v_tiles), unit = (int64_t)2 * KO * Y::S * kUnit;
-    const int64_t nr = n_tiles * 32, vr = v_tiles * 32;
-    const int64_t row_groups = C.grad ? workgroups<Y, KO, kRows>(n_tiles) : workgroups<Y, KO, kNll>(n_tiles), item_groups = workgroups<Y, KO, kItems>(v_tiles);
-    const int row_splits = pick_splits(row_groups, v_tiles, C.cus), item_splits = pick_splits(item_groups, n_tiles, C.cus);
-    Space W = {C.ws, 0};
-    Matrix mw = {C.w, C.ldw, C.v, nullptr, 0, 1.0f, nullptr, nullptr, nullptr, nullptr};
-    // (the sign of the scale goes into the packed x, so that logits rise with the product)
-    Matrix mx = {C.x, C.ldx, C.n, C.grad ? C.target : nullptr, C.v, C.scale < 0.0f ? -1.0f : 1.0f, nullptr, nullptr, nullptr, nullptr};
-    PrepArgs P = {};
-    fill_prepare(P, C, nt * 32, vt * 32);
-    mw.by_row = W.take<char>(vt * unit);
-    mx.by_row = W.take<char>(nt * unit);
-    P.bias2 = W.take<float>(vt * 32 * 4 + kOneTileMore);
-    P.meta = W.take<int32_t>(nt * 32 * 4 + kOneTileMore);
-    if (Y::scaled) {
-        mw.exps = W.take<int32_t>(vt * 4);
-        mx.exps = W.take<int32_t>(nt * 4);
-    }
-    float *const stats = W.take<float>((int64_t)row_splits * 3 * nr * 4), *reg_bias = nullptr, *target_log = nullptr, *item_stats = nullptr, *part = nullptr;
-    if (C.grad) {
-        mw.by_col = W.take<char>(vt * unit);
-        mx.by_col = W.take<char>(nt * unit);
-        if (Y::scaled) {
-            P.cols = 2 * KP;
-            P.col_top = mw.col_top = W.take<uint32_t>(2 * KP * 4);
-            mx.col_top = mw.col_top + KP;
-        }
-        reg_bias = W.take<float>(nt * 32 * 4 + kOneTileMore);
-        target_log = W.take<float>(nt * 32 * 4);
-        P.wpow = W.take<float>(4);
-        const int64_t rows_part = row_splits * nr * KP * 4, items_part = item_splits > 1 ? item_splits * vr * KP * 4 : 0;
-        part = W.take<float>(rows_part > items_part ? rows_part : items_part);   // (the rows' is read before the items' is written)
-        if (item_splits > 1)
-            item_stats = W.take<float>((int64_t)item_splits * 3 * vr * 4);
-    }
-    if (!C.ws)
-        return W.used;
-    if (C.ws_bytes < W.used)
-        return HPF_EINVAL;
-
-    prepare_kernel<<<prepare_blocks(P.np, P.vp), 256, 0, C.st>>>(P);
-    if (Y::scaled && C.grad) {
-        const int most = C.cus, wb = (int)(C.v / 128 < 1 ? 1 : C.v / 128 > most ? most : C.v / 128), xb = (int)(C.n / 128 < 1 ? 1 : C.n / 128 > most ? most : C.n / 128);
-        columns_kernel<<<wb + xb, 1024, 0, C.st>>>(mw, mx, (int)C.k, wb);
-    }
-    pack_kernel<Y, KO><<<(unsigned)(v_tiles + n_tiles), 256, 0, C.st>>>(mw, mx, (int)C.k, (int)v_tiles);
-
-    PassArgs A = {};
-    A.still = mx.by_row;
-    A.by_row = mw.by_row;
-    A.by_col = mw.by_col;
-    A.still_exp = mx.exps;
-    A.stream_exp = mw.exps;
-    A.reg_bias = P.bias2;
-    A.meta = P.meta;
-    A.stats = stats;
-    A.part = part;
-    A.still_tiles = n_tiles;
-    A.still_rows = nr;
-    A.stream_tiles = v_tiles;
-    A.c = fabsf(C.scale) * kLog2e;
-    A.splits = row_splits;
-    A.bias = C.bias != nullptr;
-    FinishArgs F = {};
-    fill_finish(F, C);
-    F.stats = stats;
-    F.part = part;
-    F.wpow = P.wpow;
-    F.col_top = mw.col_top;
-    F.reg_bias = reg_bias;
-    F.target_log = target_log;
-    F.meta = P.meta;
-    F.dx = C.dx;
-    F.rows = nr;
-    F.KP = KP;
-    F.splits = row_splits;
-    if (!C.grad) {
-        launch_pass<Y, KO, kNll>(A, row_groups, C.st);
-        finish_rows_kernel<Y, false><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
-        return (int)hipGetLastError();
-    }
-    launch_pass<Y, KO, kRows>(A, row_groups, C.st);
-    finish_rows_kernel<Y, true><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
-
-    A.still = mw.by_row;
-    A.by_row = mx.by_row;
-    A.by_col = mx.by_col;
-    A.still_exp = mw.exps;
-    A.stream_exp = mx.exps;
-    A.reg_bias = reg_bias;
-    A.lane_bias = P.bias2;
-    A.target_log = target_log;
-    A.stats = item_stats;
-    A.still_tiles = v_tiles;
-    A.still_rows = vr;
-    A.stream_tiles = n_tiles;
-    A.splits = item_splits;
-    if (item_splits == 1) {
-        A.out = C.dw;
-        A.dbias = C.bias ? C.dbias : nullptr;
-        A.col_top = mx.col_top;
-        A.wpow = P.wpow;
-        A.ld_out = C.lddw;
-        A.count = C.v;
-        A.K = (int)C.k;
-        A.quads = C.lddw % 4 == 0 && (uintptr_t)C.dw % (4 * sizeof(T)) == 0;
-        A.scale = C.scale;
-    }
-    launch_pass<Y, KO, kItems>(A, item_groups, C.st);
-    if (item_splits > 1) {
-        const JoinArgs J = {part, item_stats, nullptr, P.wpow, mx.col_top, C.v, vr, C.lddw, (int)C.k, KP, item_splits, 0, C.scale, C.dw, C.bias ? C.dbias : nullptr};
-        join_kernel<Y><<<join_blocks(C.v, KP), 256, 0, C.st>>>(J);
-    }
-    return (int)hipGetLastError();
-}
-
-// wider rows
-template <class Y> int64_t run_wide(const Call &C)
-{
-    typedef typename Y::t T;
-    const int KO = (int)((C.k + 31) / 32 + 1) / 2 * 2, KP = 32 * KO, CB = 2 * KO, kg = (KO + 3) / 4;
-    const int64_t n_tiles = (C.n + 31) / 32, v_tiles = (C.v + 31) / 32, nt = tiles_padded(n_tiles), vt = tiles_padded(v_tiles), unit = (int64_t)2 * KO * Y::S * kUnit;
-    const int64_t nr = n_tiles * 32, ng = (n_tiles + 3) / 4;
-    const int row_splits = pick_splits(2 * ng, v_tiles, C.cus);
-    int64_t chunk = kChunkBytes / (ng * 4 * 32 * 32 * 2 * Y::S * 2) / 4 * 4;                 // tiles of items at a time
-    chunk = chunk < 4 ? 4 : chunk > up(v_tiles, 4) ? up(v_tiles, 4) : chunk;
-    const int dw_splits = pick_splits(2 * kg * (chunk / 4), n_tiles, C.cus), dx_splits = pick_splits(2 * kg * ng, chunk, C.cus), sum_splits = (int)(2 * ng);
-    Space S = {C.ws, 0};
-    Matrix mw = {C.w, C.ldw, C.v, nullptr, 0, 1.0f, nullptr, nullptr, nullptr, nullptr};
-    Matrix mx = {C.x, C.ldx, C.n, C.grad ? C.target : nullptr, C.v, C.scale < 0.0f ? -1.0f : 1.0f, nullptr, nullptr, nullptr, nullptr};
-    PrepArgs P = {};
-    fill_prepare(P, C, nt * 32, vt * 32);
-    mw.by_row = S.take<char>(vt * unit);
-    mx.by_row = S.take<char>(nt * unit);
-    P.bias2 = S.take<float>(vt * 32 * 4);
-    P.meta = S.take<int32_t>(nt * 32 * 4);
-    WideArgs A = {};
-    FinishArgs F = {};
-    fill_finish(F, C);
-    float *dw_part = nullptr, *dx_part = nullptr;
-    A.stats = S.take<float>((int64_t)2 * row_splits * 3 * nr * 4);
-    if (C.grad) {
-        mw.by_col = S.take<char>(vt * unit);
-        mx.by_col = S.take<char>(nt * unit);
-        F.reg_bias = S.take<float>(nt * 32 * 4);
-        F.target_log = S.take<float>(nt * 32 * 4);
-        P.wpow = S.take<float>(4);
-        dw_part = S.take<float>(dw_splits * chunk * 32 * KP * 4);
-        dx_part = S.take<float>(dx_splits * nr * KP * 4);
-        A.part_sum = S.take<float>(sum_splits * chunk * 32 * 4);
-        A.g_rows = S.take<char>(ng * 4 * chunk * 2 * Y::S * kUnit);
-        A.g_items = S.take<char>(ng * 4 * chunk * 2 * Y::S * kUnit);
-    }
-    if (!C.ws)
-        return S.used;
-    if (C.ws_bytes < S.used)
-        return HPF_EINVAL;
-
-    prepare_kernel<<<prepare_blocks(P.np, P.vp), 256, 0, C.st>>>(P);
-    pack_wide_kernel<Y><<<dim3((unsigned)v_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mw, (int)C.k, CB, KO);
-    pack_wide_kernel<Y><<<dim3((unsigned)n_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mx, (int)C.k, CB, KO);
-    A.w = mw.by_row;
-    A.x = mx.by_row;
-    A.bias = P.bias2;
-    A.meta = P.meta;
-    A.n_tiles = n_tiles;
-    A.v_tiles = v_tiles;
-    A.rows = nr;
-    A.c = fabsf(C.scale) * kLog2e;
-    A.CB = CB;
-    A.splits = row_splits;
-    A.has_bias = C.bias != nullptr;
-    wide_stats_kernel<Y><<<(unsigned)(ng * row_splits), 256, 0, C.st>>>(A);
-    F.stats = A.stats;
-    F.wpow = P.wpow;
-    F.meta = P.meta;
-    F.rows = nr;
-    F.splits = 2 * row_splits;
-    if (!C.grad) {
-        finish_rows_kernel<Y, false><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
-        return (int)hipGetLastError();
-    }
-    finish_rows_kernel<Y, true><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
-    A.reg_bias = F.reg_bias;
-    A.target_log = F.target_log;
-    for (int64_t v0 = 0; v0 < v_tiles; v0 += chunk) {
-        A.v0 = v0;
-        A.v_count = v_tiles - v0 < chunk ? v_tiles - v0 : chunk;
-        wide_g_kernel<Y><<<(unsigned)(ng * ((A.v_count + 3) / 4)), 256, 0, C.st>>>(A);
-        ProductArgs D = {A.g_rows, mw.by_col + v0 * unit, n_tiles, A.v_count * 2, A.v_count, KO, dx_splits, dx_part, v0 > 0};
-        wide_product_kernel<Y><<<(unsigned)(ng * kg * dx_splits), 256, 0, C.st>>>(D);
-        D = {A.g_items, mx.by_col, A.v_count, n_tiles * 2, n_tiles, KO, dw_splits, dw_part, 0};
-        wide_product_kernel<Y><<<(unsigned)((A.v_count + 3) / 4 * kg * dw_splits), 256, 0, C.st>>>(D);
-        const int64_t first = v0 * 32, count = C.v - first < A.v_count * 32 ? C.v - first : A.v_count * 32;
-        const JoinArgs J = {dw_part, nullptr, A.part_sum, P.wpow, nullptr, count, A.v_count * 32, C.lddw, (int)C.k, KP, dw_splits, sum_splits, C.scale,
-                            (T *)C.dw + first * C.lddw, C.bias ? C.dbias + first : nullptr};
-        join_kernel<Y><<<join_blocks(count, KP), 256, 0, C.st>>>(J);
-    }
-    const JoinArgs J = {dx_part, nullptr, nullptr, P.wpow, nullptr, C.n, nr, C.lddx, (int)C.k, KP, dx_splits, 0, C.scale, C.dx, nullptr};
-    join_kernel<Y><<<join_blocks(C.n, KP), 256, 0, C.st>>>(J);
-    return (int)hipGetLastError();
-}
-
-// a few rows, no gradients (Y as the products take it: W32 for 32 bits).  A wavefront holds two tiles' rows as they are: 256 registers
-// have room for 2 x 128 values of 32 bits, or 2 x 256 of 16, a row.
-template <class Y> bool is_few(const Call &C) { return !C.grad && C.n <= 64 && C.k <= (Y::S == 1 ? 256 : 128); }
-
-template <class Y, int QB, int CB> void launch_few(const FewArgs &A, unsigned grid, hipStream_t st)
-{
-    const int bytes = QB * CB * Y::S * kUnit + 2 * 32 * 16 * CB * (int)sizeof(typename Y::t);   // at most 48 + 32 KB
-    few_kernel<Y, QB, CB><<<grid, kFewWaves * 64, bytes, st>>>(A);
-}
-template <class Y, int QB> void launch_few_rows(const FewArgs &A, unsigned grid, hipStream_t st)
-{
-    if (A.K <= 32)
-        launch_few<Y, QB, 2>(A, grid, st);
-    else if (A.K <= 64)
-        launch_few<Y, QB, 4>(A, grid, st);
-    else if (A.K <= 112)
-        launch_few<Y, QB, 7>(A, grid, st);
-    else if (A.K <= 128)
-        launch_few<Y, QB, 8>(A, grid, st);
-    else if constexpr (Y::S == 1) {
-        if (A.K <= 208)
-            launch_few<Y, QB, 13>(A, grid, st);
-        else
-            launch_few<Y, QB, 16>(A, grid, st);
-    }
-}
-
-template <class Y> int64_t run_few(const Call &C)
-{
-    FewArgs A = {};
-    A.rows = up(C.n, 32);
-    A.v_tiles = (C.v + 31) / 32;
-    A.K = (int)C.k;
-    int64_t grid = (A.v_tiles + kFewWaves - 1) / kFewWaves;   // two wavefronts a SIMD at most: what its registers have room for
-    grid = grid > C.cus ? C.cus : grid;
-    Space S = {C.ws, 0};
-    A.stats = S.take<float>(grid * 3 * A.rows * 4);
-    if (!C.ws)
-        return S.used;
-    if (C.ws_bytes < S.used)
-        return HPF_EINVAL;
-    A.x = C.x;
-    A.w = C.w;
-    A.target = C.target;
-    A.bias = C.bias;
-    A.N = C.n;
-    A.V = C.v;
-    A.ldx = C.ldx;
-    A.ldw = C.ldw;
-    A.c = fabsf(C.scale) * kLog2e;
-    A.sign = C.scale < 0.0f ? -1.0f : 1.0f;
-    if (C.n <= 32)
-        launch_few_rows<Y, 1>(A, (unsigned)grid, C.st);
-    else
-        launch_few_rows<Y, 2>(A, (unsigned)grid, C.st);
-    FinishArgs F = {};
-    fill_finish(F, C);
-    F.stats = A.stats;
-    F.rows = A.rows;
-    F.splits = (int)grid;
-    finish_rows_kernel<Y, false><<<(unsigned)(A.rows / 4), 256, 0, C.st>>>(F);
-    return (int)hipGetLastError();
-}
-
-template <class Y> int64_t run_any_narrow(const Call &C)
-{
-    switch ((C.k + 31) / 32) {
-    case 1: return run_narrow<Y, 1>(C);
-    case 2: return run_narrow<Y, 2>(C);
-    case 3: return run_narrow<Y, 3>(C);
-    case 4: return run_narrow<Y, 4>(C);
-    case 5: return run_narrow<Y, 5>(C);
-    case 6: return run_narrow<Y, 6>(C);
-    case 7: return run_narrow<Y, 7>(C);
-    default: return run_narrow<Y, 8>(C);
-    }
-}
-
-int64_t run(int type, const Call &C)
-{
-    const bool narrow = C.k <= 256;
-    if (type == HPF_F32)
-        return is_few<W32>(C) ? run_few<W32>(C) : narrow ? run_any_narrow<F32>(C) : run_wide<W32>(C);
-    if (type == HPF_BF16)
-        return is_few<B16>(C) ? run_few<B16>(C) : narrow ? run_any_narrow<B16>(C) : run_wide<B16>(C);
-    return is_few<H16>(C) ? run_few<H16>(C) : narrow ? run_any_narrow<H16>(C) : run_wide<H16>(C);
-}
-
-bool sizes_ok(int64_t n, int64_t v, int64_t k) { return n >= 0 && v > 0 && k > 0 && n < kNoTarget - 31 && v < kNoTarget - 31 && k < (1 << 20); }
+bool sizes_ok(int64_t n, int64_t v, int64_t k) { return n >= 0 && v > 0 && k > 0 && n < hpf_softmax::kNoTarget - 31 && v < hpf_softmax::kNoTarget - 31 && k < (1 << 20); }
 
 }  // namespace
 
@@ -1807,6 +73,7 @@ extern "C" int hpf_hip_softmax_nll_grad(const void *x, int64_t ldx, const void *
         return HPF_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
     if (n == 0) {              // no rows: the items' gradients are zero
+        using hpf_softmax::zero_rows_kernel;
         if (type == HPF_F32)
             zero_rows_kernel<<<1024, 256, 0, st>>>((float *)ditems, v, (int)k, ld_ditems);
         else
