@@ -726,17 +726,18 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
 // Rows too wide for a wavefront's registers (k > 256): plain tiled products of packed matrices, the catalogue in chunks.  The
 // statistics come from a first run over all logits; then, chunk by chunk, G is written in both operand layouts (16-bit parts,
 // a chunk at a time: at most kChunkBytes) and multiplied with the items (dx, summed over the chunks) and with x (dw).
-// Bound by the matrix instructions: 8 N V K operations, 128 x 128 outputs a workgroup, 64 x 64 a wavefront.
+// Bound by the matrix instructions: 8 N V K operations.  256 x 128 outputs a workgroup, 128 x 64 a wavefront: six operands read from
+// shared memory for eight products (four for four, 64 x 64, keep shared memory as busy as the matrix units).
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int64_t kChunkBytes = 192ll << 20;
 
-template <class Y, int KC_> struct Wide {
-    static constexpr int S = Y::S, KC = KC_;                // units of the contraction a stage
-    static constexpr int stage = 8 * KC * S * kUnit;        // 4 tiles of each matrix
+template <class Y> struct Wide {
+    static constexpr int S = Y::S, KC = S == 1 ? 2 : 1;     // units of the contraction a stage
+    static constexpr int stage = 12 * KC * S * kUnit;       // 8 tiles of one matrix, 4 of the other
 };
-template <class Y> struct Logits : Wide<Y, Y::S == 1 ? 4 : 2> {};
+constexpr int kWideA = 8, kWideB = 4;
 
-// For each group: the 128 x 128 product of 4 + 4 tiles over `steps` stages, handed to `done(group, acc)`.  a(group, step, tile) and
+// For each group: the 256 x 128 product of 8 + 4 tiles over `steps` stages, handed to `done(group, acc)`.  a(group, step, tile) and
 // b(group, step, tile) are a tile's KC S consecutive units.
 template <class Y, class Z, class A, class B, class D>
 __device__ __forceinline__ void wide_core(char *lds, int64_t groups, int steps, const A &a, const B &b, const D &done)
@@ -744,20 +745,22 @@ __device__ __forceinline__ void wide_core(char *lds, int64_t groups, int steps, 
     constexpr int S = Z::S, KC = Z::KC, per = KC * S;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
     auto stage = [&](int64_t g, int step, int buf) {
-        const char *pa = a(g, step, wave), *pb = b(g, step, wave);       // wavefront w brings tile w of each matrix
+        // wavefront w brings tiles w and w + 4 of the first matrix and w of the other
+        const char *pa = a(g, step, wave), *pc = a(g, step, wave + 4), *pb = b(g, step, wave);
 #pragma unroll
         for (int u = 0; u < per; ++u) {
             stage_unit(pa + u * kUnit, lds + buf * Z::stage + (wave * per + u) * kUnit);
-            stage_unit(pb + u * kUnit, lds + buf * Z::stage + ((4 + wave) * per + u) * kUnit);
+            stage_unit(pc + u * kUnit, lds + buf * Z::stage + ((4 + wave) * per + u) * kUnit);
+            stage_unit(pb + u * kUnit, lds + buf * Z::stage + ((8 + wave) * per + u) * kUnit);
         }
     };
-    f32x16 acc[2][2];
+    f32x16 acc[4][2];
     int buf = 0;
     if (groups > 0 && steps > 0)
         stage(0, 0, 0);
     for (int64_t g = 0; g < groups; ++g) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 4; ++i)
             for (int j = 0; j < 2; ++j)
                 acc[i][j] = (f32x16)(0.0f);
         for (int step = 0; step < steps; ++step, buf ^= 1) {
@@ -769,15 +772,17 @@ __device__ __forceinline__ void wide_core(char *lds, int64_t groups, int steps, 
             const char *at = lds + buf * Z::stage + lane * 16;
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
-                Parts<Y> x[2], y[2];
+                Parts<Y> x[4], y[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    for (int s = 0; s < S; ++s) {
-                        x[i].p[s] = *(const typename Y::m::v8 *)(at + ((2 * wa + i) * per + c * S + s) * kUnit);
-                        y[i].p[s] = *(const typename Y::m::v8 *)(at + ((4 + 2 * wb + i) * per + c * S + s) * kUnit);
-                    }
+                for (int i = 0; i < 4; ++i)
+                    for (int s = 0; s < S; ++s)
+                        x[i].p[s] = *(const typename Y::m::v8 *)(at + ((4 * wa + i) * per + c * S + s) * kUnit);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int j = 0; j < 2; ++j)
+                    for (int s = 0; s < S; ++s)
+                        y[j].p[s] = *(const typename Y::m::v8 *)(at + ((8 + 2 * wb + j) * per + c * S + s) * kUnit);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
                         acc[i][j] = product<Y>(x[i], y[j], acc[i][j]);
@@ -818,13 +823,13 @@ __device__ __forceinline__ void wide_bias(f32x16 &x, const WideArgs &A, int64_t 
 
 template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(WideArgs A)
 {
-    typedef Logits<Y> Z;
+    typedef Wide<Y> Z;
     __shared__ __attribute__((aligned(1024))) char lds[2 * Z::stage];
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
     const int sp = blockIdx.x % A.splits;
     const int64_t n0 = (int64_t)(blockIdx.x / A.splits) * 4;
-    const int64_t all = (A.v_tiles + 3) / 4, g0 = all * sp / A.splits, g1 = all * (sp + 1) / A.splits;
+    const int64_t all = (A.v_tiles + kWideA - 1) / kWideA, g0 = all * sp / A.splits, g1 = all * (sp + 1) / A.splits;
     int target[2];
     float top[2], at[2];
     Sum sum[2];
@@ -838,12 +843,12 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(W
     }
     wide_core<Y, Z>(
         lds, g1 - g0, A.CB / Z::KC,
-        [&](int64_t g, int step, int tile) { return A.w + (((g0 + g) * 4 + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
+        [&](int64_t g, int step, int tile) { return A.w + (((g0 + g) * kWideA + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
         [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
-        [&](int64_t g, f32x16 (&acc)[2][2]) {
+        [&](int64_t g, f32x16 (&acc)[4][2]) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t tile = (g0 + g) * 4 + 2 * wa + i;
+            for (int i = 0; i < 4; ++i) {
+                const int64_t tile = (g0 + g) * kWideA + 4 * wa + i;
                 if (tile >= A.v_tiles)
                     break;
 #pragma unroll
@@ -864,10 +869,10 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(W
     }
 }
 
-// G of 4 tiles of rows against 4 tiles of items of the chunk, in both layouts, and the sums over its rows
+// G of 4 tiles of rows against 8 tiles of items of the chunk, in both layouts, and the sums over its rows
 template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideArgs A)
 {
-    typedef Logits<Y> Z;
+    typedef Wide<Y> Z;
     typedef typename Y::m::e e;
     constexpr int S = Y::S;
     __shared__ __attribute__((aligned(1024))) char lds[2 * Z::stage];
@@ -875,7 +880,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
     e(*turn)[36] = turn_all[wave];
-    const int64_t ngroups = (A.n_tiles + 3) / 4, n0 = blockIdx.x % ngroups * 4, vg = blockIdx.x / ngroups * 4;   // vg: within the chunk
+    const int64_t ngroups = (A.n_tiles + 3) / 4, n0 = blockIdx.x % ngroups * 4, vg = blockIdx.x / ngroups * kWideA;   // vg: within the chunk
     int meta[2];
     float down[2], tg[2];
 #pragma unroll
@@ -890,10 +895,10 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
         lds, 1, A.CB / Z::KC,
         [&](int64_t, int step, int tile) { return A.w + ((A.v0 + vg + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
         [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
-        [&](int64_t, f32x16 (&acc)[2][2]) {
+        [&](int64_t, f32x16 (&acc)[4][2]) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t vt = vg + 2 * wa + i, tile = A.v0 + vt;
+            for (int i = 0; i < 4; ++i) {
+                const int64_t vt = vg + 4 * wa + i, tile = A.v0 + vt;
                 if (vt >= A.v_count)
                     break;
                 f32x16 total = (f32x16)(0.0f);
@@ -960,49 +965,90 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
         });
 }
 
-// c[m][k] = sum over the contraction's tiles of a (by_row units, U of them a tile) times b (by_col units)
+// c[m][k] = sum over the contraction's tiles of a (by_row units, `a_units` of them a tile) times b (by_col units)
 struct ProductArgs {
     const char *a, *b;
     int64_t a_tiles, a_units, tiles;      // output tiles, units of one, contraction tiles (32 each)
     int KO, splits;
     float *part;                          // [split][32 a_tiles][32 KO] sums; `more`: added to what is there
     int more;
+    void *out;                            // or the results themselves: times scale wpow 2^-shift, `count` rows of K
+    const float *wpow;
+    int64_t count, ld;
+    int K;
+    float scale;
 };
 
 template <class Y> __global__ __launch_bounds__(256, 2) void wide_product_kernel(ProductArgs A)
 {
-    typedef Wide<Y, 2> Z;
+    typedef Wide<Y> Z;
     __shared__ __attribute__((aligned(1024))) char lds[2 * Z::stage];
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
-    const int kgroups = (A.KO + 3) / 4;
-    int64_t id = blockIdx.x;
-    const int kg = (int)(id % kgroups) * 4;
-    id /= kgroups;
-    const int sp = (int)(id % A.splits);
-    const int64_t m0 = id / A.splits * 4;
-    const int64_t s0 = A.tiles * sp / A.splits, s1 = A.tiles * (sp + 1) / A.splits;   // a contraction tile a stage
+    const unsigned kgroups = (A.KO + kWideB - 1) / kWideB;
+    // workgroups whose ids are equal modulo 8 share a die: those of one piece of the contraction, or of one group of rows
+    unsigned sp = 0, id = blockIdx.x, kg, mg;
+    if (A.splits > 1) {
+        sp = id % A.splits;
+        id /= A.splits;
+        kg = id % kgroups;
+        mg = id / kgroups;
+    } else {
+        kg = id / 8 % kgroups;
+        mg = id % 8 + id / 8 / kgroups * 8;
+    }
+    const int64_t m0 = (int64_t)mg * kWideA;
+    const int k0 = (int)kg * kWideB;
+    if (m0 >= A.a_tiles)
+        return;
+    const int64_t all = A.tiles * (2 / Z::KC), s0 = all * sp / A.splits, s1 = all * (sp + 1) / A.splits;   // stages of KC units
     wide_core<Y, Z>(
         lds, 1, (int)(s1 - s0),
         [&](int64_t, int step, int tile) { return A.a + ((m0 + tile) * A.a_units + (s0 + step) * Z::KC) * Z::S * kUnit; },
-        [&](int64_t, int step, int tile) { return A.b + ((s0 + step) * A.KO + (kg + tile < A.KO ? kg + tile : A.KO - 1)) * Z::KC * Z::S * kUnit; },
-        [&](int64_t, f32x16 (&acc)[2][2]) {
+        [&](int64_t, int step, int tile) {
+            const int64_t u = (s0 + step) * Z::KC;
+            return A.b + (((u >> 1) * A.KO + (k0 + tile < A.KO ? k0 + tile : A.KO - 1)) * 2 + (u & 1)) * Z::S * kUnit;
+        },
+        [&](int64_t, f32x16 (&acc)[4][2]) {
+            const float f = A.out ? A.scale * *A.wpow * __builtin_amdgcn_exp2f(-(float)Y::shift) : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int64_t mt = m0 + 2 * wa + i;
-                    const int ko = kg + 2 * wb + j;
+                    const int64_t mt = m0 + 4 * wa + i;
+                    const int ko = k0 + 2 * wb + j, k = 32 * ko + low;
                     if (mt >= A.a_tiles || ko >= A.KO)
                         continue;
-                    float *to = A.part + ((sp * A.a_tiles + mt) * 32) * (int64_t)(32 * A.KO) + 32 * ko + low;
+                    if (A.out) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int64_t m = mt * 32 + row_of(r, h);
+                            if (m < A.count && k < A.K)
+                                ((typename Y::t *)A.out)[m * A.ld + k] = (typename Y::t)(acc[i][j][r] * f);
+                        }
+                        continue;
+                    }
+                    float *to = A.part + ((sp * A.a_tiles + mt) * 32) * (int64_t)(32 * A.KO) + k;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        float *o = to + (row_of(r, h)) * (int64_t)(32 * A.KO);
+                        float *o = to + row_of(r, h) * (int64_t)(32 * A.KO);
                         *o = A.more ? *o + acc[i][j][r] : acc[i][j][r];
                     }
                 }
         });
+}
+
+// dbias of a chunk: wpow 2^-shift times the sums of its rows' groups
+static __global__ __launch_bounds__(256) void wide_sums_kernel(const float *sums, int64_t rows, int groups, const float *wpow, int shift, int64_t count, float *dbias)
+{
+    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (v >= count)
+        return;
+    float all = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < groups; ++s)
+        all += sums[s * rows + v];
+    dbias[v] = ldexpf(all * *wpow, -shift);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1305,11 +1351,11 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__(kFewWaves * 64, 
 
 // joins the splits of a product with G: out = scale wpow sum, dbias = wpow sum (four columns a thread)
 struct JoinArgs {
-    const float *part, *tops, *sums;       // tops (ranged passes): [split][3][rows] with the sums behind, else NULL
+    const float *part, *tops;              // tops (the passes' pieces): [split][3][rows] with the sums behind, else NULL
     const float *wpow;
     const uint32_t *col_top;
     int64_t count, rows, ld;
-    int K, KP, splits, sum_splits;
+    int K, KP, splits;
     float scale;
     void *out;
     float *dbias;
@@ -1343,12 +1389,8 @@ template <class Y> __global__ __launch_bounds__(256) void join_kernel(JoinArgs A
         }
     if (A.dbias && k == 0) {
         float all = 0.0f;
-        if (A.tops)
-            for (int s = 0; s < A.splits; ++s)
-                all += times_power(A.tops[(3 * s + 1) * A.rows + v], A.tops[3 * s * A.rows + v] - top);
-        else
-            for (int s = 0; s < A.sum_splits; ++s)
-                all += A.sums[s * A.rows + v];
+        for (int s = 0; s < A.splits; ++s)
+            all += times_power(A.tops[(3 * s + 1) * A.rows + v], A.tops[3 * s * A.rows + v] - top);
         A.dbias[v] = times_power(all * *A.wpow, top - (float)Y::shift);
     }
 }
@@ -1366,24 +1408,17 @@ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 constexpr int kMostSplits = 256;      // a row's pieces are joined by one wavefront
 inline int64_t tiles_padded(int64_t tiles) { return up(tiles, kPadTiles); }
 
-// How many pieces the streamed side is cut into: enough workgroups for four on each compute unit with 8 tiles or more each, in eights (one
-// a die) once there are that many; where that leaves compute units idle, down to 2 tiles each.
-inline int pick_splits(int64_t workgroups, int64_t stream_tiles, int cus)
+// How many pieces a contraction of so many units is cut into for workgroups that would not fill the chip: up to a full round of them, in
+// eights (one a die) once there are eight.
+inline int wide_splits(int64_t workgroups, int64_t units, int64_t room)
 {
-    int64_t s = (4 * cus + workgroups - 1) / workgroups;
-    if (s > stream_tiles / 8)
-        s = stream_tiles / 8;
-    if (s * workgroups < cus) {
-        s = (cus + workgroups - 1) / workgroups;
-        if (s > stream_tiles / 2)
-            s = stream_tiles / 2;
-    }
-    if (s > 8)
-        s = s / 8 * 8;
-    return s < 1 ? 1 : s > kMostSplits ? kMostSplits : (int)s;
+    int64_t s = room / workgroups;
+    s = s > units ? units : s;
+    s = s > 8 ? s / 8 * 8 : s;
+    return s < 1 ? 1 : s > kMostSplits / 2 ? kMostSplits / 2 : (int)s;
 }
 
-// The same for the passes, by an estimate of their time in microseconds: rounds of the workgroups that are resident together, each with
+// For the passes, by an estimate of their time in microseconds: rounds of the workgroups that are resident together, each with
 // its start and its stages, whose cost grows with the wavefronts that share a SIMD; and what it takes to join the pieces.  More than
 // eight come in eights.
 template <class Y, int KO, int ODD, int MODE> int pass_splits(int64_t still_tiles, int64_t stream_tiles, int cus)
@@ -1596,7 +1631,7 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
     }
     launch_pass<Y, KO, ODD, kItems>(A, item_groups, C.st);
     if (item_splits > 1) {
-        const JoinArgs J = {part, item_stats, nullptr, P.wpow, mx.col_top, C.v, vr, C.lddw, (int)C.k, KP, item_splits, 0, C.scale, C.dw, C.bias ? C.dbias : nullptr};
+        const JoinArgs J = {part, item_stats, P.wpow, mx.col_top, C.v, vr, C.lddw, (int)C.k, KP, item_splits, C.scale, C.dw, C.bias ? C.dbias : nullptr};
         join_kernel<Y><<<join_blocks(C.v, KP), 256, 0, C.st>>>(J);
     }
     return (int)hipGetLastError();
@@ -1606,13 +1641,15 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
 template <class Y> int64_t run_wide(const Call &C)
 {
     typedef typename Y::t T;
-    const int KO = (int)((C.k + 31) / 32 + 1) / 2 * 2, KP = 32 * KO, CB = 2 * KO, kg = (KO + 3) / 4;
+    const int KO = (int)((C.k + 31) / 32 + 1) / 2 * 2, KP = 32 * KO, CB = 2 * KO, kg = (KO + kWideB - 1) / kWideB;
     const int64_t n_tiles = (C.n + 31) / 32, v_tiles = (C.v + 31) / 32, nt = tiles_padded(n_tiles), vt = tiles_padded(v_tiles), unit = (int64_t)2 * KO * Y::S * kUnit;
-    const int64_t nr = n_tiles * 32, ng = (n_tiles + 3) / 4;
-    const int row_splits = pick_splits(2 * ng, v_tiles, C.cus);
-    int64_t chunk = kChunkBytes / (ng * 4 * 32 * 32 * 2 * Y::S * 2) / 4 * 4;                 // tiles of items at a time
-    chunk = chunk < 4 ? 4 : chunk > up(v_tiles, 4) ? up(v_tiles, 4) : chunk;
-    const int dw_splits = pick_splits(2 * kg * (chunk / 4), n_tiles, C.cus), dx_splits = pick_splits(2 * kg * ng, chunk, C.cus), sum_splits = (int)(2 * ng);
+    const int64_t nr = n_tiles * 32, nb = (n_tiles + kWideB - 1) / kWideB, na = nt / kWideA, room = 2 * C.cus;   // workgroups that are resident
+    const int row_splits = wide_splits(nb, vt / kWideA, room);
+    // tiles of items at a time: what kChunkBytes hold, as full rounds of the products' workgroups if that is a round or more
+    const int64_t round = kWideA * ((room + kg - 1) / kg), most = kChunkBytes / (nt * 32 * 32 * 2 * Y::S * 2);
+    int64_t chunk = most >= round ? most / round * round : up(most < 1 ? 1 : most, kWideA);
+    chunk = chunk > vt ? vt : chunk;
+    const int dx_splits = wide_splits(na * kg, chunk / 4, room), dw_splits = wide_splits(chunk / kWideA * kg, n_tiles / 4, room);
     Space S = {C.ws, 0};
     Matrix mw = {C.w, C.ldw, C.v, nullptr, 0, 1.0f, nullptr, nullptr, nullptr, nullptr};
     Matrix mx = {C.x, C.ldx, C.n, C.grad ? C.target : nullptr, C.v, C.scale < 0.0f ? -1.0f : 1.0f, nullptr, nullptr, nullptr, nullptr};
@@ -1633,11 +1670,12 @@ template <class Y> int64_t run_wide(const Call &C)
         F.reg_bias = S.take<float>(nt * 32 * 4);
         F.target_log = S.take<float>(nt * 32 * 4);
         P.wpow = S.take<float>(4);
-        dw_part = S.take<float>(dw_splits * chunk * 32 * KP * 4);
+        if (dw_splits > 1)
+            dw_part = S.take<float>(dw_splits * chunk * 32 * KP * 4);
         dx_part = S.take<float>(dx_splits * nr * KP * 4);
-        A.part_sum = S.take<float>(sum_splits * chunk * 32 * 4);
-        A.g_rows = S.take<char>(ng * 4 * chunk * 2 * Y::S * kUnit);
-        A.g_items = S.take<char>(ng * 4 * chunk * 2 * Y::S * kUnit);
+        A.part_sum = S.take<float>(2 * nb * chunk * 32 * 4);
+        A.g_rows = S.take<char>(nt * chunk * 2 * Y::S * kUnit);
+        A.g_items = S.take<char>(nt * chunk * 2 * Y::S * kUnit);
     }
     if (!C.ws)
         return S.used;
@@ -1658,7 +1696,7 @@ template <class Y> int64_t run_wide(const Call &C)
     A.CB = CB;
     A.splits = row_splits;
     A.has_bias = C.bias != nullptr;
-    wide_stats_kernel<Y><<<(unsigned)(ng * row_splits), 256, 0, C.st>>>(A);
+    wide_stats_kernel<Y><<<(unsigned)(nb * row_splits), 256, 0, C.st>>>(A);
     F.stats = A.stats;
     F.wpow = P.wpow;
     F.meta = P.meta;
@@ -1674,17 +1712,44 @@ template <class Y> int64_t run_wide(const Call &C)
     for (int64_t v0 = 0; v0 < v_tiles; v0 += chunk) {
         A.v0 = v0;
         A.v_count = v_tiles - v0 < chunk ? v_tiles - v0 : chunk;
-        wide_g_kernel<Y><<<(unsigned)(ng * ((A.v_count + 3) / 4)), 256, 0, C.st>>>(A);
-        ProductArgs D = {A.g_rows, mw.by_col + v0 * unit, n_tiles, A.v_count * 2, A.v_count, KO, dx_splits, dx_part, v0 > 0};
-        wide_product_kernel<Y><<<(unsigned)(ng * kg * dx_splits), 256, 0, C.st>>>(D);
-        D = {A.g_items, mx.by_col, A.v_count, n_tiles * 2, n_tiles, KO, dw_splits, dw_part, 0};
-        wide_product_kernel<Y><<<(unsigned)((A.v_count + 3) / 4 * kg * dw_splits), 256, 0, C.st>>>(D);
-        const int64_t first = v0 * 32, count = C.v - first < A.v_count * 32 ? C.v - first : A.v_count * 32;
-        const JoinArgs J = {dw_part, nullptr, A.part_sum, P.wpow, nullptr, count, A.v_count * 32, C.lddw, (int)C.k, KP, dw_splits, sum_splits, C.scale,
-                            (T *)C.dw + first * C.lddw, C.bias ? C.dbias + first : nullptr};
-        join_kernel<Y><<<join_blocks(count, KP), 256, 0, C.st>>>(J);
+        const int64_t vg = (A.v_count + kWideA - 1) / kWideA, first = v0 * 32, count = C.v - first < A.v_count * 32 ? C.v - first : A.v_count * 32;
+        wide_g_kernel<Y><<<(unsigned)(nb * vg), 256, 0, C.st>>>(A);
+        ProductArgs D = {};
+        D.a = A.g_rows;
+        D.b = mw.by_col + v0 * unit;
+        D.a_tiles = n_tiles;
+        D.a_units = A.v_count * 2;
+        D.tiles = A.v_count;
+        D.KO = KO;
+        D.splits = dx_splits;
+        D.part = dx_part;
+        D.more = v0 > 0;
+        wide_product_kernel<Y><<<(unsigned)(up(na, 8) * kg * dx_splits), 256, 0, C.st>>>(D);
+        D.a = A.g_items;
+        D.b = mx.by_col;
+        D.a_tiles = A.v_count;
+        D.a_units = n_tiles * 2;
+        D.tiles = n_tiles;
+        D.splits = dw_splits;
+        D.part = dw_part;
+        D.more = 0;
+        if (dw_splits == 1) {
+            D.out = (T *)C.dw + first * C.lddw;
+            D.wpow = P.wpow;
+            D.count = count;
+            D.ld = C.lddw;
+            D.K = (int)C.k;
+            D.scale = C.scale;
+        }
+        wide_product_kernel<Y><<<(unsigned)(up(vg, 8) * kg * dw_splits), 256, 0, C.st>>>(D);
+        if (dw_splits > 1) {
+            const JoinArgs J = {dw_part, nullptr, P.wpow, nullptr, count, A.v_count * 32, C.lddw, (int)C.k, KP, dw_splits, C.scale, (T *)C.dw + first * C.lddw, nullptr};
+            join_kernel<Y><<<join_blocks(count, KP), 256, 0, C.st>>>(J);
+        }
+        if (C.bias)
+            wide_sums_kernel<<<(unsigned)((count + 255) / 256), 256, 0, C.st>>>(A.part_sum, A.v_count * 32, (int)(2 * nb), P.wpow, Y::shift, count, C.dbias + first);
     }
-    const JoinArgs J = {dx_part, nullptr, nullptr, P.wpow, nullptr, C.n, nr, C.lddx, (int)C.k, KP, dx_splits, 0, C.scale, C.dx, nullptr};
+    const JoinArgs J = {dx_part, nullptr, P.wpow, nullptr, C.n, nr, C.lddx, (int)C.k, KP, dx_splits, C.scale, C.dx, nullptr};
     join_kernel<Y><<<join_blocks(C.n, KP), 256, 0, C.st>>>(J);
     return (int)hipGetLastError();
 }
