@@ -312,8 +312,9 @@ template <class Y, int KO> __global__ __launch_bounds__(256) void pack_kernel(Ma
     }
 }
 
-// the same for rows of any width, without scales: 32 rows x 128 columns a workgroup
-template <class Y> __global__ __launch_bounds__(256) void pack_wide_kernel(Matrix M, int K, int CB, int KO)
+// The same for rows of any width, without scales: 32 rows x 128 columns a workgroup.  `pitch` units from tile to tile, an odd number: the
+// tiles that a product reads side by side would else lie a power of two apart, on the same channels of the caches.
+template <class Y> __global__ __launch_bounds__(256) void pack_wide_kernel(Matrix M, int K, int CB, int KO, int pitch)
 {
     __shared__ float tile[32][129];
     const int64_t rb = blockIdx.x;
@@ -335,7 +336,7 @@ template <class Y> __global__ __launch_bounds__(256) void pack_wide_kernel(Matri
             for (int j = 0; j < 8; ++j)
                 split<Y>(M.sign * tile[low][16 * u + 8 * h + j], q, j);
             for (int s = 0; s < Y::S; ++s)
-                *(typename Y::m::v8 *)(M.by_row + (((rb * CB + cb) * Y::S + s) * 64 + lane) * 16) = q.p[s];
+                *(typename Y::m::v8 *)(M.by_row + (((rb * pitch + cb) * Y::S + s) * 64 + lane) * 16) = q.p[s];
         }
         const int ko = blockIdx.y * 4 + (u >> 1), t = u & 1;
         if (M.by_col && ko < KO) {
@@ -800,7 +801,8 @@ struct WideArgs {
     char *g_rows, *g_items;         // G of a chunk: rows n / contraction v, and rows v / contraction n
     int64_t n_tiles, v_tiles, rows, v0, v_count;   // tiles; v0, v_count: the chunk
     float c;
-    int CB, splits, has_bias;
+    int CB, pitch, splits, has_bias;   // pitch: units from tile to tile of w and x
+    int64_t g_rows_pitch, g_items_pitch;
 };
 
 // logits in base 2 of one 32 x 32 block: lane: row n, register: item
@@ -843,8 +845,8 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(W
     }
     wide_core<Y, Z>(
         lds, g1 - g0, A.CB / Z::KC,
-        [&](int64_t g, int step, int tile) { return A.w + (((g0 + g) * kWideA + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
-        [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
+        [&](int64_t g, int step, int tile) { return A.w + (((g0 + g) * kWideA + tile) * A.pitch + step * Z::KC) * Z::S * kUnit; },
+        [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.pitch + step * Z::KC) * Z::S * kUnit; },
         [&](int64_t g, f32x16 (&acc)[4][2]) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -893,8 +895,8 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
     }
     wide_core<Y, Z>(
         lds, 1, A.CB / Z::KC,
-        [&](int64_t, int step, int tile) { return A.w + ((A.v0 + vg + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
-        [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
+        [&](int64_t, int step, int tile) { return A.w + ((A.v0 + vg + tile) * A.pitch + step * Z::KC) * Z::S * kUnit; },
+        [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.pitch + step * Z::KC) * Z::S * kUnit; },
         [&](int64_t, f32x16 (&acc)[4][2]) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -934,7 +936,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
                     for (int s = 0; s < S; ++s) {
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
-                            *(typename Y::m::v8 *)(A.g_rows + (((nt * A.v_count + vt) * 2 + t) * S + s) * kUnit + lane * 16) = p[t].p[s];
+                            *(typename Y::m::v8 *)(A.g_rows + ((nt * A.g_rows_pitch + vt * 2 + t) * S + s) * kUnit + lane * 16) = p[t].p[s];
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
                             turn[low][row_of(r, h)] = p[r >> 3].p[s][r & 7];
@@ -946,7 +948,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
 #pragma unroll
                             for (int r = 0; r < 8; ++r)
                                 q[r] = turn[16 * t + row_of(r, h)][low];
-                            *(typename Y::m::v8 *)(A.g_items + (((vt * A.n_tiles + nt) * 2 + t) * S + s) * kUnit + lane * 16) = q;
+                            *(typename Y::m::v8 *)(A.g_items + ((vt * A.g_items_pitch + nt * 2 + t) * S + s) * kUnit + lane * 16) = q;
                         }
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                     }
@@ -968,9 +970,9 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
 // c[m][k] = sum over the contraction's tiles of a (by_row units, `a_units` of them a tile) times b (by_col units)
 struct ProductArgs {
     const char *a, *b;
-    int64_t a_tiles, a_units, tiles;      // output tiles, units of one, contraction tiles (32 each)
+    int64_t a_tiles, a_units, tiles;      // output tiles, units from one to the next, contraction tiles (32 each)
     int KO, splits;
-    float *part;                          // [split][32 a_tiles][32 KO] sums; `more`: added to what is there
+    float *part;                          // [split][32 a_tiles][32 KO] sums; `more`: what is there goes in too
     int more;
     void *out;                            // or the results themselves: times scale wpow 2^-shift, `count` rows of K
     const float *wpow;
@@ -979,13 +981,25 @@ struct ProductArgs {
     float scale;
 };
 
-template <class Y> __global__ __launch_bounds__(256, 2) void wide_product_kernel(ProductArgs A)
+// 256 x 256 outputs a workgroup, 128 x 128 a wavefront and one wavefront a SIMD: eight operands for sixteen products, since shared memory
+// bounds smaller tiles.  Stages lie in a ring: while one is multiplied the first operands of the next are read, and the one after
+// that is known to have arrived.
+template <class Y> struct Ring {
+    static constexpr int S = Y::S, KC = S == 1 ? 2 : 1, per = KC * S, tiles = 16;
+    static constexpr int depth = S == 1 ? 4 : 3;               // 128 or 144 KB
+    static constexpr int stage = tiles * per * kUnit;
+    static constexpr int loads = tiles / 4 * per;              // of a wavefront, a stage
+};
+constexpr int kProductA = 8, kProductB = 8;                    // tiles of a workgroup
+
+template <class Y> __global__ __launch_bounds__(256, 1) void wide_product_kernel(ProductArgs A)
 {
-    typedef Wide<Y> Z;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * Z::stage];
+    typedef Ring<Y> Z;
+    constexpr int S = Y::S, KC = Z::KC, per = Z::per;
+    __shared__ __attribute__((aligned(1024))) char lds[Z::depth * Z::stage];
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
-    const unsigned kgroups = (A.KO + kWideB - 1) / kWideB;
+    const unsigned kgroups = (A.KO + kProductB - 1) / kProductB;
     // workgroups whose ids are equal modulo 8 share a die: those of one piece of the contraction, or of one group of rows
     unsigned sp = 0, id = blockIdx.x, kg, mg;
     if (A.splits > 1) {
@@ -997,45 +1011,110 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_product_kernel
         kg = id / 8 % kgroups;
         mg = id % 8 + id / 8 / kgroups * 8;
     }
-    const int64_t m0 = (int64_t)mg * kWideA;
-    const int k0 = (int)kg * kWideB;
+    const int64_t m0 = (int64_t)mg * kProductA;
+    const int k0 = (int)kg * kProductB;
     if (m0 >= A.a_tiles)
         return;
-    const int64_t all = A.tiles * (2 / Z::KC), s0 = all * sp / A.splits, s1 = all * (sp + 1) / A.splits;   // stages of KC units
-    wide_core<Y, Z>(
-        lds, 1, (int)(s1 - s0),
-        [&](int64_t, int step, int tile) { return A.a + ((m0 + tile) * A.a_units + (s0 + step) * Z::KC) * Z::S * kUnit; },
-        [&](int64_t, int step, int tile) {
-            const int64_t u = (s0 + step) * Z::KC;
-            return A.b + (((u >> 1) * A.KO + (k0 + tile < A.KO ? k0 + tile : A.KO - 1)) * 2 + (u & 1)) * Z::S * kUnit;
-        },
-        [&](int64_t, f32x16 (&acc)[4][2]) {
-            const float f = A.out ? A.scale * *A.wpow * __builtin_amdgcn_exp2f(-(float)Y::shift) : 0.0f;
+    const int64_t all = A.tiles * (2 / KC), s0 = all * sp / A.splits, s1 = all * (sp + 1) / A.splits;   // stages of KC units
+    const int steps = (int)(s1 - s0);
+
+    // wavefront w brings tiles w and w + 4 of each matrix
+    const char *const pa = A.a + (m0 + wave) * A.a_units * S * kUnit, *const pc = A.a + (m0 + wave + 4) * A.a_units * S * kUnit;
+    const int kb = k0 + wave < A.KO ? k0 + wave : A.KO - 1, kd = k0 + wave + 4 < A.KO ? k0 + wave + 4 : A.KO - 1;
+    auto stage = [&](int step) {
+        char *const to = lds + step % Z::depth * Z::stage;
+        const int64_t u = (s0 + step) * KC, row = (u >> 1) * A.KO;
+        const char *const b = A.b + ((row + kb) * 2 + (u & 1)) * S * kUnit, *const d = A.b + ((row + kd) * 2 + (u & 1)) * S * kUnit;
+#pragma unroll
+        for (int i = 0; i < per; ++i) {
+            stage_unit(pa + (u * S + i) * kUnit, to + (wave * per + i) * kUnit);
+            stage_unit(pc + (u * S + i) * kUnit, to + ((4 + wave) * per + i) * kUnit);
+            stage_unit(b + i * kUnit, to + ((8 + wave) * per + i) * kUnit);
+            stage_unit(d + i * kUnit, to + ((12 + wave) * per + i) * kUnit);
+        }
+    };
+    struct Operands { Parts<Y> x[4], y[4]; };
+    auto fetch = [&](int step, int c) {
+        const char *const at = lds + step % Z::depth * Z::stage + lane * 16 + c * S * kUnit;
+        Operands o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            for (int s = 0; s < S; ++s) {
+                o.x[i].p[s] = *(const typename Y::m::v8 *)(at + ((4 * wa + i) * per + s) * kUnit);
+                o.y[i].p[s] = *(const typename Y::m::v8 *)(at + ((8 + 4 * wb + i) * per + s) * kUnit);
+            }
+        return o;
+    };
+
+    for (int s = 0; s < Z::depth - 1 && s < steps; ++s)
+        stage(s);
+    // one value of block (i, j): row row_of(r, h), column low
+    auto place = [&](int i, int j, int r) { return A.part + ((sp * A.a_tiles + m0 + 4 * wa + i) * 32 + row_of(r, h)) * (int64_t)(32 * A.KO) + 32 * (k0 + 4 * wb + j) + low; };
+    auto mine = [&](int i, int j) { return m0 + 4 * wa + i < A.a_tiles && k0 + 4 * wb + j < A.KO; };
+    f32x16 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc[i][j] = (f32x16)(0.0f);
+            if (A.more && mine(i, j))          // (all loads ahead of all stores: one by one they would wait for each other)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    acc[i][j][r] = *place(i, j, r);
+        }
+    staged_barrier();
+    Operands now;
+    if (steps > 0)
+        now = fetch(0, 0);
+    for (int step = 0; step < steps; ++step) {
+        // Here stages up to step + 1 have arrived for every wavefront, and all have read step - 1, whose place this one takes.
+        if (step + Z::depth - 1 < steps)
+            stage(step + Z::depth - 1);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const Operands next = c + 1 < KC ? fetch(step, c + 1) : fetch(step + 1 < steps ? step + 1 : step, 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int64_t mt = m0 + 4 * wa + i;
-                    const int ko = k0 + 2 * wb + j, k = 32 * ko + low;
-                    if (mt >= A.a_tiles || ko >= A.KO)
-                        continue;
-                    if (A.out) {
+                for (int j = 0; j < 4; ++j)
+                    acc[i][j] = product<Y>(now.x[i], now.y[j], acc[i][j]);
+            if constexpr (S == 1)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int64_t m = mt * 32 + row_of(r, h);
-                            if (m < A.count && k < A.K)
-                                ((typename Y::t *)A.out)[m * A.ld + k] = (typename Y::t)(acc[i][j][r] * f);
-                        }
-                        continue;
-                    }
-                    float *to = A.part + ((sp * A.a_tiles + mt) * 32) * (int64_t)(32 * A.KO) + k;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float *o = to + row_of(r, h) * (int64_t)(32 * A.KO);
-                        *o = A.more ? *o + acc[i][j][r] : acc[i][j][r];
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
                 }
-        });
+            now = next;
+        }
+        // step + 2 has to be there before the next step reads ahead: all but the latest stage's loads, if one is on its way behind it
+        if (Z::depth == 4 && step + 3 < steps)
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(Z::loads) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+
+    const float f = A.out ? A.scale * *A.wpow * __builtin_amdgcn_exp2f(-(float)Y::shift) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (!mine(i, j))
+                continue;
+            if (A.out) {
+                const int k = 32 * (k0 + 4 * wb + j) + low;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int64_t m = (m0 + 4 * wa + i) * 32 + row_of(r, h);
+                    if (m < A.count && k < A.K)
+                        ((typename Y::t *)A.out)[m * A.ld + k] = (typename Y::t)(acc[i][j][r] * f);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    *place(i, j, r) = acc[i][j][r];
+            }
+        }
 }
 
 // dbias of a chunk: wpow 2^-shift times the sums of its rows' groups
@@ -1641,22 +1720,25 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
 template <class Y> int64_t run_wide(const Call &C)
 {
     typedef typename Y::t T;
-    const int KO = (int)((C.k + 31) / 32 + 1) / 2 * 2, KP = 32 * KO, CB = 2 * KO, kg = (KO + kWideB - 1) / kWideB;
-    const int64_t n_tiles = (C.n + 31) / 32, v_tiles = (C.v + 31) / 32, nt = tiles_padded(n_tiles), vt = tiles_padded(v_tiles), unit = (int64_t)2 * KO * Y::S * kUnit;
-    const int64_t nr = n_tiles * 32, nb = (n_tiles + kWideB - 1) / kWideB, na = nt / kWideA, room = 2 * C.cus;   // workgroups that are resident
-    const int row_splits = wide_splits(nb, vt / kWideA, room);
+    const int KO = (int)((C.k + 31) / 32 + 1) / 2 * 2, KP = 32 * KO, CB = 2 * KO, kg = (KO + kProductB - 1) / kProductB;
+    const int64_t n_tiles = (C.n + 31) / 32, v_tiles = (C.v + 31) / 32, nt = tiles_padded(n_tiles), vt = tiles_padded(v_tiles), unit = (int64_t)2 * KO * Y::S * kUnit, row_unit = (int64_t)(CB + 1) * Y::S * kUnit;
+    const int64_t nr = n_tiles * 32, nb = (n_tiles + kWideB - 1) / kWideB, na = nt / kProductA, room = C.cus;   // the products' workgroups that are resident
+    const int row_splits = wide_splits(nb, vt / kWideA, 2 * room);
     // tiles of items at a time: what kChunkBytes hold, as full rounds of the products' workgroups if that is a round or more
-    const int64_t round = kWideA * ((room + kg - 1) / kg), most = kChunkBytes / (nt * 32 * 32 * 2 * Y::S * 2);
+    const int64_t round = kProductA * ((room + kg - 1) / kg), most = kChunkBytes / (nt * 32 * 32 * 2 * Y::S * 2);
     int64_t chunk = most >= round ? most / round * round : up(most < 1 ? 1 : most, kWideA);
     chunk = chunk > vt ? vt : chunk;
-    const int dx_splits = wide_splits(na * kg, chunk / 4, room), dw_splits = wide_splits(chunk / kWideA * kg, n_tiles / 4, room);
+    const int dx_splits = wide_splits(na * kg, chunk / 4, room);
+    const auto dw_splits_of = [&](int64_t tiles) { return wide_splits((tiles + kProductA - 1) / kProductA * kg, n_tiles / 4, room); };
+    const int64_t last = v_tiles % chunk ? v_tiles % chunk : chunk;
+    const int64_t dw_rows = 32 * (dw_splits_of(chunk) * chunk > dw_splits_of(last) * last ? dw_splits_of(chunk) * chunk : dw_splits_of(last) * last);
     Space S = {C.ws, 0};
     Matrix mw = {C.w, C.ldw, C.v, nullptr, 0, 1.0f, nullptr, nullptr, nullptr, nullptr};
     Matrix mx = {C.x, C.ldx, C.n, C.grad ? C.target : nullptr, C.v, C.scale < 0.0f ? -1.0f : 1.0f, nullptr, nullptr, nullptr, nullptr};
     PrepArgs P = {};
     fill_prepare(P, C, nt * 32, vt * 32);
-    mw.by_row = S.take<char>(vt * unit);
-    mx.by_row = S.take<char>(nt * unit);
+    mw.by_row = S.take<char>(vt * row_unit);
+    mx.by_row = S.take<char>(nt * row_unit);
     P.bias2 = S.take<float>(vt * 32 * 4);
     P.meta = S.take<int32_t>(nt * 32 * 4);
     WideArgs A = {};
@@ -1670,12 +1752,11 @@ template <class Y> int64_t run_wide(const Call &C)
         F.reg_bias = S.take<float>(nt * 32 * 4);
         F.target_log = S.take<float>(nt * 32 * 4);
         P.wpow = S.take<float>(4);
-        if (dw_splits > 1)
-            dw_part = S.take<float>(dw_splits * chunk * 32 * KP * 4);
+        dw_part = S.take<float>(dw_splits_of(chunk) > 1 || dw_splits_of(last) > 1 ? dw_rows * KP * 4 : 4);
         dx_part = S.take<float>(dx_splits * nr * KP * 4);
         A.part_sum = S.take<float>(2 * nb * chunk * 32 * 4);
-        A.g_rows = S.take<char>(nt * chunk * 2 * Y::S * kUnit);
-        A.g_items = S.take<char>(nt * chunk * 2 * Y::S * kUnit);
+        A.g_rows = S.take<char>(nt * (chunk * 2 + 1) * Y::S * kUnit);
+        A.g_items = S.take<char>(chunk * (nt * 2 + 1) * Y::S * kUnit);
     }
     if (!C.ws)
         return S.used;
@@ -1683,8 +1764,8 @@ template <class Y> int64_t run_wide(const Call &C)
         return HPF_EINVAL;
 
     prepare_kernel<<<prepare_blocks(P.np, P.vp), 256, 0, C.st>>>(P);
-    pack_wide_kernel<Y><<<dim3((unsigned)v_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mw, (int)C.k, CB, KO);
-    pack_wide_kernel<Y><<<dim3((unsigned)n_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mx, (int)C.k, CB, KO);
+    pack_wide_kernel<Y><<<dim3((unsigned)v_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mw, (int)C.k, CB, KO, CB + 1);
+    pack_wide_kernel<Y><<<dim3((unsigned)n_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mx, (int)C.k, CB, KO, CB + 1);
     A.w = mw.by_row;
     A.x = mx.by_row;
     A.bias = P.bias2;
@@ -1694,6 +1775,8 @@ template <class Y> int64_t run_wide(const Call &C)
     A.rows = nr;
     A.c = fabsf(C.scale) * kLog2e;
     A.CB = CB;
+    A.pitch = CB + 1;
+    A.g_items_pitch = n_tiles * 2 + 1;
     A.splits = row_splits;
     A.has_bias = C.bias != nullptr;
     wide_stats_kernel<Y><<<(unsigned)(nb * row_splits), 256, 0, C.st>>>(A);
@@ -1712,13 +1795,15 @@ template <class Y> int64_t run_wide(const Call &C)
     for (int64_t v0 = 0; v0 < v_tiles; v0 += chunk) {
         A.v0 = v0;
         A.v_count = v_tiles - v0 < chunk ? v_tiles - v0 : chunk;
+        const int dw_splits = dw_splits_of(A.v_count);
         const int64_t vg = (A.v_count + kWideA - 1) / kWideA, first = v0 * 32, count = C.v - first < A.v_count * 32 ? C.v - first : A.v_count * 32;
+        A.g_rows_pitch = A.v_count * 2 + 1;
         wide_g_kernel<Y><<<(unsigned)(nb * vg), 256, 0, C.st>>>(A);
         ProductArgs D = {};
         D.a = A.g_rows;
         D.b = mw.by_col + v0 * unit;
         D.a_tiles = n_tiles;
-        D.a_units = A.v_count * 2;
+        D.a_units = A.g_rows_pitch;
         D.tiles = A.v_count;
         D.KO = KO;
         D.splits = dx_splits;
@@ -1728,11 +1813,12 @@ template <class Y> int64_t run_wide(const Call &C)
         D.a = A.g_items;
         D.b = mx.by_col;
         D.a_tiles = A.v_count;
-        D.a_units = n_tiles * 2;
+        D.a_units = A.g_items_pitch;
         D.tiles = n_tiles;
         D.splits = dw_splits;
         D.part = dw_part;
         D.more = 0;
+        D.out = nullptr;
         if (dw_splits == 1) {
             D.out = (T *)C.dw + first * C.lddw;
             D.wpow = P.wpow;
