@@ -730,11 +730,13 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
 // Bound by the matrix instructions: 8 N V K operations.  256 x 128 outputs a workgroup, 128 x 64 a wavefront: six operands read from
 // shared memory for eight products (four for four, 64 x 64, keep shared memory as busy as the matrix units).
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int64_t kChunkBytes = 192ll << 20;
+constexpr int64_t kChunkBytes = 512ll << 20;
 
 template <class Y> struct Wide {
-    static constexpr int S = Y::S, KC = S == 1 ? 2 : 1;     // units of the contraction a stage
-    static constexpr int stage = 12 * KC * S * kUnit;       // 8 tiles of one matrix, 4 of the other
+    static constexpr int S = Y::S, KC = S == 1 ? 2 : 1, per = KC * S;   // units of the contraction a stage, of one tile
+    static constexpr int stage = 12 * per * kUnit;          // 8 tiles of one matrix, 4 of the other
+    static constexpr int depth = S == 1 ? 3 : 2;            // stages in a ring: two workgroups a compute unit have 144 KB
+    static constexpr int loads = 3 * per;                   // of a wavefront, a stage
 };
 constexpr int kWideA = 8, kWideB = 4;
 
@@ -743,34 +745,49 @@ constexpr int kWideA = 8, kWideB = 4;
 template <class Y, class Z, class A, class B, class D>
 __device__ __forceinline__ void wide_core(char *lds, int64_t groups, int steps, const A &a, const B &b, const D &done)
 {
-    constexpr int S = Z::S, KC = Z::KC, per = KC * S;
+    constexpr int S = Z::S, KC = Z::KC, per = Z::per;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
-    auto stage = [&](int64_t g, int step, int buf) {
+    int64_t ahead_g = 0;                       // the next stage to bring, and its place in the ring
+    int ahead = 0, to_ring = 0, ring = 0;
+    auto bring = [&]() {
+        if (ahead_g >= groups)
+            return;
         // wavefront w brings tiles w and w + 4 of the first matrix and w of the other
-        const char *pa = a(g, step, wave), *pc = a(g, step, wave + 4), *pb = b(g, step, wave);
+        const char *pa = a(ahead_g, ahead, wave), *pc = a(ahead_g, ahead, wave + 4), *pb = b(ahead_g, ahead, wave);
+        char *const to = lds + to_ring * Z::stage;
 #pragma unroll
         for (int u = 0; u < per; ++u) {
-            stage_unit(pa + u * kUnit, lds + buf * Z::stage + (wave * per + u) * kUnit);
-            stage_unit(pc + u * kUnit, lds + buf * Z::stage + ((4 + wave) * per + u) * kUnit);
-            stage_unit(pb + u * kUnit, lds + buf * Z::stage + ((8 + wave) * per + u) * kUnit);
+            stage_unit(pa + u * kUnit, to + (wave * per + u) * kUnit);
+            stage_unit(pc + u * kUnit, to + ((4 + wave) * per + u) * kUnit);
+            stage_unit(pb + u * kUnit, to + ((8 + wave) * per + u) * kUnit);
+        }
+        to_ring = to_ring + 1 == Z::depth ? 0 : to_ring + 1;
+        if (++ahead == steps) {
+            ahead = 0;
+            ++ahead_g;
         }
     };
     f32x16 acc[4][2];
-    int buf = 0;
-    if (groups > 0 && steps > 0)
-        stage(0, 0, 0);
+    if (steps <= 0)
+        return;
+    for (int i = 0; i < Z::depth - 1; ++i)
+        bring();
     for (int64_t g = 0; g < groups; ++g) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             for (int j = 0; j < 2; ++j)
                 acc[i][j] = (f32x16)(0.0f);
-        for (int step = 0; step < steps; ++step, buf ^= 1) {
-            staged_barrier();                      // this stage has arrived, the other has been read
-            if (step + 1 < steps)
-                stage(g, step + 1, buf ^ 1);
-            else if (g + 1 < groups)   // (groups of one length: steps > 0 here)
-                stage(g + 1, 0, buf ^ 1);
-            const char *at = lds + buf * Z::stage + lane * 16;
+        for (int step = 0; step < steps; ++step) {
+            // This stage has arrived and the one before it has been read.  The stage behind it may be on its way still -- but where
+            // other accesses came between them (a group's end) or none follows, all are waited for.
+            if (Z::depth > 2 && step > 0 && ahead_g < groups)
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Z::loads) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            bring();
+            const char *at = lds + ring * Z::stage + lane * 16;
+            ring = ring + 1 == Z::depth ? 0 : ring + 1;
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
                 Parts<Y> x[4], y[2];
@@ -826,7 +843,7 @@ __device__ __forceinline__ void wide_bias(f32x16 &x, const WideArgs &A, int64_t 
 template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(WideArgs A)
 {
     typedef Wide<Y> Z;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * Z::stage];
+    __shared__ __attribute__((aligned(1024))) char lds[Z::depth * Z::stage];
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
     const int sp = blockIdx.x % A.splits;
@@ -877,11 +894,10 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
     typedef Wide<Y> Z;
     typedef typename Y::m::e e;
     constexpr int S = Y::S;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * Z::stage];
-    __shared__ __attribute__((aligned(16))) e turn_all[4][32][36];      // a block a wavefront, to exchange its lanes and registers
+    __shared__ __attribute__((aligned(1024))) char lds[Z::depth * Z::stage];
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
-    e(*turn)[36] = turn_all[wave];
+    e(*const turn)[36] = (e(*)[36])(lds + wave * 2304);      // a block a wavefront, to exchange its lanes and registers: where the stages were
     const int64_t ngroups = (A.n_tiles + 3) / 4, n0 = blockIdx.x % ngroups * 4, vg = blockIdx.x / ngroups * kWideA;   // vg: within the chunk
     int meta[2];
     float down[2], tg[2];
@@ -898,6 +914,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
         [&](int64_t, int step, int tile) { return A.w + ((A.v0 + vg + tile) * A.pitch + step * Z::KC) * Z::S * kUnit; },
         [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.pitch + step * Z::KC) * Z::S * kUnit; },
         [&](int64_t, f32x16 (&acc)[4][2]) {
+            __syncthreads();                   // the last stage has been read by every wavefront
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int64_t vt = vg + 4 * wa + i, tile = A.v0 + vt;
@@ -1724,10 +1741,10 @@ template <class Y> int64_t run_wide(const Call &C)
     const int64_t n_tiles = (C.n + 31) / 32, v_tiles = (C.v + 31) / 32, nt = tiles_padded(n_tiles), vt = tiles_padded(v_tiles), unit = (int64_t)2 * KO * Y::S * kUnit, row_unit = (int64_t)(CB + 1) * Y::S * kUnit;
     const int64_t nr = n_tiles * 32, nb = (n_tiles + kWideB - 1) / kWideB, na = nt / kProductA, room = C.cus;   // the products' workgroups that are resident
     const int row_splits = wide_splits(nb, vt / kWideA, 2 * room);
-    // tiles of items at a time: what kChunkBytes hold, as full rounds of the products' workgroups if that is a round or more
-    const int64_t round = kProductA * ((room + kg - 1) / kg), most = kChunkBytes / (nt * 32 * 32 * 2 * Y::S * 2);
-    int64_t chunk = most >= round ? most / round * round : up(most < 1 ? 1 : most, kWideA);
-    chunk = chunk > vt ? vt : chunk;
+    // tiles of items at a time: equal chunks of what kChunkBytes hold
+    int64_t most = kChunkBytes / (nt * 32 * 32 * 2 * Y::S * 2) / kWideA * kWideA;
+    most = most < kWideA ? kWideA : most;
+    const int64_t chunks = (v_tiles + most - 1) / most, chunk = up((v_tiles + chunks - 1) / chunks, kWideA);
     const int dx_splits = wide_splits(na * kg, chunk / 4, room);
     const auto dw_splits_of = [&](int64_t tiles) { return wide_splits((tiles + kProductA - 1) / kProductA * kg, n_tiles / 4, room); };
     const int64_t last = v_tiles % chunk ? v_tiles % chunk : chunk;
