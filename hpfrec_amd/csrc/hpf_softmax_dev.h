@@ -1261,9 +1261,10 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
 
 // ---------------------------------------------------------------------------------------------------------------------
 // A few rows (up to 64) without gradients: what serving asks for.  Bound by reading the items once, so nothing is packed: a
-// wavefront takes a tile of 32 items straight from the table, two operands' halves of a row a lane, and splits them as it
-// goes; the rows lie in shared memory as operands.  (Three bfloat16 parts for 32-bit matrices: they need no scale, and the
-// matrix instructions have time to spare.)
+// wavefront reads a tile of 32 items as it lies in the table, 16 bytes a lane and neighbours side by side (reading operands -- 16 bytes
+// of each row -- fetched every line four times), turns it into operands through shared memory of its own, and splits it as it goes;
+// the rows lie in shared memory as operands.  (Three bfloat16 parts for 32-bit matrices: they need no scale, and the matrix
+// instructions have time to spare.)
 // ---------------------------------------------------------------------------------------------------------------------
 struct FewArgs {
     const void *x, *w;
@@ -1271,20 +1272,14 @@ struct FewArgs {
     const float *bias;
     float *stats;                  // [workgroup][3][rows]
     int64_t N, V, ldx, ldw, rows, v_tiles;
-    int K;
+    int K, groups;                 // groups: workgroups
     float c, sign;
 };
 
-constexpr int kFewWaves = 8;
-
-// 8 values as words, from any address that suits their type
+// 8 values as words
 template <class T> struct Raw { uint32_t v[2 * sizeof(T)]; };
-template <class T> __device__ __forceinline__ Raw<T> load8(const T *p)
-{
-    Raw<T> r;
-    __builtin_memcpy(&r, p, sizeof(r));
-    return r;
-}
+typedef uint32_t Chunk __attribute__((ext_vector_type(4)));
+typedef Chunk LooseChunk __attribute__((aligned(2)));     // anywhere in a table
 template <class T> __device__ __forceinline__ void zeros_from(Raw<T> &r, int left)   // `left` of the 8 are values (fewer than none: none)
 {
 #pragma unroll
@@ -1309,48 +1304,73 @@ template <class Y> __device__ __forceinline__ Parts<Y> parts_of(const Raw<typena
 }
 
 // QB: tiles of 32 rows; CB: operands of a row, K / 16 or more
-template <class Y, int QB, int CB> __global__ __launch_bounds__(kFewWaves * 64, 2) void few_kernel(FewArgs A)
+template <class Y, int QB, int CB> struct FewShape {
+    static constexpr int chunks = CB * (int)sizeof(typename Y::t);        // of 16 bytes, a row
+    static constexpr int rows_bytes = QB * CB * Y::S * kUnit, own = chunks * 512;   // the rows' operands; a wavefront's tile
+    static constexpr int waves = rows_bytes + 8 * own <= 152 << 10 ? 8 : 4, bytes = rows_bytes + waves * own;
+};
+
+template <class Y, int QB, int CB> __global__ __launch_bounds__((FewShape<Y, QB, CB>::waves * 64), (FewShape<Y, QB, CB>::waves / 4)) void few_kernel(FewArgs A)
 {
-    constexpr int S = Y::S;
+    typedef FewShape<Y, QB, CB> Z;
+    constexpr int S = Y::S, NC = Z::chunks;
     typedef typename Y::t T;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
-    __shared__ float join[kFewWaves][QB][3][32];
+    __shared__ float join[Z::waves][QB][3][32];
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t step = (int64_t)gridDim.x * kFewWaves, fast = A.V >= 64 ? (A.V - 32) / 32 : 0;
-    Raw<T> next[CB];
-    // A tile's rows are read in whole operands, beyond their own end, where 32 rows or more follow (K > 8 CB or CB is 2: no further than
-    // that); the last one or two tiles go through shared memory, which holds zeros there.
-    auto load = [&](int64_t tile) {
-        const int64_t v = tile * 32 + low;
-        if (tile < fast) {
-            const T *row = (const T *)A.w + v * A.ldw + 8 * h;
+    const int64_t step = (int64_t)gridDim.x * Z::waves, fast = A.V >= 64 ? (A.V - 32) / 32 : 0;
+    char *const own = lds + Z::rows_bytes + wave * Z::own;
+
+    // chunk p = 64 i + lane of a tile: row p / NC, bytes 16 (p % NC) on.  A row's last chunks reach beyond its end: where 32 rows or more
+    // follow (K > 8 CB or CB is 2: no further than that), what is there is read and zeroed later; the last one or two tiles are read
+    // value by value.
+    Chunk next[NC / 2];
+    uint32_t from[NC / 2];                 // bytes from the tile's start
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
-                next[cb] = load8(row + 16 * cb);
+    for (int i = 0; i < NC / 2; ++i)
+        from[i] = (uint32_t)((64 * i + lane) / NC) * (uint32_t)(A.ldw * sizeof(T)) + (64 * i + lane) % NC * 16;
+    auto load = [&](int64_t tile) __attribute__((always_inline)) {
+        const char *const start = (const char *)A.w + tile * 32 * A.ldw * (int64_t)sizeof(T);
+        if (tile < fast) {
+#pragma unroll
+            for (int i = 0; i < NC / 2; ++i)
+                next[i] = *(const LooseChunk *)(start + from[i]);
         } else {
-            T *const copy = (T *)(lds + QB * CB * S * kUnit) + (tile - fast) * 32 * 16 * CB;
-            for (int i = lane; i < 32 * 16 * CB; i += 64) {
-                const int r = i / (16 * CB), k = i % (16 * CB);
-                copy[i] = tile * 32 + r < A.V && k < A.K ? ((const T *)A.w)[(tile * 32 + r) * A.ldw + k] : (T)0.0f;
+#pragma unroll 1
+            for (int i = 0; i < NC / 2; ++i) {      // through shared memory: a register cannot be chosen by i
+                const int r = (64 * i + lane) / NC, k = (64 * i + lane) % NC * (16 / (int)sizeof(T));
+#pragma unroll
+                for (int j = 0; j < (int)(16 / sizeof(T)); ++j)
+                    ((T *)(own + (64 * i + lane) * 16))[j] = tile * 32 + r < A.V && k + j < A.K ? ((const T *)A.w)[(tile * 32 + r) * A.ldw + k + j] : (T)0.0f;
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
-                next[cb] = load8(copy + low * 16 * CB + 16 * cb + 8 * h);
+            for (int i = 0; i < NC / 2; ++i)
+                next[i] = *(const Chunk *)(own + (64 * i + lane) * 16);
         }
     };
-    int64_t tile = (int64_t)blockIdx.x * kFewWaves + wave;
+    // where chunk c of row r lies: rows side by side, each chunk's a place further on (no two of eight neighbours on one bank, written or read)
+    auto place = [&](int c, int r) { return own + c * 512 + ((r + c) & 31) * 16; };
+
+    int64_t tile = (int64_t)blockIdx.x * Z::waves + wave;
     if (tile < A.v_tiles)
         load(tile);
-    for (int u = wave; u < QB * CB; u += kFewWaves) {
+    for (int u = wave; u < QB * CB; u += Z::waves) {
         const int q = u / CB, cb = u % CB;
         const int64_t n = q * 32 + low;
         Parts<Y> p;
+        const T *const row = (const T *)A.x + (n < A.N ? n : 0) * A.ldx + 16 * cb + 8 * h;
+        if (16 * cb + 16 <= A.K) {
+            struct Eight { T v[8]; } r;
+            __builtin_memcpy(&r, row, sizeof(r));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int k = 16 * cb + 8 * h + j;
-            split<Y>(n < A.N && k < A.K ? A.sign * (float)((const T *)A.x)[n * A.ldx + k] : 0.0f, p, j);
+            for (int j = 0; j < 8; ++j)
+                split<Y>(n < A.N ? A.sign * (float)r.v[j] : 0.0f, p, j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                split<Y>(n < A.N && 16 * cb + 8 * h + j < A.K ? A.sign * (float)row[j] : 0.0f, p, j);
         }
         for (int s = 0; s < S; ++s)
             *(typename Y::m::v8 *)(lds + (u * S + s) * kUnit + lane * 16) = p.p[s];
@@ -1368,10 +1388,13 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__(kFewWaves * 64, 
     }
     __syncthreads();
     for (; tile < A.v_tiles; tile += step) {
-        Raw<T> cur[CB];
+        // (one wavefront's own memory: its accesses are served in order)
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
-            cur[cb] = next[cb];
+        for (int i = 0; i < NC / 2; ++i)
+            *(Chunk *)place((64 * i + lane) % NC, (64 * i + lane) / NC) = next[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (tile + step < fast)
+            load(tile + step);
         f32x4 b[4];
         const bool whole = tile < fast;
 #pragma unroll
@@ -1388,17 +1411,23 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__(kFewWaves * 64, 
                 }
             }
         }
-        if (tile + step < A.v_tiles)
-            load(tile + step);
         f32x16 z[QB];
 #pragma unroll
         for (int q = 0; q < QB; ++q)
             z[q] = (f32x16)(0.0f);
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
+            Raw<T> raw;
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+                const Chunk c = *(const Chunk *)place((2 * cb + h) * (int)sizeof(T) / 2 + i, low);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    raw.v[4 * i + j] = c[j];
+            }
             if (16 * cb + 16 > A.K)
-                zeros_from(cur[cb], A.K - 16 * cb - 8 * h);
-            const Parts<Y> a = parts_of<Y>(cur[cb]);
+                zeros_from(raw, A.K - 16 * cb - 8 * h);
+            const Parts<Y> a = parts_of<Y>(raw);
 #pragma unroll
             for (int q = 0; q < QB; ++q) {
                 Parts<Y> y;
@@ -1407,6 +1436,9 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__(kFewWaves * 64, 
                 z[q] = product<Y>(a, y, z[q]);
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (tile + step >= fast && tile + step < A.v_tiles)      // (the slow way goes through `own`: the operands have been read)
+            load(tile + step);
 #pragma unroll
         for (int q = 0; q < QB; ++q) {
             f32x16 &x = z[q];
@@ -1432,11 +1464,11 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__(kFewWaves * 64, 
     if (threadIdx.x < 32 * QB) {
         const int q = threadIdx.x >> 5;
         float m = kNothing, all = 0.0f, hit = -INFINITY;
-        for (int i = 0; i < kFewWaves; ++i) {
+        for (int i = 0; i < Z::waves; ++i) {
             m = fmaxf(m, join[i][q][0][low]);
             hit = larger(hit, join[i][q][2][low]);
         }
-        for (int i = 0; i < kFewWaves; ++i)
+        for (int i = 0; i < Z::waves; ++i)
             all += times_power(join[i][q][1][low], join[i][q][0][low] - m);
         float *to = A.stats + (int64_t)blockIdx.x * 3 * A.rows + threadIdx.x;
         to[0] = m;
@@ -1857,30 +1889,33 @@ template <class Y> int64_t run_wide(const Call &C)
     return (int)hipGetLastError();
 }
 
-// a few rows, no gradients (Y as the products take it: W32 for 32 bits).  A wavefront holds two tiles' rows as they are: 256 registers
-// have room for 2 x 128 values of 32 bits, or 2 x 256 of 16, a row.
-template <class Y> bool is_few(const Call &C) { return !C.grad && C.n <= 64 && C.k <= (Y::S == 1 ? 256 : 128); }
+// a few rows, no gradients (Y as the products take it: W32 for 32 bits), as wide as shared memory has room for them and a tile
+template <class Y> bool is_few(const Call &C) { return !C.grad && C.n <= 64 && C.k <= (Y::S == 1 ? 256 : 128) && C.ldw < (1 << 24); }
 
-template <class Y, int QB, int CB> void launch_few(const FewArgs &A, unsigned grid, hipStream_t st)
+template <class Y, int QB, int CB> void launch_few(FewArgs &A, int cus, hipStream_t st)
 {
-    const int bytes = QB * CB * Y::S * kUnit + 2 * 32 * 16 * CB * (int)sizeof(typename Y::t);   // at most 48 + 32 KB
-    few_kernel<Y, QB, CB><<<grid, kFewWaves * 64, bytes, st>>>(A);
+    typedef FewShape<Y, QB, CB> Z;
+    const int64_t grid = (A.v_tiles + Z::waves - 1) / Z::waves;
+    A.groups = (int)(grid > cus ? cus : grid);
+    if (Z::bytes > 64 << 10)
+        (void)hipFuncSetAttribute((const void *)few_kernel<Y, QB, CB>, hipFuncAttributeMaxDynamicSharedMemorySize, Z::bytes);
+    few_kernel<Y, QB, CB><<<A.groups, Z::waves * 64, Z::bytes, st>>>(A);
 }
-template <class Y, int QB> void launch_few_rows(const FewArgs &A, unsigned grid, hipStream_t st)
+template <class Y, int QB> void launch_few_rows(FewArgs &A, int cus, hipStream_t st)
 {
     if (A.K <= 32)
-        launch_few<Y, QB, 2>(A, grid, st);
+        launch_few<Y, QB, 2>(A, cus, st);
     else if (A.K <= 64)
-        launch_few<Y, QB, 4>(A, grid, st);
+        launch_few<Y, QB, 4>(A, cus, st);
     else if (A.K <= 112)
-        launch_few<Y, QB, 7>(A, grid, st);
+        launch_few<Y, QB, 7>(A, cus, st);
     else if (A.K <= 128)
-        launch_few<Y, QB, 8>(A, grid, st);
+        launch_few<Y, QB, 8>(A, cus, st);
     else if constexpr (Y::S == 1) {
         if (A.K <= 208)
-            launch_few<Y, QB, 13>(A, grid, st);
+            launch_few<Y, QB, 13>(A, cus, st);
         else
-            launch_few<Y, QB, 16>(A, grid, st);
+            launch_few<Y, QB, 16>(A, cus, st);
     }
 }
 
@@ -1890,10 +1925,8 @@ template <class Y> int64_t run_few(const Call &C)
     A.rows = up(C.n, 32);
     A.v_tiles = (C.v + 31) / 32;
     A.K = (int)C.k;
-    int64_t grid = (A.v_tiles + kFewWaves - 1) / kFewWaves;   // two wavefronts a SIMD at most: what its registers have room for
-    grid = grid > C.cus ? C.cus : grid;
     Space S = {C.ws, 0};
-    A.stats = S.take<float>(grid * 3 * A.rows * 4);
+    A.stats = S.take<float>((int64_t)C.cus * 3 * A.rows * 4);
     if (!C.ws)
         return S.used;
     if (C.ws_bytes < S.used)
@@ -1909,14 +1942,14 @@ template <class Y> int64_t run_few(const Call &C)
     A.c = fabsf(C.scale) * kLog2e;
     A.sign = C.scale < 0.0f ? -1.0f : 1.0f;
     if (C.n <= 32)
-        launch_few_rows<Y, 1>(A, (unsigned)grid, C.st);
+        launch_few_rows<Y, 1>(A, C.cus, C.st);
     else
-        launch_few_rows<Y, 2>(A, (unsigned)grid, C.st);
+        launch_few_rows<Y, 2>(A, C.cus, C.st);
     FinishArgs F = {};
     fill_finish(F, C);
     F.stats = A.stats;
     F.rows = A.rows;
-    F.splits = (int)grid;
+    F.splits = A.groups;
     finish_rows_kernel<Y, false><<<(unsigned)(A.rows / 4), 256, 0, C.st>>>(F);
     return (int)hipGetLastError();
 }
