@@ -126,6 +126,11 @@ __device__ __forceinline__ float halves_max(float x)
 }
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 
+// Workgroups of launches that may pass 2^32 threads are numbered over two dimensions: see blocks_of().
+constexpr int kGridX = 1 << 16;
+__device__ __forceinline__ int64_t block_number() { return (int64_t)blockIdx.y * kGridX + blockIdx.x; }
+inline dim3 blocks_of(int64_t n) { return dim3((unsigned)(n < kGridX ? n : kGridX), (unsigned)((n + kGridX - 1) / kGridX)); }
+
 // a word that earlier launches wrote, the same for all lanes
 __device__ __forceinline__ int uniform_word(const int32_t *p) { return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p; }
 
@@ -135,6 +140,9 @@ constexpr int kUnit = 1024;
 // the exponent that brings a largest magnitude into [2^14, 2^15) when it is taken away; 0 for nothing but zeros
 __device__ __forceinline__ int half_exponent(float top) { return top > 0.0f ? (int)(__float_as_uint(top) >> 23) - 127 - 14 : 0; }
 __device__ __forceinline__ float finite_size(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }
+
+// a bias that takes its item out: what remains of it in base 2 is no number above kNothing
+__device__ __forceinline__ bool masks(float bias) { return bias * kLog2e <= kNothing; }
 
 __device__ __forceinline__ float wave_max(float m)
 {
@@ -148,67 +156,69 @@ __device__ __forceinline__ float wave_max(float m)
 // ---------------------------------------------------------------------------------------------------------------------
 struct PrepArgs {
     const int64_t *target;
-    const float *bias, *weight;
+    const float *bias;
     int64_t N, V, np, vp;          // np, vp: padded
     float *bias2;                  // bias in base 2, -inf beyond the catalogue
-    int32_t *meta;                 // targets as 32-bit numbers, kNoTarget where there is none
-    float *wpow;                   // the smallest power of two above every |weight| (1 if there is none): G is held as a share of it
-    uint32_t *col_top;             // largest magnitudes of the columns (bits): zeros before they are looked for
-    int cols;
+    int32_t *meta;                 // targets as 32-bit numbers, kNoTarget where there is none or a masked one
+    uint32_t *zero;                // what later launches take maxima into
+    int zeros;
 };
 
-// block 0: weights and zeros; the others: an item and a row a thread
+// an item and a row a thread
 static __global__ __launch_bounds__(256) void prepare_kernel(PrepArgs A)
 {
-    if (blockIdx.x == 0) {
-        __shared__ float top[4];
-        for (int c = threadIdx.x; c < A.cols; c += 256)
-            A.col_top[c] = 0;
-        if (!A.wpow)
-            return;
-        float m = 0.0f;
-        if (A.weight) {
-            int64_t n = threadIdx.x;
-            for (; n + 768 < A.N; n += 1024)
-                m = fmaxf(fmaxf(m, fmaxf(fabsf(A.weight[n]), fabsf(A.weight[n + 256]))),
-                          fmaxf(fabsf(A.weight[n + 512]), fabsf(A.weight[n + 768])));
-            for (; n < A.N; n += 256)
-                m = fmaxf(m, fabsf(A.weight[n]));
-        }
-        m = wave_max(m);
-        if ((threadIdx.x & 63) == 0)
-            top[threadIdx.x >> 6] = m;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            int e = 0;
-            if (m > 0.0f && m < INFINITY)
-                frexpf(m, &e);                       // m in [2^(e-1), 2^e)
-            A.wpow[0] = ldexpf(1.0f, e > 100 ? 100 : e < -100 ? -100 : e);
-        }
-        return;
-    }
-    const int64_t i = (int64_t)(blockIdx.x - 1) * 256 + threadIdx.x;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < A.zeros)
+        A.zero[i] = 0;
     if (i < A.vp)
         A.bias2[i] = i >= A.V ? -INFINITY : A.bias ? A.bias[i] * kLog2e : 0.0f;
     if (i < A.np) {
         const int64_t t = i < A.N ? A.target[i] : -1;
-        A.meta[i] = t >= 0 && t < A.V ? (int32_t)t : kNoTarget;
+        A.meta[i] = t >= 0 && t < A.V && !(A.bias && masks(A.bias[t])) ? (int32_t)t : kNoTarget;
     }
 }
 
 struct Matrix {
     const void *p;
     int64_t ld, rows;
-    const int64_t *target;         // of x with its gradients: rows without a target count as zeros (whatever they hold must not
-    int64_t items;                 // reach a sum)
     float sign;                    // goes into by_row
+    const float *bias2;            // items with a bias: theirs
+    const int32_t *meta;           // x with its gradients: its targets
+    const float *weight;           //   its weights (NULL: ones), and the largest magnitude among them (bits)
+    uint32_t *weight_top;
     char *by_row, *by_col;
-    int32_t *exps;                 // scaled: of the tiles, and of the columns (as magnitudes' bits)
-    uint32_t *col_top;
+    int32_t *exps;                 // scaled: of the tiles, or with `each` of the rows
+    int each;
+    uint32_t *col_top;             // scaled: of the columns (as magnitudes' bits)
 };
 
-__device__ __forceinline__ bool counts(const Matrix &M, int64_t row) { return row < M.rows && !(M.target && (uint64_t)M.target[row] >= (uint64_t)M.items); }
+// Rows that take no part count as zeros, since whatever they hold must reach no sum and no scale: masked items, and in the gradients
+// rows without a target or with a masked one.
+__device__ __forceinline__ bool takes_part(const Matrix &M, int64_t row)
+{
+    return row < M.rows && !(M.bias2 && M.bias2[row] <= kNothing) && !(M.meta && M.meta[row] == kNoTarget);
+}
+__device__ __forceinline__ uint32_t tile_rows(const Matrix &M, int64_t tile)      // a bit a row
+{
+    return (uint32_t)__ballot(takes_part(M, tile * 32 + (threadIdx.x & 31)));
+}
+
+// by one wavefront for a tile of x
+__device__ __forceinline__ void largest_weight(const Matrix &M, int64_t tile, uint32_t rows)
+{
+    const int low = threadIdx.x & 31;
+    const float top = wave_max(rows >> low & 1 ? M.weight ? fabsf(M.weight[tile * 32 + low]) : 1.0f : 0.0f);
+    if ((threadIdx.x & 63) == 0 && __float_as_uint(top) > __hip_atomic_load(M.weight_top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+        atomicMax(M.weight_top, __float_as_uint(top));
+}
+
+// G is held as a share of the power of two above every |weight| (2^-100 .. 2^100; 1 where there is none or no finite one)
+__device__ __forceinline__ int weight_exponent(const uint32_t *top)
+{
+    const uint32_t bits = *top;
+    const int e = (int)(bits >> 23) - 126;
+    return bits == 0 || bits >= 0x7F800000u ? 0 : e > 100 ? 100 : e < -100 ? -100 : e;
+}
 
 // Largest magnitudes of the columns of both matrices; a wavefront reads whole rows, 8 at a time.  One workgroup of 16 wavefronts a compute
 // unit: each ends in an atomic maximum a column, and those of one column are served one after the other (about 60 ns each).
@@ -227,12 +237,13 @@ static __global__ __launch_bounds__(1024) void columns_kernel(Matrix W, Matrix X
             if (64 * j < K)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const int64_t row = r + i * step < M.rows ? r + i * step : r;      // (a row twice changes no maximum)
+                    const int64_t row = r + i * step < M.rows ? r + i * step : r;
                     x[i][j] = ((const float *)M.p)[row * M.ld + (lane + 64 * j < K ? lane + 64 * j : K - 1)];
                 }
+        const uint64_t rows = __ballot(takes_part(M, r + (lane & 7) * step));
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (!M.target || counts(M, r + i * step < M.rows ? r + i * step : r))
+            if (rows >> i & 1)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (64 * j < K)
@@ -255,30 +266,43 @@ static __global__ __launch_bounds__(1024) void columns_kernel(Matrix W, Matrix X
 // columns 16 cb + 8 (lane / 32) + j).  `by_col`: tile after tile, in it (K / 32) x 2 units (lane: column 32 ko + lane % 32, rows
 // 16 t + 8 (j / 4) + 4 (lane / 32) + j % 4: the order of a product's output registers).  Columns and rows beyond the matrix
 // are zero.  Bound by memory: read once for both forms.
-template <class Y, int KO> __global__ __launch_bounds__(256) void pack_kernel(Matrix W, Matrix X, int K, int CB, int w_tiles)
+template <class Y, int KO> __global__ __launch_bounds__(256) void pack_kernel(Matrix W, Matrix X, int K, int CB, int64_t w_tiles)
 {
     constexpr int KP = 32 * KO;
     __shared__ float tile[32][KP + 1];
-    __shared__ float tops[4];
-    const bool second = (int)blockIdx.x >= w_tiles;
+    __shared__ float tops[32];
+    const int64_t id = block_number();
+    const bool second = id >= w_tiles;
     const Matrix &M = second ? X : W;
-    const int64_t rb = second ? blockIdx.x - w_tiles : blockIdx.x;
+    const int64_t rb = second ? id - w_tiles : id;
+    if (rb * 32 >= M.rows)
+        return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, low = lane & 31, h = lane >> 5;
+    const uint32_t rows = tile_rows(M, rb);
+    if (M.weight_top && wave == 0)
+        largest_weight(M, rb, rows);
     float top = 0.0f;
+#pragma unroll 4
     for (int i = 0; i < 8; ++i) {
         const int r = wave * 8 + i;
-        const int64_t row = rb * 32 + r;
-        const bool in = counts(M, row);
+        const int64_t row = rb * 32 + r < M.rows ? rb * 32 + r : rb * 32;
 #pragma unroll
         for (int j = 0; j < (KP + 63) / 64; ++j) {
             const int c = lane + 64 * j;
-            const float x = in && c < K ? (float)((const typename Y::t *)M.p)[row * M.ld + c] : 0.0f;
+            float x = (float)((const typename Y::t *)M.p)[row * M.ld + (c < K ? c : K - 1)];
+            x = (rows >> r & 1) && c < K ? x : 0.0f;
             if (c < KP)
                 tile[r][c] = x;
             top = fmaxf(top, finite_size(x));
         }
+        if (Y::scaled && M.each) {
+            top = wave_max(top);
+            if (lane == 0)
+                tops[r] = top;
+            top = 0.0f;
+        }
     }
-    if constexpr (Y::scaled) {
+    if (Y::scaled && !M.each) {
         top = wave_max(top);
         if (lane == 0)
             tops[wave] = top;
@@ -286,8 +310,10 @@ template <class Y, int KO> __global__ __launch_bounds__(256) void pack_kernel(Ma
     __syncthreads();
     int e = 0;
     if constexpr (Y::scaled) {
-        e = half_exponent(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-        if (threadIdx.x == 0)
+        e = half_exponent(M.each ? tops[low] : fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+        if (M.each && threadIdx.x < 32)
+            M.exps[rb * 32 + low] = e;
+        else if (!M.each && threadIdx.x == 0)
             M.exps[rb] = e;
     }
     for (int cb = wave; cb < CB; cb += 4) {
@@ -319,11 +345,15 @@ template <class Y> __global__ __launch_bounds__(256) void pack_wide_kernel(Matri
     __shared__ float tile[32][129];
     const int64_t rb = blockIdx.x;
     const int c0 = blockIdx.y * 128;
+    const uint32_t rows = tile_rows(M, rb);
+    if (M.weight_top && blockIdx.y == 0 && threadIdx.x < 64)
+        largest_weight(M, rb, rows);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int at = i * 256 + threadIdx.x, r = at >> 7, c = c0 + (at & 127);
-        const int64_t row = rb * 32 + r;
-        tile[r][at & 127] = c < K && counts(M, row) ? (float)((const typename Y::t *)M.p)[row * M.ld + c] : 0.0f;
+        const int64_t row = rb * 32 + r < M.rows ? rb * 32 + r : rb * 32;
+        const float x = (float)((const typename Y::t *)M.p)[row * M.ld + (c < K ? c : K - 1)];
+        tile[r][at & 127] = (rows >> r & 1) && c < K ? x : 0.0f;
     }
     __syncthreads();
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
@@ -358,8 +388,8 @@ enum { kNll, kRows, kItems };
 struct PassArgs {
     const char *still;              // stationary matrix, by_row
     const char *by_row, *by_col;    // streamed matrix
-    const int32_t *still_exp, *stream_exp;   // scaled: their tiles'
-    const float *reg_bias;          // per streamed row: rows passes: its bias (base 2); items pass: log2(|weight| / wpow) - lse
+    const int32_t *still_exp, *stream_exp;   // scaled: their tiles' (stationary rows without gradients: each row's)
+    const float *reg_bias;          // per streamed row: rows passes: its bias (base 2); items pass: log2(|weight|), less weight_exponent, less lse
     const float *lane_bias;         // items pass: the stationary item's bias
     const int32_t *meta;            // items pass: per streamed row its target and flag; rows passes: per stationary row
     const float *target_log;        // items pass: per streamed row, log2 of |G| at its target
@@ -372,7 +402,7 @@ struct PassArgs {
     void *out;
     float *dbias;
     const uint32_t *col_top;
-    const float *wpow;
+    const uint32_t *weight_top;
     int64_t ld_out, count;
     int K, quads;                   // quads: rows of `out` allow four values at once
     float scale;
@@ -527,7 +557,7 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
             }
         target[q] = MODE != kItems && in ? A.meta[(q0 + q) * 32 + low] : kNoTarget;
         lane_bias[q] = MODE == kItems && in && A.bias ? A.lane_bias[(q0 + q) * 32 + low] : 0.0f;
-        still_exp[q] = Y::scaled && in ? uniform_word(A.still_exp + q0 + q) : 0;
+        still_exp[q] = Y::scaled && in ? MODE == kNll ? A.still_exp[(q0 + q) * 32 + low] : uniform_word(A.still_exp + q0 + q) : 0;
     }
 
     f32x16 acc[QB][MODE == kNll ? 1 : KO];
@@ -604,7 +634,7 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
             for (int q = 0; q < QB; ++q) {
                 f32x16 &x = z[q];
                 float c = Y::scaled ? ldexpf(A.c, stream_exp + still_exp[q]) : A.c;
-                if (biased || c == 0.0f) {
+                if (biased || __any(c == 0.0f)) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const f32x4 b = *(const f32x4 *)(side + (8 * i + 4 * h) * 4);
@@ -681,10 +711,10 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
             break;
         const int64_t row = (q0 + q) * 32 + low;
         if (MODE == kItems && A.out) {             // the whole sum: the gradients themselves
-            const float both = sum[q].s + other_half(sum[q].s), wpow = *A.wpow, e = top[q] - (float)Y::shift;
+            const float both = sum[q].s + other_half(sum[q].s), e = top[q] - (float)Y::shift + (float)weight_exponent(A.weight_top);
             if (row < A.count) {
                 if (A.dbias && h == 0)
-                    A.dbias[row] = times_power(both * wpow, e);
+                    A.dbias[row] = times_power(both, e);
                 typedef typename Y::t T;
                 T *to = (T *)A.out + row * A.ld_out;
                 if constexpr (MODE != kNll)
@@ -697,7 +727,7 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const int ce = Y::scaled && k + j < A.K ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
-                                o.v[j] = (T)times_power(acc[q][ko][4 * i + j] * (A.scale * wpow), e + (float)ce);
+                                o.v[j] = (T)times_power(acc[q][ko][4 * i + j] * A.scale, e + (float)ce);
                             }
                             if (A.quads && k + 4 <= A.K)
                                 *(Quad *)(to + k) = o;
@@ -991,8 +1021,8 @@ struct ProductArgs {
     int KO, splits;
     float *part;                          // [split][32 a_tiles][32 KO] sums; `more`: what is there goes in too
     int more;
-    void *out;                            // or the results themselves: times scale wpow 2^-shift, `count` rows of K
-    const float *wpow;
+    void *out;                            // or the results themselves: times scale 2^(weight_exponent - shift), `count` rows of K
+    const uint32_t *weight_top;
     int64_t count, ld;
     int K;
     float scale;
@@ -1111,7 +1141,7 @@ template <class Y> __global__ __launch_bounds__(256, 1) void wide_product_kernel
             asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     }
 
-    const float f = A.out ? A.scale * *A.wpow * __builtin_amdgcn_exp2f(-(float)Y::shift) : 0.0f;
+    const float f = A.out ? A.scale * __builtin_amdgcn_exp2f((float)(weight_exponent(A.weight_top) - Y::shift)) : 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1134,8 +1164,8 @@ template <class Y> __global__ __launch_bounds__(256, 1) void wide_product_kernel
         }
 }
 
-// dbias of a chunk: wpow 2^-shift times the sums of its rows' groups
-static __global__ __launch_bounds__(256) void wide_sums_kernel(const float *sums, int64_t rows, int groups, const float *wpow, int shift, int64_t count, float *dbias)
+// dbias of a chunk: 2^(weight_exponent - shift) times the sums of its rows' groups
+static __global__ __launch_bounds__(256) void wide_sums_kernel(const float *sums, int64_t rows, int groups, const uint32_t *weight_top, int shift, int64_t count, float *dbias)
 {
     const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (v >= count)
@@ -1144,7 +1174,7 @@ static __global__ __launch_bounds__(256) void wide_sums_kernel(const float *sums
 #pragma unroll 4
     for (int s = 0; s < groups; ++s)
         all += sums[s * rows + v];
-    dbias[v] = ldexpf(all * *wpow, -shift);
+    dbias[v] = ldexpf(all, weight_exponent(weight_top) - shift);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1153,7 +1183,8 @@ static __global__ __launch_bounds__(256) void wide_sums_kernel(const float *sums
 struct FinishArgs {
     const float *stats, *part;
     const int64_t *target;
-    const float *weight, *wpow;
+    const float *bias, *weight;
+    const uint32_t *weight_top;
     const void *w;                 // items, for the target's own row
     const uint32_t *col_top;
     float *loss, *lse, *reg_bias, *target_log;
@@ -1167,7 +1198,7 @@ struct FinishArgs {
 template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows_kernel(FinishArgs A)
 {
     const int lane = threadIdx.x & 63;
-    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t n = block_number() * 4 + (threadIdx.x >> 6);
     if (n >= A.rows)
         return;
     if (n >= A.N) {                // rows that only fill the last tile: no share of any sum
@@ -1206,7 +1237,7 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
         loss = __builtin_nanf("");
         alive = false;
     } else if (t >= 0) {
-        if (!(at > kNothing) && at == at && all == all) {   // a masked target
+        if ((A.bias && masks(A.bias[t])) || (!(at > kNothing) && at == at && all == all)) {   // a masked target
             loss = INFINITY;
             alive = false;
         } else if (own > 0.0f && rest < 0x1p20f * own) {
@@ -1221,7 +1252,7 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
             A.lse[n] = lse2 * kLn2;
     }
     if constexpr (GRAD) {
-        const float weight = alive ? (A.weight ? A.weight[n] : 1.0f) : 0.0f, share = fabsf(weight) / *A.wpow;
+        const float weight = alive ? (A.weight ? A.weight[n] : 1.0f) : 0.0f, share = ldexpf(fabsf(weight), -weight_exponent(A.weight_top));
         if (lane == 0) {
             A.reg_bias[n] = alive ? log2f(share) - lse2 : -INFINITY;
             A.target_log[n] = alive ? log2f(share * (rest / all)) : -INFINITY;
@@ -1411,6 +1442,11 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__((FewShape<Y, QB,
                 }
             }
         }
+        float least = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            least = fminf(least, b[i >> 2][i & 3]);
+        const bool masked = __any(least <= kNothing);
         f32x16 z[QB];
 #pragma unroll
         for (int q = 0; q < QB; ++q)
@@ -1445,6 +1481,10 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__((FewShape<Y, QB,
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 x[i] = fmaf(x[i], A.c, b[i >> 2][i & 3]);
+            if (masked)              // whatever their rows hold
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    x[i] = b[i >> 2][i & 3] <= kNothing ? -INFINITY : x[i];
             take_target(x, 1.0f, (int)tile, h, target[q], at[q]);
             exponentials<Y>(x, 1.0f, top[q], sum[q], [](float) {});
             sum[q].add(sum16(x));
@@ -1477,11 +1517,10 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__((FewShape<Y, QB,
     }
 }
 
-// joins the splits of a product with G: out = scale wpow sum, dbias = wpow sum (four columns a thread)
+// joins the splits of a product with G: out = scale 2^weight_exponent sum, dbias = 2^weight_exponent sum (four columns a thread)
 struct JoinArgs {
     const float *part, *tops;              // tops (the passes' pieces): [split][3][rows] with the sums behind, else NULL
-    const float *wpow;
-    const uint32_t *col_top;
+    const uint32_t *weight_top, *col_top;
     int64_t count, rows, ld;
     int K, KP, splits;
     float scale;
@@ -1492,7 +1531,7 @@ struct JoinArgs {
 template <class Y> __global__ __launch_bounds__(256) void join_kernel(JoinArgs A)
 {
     const int quads = A.KP / 4;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, v = id / quads;
+    const int64_t id = block_number() * 256 + threadIdx.x, v = id / quads;
     const int k = (int)(id - v * quads) * 4;
     if (v >= A.count)
         return;
@@ -1500,6 +1539,7 @@ template <class Y> __global__ __launch_bounds__(256) void join_kernel(JoinArgs A
     if (A.tops)
         for (int s = 0; s < A.splits; ++s)
             top = fmaxf(top, A.tops[3 * s * A.rows + v]);
+    const float e = top - (float)Y::shift + (float)weight_exponent(A.weight_top);
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int s = 0; s < A.splits; ++s) {
@@ -1513,13 +1553,13 @@ template <class Y> __global__ __launch_bounds__(256) void join_kernel(JoinArgs A
     for (int j = 0; j < 4; ++j)
         if (k + j < A.K) {
             const int ce = Y::scaled ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
-            ((typename Y::t *)A.out)[v * A.ld + k + j] = (typename Y::t)times_power(sum[j] * (A.scale * *A.wpow), top - (float)Y::shift + (float)ce);
+            ((typename Y::t *)A.out)[v * A.ld + k + j] = (typename Y::t)times_power(sum[j] * A.scale, e + (float)ce);
         }
     if (A.dbias && k == 0) {
         float all = 0.0f;
         for (int s = 0; s < A.splits; ++s)
             all += times_power(A.tops[(3 * s + 1) * A.rows + v], A.tops[3 * s * A.rows + v] - top);
-        A.dbias[v] = times_power(all * *A.wpow, top - (float)Y::shift);
+        A.dbias[v] = times_power(all, e);
     }
 }
 
@@ -1619,18 +1659,36 @@ inline void fill_prepare(PrepArgs &P, const Call &C, int64_t np, int64_t vp)
 {
     P.target = C.target;
     P.bias = C.bias;
-    P.weight = C.weight;
     P.N = C.n;
     P.V = C.v;
     P.np = np;
     P.vp = vp;
 }
-inline unsigned join_blocks(int64_t rows, int KP) { return (unsigned)((rows * (KP / 4) + 255) / 256); }
-inline unsigned prepare_blocks(int64_t np, int64_t vp) { return (unsigned)((np > vp ? np : vp) + 255) / 256 + 1; }
+inline dim3 join_blocks(int64_t rows, int KP) { return blocks_of((rows * (KP / 4) + 255) / 256); }
+inline unsigned prepare_blocks(const PrepArgs &P)
+{
+    const int64_t most = P.np > P.vp ? P.np : P.vp;
+    return (unsigned)(((most > P.zeros ? most : P.zeros) + 255) / 256);
+}
+
+inline void fill_matrices(Matrix &w, Matrix &x, const Call &C)
+{
+    w.p = C.w;
+    w.ld = C.ldw;
+    w.rows = C.v;
+    w.sign = 1.0f;
+    x.p = C.x;
+    x.ld = C.ldx;
+    x.rows = C.n;
+    x.sign = C.scale < 0.0f ? -1.0f : 1.0f;       // the sign of the scale, so that logits rise with the product
+    x.weight = C.weight;
+    x.each = !C.grad;
+}
 
 inline void fill_finish(FinishArgs &F, const Call &C)
 {
     F.target = C.target;
+    F.bias = C.bias;
     F.weight = C.weight;
     F.w = C.w;
     F.loss = C.loss;
@@ -1654,31 +1712,32 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
     const int row_splits = C.grad ? pass_splits<Y, KO, ODD, kRows>(n_tiles, v_tiles, C.cus) : pass_splits<Y, KO, ODD, kNll>(n_tiles, v_tiles, C.cus);
     const int item_splits = pass_splits<Y, KO, ODD, kItems>(v_tiles, n_tiles, C.cus);
     Space W = {C.ws, 0};
-    Matrix mw = {C.w, C.ldw, C.v, nullptr, 0, 1.0f, nullptr, nullptr, nullptr, nullptr};
-    // (the sign of the scale goes into the packed x, so that logits rise with the product)
-    Matrix mx = {C.x, C.ldx, C.n, C.grad ? C.target : nullptr, C.v, C.scale < 0.0f ? -1.0f : 1.0f, nullptr, nullptr, nullptr, nullptr};
+    Matrix mw = {}, mx = {};
+    fill_matrices(mw, mx, C);
     PrepArgs P = {};
     fill_prepare(P, C, nt * 32, vt * 32);
     mw.by_row = W.take<char>(vt * row_unit);
     mx.by_row = W.take<char>(nt * row_unit);
     P.bias2 = W.take<float>(vt * 32 * 4 + kOneTileMore);
     P.meta = W.take<int32_t>(nt * 32 * 4 + kOneTileMore);
+    mw.bias2 = C.bias ? P.bias2 : nullptr;
+    mx.meta = C.grad ? P.meta : nullptr;
     if (Y::scaled) {
         mw.exps = W.take<int32_t>(vt * 4);
-        mx.exps = W.take<int32_t>(nt * 4);
+        mx.exps = W.take<int32_t>(nt * (C.grad ? 4 : 32 * 4));
     }
     float *const stats = W.take<float>((int64_t)row_splits * 3 * nr * 4), *reg_bias = nullptr, *target_log = nullptr, *item_stats = nullptr, *part = nullptr;
     if (C.grad) {
         mw.by_col = W.take<char>(vt * col_unit);
         mx.by_col = W.take<char>(nt * col_unit);
+        P.zeros = Y::scaled ? 1 + 2 * KP : 1;
+        P.zero = mx.weight_top = W.take<uint32_t>(P.zeros * 4);
         if (Y::scaled) {
-            P.cols = 2 * KP;
-            P.col_top = mw.col_top = W.take<uint32_t>(2 * KP * 4);
+            mw.col_top = P.zero + 1;
             mx.col_top = mw.col_top + KP;
         }
         reg_bias = W.take<float>(nt * 32 * 4 + kOneTileMore);
         target_log = W.take<float>(nt * 32 * 4);
-        P.wpow = W.take<float>(4);
         const int64_t rows_part = row_splits * nr * KP * 4, items_part = item_splits > 1 ? item_splits * vr * KP * 4 : 0;
         part = W.take<float>(rows_part > items_part ? rows_part : items_part);   // (the rows' is read before the items' is written)
         if (item_splits > 1)
@@ -1689,12 +1748,12 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
     if (C.ws_bytes < W.used)
         return HPF_EINVAL;
 
-    prepare_kernel<<<prepare_blocks(P.np, P.vp), 256, 0, C.st>>>(P);
+    prepare_kernel<<<prepare_blocks(P), 256, 0, C.st>>>(P);
     if (Y::scaled && C.grad) {
         const int most = C.cus, wb = (int)(C.v / 128 < 1 ? 1 : C.v / 128 > most ? most : C.v / 128), xb = (int)(C.n / 128 < 1 ? 1 : C.n / 128 > most ? most : C.n / 128);
         columns_kernel<<<wb + xb, 1024, 0, C.st>>>(mw, mx, (int)C.k, wb);
     }
-    pack_kernel<Y, KO><<<(unsigned)(v_tiles + n_tiles), 256, 0, C.st>>>(mw, mx, (int)C.k, CB, (int)v_tiles);
+    pack_kernel<Y, KO><<<blocks_of(v_tiles + n_tiles), 256, 0, C.st>>>(mw, mx, (int)C.k, CB, v_tiles);
 
     PassArgs A = {};
     A.still = mx.by_row;
@@ -1716,7 +1775,7 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
     fill_finish(F, C);
     F.stats = stats;
     F.part = part;
-    F.wpow = P.wpow;
+    F.weight_top = mx.weight_top;
     F.col_top = mw.col_top;
     F.reg_bias = reg_bias;
     F.target_log = target_log;
@@ -1727,11 +1786,11 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
     F.splits = row_splits;
     if (!C.grad) {
         launch_pass<Y, KO, ODD, kNll>(A, row_groups, C.st);
-        finish_rows_kernel<Y, false><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
+        finish_rows_kernel<Y, false><<<blocks_of((nr + 3) / 4), 256, 0, C.st>>>(F);
         return (int)hipGetLastError();
     }
     launch_pass<Y, KO, ODD, kRows>(A, row_groups, C.st);
-    finish_rows_kernel<Y, true><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
+    finish_rows_kernel<Y, true><<<blocks_of((nr + 3) / 4), 256, 0, C.st>>>(F);
 
     A.still = mw.by_row;
     A.by_row = mx.by_row;
@@ -1750,7 +1809,7 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
         A.out = C.dw;
         A.dbias = C.bias ? C.dbias : nullptr;
         A.col_top = mx.col_top;
-        A.wpow = P.wpow;
+        A.weight_top = mx.weight_top;
         A.ld_out = C.lddw;
         A.count = C.v;
         A.K = (int)C.k;
@@ -1759,7 +1818,7 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
     }
     launch_pass<Y, KO, ODD, kItems>(A, item_groups, C.st);
     if (item_splits > 1) {
-        const JoinArgs J = {part, item_stats, P.wpow, mx.col_top, C.v, vr, C.lddw, (int)C.k, KP, item_splits, C.scale, C.dw, C.bias ? C.dbias : nullptr};
+        const JoinArgs J = {part, item_stats, mx.weight_top, mx.col_top, C.v, vr, C.lddw, (int)C.k, KP, item_splits, C.scale, C.dw, C.bias ? C.dbias : nullptr};
         join_kernel<Y><<<join_blocks(C.v, KP), 256, 0, C.st>>>(J);
     }
     return (int)hipGetLastError();
@@ -1782,14 +1841,16 @@ template <class Y> int64_t run_wide(const Call &C)
     const int64_t last = v_tiles % chunk ? v_tiles % chunk : chunk;
     const int64_t dw_rows = 32 * (dw_splits_of(chunk) * chunk > dw_splits_of(last) * last ? dw_splits_of(chunk) * chunk : dw_splits_of(last) * last);
     Space S = {C.ws, 0};
-    Matrix mw = {C.w, C.ldw, C.v, nullptr, 0, 1.0f, nullptr, nullptr, nullptr, nullptr};
-    Matrix mx = {C.x, C.ldx, C.n, C.grad ? C.target : nullptr, C.v, C.scale < 0.0f ? -1.0f : 1.0f, nullptr, nullptr, nullptr, nullptr};
+    Matrix mw = {}, mx = {};
+    fill_matrices(mw, mx, C);
     PrepArgs P = {};
     fill_prepare(P, C, nt * 32, vt * 32);
     mw.by_row = S.take<char>(vt * row_unit);
     mx.by_row = S.take<char>(nt * row_unit);
     P.bias2 = S.take<float>(vt * 32 * 4);
     P.meta = S.take<int32_t>(nt * 32 * 4);
+    mw.bias2 = C.bias ? P.bias2 : nullptr;
+    mx.meta = C.grad ? P.meta : nullptr;
     WideArgs A = {};
     FinishArgs F = {};
     fill_finish(F, C);
@@ -1800,7 +1861,8 @@ template <class Y> int64_t run_wide(const Call &C)
         mx.by_col = S.take<char>(nt * unit);
         F.reg_bias = S.take<float>(nt * 32 * 4);
         F.target_log = S.take<float>(nt * 32 * 4);
-        P.wpow = S.take<float>(4);
+        P.zeros = 1;
+        P.zero = mx.weight_top = S.take<uint32_t>(4);
         dw_part = S.take<float>(dw_splits_of(chunk) > 1 || dw_splits_of(last) > 1 ? dw_rows * KP * 4 : 4);
         dx_part = S.take<float>(dx_splits * nr * KP * 4);
         A.part_sum = S.take<float>(2 * nb * chunk * 32 * 4);
@@ -1812,7 +1874,7 @@ template <class Y> int64_t run_wide(const Call &C)
     if (C.ws_bytes < S.used)
         return HPF_EINVAL;
 
-    prepare_kernel<<<prepare_blocks(P.np, P.vp), 256, 0, C.st>>>(P);
+    prepare_kernel<<<prepare_blocks(P), 256, 0, C.st>>>(P);
     pack_wide_kernel<Y><<<dim3((unsigned)v_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mw, (int)C.k, CB, KO, CB + 1);
     pack_wide_kernel<Y><<<dim3((unsigned)n_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mx, (int)C.k, CB, KO, CB + 1);
     A.w = mw.by_row;
@@ -1830,15 +1892,15 @@ template <class Y> int64_t run_wide(const Call &C)
     A.has_bias = C.bias != nullptr;
     wide_stats_kernel<Y><<<(unsigned)(nb * row_splits), 256, 0, C.st>>>(A);
     F.stats = A.stats;
-    F.wpow = P.wpow;
+    F.weight_top = mx.weight_top;
     F.meta = P.meta;
     F.rows = nr;
     F.splits = 2 * row_splits;
     if (!C.grad) {
-        finish_rows_kernel<Y, false><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
+        finish_rows_kernel<Y, false><<<blocks_of((nr + 3) / 4), 256, 0, C.st>>>(F);
         return (int)hipGetLastError();
     }
-    finish_rows_kernel<Y, true><<<(unsigned)((nr + 3) / 4), 256, 0, C.st>>>(F);
+    finish_rows_kernel<Y, true><<<blocks_of((nr + 3) / 4), 256, 0, C.st>>>(F);
     A.reg_bias = F.reg_bias;
     A.target_log = F.target_log;
     for (int64_t v0 = 0; v0 < v_tiles; v0 += chunk) {
@@ -1870,7 +1932,7 @@ template <class Y> int64_t run_wide(const Call &C)
         D.out = nullptr;
         if (dw_splits == 1) {
             D.out = (T *)C.dw + first * C.lddw;
-            D.wpow = P.wpow;
+            D.weight_top = mx.weight_top;
             D.count = count;
             D.ld = C.lddw;
             D.K = (int)C.k;
@@ -1878,13 +1940,13 @@ template <class Y> int64_t run_wide(const Call &C)
         }
         wide_product_kernel<Y><<<(unsigned)(up(vg, 8) * kg * dw_splits), 256, 0, C.st>>>(D);
         if (dw_splits > 1) {
-            const JoinArgs J = {dw_part, nullptr, P.wpow, nullptr, count, A.v_count * 32, C.lddw, (int)C.k, KP, dw_splits, C.scale, (T *)C.dw + first * C.lddw, nullptr};
+            const JoinArgs J = {dw_part, nullptr, mx.weight_top, nullptr, count, A.v_count * 32, C.lddw, (int)C.k, KP, dw_splits, C.scale, (T *)C.dw + first * C.lddw, nullptr};
             join_kernel<Y><<<join_blocks(count, KP), 256, 0, C.st>>>(J);
         }
         if (C.bias)
-            wide_sums_kernel<<<(unsigned)((count + 255) / 256), 256, 0, C.st>>>(A.part_sum, A.v_count * 32, (int)(2 * nb), P.wpow, Y::shift, count, C.dbias + first);
+            wide_sums_kernel<<<(unsigned)((count + 255) / 256), 256, 0, C.st>>>(A.part_sum, A.v_count * 32, (int)(2 * nb), mx.weight_top, Y::shift, count, C.dbias + first);
     }
-    const JoinArgs J = {dx_part, nullptr, P.wpow, nullptr, C.n, nr, C.lddx, (int)C.k, KP, dx_splits, C.scale, C.dx, nullptr};
+    const JoinArgs J = {dx_part, nullptr, mx.weight_top, nullptr, C.n, nr, C.lddx, (int)C.k, KP, dx_splits, C.scale, C.dx, nullptr};
     join_kernel<Y><<<join_blocks(C.n, KP), 256, 0, C.st>>>(J);
     return (int)hipGetLastError();
 }

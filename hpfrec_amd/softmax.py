@@ -55,6 +55,8 @@ def _inputs(ops, x, items, target, bias, scale):
         raise ValueError("items is empty")
     if max(n, v) >= 2 ** 30 - 32:
         raise ValueError("more than 2^30 - 33 rows")
+    if k >= 2 ** 20:
+        raise ValueError("rows of 2^20 values or more")
     _vector(target, "target", ops, torch.int64, n)
     if bias is not None:
         _vector(bias, "bias", ops, torch.float32, v)
@@ -70,7 +72,8 @@ def softmax_nll(ops, x, items, target, bias=None, scale=1.0):
     x       [n, k] float32, bfloat16 or float16, rows contiguous (a stride between them is allowed: `table[:, :k]`)
     items   [v, k] of the same type
     target  int64 [n]; negative: no target, loss 0.  An id of v or more gives a loss of NaN
-    bias    float32 [v] or None; -inf (or the type's lowest value) takes an item out.  A masked target's loss is +inf"""
+    bias    float32 [v] or None; -inf (or the type's lowest value) takes an item out, whatever its row holds.  A masked target's
+            loss is +inf"""
     n, v, k, ldx, ldi = _inputs(ops, x, items, target, bias, scale)
     loss, lse = (torch.empty(n, dtype=torch.float32, device=x.device) for _ in range(2))
     if n:

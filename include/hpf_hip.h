@@ -734,11 +734,14 @@ int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors, int param_
  * weight (NULL: ones), bias (NULL: none), loss, lse (nll only, may be NULL) and dbias (given exactly when bias is) float32.
  * Sums and statistics are float32; dx and ditems are rounded once, to `type`.  Equal calls give equal results.
  *   - target < 0: loss 0; target >= v: loss NaN.  Neither takes part in the gradients, whatever its x holds.
- *   - A logit of -2^126 ln 2 or less is masked (a bias of -inf, or of the type's lowest value): probability zero.  A row
- *     whose target is masked -- or everything -- has loss +inf and takes no part in the gradients; lse of nothing is -inf.
- *   - NaN and +inf logits give NaN losses and gradients.
+ *   - An item whose bias is below -5.9e37 (-2^126 ln 2; -inf, or the type's lowest value) is masked: probability zero,
+ *     whatever its row holds.  So is a single logit down there.  A row whose target is masked -- or everything -- has loss
+ *     +inf and takes no part in the gradients; lse of nothing is -inf.
+ *   - NaN and +inf logits of other items give NaN losses and gradients; so do weights that are infinite or NaN.
+ *   - float32, k <= 256: values below 2^-17 of the largest of their 32 rows (of 32 consecutive rows of items, or of x in the
+ *     gradients) or of their column are held to 2^-40 of it.  HPF_F16, k > 256: G below 2^-38 of the largest weight is zero.
  * workspace: hpf_hip_softmax_workspace bytes (same sizes, type, grad and cu_count) at a multiple of 256; free again when
- * the call's work is done.  n, v < 2^30 - 32.  cu_count: compute units the launch grids are made for.
+ * the call's work is done.  n, v < 2^30 - 32, k < 2^20.  cu_count: compute units the launch grids are made for.
  */
 int64_t hpf_hip_softmax_workspace(int64_t n, int64_t v, int64_t k, int type, int grad, int cu_count);
 int hpf_hip_softmax_nll(const void *x, int64_t ldx, const void *items, int64_t ld_items, const int64_t *target,

@@ -58,6 +58,7 @@ _REFUSED = [
     (dict(x=torch.ones(4, 0), items=torch.ones(7, 0)), "items is empty"),
     (dict(x=torch.ones(5, 4).t()), "contiguous rows"),
     (dict(x=torch.ones(1, 5).expand(4, 5)), "overlap"),
+    (dict(x=torch.ones(4, 2 ** 20), items=torch.ones(1, 2 ** 20), bias=None), "2\\^20"),
     (dict(target=torch.zeros(4, dtype=torch.int32)), "target"),
     (dict(target=torch.zeros(3, dtype=torch.int64)), "target"),
     (dict(target=torch.zeros(8, dtype=torch.int64)[::2]), "target"),
@@ -367,6 +368,54 @@ def test_nan_and_padding(ops, k, kind):
     assert bool(torch.isnan(loss[live]).all())
     loss, lse = softmax.softmax_nll(ops, **{a: b for a, b in c.items() if a != "weight"})
     assert bool(torch.isnan(loss[live]).all()) and bool(torch.isnan(lse[1:]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [40, 90])
+@pytest.mark.parametrize("k", [50, 300])
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+def test_what_takes_no_part_may_hold_anything(ops, kind, k, n):
+    """Rows and weights without a target, rows with a masked target, masked items: NaN, infinite or as large as the type goes, they
+    change no bit of the rest."""
+    c = _case(n, 300, k, kind, True, seed=30)
+    out = torch.zeros(300, dtype=torch.bool, device="cuda:0")
+    out[::7] = True
+    out[64:96] = True                        # a whole tile
+    c["bias"] = torch.where(out, float("-inf"), c["bias"])
+    c["target"] = torch.where((c["target"] >= 0) & out[c["target"].clamp(min=0)], 2, c["target"])
+    c["target"][3] = 70                      # masked
+    gone = (c["target"] < 0) | (c["target"] == 70)
+    big = torch.finfo(kind).max / 4
+    filled = lambda value, values: dict(c, x=torch.where(gone[:, None], value, c["x"]), items=torch.where(out[:, None], value, c["items"]),  # noqa: E731
+                                        weight=torch.where(gone, values, c["weight"]))
+    nll, grad = _both(ops, filled(0.0, 0.0))
+    assert bool((nll[0][3] == float("inf")).all()) and bool(torch.isfinite(grad[0][~gone]).all())
+    for value in (big, -big, float("inf"), float("nan")):
+        (loss, lse), got = _both(ops, filled(value, 1e38 if abs(value) == big else value))
+        assert torch.equal(loss, nll[0]) and torch.equal(lse[~gone], nll[1][~gone])
+        for a, b in zip(got, grad):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n, v, k", [(2200003, 3, 2), (70001, 40, 1000)])
+def test_launches_of_over_65536_workgroups(ops, n, v, k):
+    """Results of all rows against the same rows in a call of their own."""
+    c = _case(n, v, k, F16, True, seed=31)
+    loss, dx, _, dbias = softmax.softmax_nll_grad(ops, **c)
+    e = _exact(**{a: b[-500:] if a in ("x", "target", "weight") else b for a, b in c.items()})
+    wmax = 2 * float(c["weight"].abs().max())
+    b = _bounds(e, F16, c["bias"], c["scale"], k, wmax)
+    _close((loss[-500:], dx[-500:]), e, b, ("loss", "dx"))
+    g = torch.zeros(v, dtype=torch.float64, device="cuda:0")
+    slack = torch.zeros_like(g)
+    for i in range(0, n, 200000):
+        e = _exact(**{a: b[i:i + 200000] if a in ("x", "target", "weight") else b for a, b in c.items()})
+        b = _bounds(e, F16, c["bias"], c["scale"], k, wmax)
+        g += e["dbias"]
+        slack += b["dbias"] + e["g"].abs().sum(dim=0) * 4 * math.sqrt(n) * U
+        _close((loss[i:i + 200000], dx[i:i + 200000]), e, b, ("loss", "dx"))
+    assert bool(((dbias.double() - g).abs() <= slack).all())
 
 
 @pytest.mark.gpu
