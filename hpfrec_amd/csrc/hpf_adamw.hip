@@ -29,6 +29,7 @@ constexpr int kBlock = 256;              // values per wavefront pass = values p
 constexpr int kAtOnce = 2;               // blocks of a wavefront in flight
 constexpr int kMaxTensors = 40;          // per launch: their descriptors travel in the kernel's arguments
 constexpr int kTicketShift = 40;         // the step counter's upper bits count the workgroups that are done
+constexpr int kMaxGrid = 1 << 22;        // what fits there
 
 struct Tensor {
     void *p;
@@ -401,7 +402,7 @@ extern "C" int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors,
         if (blocks == 0 && !A.advance)
             break;
         const int64_t want = (blocks + 7) / 8;       // four wavefronts of kAtOnce blocks
-        const int grid = (int)(want < 1 ? 1 : want < grid_blocks ? want : grid_blocks);
+        const int most = grid_blocks < kMaxGrid ? grid_blocks : kMaxGrid, grid = (int)(want < 1 ? 1 : want < most ? want : most);
         const hipStream_t st = (hipStream_t)stream;
         const int rc = param_type == HPF_F32    ? launch_g<float>(A, grad_type, state_bits, grid, st)
                        : param_type == HPF_BF16 ? launch_g<__bf16>(A, grad_type, state_bits, grid, st)

@@ -697,7 +697,7 @@ int hpf_hip_p2p_pull_f32(void *region, int kind, uint32_t epoch, int src_rank, i
  * One AdamW step (decoupled weight decay) over a list of tensors, up to 40 of them a launch:
  *   m <- b1 m + (1 - b1) g;  v <- b2 v + (1 - b2) g^2
  *   p <- p (1 - lr weight_decay) - (lr / (1 - b1^t)) m / (sqrt(v) / sqrt(1 - b2^t) + eps),   t = *step + 1
- * `tensors` is read on the HOST during the call; everything it points to is device memory.  step (device, >= 0) becomes t
+ * `tensors` is read on the HOST during the call; everything it points to is device memory.  step (device, 0 .. 2^40 - 2) becomes t
  * at the end of the call if `advance` is set, so a captured call counts its replays; lr_dev (device, may be NULL) replaces
  * lr.  param_type / grad_type: HPF_F32, HPF_BF16 or HPF_F16, alike for all tensors of a call; 16-bit parameters have a
  * float32 master, which is what the step works on (param = master rounded to nearest).
