@@ -421,9 +421,8 @@ __device__ __forceinline__ void staged_barrier()
 template <class Y, int KO, int ODD, int MODE> struct Shape {
     static constexpr int S = Y::S, CB = 2 * KO - ODD;
     static constexpr int row_units = CB * S, col_units = MODE == kNll ? 0 : 2 * KO * S, units = row_units + col_units;   // per tile
-    static constexpr int waves = S == 2 && KO > 4 && MODE != kNll ? 1 : S * KO <= 4 ? 3 : 2;    // per SIMD: 512, 256 or 168 registers
+    static constexpr int waves = S == 2 && KO > 4 && MODE != kNll ? 1 : (S + (MODE == kNll ? 0 : 2)) * KO <= 9 ? 3 : 2;    // per SIMD: 512, 256 or 168 registers
     static constexpr int NW = S * KO >= 7 && waves == 2 ? 8 : 4;              // wavefronts: eight share a tile where it is large
-    static constexpr int QB = S * KO <= 2 ? 2 : 1;                            // stationary tiles of a wavefront
     static constexpr int RT = units <= 4 ? 4 : units <= 12 ? 2 : 1;           // streamed tiles a stage
     static constexpr int side = RT * 64 * 4 * (MODE == kItems ? 2 : 1);       // reg_bias (and meta) of a stage: 64 values a tile, 32 of them its own
     static constexpr int stage = RT * units * kUnit + side;
@@ -532,64 +531,53 @@ template <class Y, int KO, int ODD, int MODE>
 __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, ODD, MODE>::waves)) void pass_kernel(PassArgs A)
 {
     typedef Shape<Y, KO, ODD, MODE> Z;
-    constexpr int S = Z::S, CB = Z::CB, QB = Z::QB, RT = Z::RT, NW = Z::NW;
+    constexpr int S = Z::S, CB = Z::CB, RT = Z::RT, NW = Z::NW;
     __shared__ __attribute__((aligned(1024))) char lds[2][Z::stage];
 
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int sp = blockIdx.x;      // equal splits stream the same tiles: where there are eight, they meet on one die and its cache
-    const int64_t q0 = (((int64_t)blockIdx.z * kGridY + blockIdx.y) * NW + wave) * QB;
-    if (q0 - wave * QB >= A.still_tiles)
+    const int64_t mine = ((int64_t)blockIdx.z * kGridY + blockIdx.y) * NW + wave;     // the stationary tile
+    if (mine - wave >= A.still_tiles)
         return;
-    const int64_t g0 = (int64_t)A.base * sp + (sp < A.more ? sp : A.more), g1 = g0 + A.base + (sp < A.more);
+    const bool in = mine < A.still_tiles;
+    const int g0 = A.base * sp + (sp < A.more ? sp : A.more), g1 = g0 + A.base + (sp < A.more);      // (at most 2^25 tiles)
 
-    Parts<Y> still[QB][CB];
-    int target[QB], still_exp[QB];
-    float lane_bias[QB];
+    Parts<Y> still[CB];
 #pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        const bool in = q0 + q < A.still_tiles;
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
-            for (int s = 0; s < S; ++s) {
-                typename Y::m::v8 z = {};
-                still[q][cb].p[s] = in ? *(const typename Y::m::v8 *)(A.still + (((q0 + q) * CB + cb) * S + s) * kUnit + lane * 16) : z;
-            }
-        target[q] = MODE != kItems && in ? A.meta[(q0 + q) * 32 + low] : kNoTarget;
-        lane_bias[q] = MODE == kItems && in && A.bias ? A.lane_bias[(q0 + q) * 32 + low] : 0.0f;
-        still_exp[q] = Y::scaled && in ? MODE == kNll ? A.still_exp[(q0 + q) * 32 + low] : uniform_word(A.still_exp + q0 + q) : 0;
-    }
+    for (int cb = 0; cb < CB; ++cb)
+        for (int s = 0; s < S; ++s) {
+            typename Y::m::v8 z = {};
+            still[cb].p[s] = in ? *(const typename Y::m::v8 *)(A.still + ((mine * CB + cb) * S + s) * kUnit + lane * 16) : z;
+        }
+    const int target = MODE != kItems && in ? A.meta[mine * 32 + low] : kNoTarget;
+    const float lane_bias = MODE == kItems && in && A.bias ? A.lane_bias[mine * 32 + low] : 0.0f;
+    const int still_exp = Y::scaled && in ? MODE == kNll ? A.still_exp[mine * 32 + low] : uniform_word(A.still_exp + mine) : 0;
 
-    f32x16 acc[QB][MODE == kNll ? 1 : KO];
-    float top[QB], at[QB];
-    Sum sum[QB];
-#pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        top[q] = MODE == kItems && !Y::ranged ? 0.0f : kNothing;
-        sum[q] = {0.0f, 0.0f};
-        at[q] = -INFINITY;
-        if constexpr (MODE != kNll)
-            for (int ko = 0; ko < KO; ++ko)
-                acc[q][ko] = (f32x16)(0.0f);
-    }
+    f32x16 acc[MODE == kNll ? 1 : KO];
+    if constexpr (MODE != kNll)
+        for (int ko = 0; ko < KO; ++ko)
+            acc[ko] = (f32x16)(0.0f);
+    float top = MODE == kItems && !Y::ranged ? 0.0f : kNothing, at = -INFINITY;
+    Sum sum = {0.0f, 0.0f};
 
-    auto stage = [&](int64_t g, int buf) {
-        const char *from = A.by_row + g * RT * Z::row_units * kUnit;
+    auto stage = [&](int g, int buf) {
+        const char *from = A.by_row + (int64_t)g * RT * Z::row_units * kUnit;
 #pragma unroll
         for (int u = 0; u < RT * Z::row_units; u += NW)
             if (u + wave < RT * Z::row_units)
                 stage_unit(from + (u + wave) * kUnit, &lds[buf][(u + wave) * kUnit]);
         if constexpr (MODE != kNll) {
-            from = A.by_col + g * RT * Z::col_units * kUnit;
+            from = A.by_col + (int64_t)g * RT * Z::col_units * kUnit;
 #pragma unroll
             for (int u = 0; u < RT * Z::col_units; u += NW)
                 if (u + wave < RT * Z::col_units)
                     stage_unit(from + (u + wave) * kUnit, &lds[buf][(RT * Z::row_units + u + wave) * kUnit]);
         }
         if (wave < RT) {
-            stage_words(A.reg_bias + (g * RT + wave) * 32, &lds[buf][RT * Z::units * kUnit + wave * 256]);
+            stage_words(A.reg_bias + ((int64_t)g * RT + wave) * 32, &lds[buf][RT * Z::units * kUnit + wave * 256]);
             if constexpr (MODE == kItems)
-                stage_words(A.meta + (g * RT + wave) * 32, &lds[buf][RT * Z::units * kUnit + (RT + wave) * 256]);
+                stage_words(A.meta + ((int64_t)g * RT + wave) * 32, &lds[buf][RT * Z::units * kUnit + (RT + wave) * 256]);
         }
     };
     auto fetch = [&](const char *unit) {
@@ -601,155 +589,136 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
 
     if (g0 < g1)
         stage(g0, 0);
-    for (int64_t g = g0; g < g1; ++g) {
-        const int buf = (int)(g - g0) & 1;
+    for (int g = g0; g < g1; ++g) {
+        const int buf = (g - g0) & 1;
         staged_barrier();                         // this group has arrived, and the other buffer has been read
         if (g + 1 < g1)
             stage(g + 1, buf ^ 1);
 #pragma unroll 1
         for (int rt = 0; rt < RT; ++rt) {
-            const int64_t tile = g * RT + rt;
-            if (tile >= A.stream_tiles)
+            const int tile = (int)g * RT + rt;
+            if (tile >= (int)A.stream_tiles)
                 break;
             const char *rows = &lds[buf][rt * Z::row_units * kUnit], *cols = &lds[buf][(RT * Z::row_units + rt * Z::col_units) * kUnit];
             const char *side = &lds[buf][RT * Z::units * kUnit + rt * 256];
-            const bool biased = MODE == kItems || A.bias || tile == A.stream_tiles - 1;
+            const bool biased = MODE == kItems || A.bias || tile == (int)A.stream_tiles - 1;
             const int stream_exp = Y::scaled ? uniform_word(A.stream_exp + tile) : 0;
 
-            f32x16 z[QB];
+            f32x16 x = (f32x16)(0.0f);
 #pragma unroll
-            for (int q = 0; q < QB; ++q)
-                z[q] = (f32x16)(0.0f);
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
-                const Parts<Y> a = fetch(rows + cb * S * kUnit);
-#pragma unroll
-                for (int q = 0; q < QB; ++q)
-                    z[q] = product<Y>(a, still[q][cb], z[q]);
-            }
-            order_reads<S, QB * (2 * S - 1), CB>();
+            for (int cb = 0; cb < CB; ++cb)
+                x = product<Y>(fetch(rows + cb * S * kUnit), still[cb], x);
+            order_reads<S, 2 * S - 1, CB>();
 
-            Parts<Y> p[QB][2];
+            float c = Y::scaled ? ldexpf(A.c, stream_exp + still_exp) : A.c;
+            if (biased || __any(c == 0.0f)) {
 #pragma unroll
-            for (int q = 0; q < QB; ++q) {
-                f32x16 &x = z[q];
-                float c = Y::scaled ? ldexpf(A.c, stream_exp + still_exp[q]) : A.c;
-                if (biased || __any(c == 0.0f)) {
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 b = *(const f32x4 *)(side + (8 * i + 4 * h) * 4);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 b = *(const f32x4 *)(side + (8 * i + 4 * h) * 4);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            x[4 * i + j] = fmaf(x[4 * i + j], c, b[j]);
-                    }
-                    c = 1.0f;
+                    for (int j = 0; j < 4; ++j)
+                        x[4 * i + j] = fmaf(x[4 * i + j], c, b[j]);
                 }
-                const auto rescale = [&](float f) {
-                    if constexpr (MODE != kNll)
-#pragma unroll
-                        for (int ko = 0; ko < KO; ++ko)
-                            acc[q][ko] *= f;
-                };
-                if constexpr (MODE == kItems) {
-                    if (A.bias)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            x[i] += lane_bias[q];
-                    const int meta = ((const int32_t *)(side + RT * 256))[low];
-                    unsigned flip = 0;             // registers of negative G: negative weights, and targets of positive ones
-                    const bool hit = __any(((meta & ~kNegative) >> 5) == (int)(q0 + q)), negative = __any(meta & kNegative);
-                    if (hit || negative) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int r = row_of(i, h), of = __shfl(meta, r);
-                            const bool mine = (of & ~kNegative) == (int)(q0 + q) * 32 + low;
-                            if (mine)
-                                x[i] = A.target_log[tile * 32 + r];
-                            flip |= (unsigned)(mine != ((of & kNegative) != 0)) << i;
-                        }
-                    }
-                    if constexpr (Y::ranged) {
-                        exponentials<Y>(x, c, top[q], sum[q], rescale);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            x[i] = __builtin_amdgcn_exp2f(x[i]);
-                    }
-                    if (hit || negative)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            x[i] = flip >> i & 1 ? -x[i] : x[i];
-                    if (A.bias)
-                        sum[q].add(sum16(x));
-                } else {
-                    take_target(x, c, (int)tile, h, target[q], at[q]);
-                    exponentials<Y>(x, c, top[q], sum[q], rescale);
-                    sum[q].add(sum16(x));
-                }
+                c = 1.0f;
+            }
+            const auto rescale = [&](float f) {
                 if constexpr (MODE != kNll)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2)
-                        split2<Y>(x[i], x[i + 1], p[q][i >> 3], i & 7);
+                    for (int ko = 0; ko < KO; ++ko)
+                        acc[ko] *= f;
+            };
+            if constexpr (MODE == kItems) {
+                if (A.bias)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        x[i] += lane_bias;
+                const int meta = ((const int32_t *)(side + RT * 256))[low];
+                unsigned flip = 0;             // registers of negative G: negative weights, and targets of positive ones
+                const bool hit = __any(((meta & ~kNegative) >> 5) == (int)mine), negative = __any(meta & kNegative);
+                if (hit || negative) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = row_of(i, h), of = __shfl(meta, r);
+                        const bool own = (of & ~kNegative) == (int)mine * 32 + low;
+                        if (own)
+                            x[i] = A.target_log[(int64_t)tile * 32 + r];
+                        flip |= (unsigned)(own != ((of & kNegative) != 0)) << i;
+                    }
+                }
+                if constexpr (Y::ranged) {
+                    exponentials<Y>(x, c, top, sum, rescale);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        x[i] = __builtin_amdgcn_exp2f(x[i]);
+                }
+                if (hit || negative)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        x[i] = flip >> i & 1 ? -x[i] : x[i];
+                if (A.bias)
+                    sum.add(sum16(x));
+            } else {
+                take_target(x, c, tile, h, target, at);
+                exponentials<Y>(x, c, top, sum, rescale);
+                sum.add(sum16(x));
             }
 
             if constexpr (MODE != kNll) {
+                Parts<Y> p[2];
 #pragma unroll
-                for (int u = 0; u < 2 * KO; ++u) {
-                    const Parts<Y> a = fetch(cols + u * S * kUnit);
+                for (int i = 0; i < 16; i += 2)
+                    split2<Y>(x[i], x[i + 1], p[i >> 3], i & 7);
 #pragma unroll
-                    for (int q = 0; q < QB; ++q)
-                        acc[q][u >> 1] = product<Y>(a, p[q][u & 1], acc[q][u >> 1]);
-                }
-                order_reads<S, QB * (2 * S - 1), 2 * KO>();
+                for (int u = 0; u < 2 * KO; ++u)
+                    acc[u >> 1] = product<Y>(fetch(cols + u * S * kUnit), p[u & 1], acc[u >> 1]);
+                order_reads<S, 2 * S - 1, 2 * KO>();
             }
         }
     }
 
+    if (!in)
+        return;
+    const int64_t row = mine * 32 + low;
+    if (MODE == kItems && A.out) {             // the whole sum: the gradients themselves
+        const float both = sum.s + other_half(sum.s), e = top - (float)Y::shift + (float)weight_exponent(A.weight_top);
+        if (row < A.count) {
+            if (A.dbias && h == 0)
+                A.dbias[row] = times_power(both, e);
+            typedef typename Y::t T;
+            T *to = (T *)A.out + row * A.ld_out;
+            if constexpr (MODE != kNll)
 #pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        if (q0 + q >= A.still_tiles)
-            break;
-        const int64_t row = (q0 + q) * 32 + low;
-        if (MODE == kItems && A.out) {             // the whole sum: the gradients themselves
-            const float both = sum[q].s + other_half(sum[q].s), e = top[q] - (float)Y::shift + (float)weight_exponent(A.weight_top);
-            if (row < A.count) {
-                if (A.dbias && h == 0)
-                    A.dbias[row] = times_power(both, e);
-                typedef typename Y::t T;
-                T *to = (T *)A.out + row * A.ld_out;
-                if constexpr (MODE != kNll)
+                for (int ko = 0; ko < KO; ++ko)
 #pragma unroll
-                    for (int ko = 0; ko < KO; ++ko)
+                    for (int i = 0; i < 4; ++i) {
+                        const int k = 32 * ko + 8 * i + 4 * h;
+                        struct alignas(4 * sizeof(T)) Quad { T v[4]; } o;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int k = 32 * ko + 8 * i + 4 * h;
-                            struct alignas(4 * sizeof(T)) Quad { T v[4]; } o;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int ce = Y::scaled && k + j < A.K ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
-                                o.v[j] = (T)times_power(acc[q][ko][4 * i + j] * A.scale, e + (float)ce);
-                            }
-                            if (A.quads && k + 4 <= A.K)
-                                *(Quad *)(to + k) = o;
-                            else
-                                for (int j = 0; j < 4; ++j)
-                                    if (k + j < A.K)
-                                        to[k + j] = o.v[j];
+                        for (int j = 0; j < 4; ++j) {
+                            const int ce = Y::scaled && k + j < A.K ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
+                            o.v[j] = (T)times_power(acc[ko][4 * i + j] * A.scale, e + (float)ce);
                         }
+                        if (A.quads && k + 4 <= A.K)
+                            *(Quad *)(to + k) = o;
+                        else
+                            for (int j = 0; j < 4; ++j)
+                                if (k + j < A.K)
+                                    to[k + j] = o.v[j];
+                    }
+        }
+        return;
+    }
+    store_stats(A.stats + (int64_t)sp * 3 * A.still_rows + row, A.still_rows, h, top, sum, at);
+    if constexpr (MODE != kNll) {
+        float *to = A.part + (sp * A.still_rows + row) * (32 * KO) + 4 * h;
+#pragma unroll
+        for (int ko = 0; ko < KO; ++ko)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 o = {acc[ko][4 * i], acc[ko][4 * i + 1], acc[ko][4 * i + 2], acc[ko][4 * i + 3]};
+                *(f32x4 *)(to + 32 * ko + 8 * i) = o;
             }
-            continue;
-        }
-        store_stats(A.stats + (int64_t)sp * 3 * A.still_rows + row, A.still_rows, h, top[q], sum[q], at[q]);
-        if constexpr (MODE != kNll) {
-            float *to = A.part + (sp * A.still_rows + row) * (32 * KO) + 4 * h;
-#pragma unroll
-            for (int ko = 0; ko < KO; ++ko)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f32x4 o = {acc[q][ko][4 * i], acc[q][ko][4 * i + 1], acc[q][ko][4 * i + 2], acc[q][ko][4 * i + 3]};
-                    *(f32x4 *)(to + 32 * ko + 8 * i) = o;
-                }
-        }
     }
 }
 
@@ -760,13 +729,11 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
 // Bound by the matrix instructions: 8 N V K operations.  256 x 128 outputs a workgroup, 128 x 64 a wavefront: six operands read from
 // shared memory for eight products (four for four, 64 x 64, keep shared memory as busy as the matrix units).
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int64_t kChunkBytes = 512ll << 20;
+constexpr int64_t kChunkBytes = 1024ll << 20;
 
 template <class Y> struct Wide {
     static constexpr int S = Y::S, KC = S == 1 ? 2 : 1, per = KC * S;   // units of the contraction a stage, of one tile
     static constexpr int stage = 12 * per * kUnit;          // 8 tiles of one matrix, 4 of the other
-    static constexpr int depth = S == 1 ? 3 : 2;            // stages in a ring: two workgroups a compute unit have 144 KB
-    static constexpr int loads = 3 * per;                   // of a wavefront, a stage
 };
 constexpr int kWideA = 8, kWideB = 4;
 
@@ -777,21 +744,19 @@ __device__ __forceinline__ void wide_core(char *lds, int64_t groups, int steps, 
 {
     constexpr int S = Z::S, KC = Z::KC, per = Z::per;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
-    int64_t ahead_g = 0;                       // the next stage to bring, and its place in the ring
-    int ahead = 0, to_ring = 0, ring = 0;
-    auto bring = [&]() {
+    int64_t ahead_g = 0;                       // the next stage to bring
+    int ahead = 0, buf = 0;
+    auto bring = [&](char *to) {
         if (ahead_g >= groups)
             return;
         // wavefront w brings tiles w and w + 4 of the first matrix and w of the other
         const char *pa = a(ahead_g, ahead, wave), *pc = a(ahead_g, ahead, wave + 4), *pb = b(ahead_g, ahead, wave);
-        char *const to = lds + to_ring * Z::stage;
 #pragma unroll
         for (int u = 0; u < per; ++u) {
             stage_unit(pa + u * kUnit, to + (wave * per + u) * kUnit);
             stage_unit(pc + u * kUnit, to + ((4 + wave) * per + u) * kUnit);
             stage_unit(pb + u * kUnit, to + ((8 + wave) * per + u) * kUnit);
         }
-        to_ring = to_ring + 1 == Z::depth ? 0 : to_ring + 1;
         if (++ahead == steps) {
             ahead = 0;
             ++ahead_g;
@@ -800,24 +765,17 @@ __device__ __forceinline__ void wide_core(char *lds, int64_t groups, int steps, 
     f32x16 acc[4][2];
     if (steps <= 0)
         return;
-    for (int i = 0; i < Z::depth - 1; ++i)
-        bring();
+    bring(lds);
     for (int64_t g = 0; g < groups; ++g) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             for (int j = 0; j < 2; ++j)
                 acc[i][j] = (f32x16)(0.0f);
         for (int step = 0; step < steps; ++step) {
-            // This stage has arrived and the one before it has been read.  The stage behind it may be on its way still -- but where
-            // other accesses came between them (a group's end) or none follows, all are waited for.
-            if (Z::depth > 2 && step > 0 && ahead_g < groups)
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Z::loads) : "memory");
-            else
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            bring();
-            const char *at = lds + ring * Z::stage + lane * 16;
-            ring = ring + 1 == Z::depth ? 0 : ring + 1;
+            staged_barrier();                      // this stage has arrived, and the one before it has been read
+            bring(lds + (buf ^ 1) * Z::stage);
+            const char *at = lds + buf * Z::stage + lane * 16;
+            buf ^= 1;
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
                 Parts<Y> x[4], y[2];
@@ -873,7 +831,7 @@ __device__ __forceinline__ void wide_bias(f32x16 &x, const WideArgs &A, int64_t 
 template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(WideArgs A)
 {
     typedef Wide<Y> Z;
-    __shared__ __attribute__((aligned(1024))) char lds[Z::depth * Z::stage];
+    __shared__ __attribute__((aligned(1024))) char lds[2 * Z::stage];
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
     const int sp = blockIdx.x % A.splits;
@@ -924,7 +882,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
     typedef Wide<Y> Z;
     typedef typename Y::m::e e;
     constexpr int S = Y::S;
-    __shared__ __attribute__((aligned(1024))) char lds[Z::depth * Z::stage];
+    __shared__ __attribute__((aligned(1024))) char lds[2 * Z::stage];
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wa = wave >> 1, wb = wave & 1;
     e(*const turn)[36] = (e(*)[36])(lds + wave * 2304);      // a block a wavefront, to exchange its lanes and registers: where the stages were
@@ -1576,14 +1534,22 @@ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 constexpr int kMostSplits = 256;      // a row's pieces are joined by one wavefront
 inline int64_t tiles_padded(int64_t tiles) { return up(tiles, kPadTiles); }
 
-// How many pieces a contraction of so many units is cut into for workgroups that would not fill the chip: up to a full round of them, in
-// eights (one a die) once there are eight.
-inline int wide_splits(int64_t workgroups, int64_t units, int64_t room)
+// How many pieces a contraction of so many units is cut into, for a launch of `workgroups` tiles of which `room` are resident together:
+// by an estimate of its time in microseconds -- rounds of workgroups, each with its start, its units and what it writes of its
+// piece, and the pieces' join.  More than eight come in eights (one a die).
+inline int wide_splits(int64_t workgroups, int64_t units, int64_t room, double unit_us, double start_us, double piece_us)
 {
-    int64_t s = room / workgroups;
-    s = s > units ? units : s;
-    s = s > 8 ? s / 8 * 8 : s;
-    return s < 1 ? 1 : s > kMostSplits / 2 ? kMostSplits / 2 : (int)s;
+    double best = 0.0;
+    int at = 0;
+    for (int s = 1; s <= kMostSplits / 2 && (s == 1 || s <= units); s += s < 8 ? 1 : 8) {
+        const int64_t rounds = (workgroups * s + room - 1) / room;
+        const double us = rounds * (start_us + (double)((units + s - 1) / s) * unit_us) + (s > 1 ? (double)workgroups * s / room * piece_us : 0.0);
+        if (!at || us < best) {
+            best = us;
+            at = s;
+        }
+    }
+    return at;
 }
 
 // For the passes, by an estimate of their time in microseconds: rounds of the workgroups that are resident together, each with
@@ -1592,9 +1558,9 @@ inline int wide_splits(int64_t workgroups, int64_t units, int64_t room)
 template <class Y, int KO, int ODD, int MODE> int pass_splits(int64_t still_tiles, int64_t stream_tiles, int cus)
 {
     typedef Shape<Y, KO, ODD, MODE> Z;
-    const int64_t groups = (still_tiles + Z::NW * Z::QB - 1) / (Z::NW * Z::QB), stages = (stream_tiles + Z::RT - 1) / Z::RT;
+    const int64_t groups = (still_tiles + Z::NW - 1) / Z::NW, stages = (stream_tiles + Z::RT - 1) / Z::RT;
     const double products = (Z::CB + (MODE == kNll ? 0 : 2 * KO)) * (2 * Y::S - 1);
-    const double stage_us = Z::RT * Z::QB * (16 * products + 700) / 2000;              // one wavefront's, with others beside it
+    const double stage_us = Z::RT * (16 * products + 700) / 2000;              // one wavefront's, with others beside it
     const double join_us = MODE == kNll ? 0.0 : 32.0 * still_tiles * 32 * KO * 8 / 4e6;   // a piece written and read again, at 4 TB/s
     const int64_t room = (int64_t)cus * Z::waves * 4 / Z::NW;
     double best = 0.0;
@@ -1643,7 +1609,7 @@ constexpr int64_t kOneTileMore = 64 * 4;    // staging reads 64 words for a tile
 template <class Y, int KO, int ODD, int MODE> int64_t workgroups(int64_t tiles)
 {
     typedef Shape<Y, KO, ODD, MODE> Z;
-    return (tiles + Z::NW * Z::QB - 1) / (Z::NW * Z::QB);
+    return (tiles + Z::NW - 1) / Z::NW;
 }
 
 template <class Y, int KO, int ODD, int MODE> void launch_pass(PassArgs &A, int64_t groups, hipStream_t st)
@@ -1831,13 +1797,17 @@ template <class Y> int64_t run_wide(const Call &C)
     const int KO = (int)((C.k + 31) / 32 + 1) / 2 * 2, KP = 32 * KO, CB = 2 * KO, kg = (KO + kProductB - 1) / kProductB;
     const int64_t n_tiles = (C.n + 31) / 32, v_tiles = (C.v + 31) / 32, nt = tiles_padded(n_tiles), vt = tiles_padded(v_tiles), unit = (int64_t)2 * KO * Y::S * kUnit, row_unit = (int64_t)(CB + 1) * Y::S * kUnit;
     const int64_t nr = n_tiles * 32, nb = (n_tiles + kWideB - 1) / kWideB, na = nt / kProductA, room = C.cus;   // the products' workgroups that are resident
-    const int row_splits = wide_splits(nb, vt / kWideA, 2 * room);
+    const int products = Y::S == 1 ? 1 : 6;
+    // a group's product of 256 x 128 x K on half a compute unit, at two thirds of its rate, and its exponentials
+    const int row_splits = wide_splits(nb, vt / kWideA, 2 * room, 0.024 * (double)KP * products + 4.0, 5.0, 0.0);
     // tiles of items at a time: equal chunks of what kChunkBytes hold
     int64_t most = kChunkBytes / (nt * 32 * 32 * 2 * Y::S * 2) / kWideA * kWideA;
     most = most < kWideA ? kWideA : most;
     const int64_t chunks = (v_tiles + most - 1) / most, chunk = up((v_tiles + chunks - 1) / chunks, kWideA);
-    const int dx_splits = wide_splits(na * kg, chunk / 4, room);
-    const auto dw_splits_of = [&](int64_t tiles) { return wide_splits((tiles + kProductA - 1) / kProductA * kg, n_tiles / 4, room); };
+    // four tiles of a 256 x 256 product; 256 KB of sums written by every compute unit at once, and read again
+    const double unit_us = 3.2 * products, piece_us = 32.0;
+    const int dx_splits = wide_splits(na * kg, chunk / 4, room, unit_us, 5.0, piece_us);
+    const auto dw_splits_of = [&](int64_t tiles) { return wide_splits((tiles + kProductA - 1) / kProductA * kg, n_tiles / 4, room, unit_us, 5.0, piece_us); };
     const int64_t last = v_tiles % chunk ? v_tiles % chunk : chunk;
     const int64_t dw_rows = 32 * (dw_splits_of(chunk) * chunk > dw_splits_of(last) * last ? dw_splits_of(chunk) * chunk : dw_splits_of(last) * last);
     Space S = {C.ws, 0};
