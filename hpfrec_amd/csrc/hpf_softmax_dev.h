@@ -139,6 +139,12 @@ constexpr int kUnit = 1024;
 
 // the exponent that brings a largest magnitude into [2^14, 2^15) when it is taken away; 0 for nothing but zeros
 __device__ __forceinline__ int half_exponent(float top) { return top > 0.0f ? (int)(__float_as_uint(top) >> 23) - 127 - 14 : 0; }
+// of four columns (k a multiple of 4) from their largest magnitudes, which earlier launches wrote
+__device__ __forceinline__ f32x4 column_exponents(const uint32_t *top, int k)
+{
+    const f32x4 t = *(const __attribute__((address_space(4))) f32x4 *)(uintptr_t)(top + k);
+    return (f32x4){(float)half_exponent(t[0]), (float)half_exponent(t[1]), (float)half_exponent(t[2]), (float)half_exponent(t[3])};
+}
 __device__ __forceinline__ float finite_size(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.0f; }
 
 // a bias that takes its item out: what remains of it in base 2 is no number above kNothing
@@ -422,7 +428,7 @@ template <class Y, int KO, int ODD, int MODE> struct Shape {
     static constexpr int S = Y::S, CB = 2 * KO - ODD;
     static constexpr int row_units = CB * S, col_units = MODE == kNll ? 0 : 2 * KO * S, units = row_units + col_units;   // per tile
     static constexpr int waves = S == 2 && KO > 4 && MODE != kNll ? 1 : (S + (MODE == kNll ? 0 : 2)) * KO <= 9 ? 3 : 2;    // per SIMD: 512, 256 or 168 registers
-    static constexpr int NW = S * KO >= 7 && waves == 2 ? 8 : 4;              // wavefronts: eight share a tile where it is large
+    static constexpr int NW = waves == 2 ? 8 : 4;                              // wavefronts of a workgroup
     static constexpr int RT = units <= 4 ? 4 : units <= 12 ? 2 : 1;           // streamed tiles a stage
     static constexpr int side = RT * 64 * 4 * (MODE == kItems ? 2 : 1);       // reg_bias (and meta) of a stage: 64 values a tile, 32 of them its own
     static constexpr int stage = RT * units * kUnit + side;
@@ -477,15 +483,15 @@ __device__ __forceinline__ float sum16(const f32x16 &x)
     return (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]))) + (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
 }
 
-// One block of base-2 logarithms times 1 / c (lane: stationary row, register: streamed row) becomes its exponentials relative to a
-// running maximum, times 2^shift; `rescale(f)` is called where the maximum grew.  c > 0.
-template <class Y, class F> __device__ __forceinline__ void exponentials(f32x16 &x, float c, float &top, Sum &sum, const F &rescale)
+// One block (lane: stationary row, register: streamed row) whose logarithms in base 2 are c x + more becomes its exponentials relative
+// to a running maximum, times 2^shift; `rescale(f)` is called where the maximum grew.  c > 0.
+template <class Y, class F> __device__ __forceinline__ void exponentials(f32x16 &x, float c, float more, float &top, Sum &sum, const F &rescale)
 {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i)
         m = fmaxf(m, x[i]);
-    m = halves_max(m) * c;
+    m = fmaf(halves_max(m), c, more);
     if (__any(m > top)) {
         const float grown = m > top ? ceilf(m) : top, f = __builtin_amdgcn_exp2f(top - grown);
         sum.s *= f;
@@ -493,7 +499,7 @@ template <class Y, class F> __device__ __forceinline__ void exponentials(f32x16 
         top = grown;
         rescale(f);
     }
-    const float down = (float)Y::shift - top;
+    const float down = ((float)Y::shift - top) + more;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
         x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, down));
@@ -628,10 +634,6 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
                         acc[ko] *= f;
             };
             if constexpr (MODE == kItems) {
-                if (A.bias)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        x[i] += lane_bias;
                 const int meta = ((const int32_t *)(side + RT * 256))[low];
                 unsigned flip = 0;             // registers of negative G: negative weights, and targets of positive ones
                 const bool hit = __any(((meta & ~kNegative) >> 5) == (int)mine), negative = __any(meta & kNegative);
@@ -641,16 +643,16 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
                         const int r = row_of(i, h), of = __shfl(meta, r);
                         const bool own = (of & ~kNegative) == (int)mine * 32 + low;
                         if (own)
-                            x[i] = A.target_log[(int64_t)tile * 32 + r];
+                            x[i] = A.target_log[(int64_t)tile * 32 + r] - lane_bias;
                         flip |= (unsigned)(own != ((of & kNegative) != 0)) << i;
                     }
                 }
                 if constexpr (Y::ranged) {
-                    exponentials<Y>(x, c, top, sum, rescale);
+                    exponentials<Y>(x, c, lane_bias, top, sum, rescale);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        x[i] = __builtin_amdgcn_exp2f(x[i]);
+                        x[i] = __builtin_amdgcn_exp2f(x[i] + lane_bias);
                 }
                 if (hit || negative)
 #pragma unroll
@@ -660,7 +662,7 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
                     sum.add(sum16(x));
             } else {
                 take_target(x, c, tile, h, target, at);
-                exponentials<Y>(x, c, top, sum, rescale);
+                exponentials<Y>(x, c, 0.0f, top, sum, rescale);
                 sum.add(sum16(x));
             }
 
@@ -694,11 +696,10 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
                     for (int i = 0; i < 4; ++i) {
                         const int k = 32 * ko + 8 * i + 4 * h;
                         struct alignas(4 * sizeof(T)) Quad { T v[4]; } o;
+                        const f32x4 ce = Y::scaled ? column_exponents(A.col_top, k) : (f32x4)(0.0f);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int ce = Y::scaled && k + j < A.K ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
-                            o.v[j] = (T)times_power(acc[ko][4 * i + j] * A.scale, e + (float)ce);
-                        }
+                        for (int j = 0; j < 4; ++j)
+                            o.v[j] = (T)times_power(acc[ko][4 * i + j] * A.scale, e + ce[j]);
                         if (A.quads && k + 4 <= A.K)
                             *(Quad *)(to + k) = o;
                         else
@@ -863,7 +864,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(W
                     f32x16 &x = acc[i][j];
                     wide_bias(x, A, tile, h);
                     take_target(x, 1.0f, (int)tile, h, target[j], at[j]);
-                    exponentials<Y>(x, 1.0f, top[j], sum[j], [](float) {});
+                    exponentials<Y>(x, 1.0f, 0.0f, top[j], sum[j], [](float) {});
                     sum[j].add(sum16(x));
                 }
             }
@@ -1237,12 +1238,12 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 sum[j] += __shfl_xor(sum[j], d);
+        const f32x4 ce = Y::scaled && k < A.KP ? column_exponents(A.col_top, k) : (f32x4)(0.0f);
         if (lane < span)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (k + j < A.K) {
-                    const int ce = Y::scaled ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
-                    const float v = times_power(sum[j], top - peak - (float)Y::shift + (float)ce);
+                    const float v = times_power(sum[j], top - peak - (float)Y::shift + ce[j]);
                     dx[k + j] = (T)(alive ? A.scale * weight * (v / all - rest / all * (float)w[k + j]) : 0.0f);
                 }
     }
@@ -1444,7 +1445,7 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__((FewShape<Y, QB,
                 for (int i = 0; i < 16; ++i)
                     x[i] = b[i >> 2][i & 3] <= kNothing ? -INFINITY : x[i];
             take_target(x, 1.0f, (int)tile, h, target[q], at[q]);
-            exponentials<Y>(x, 1.0f, top[q], sum[q], [](float) {});
+            exponentials<Y>(x, 1.0f, 0.0f, top[q], sum[q], [](float) {});
             sum[q].add(sum16(x));
         }
     }
@@ -1507,12 +1508,11 @@ template <class Y> __global__ __launch_bounds__(256) void join_kernel(JoinArgs A
         for (int j = 0; j < 4; ++j)
             sum[j] += times_power(p[j], down);
     }
+    const f32x4 ce = Y::scaled ? column_exponents(A.col_top, k) : (f32x4)(0.0f);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (k + j < A.K) {
-            const int ce = Y::scaled ? half_exponent(__uint_as_float(A.col_top[k + j])) : 0;
-            ((typename Y::t *)A.out)[v * A.ld + k + j] = (typename Y::t)times_power(sum[j] * A.scale, e + (float)ce);
-        }
+        if (k + j < A.K)
+            ((typename Y::t *)A.out)[v * A.ld + k + j] = (typename Y::t)times_power(sum[j] * A.scale, e + ce[j]);
     if (A.dbias && k == 0) {
         float all = 0.0f;
         for (int s = 0; s < A.splits; ++s)
@@ -1697,10 +1697,11 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
         mw.by_col = W.take<char>(vt * col_unit);
         mx.by_col = W.take<char>(nt * col_unit);
         P.zeros = Y::scaled ? 1 + 2 * KP : 1;
-        P.zero = mx.weight_top = W.take<uint32_t>(P.zeros * 4);
+        P.zero = W.take<uint32_t>(P.zeros * 4);
+        mx.weight_top = P.zero + P.zeros - 1;
         if (Y::scaled) {
-            mw.col_top = P.zero + 1;
-            mx.col_top = mw.col_top + KP;
+            mw.col_top = P.zero;
+            mx.col_top = P.zero + KP;
         }
         reg_bias = W.take<float>(nt * 32 * 4 + kOneTileMore);
         target_log = W.take<float>(nt * 32 * 4);
