@@ -6,23 +6,32 @@
 //
 // Every product is a matrix instruction (32 x 32 x 16); a row's statistics are kept in base 2 (z log2(e)).
 //
-// PASSES.  A wavefront keeps 32 (or 64) rows of one matrix in registers -- the STATIONARY rows -- and the other matrix streams
-// by in tiles of 32 rows through shared memory, four wavefronts reading each.  A tile's logits come out with the stationary
-// row in the lane and the streamed row in the register, so that what belongs to a stationary row is a lane's own.
+// THREE FORMS, chosen by sizes and types alone (times: 4,096 rows with gradients, 50k items, or what is said):
+//   few rows     loss alone, up to 64 rows (they fit shared memory as operands) of up to 256 values, 128 in 32 bits: items read once,
+//                unpacked.  64 rows, 100k items: of 100 in bf16 24.8 us against 39.9 by the passes, in 32 bits 44.8 : 55.2, of
+//                256 in bf16 49.3 : 64.1; one row, 27k items of 50 in 32 bits 21.0 : 27.8
+//   passes       rows of up to 256 values, which a wavefront's registers hold: of 60 in bf16 212 us against 762 by wide products,
+//                of 256 495 : 1,013; of 50 in 32 bits 391 : 1,970, of 200 1,370 : 2,840; 100 rows, 1k items: 46 : 115
+//   wide         wider ones
+//
+// PASSES.  A wavefront keeps 32 rows of one matrix in registers -- the STATIONARY rows -- and the other matrix streams by in tiles of
+// 32 rows through shared memory, four or eight wavefronts reading each.  A tile's logits come out with the stationary row in the
+// lane and the streamed row in the register, so that what belongs to a stationary row is a lane's own.
 //   rows pass:   x stationary, w streamed: running maximum and sum of a softmax, and the sum of exp(z - max) w over the tiles
 //                -- dx before its normalisation -- in the same pass, rescaled when a maximum grows
 //   items pass:  w stationary, x streamed: G from the finished lse, and its product with x, held relative to the item's largest
-// so the logits are computed twice and nothing of their size is written.  An output register's row (8 (i / 4) + 4 (lane / 32) +
-// i % 4) is not an operand's (8 (lane / 32) + j), but a contraction may take its terms in any order: the second product's
-// other operand is laid out in the order in which the first product's output lies in the registers, and the probabilities
-// never leave the lane that made them.
+// so the logits are computed twice and nothing of their size is written: 8 N V K operations with gradients, 2 N V K without.  An
+// output register's row (8 (i / 4) + 4 (lane / 32) + i % 4) is not an operand's (8 (lane / 32) + j), but a contraction may take its
+// terms in any order: the second product's other operand is laid out in the order in which the first product's output lies in
+// the registers, and the probabilities never leave the lane that made them.
 //
 // 32-BIT MATRICES are split into two half-precision parts (11 + 11 bits of mantissa and the second's sign: a value is held to
 // 2^-23) and multiplied in three products; the fourth, low times low, is below 2^-22 of |a| |b| and of either sign.  For
 // half's range they are scaled by powers of two: 32 rows share one where rows are multiplied with rows (the largest becomes
-// 2^14 .. 2^15), all rows of a column one where the sum is over rows; what is below 2^-17 of the largest is held to 2^-40 of
-// it.  Probabilities are held times 2^14 relative to a running maximum of their row (or item).  bfloat16 and half matrices
-// take one product; their probabilities are rounded to the same type, everything else stays in 32 bits.
+// 2^14 .. 2^15; rows of x without gradients have one each), all rows of a column one where the sum is over rows; what is below
+// 2^-17 of the largest is held to 2^-40 of it.  Probabilities are held times 2^14 relative to a running maximum of their row (or
+// item).  bfloat16 and half matrices take one product; their probabilities are rounded to the same type -- up to 2^-8 or 2^-11
+// of a term, of either sign, which is what the matrices' own rounding did to theirs -- and everything else stays in 32 bits.
 //
 // A running maximum is rounded up to a whole number: rescaling by a power of two changes no digit.
 //
@@ -170,7 +179,7 @@ struct PrepArgs {
     int zeros;
 };
 
-// an item and a row a thread
+// An item and a row a thread; a launch's latency (2 us at 1,000 items, 5 at 380k).
 static __global__ __launch_bounds__(256) void prepare_kernel(PrepArgs A)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -226,8 +235,9 @@ __device__ __forceinline__ int weight_exponent(const uint32_t *top)
     return bits == 0 || bits >= 0x7F800000u ? 0 : e > 100 ? 100 : e < -100 ? -100 : e;
 }
 
-// Largest magnitudes of the columns of both matrices; a wavefront reads whole rows, 8 at a time.  One workgroup of 16 wavefronts a compute
-// unit: each ends in an atomic maximum a column, and those of one column are served one after the other (about 60 ns each).
+// Largest magnitudes of the columns of both matrices; a wavefront reads whole rows, 8 at a time.  One workgroup of 16 wavefronts a
+// compute unit: each ends in an atomic maximum a column (in no order that matters), and those of one column are served one after the
+// other.  Bound by memory: 388k rows of 100 in 54 us, 2.9 TB/s; 31k of 50 in 7.7, which is latency.
 static __global__ __launch_bounds__(1024) void columns_kernel(Matrix W, Matrix X, int K, int w_blocks)
 {
     __shared__ float top[16][256];
@@ -271,7 +281,8 @@ static __global__ __launch_bounds__(1024) void columns_kernel(Matrix W, Matrix X
 // packing: rows -> units, one workgroup 32 rows.  `by_row`: tile of 32 rows after tile, in it K / 16 units (lane: row lane % 32,
 // columns 16 cb + 8 (lane / 32) + j).  `by_col`: tile after tile, in it (K / 32) x 2 units (lane: column 32 ko + lane % 32, rows
 // 16 t + 8 (j / 4) + 4 (lane / 32) + j % 4: the order of a product's output registers).  Columns and rows beyond the matrix
-// are zero.  Bound by memory: read once for both forms.
+// are zero.  Bound by memory, read once for both forms: 388k rows of 100 in 32 bits, 155 MB in and 400 MB out, in 126 us, 4.4 TB/s;
+// 108k of 200 in bf16 36 us.
 template <class Y, int KO> __global__ __launch_bounds__(256) void pack_kernel(Matrix W, Matrix X, int K, int CB, int64_t w_tiles)
 {
     constexpr int KP = 32 * KO;
@@ -344,9 +355,9 @@ template <class Y, int KO> __global__ __launch_bounds__(256) void pack_kernel(Ma
     }
 }
 
-// The same for rows of any width, without scales: 32 rows x 128 columns a workgroup.  `pitch` units from tile to tile, an odd number: the
-// tiles that a product reads side by side would else lie a power of two apart, on the same channels of the caches.
-template <class Y> __global__ __launch_bounds__(256) void pack_wide_kernel(Matrix M, int K, int CB, int KO, int pitch)
+// The same for rows of any width, without scales: 32 rows x 128 columns a workgroup.
+// Bound by memory, short of it where rows do not begin on 16 bytes: 50,001 rows of 1000 in half precision in 105 us, 2.9 TB/s.
+template <class Y> __global__ __launch_bounds__(256) void pack_wide_kernel(Matrix M, int K, int CB, int KO)
 {
     __shared__ float tile[32][129];
     const int64_t rb = blockIdx.x;
@@ -372,7 +383,7 @@ template <class Y> __global__ __launch_bounds__(256) void pack_wide_kernel(Matri
             for (int j = 0; j < 8; ++j)
                 split<Y>(M.sign * tile[low][16 * u + 8 * h + j], q, j);
             for (int s = 0; s < Y::S; ++s)
-                *(typename Y::m::v8 *)(M.by_row + (((rb * pitch + cb) * Y::S + s) * 64 + lane) * 16) = q.p[s];
+                *(typename Y::m::v8 *)(M.by_row + (((rb * CB + cb) * Y::S + s) * 64 + lane) * 16) = q.p[s];
         }
         const int ko = blockIdx.y * 4 + (u >> 1), t = u & 1;
         if (M.by_col && ko < KO) {
@@ -423,12 +434,20 @@ __device__ __forceinline__ void staged_barrier()
     __syncthreads();
 }
 
-// KO: K / 32 rounded up; ODD: the last 16 of these columns are beyond K, and the products over columns leave them out
+// KO: K / 32 rounded up; ODD: the last 16 of these columns are beyond K, and the products with rows leave them out.
+// (Times: 4,096 rows x 50k items with gradients, or 8,192 x 100k without.)
+//   waves  a SIMD holds as many as registers allow (512, 256 or 168 each) beside the stationary rows and the sums: without gradients,
+//          of 50 in 32 bits, three 392 us, two 430; with them three 402, two 422; of 128 in bf16 three 331, two 313; of 256 in bf16
+//          two 523, one 737
+//   NW     where two share a SIMD a workgroup has all eight of a compute unit, which read each tile once: of 100 in 32 bits 586 us,
+//          four 632; of 160 in bf16 339 : 351; where three do, it is three workgroups that overlap their barriers
+//   RT     short stages cost a barrier each, long ones room: of 30 in bf16 four tiles 179 us, one 184; of 50 in 32 bits one tile 402
+//          us, two 449
 template <class Y, int KO, int ODD, int MODE> struct Shape {
     static constexpr int S = Y::S, CB = 2 * KO - ODD;
     static constexpr int row_units = CB * S, col_units = MODE == kNll ? 0 : 2 * KO * S, units = row_units + col_units;   // per tile
-    static constexpr int waves = S == 2 && KO > 4 && MODE != kNll ? 1 : (S + (MODE == kNll ? 0 : 2)) * KO <= 9 ? 3 : 2;    // per SIMD: 512, 256 or 168 registers
-    static constexpr int NW = waves == 2 ? 8 : 4;                              // wavefronts of a workgroup
+    static constexpr int waves = S == 2 && KO > 4 && MODE != kNll ? 1 : (S + (MODE == kNll ? 0 : 2)) * KO <= 9 ? 3 : 2;   // a SIMD
+    static constexpr int NW = waves == 2 ? 8 : 4;                             // wavefronts of a workgroup
     static constexpr int RT = units <= 4 ? 4 : units <= 12 ? 2 : 1;           // streamed tiles a stage
     static constexpr int side = RT * 64 * 4 * (MODE == kItems ? 2 : 1);       // reg_bias (and meta) of a stage: 64 values a tile, 32 of them its own
     static constexpr int stage = RT * units * kUnit + side;
@@ -533,6 +552,11 @@ __device__ __forceinline__ void store_stats(float *to, int64_t rows, int h, floa
 // x 2^e for whole numbers held as floats (very low ones: a maximum of nothing)
 __device__ __forceinline__ float times_power(float x, float e) { return ldexpf(x, (int)fmaxf(e, -1000.0f)); }
 
+// Bound by the matrix instructions where rows are wide and by the exponentials where they are narrow: a logit costs a wavefront's lane
+// about ten vector instructions and an exponential, and the two kinds of instruction were seen to take turns rather than to overlap
+// (raised priorities changed nothing).  8,192 x 380k of 100 in 32 bits: rows 3.40 ms, items 3.57 ms, 1.10 and 1.05 PFLOP/s of
+// half-precision products, while one of 8192 x 8192 x 8192 of the library runs at 1.16; loss alone, of 50: 1.25 ms.  8,192 x 100k of
+// 200 in bf16: 0.70 and 0.85 ms, 0.93 and 0.77 PFLOP/s.
 template <class Y, int KO, int ODD, int MODE>
 __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, ODD, MODE>::waves)) void pass_kernel(PassArgs A)
 {
@@ -727,8 +751,12 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
 // Rows too wide for a wavefront's registers (k > 256): plain tiled products of packed matrices, the catalogue in chunks.  The
 // statistics come from a first run over all logits; then, chunk by chunk, G is written in both operand layouts (16-bit parts,
 // a chunk at a time: at most kChunkBytes) and multiplied with the items (dx, summed over the chunks) and with x (dw).
-// Bound by the matrix instructions: 8 N V K operations.  256 x 128 outputs a workgroup, 128 x 64 a wavefront: six operands read from
-// shared memory for eight products (four for four, 64 x 64, keep shared memory as busy as the matrix units).
+// Bound by the matrix instructions: 8 N V K operations.  Logits are made in 256 x 128 outputs a workgroup and 128 x 64 a wavefront,
+// two workgroups a compute unit: six operands read from shared memory for eight products (four for four, 64 x 64, keep shared
+// memory as busy as the matrix units).  2,048 x 50,001 of 1000 in half precision: statistics 251 us, G 255 us (0.82 and 0.80
+// PFLOP/s; a third stage on its way cost 5 per cent), each product with G about 240 us (0.85).
+//   kChunkBytes  more is fewer launches and fuller last rounds, and memory: 4,096 x 50k of 600 in bf16 with 1 GB 1,572 us, with 512 MB
+//                1,743, with 2 GB 1,575
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int64_t kChunkBytes = 1024ll << 20;
 
@@ -807,8 +835,7 @@ struct WideArgs {
     char *g_rows, *g_items;         // G of a chunk: rows n / contraction v, and rows v / contraction n
     int64_t n_tiles, v_tiles, rows, v0, v_count;   // tiles; v0, v_count: the chunk
     float c;
-    int CB, pitch, splits, has_bias;   // pitch: units from tile to tile of w and x
-    int64_t g_rows_pitch, g_items_pitch;
+    int CB, splits, has_bias;
 };
 
 // logits in base 2 of one 32 x 32 block: lane: row n, register: item
@@ -851,8 +878,8 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(W
     }
     wide_core<Y, Z>(
         lds, g1 - g0, A.CB / Z::KC,
-        [&](int64_t g, int step, int tile) { return A.w + (((g0 + g) * kWideA + tile) * A.pitch + step * Z::KC) * Z::S * kUnit; },
-        [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.pitch + step * Z::KC) * Z::S * kUnit; },
+        [&](int64_t g, int step, int tile) { return A.w + (((g0 + g) * kWideA + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
+        [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
         [&](int64_t g, f32x16 (&acc)[4][2]) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -900,8 +927,8 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
     }
     wide_core<Y, Z>(
         lds, 1, A.CB / Z::KC,
-        [&](int64_t, int step, int tile) { return A.w + ((A.v0 + vg + tile) * A.pitch + step * Z::KC) * Z::S * kUnit; },
-        [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.pitch + step * Z::KC) * Z::S * kUnit; },
+        [&](int64_t, int step, int tile) { return A.w + ((A.v0 + vg + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
+        [&](int64_t, int step, int tile) { return A.x + ((n0 + tile) * A.CB + step * Z::KC) * Z::S * kUnit; },
         [&](int64_t, f32x16 (&acc)[4][2]) {
             __syncthreads();                   // the last stage has been read by every wavefront
 #pragma unroll
@@ -942,7 +969,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
                     for (int s = 0; s < S; ++s) {
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
-                            *(typename Y::m::v8 *)(A.g_rows + ((nt * A.g_rows_pitch + vt * 2 + t) * S + s) * kUnit + lane * 16) = p[t].p[s];
+                            *(typename Y::m::v8 *)(A.g_rows + (((nt * A.v_count + vt) * 2 + t) * S + s) * kUnit + lane * 16) = p[t].p[s];
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
                             turn[low][row_of(r, h)] = p[r >> 3].p[s][r & 7];
@@ -954,7 +981,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
 #pragma unroll
                             for (int r = 0; r < 8; ++r)
                                 q[r] = turn[16 * t + row_of(r, h)][low];
-                            *(typename Y::m::v8 *)(A.g_items + ((vt * A.g_items_pitch + nt * 2 + t) * S + s) * kUnit + lane * 16) = q;
+                            *(typename Y::m::v8 *)(A.g_items + (((vt * A.n_tiles + nt) * 2 + t) * S + s) * kUnit + lane * 16) = q;
                         }
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                     }
@@ -989,7 +1016,8 @@ struct ProductArgs {
 
 // 256 x 256 outputs a workgroup, 128 x 128 a wavefront and one wavefront a SIMD: eight operands for sixteen products, since shared memory
 // bounds smaller tiles.  Stages lie in a ring: while one is multiplied the first operands of the next are read, and the one after
-// that is known to have arrived.
+// that is known to have arrived.  2,048 x 50,001 x 1000 in half precision: 194 us with the items' results written directly, 1.06
+// PFLOP/s, and up to 300 where sums are written, joined over the chunks and pieces.
 template <class Y> struct Ring {
     static constexpr int S = Y::S, KC = S == 1 ? 2 : 1, per = KC * S, tiles = 16;
     static constexpr int depth = S == 1 ? 4 : 3;               // 128 or 144 KB
@@ -1137,7 +1165,8 @@ static __global__ __launch_bounds__(256) void wide_sums_kernel(const float *sums
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Joins a row's splits: loss and lse, what the items' side needs of the row, and dx (a wavefront a row).
+// Joins a row's splits: loss and lse, what the items' side needs of the row, and dx (a wavefront a row).  Bound by memory with
+// gradients: 4,001 rows of 64 sums in 24 pieces, 25 MB, in 10 us; by latency without (3 us for a row, 9 for 8,192).
 // ---------------------------------------------------------------------------------------------------------------------
 struct FinishArgs {
     const float *stats, *part;
@@ -1254,7 +1283,8 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
 // wavefront reads a tile of 32 items as it lies in the table, 16 bytes a lane and neighbours side by side (reading operands -- 16 bytes
 // of each row -- fetched every line four times), turns it into operands through shared memory of its own, and splits it as it goes;
 // the rows lie in shared memory as operands.  (Three bfloat16 parts for 32-bit matrices: they need no scale, and the matrix
-// instructions have time to spare.)
+// instructions have time to spare.)  61 rows, 380k items of 100 in bf16, 76 MB: 29 us, 2.6 TB/s with the launch's start and end (a
+// sum of a large tensor reads 4.0 TB/s), 42 by operands; one row, 27k of 50 in 32 bits: 8 us, which is latency.
 // ---------------------------------------------------------------------------------------------------------------------
 struct FewArgs {
     const void *x, *w;
@@ -1293,7 +1323,9 @@ template <class Y> __device__ __forceinline__ Parts<Y> parts_of(const Raw<typena
     return q;
 }
 
-// QB: tiles of 32 rows; CB: operands of a row, K / 16 or more
+// QB: tiles of 32 rows; CB: operands of a row, K / 16 or more (of six, since each is a kernel: 64 rows, 100k items of 200 in bf16 with 13
+// 42 us, with 16 48).  Eight wavefronts a workgroup where shared memory holds as many tiles beside the rows, else four; one workgroup a
+// compute unit.
 template <class Y, int QB, int CB> struct FewShape {
     static constexpr int chunks = CB * (int)sizeof(typename Y::t);        // of 16 bytes, a row
     static constexpr int rows_bytes = QB * CB * Y::S * kUnit, own = chunks * 512;   // the rows' operands; a wavefront's tile
@@ -1476,7 +1508,7 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__((FewShape<Y, QB,
     }
 }
 
-// joins the splits of a product with G: out = scale 2^weight_exponent sum, dbias = 2^weight_exponent sum (four columns a thread)
+// Joins the splits of a product with G, bound by memory (27k x 64 in three pieces, 21 MB and 7 out, in 10 us): out = scale 2^weight_exponent sum, dbias = 2^weight_exponent sum (four columns a thread)
 struct JoinArgs {
     const float *part, *tops;              // tops (the passes' pieces): [split][3][rows] with the sums behind, else NULL
     const uint32_t *weight_top, *col_top;
@@ -1536,7 +1568,8 @@ inline int64_t tiles_padded(int64_t tiles) { return up(tiles, kPadTiles); }
 
 // How many pieces a contraction of so many units is cut into, for a launch of `workgroups` tiles of which `room` are resident together:
 // by an estimate of its time in microseconds -- rounds of workgroups, each with its start, its units and what it writes of its
-// piece, and the pieces' join.  More than eight come in eights (one a die).
+// piece, and the pieces' join.  More than eight come in eights (one a die).  (As many as fill one round instead: 2,048 x 20k of 300 in
+// 32 bits 831 us against 806, 50k x 2k of 600 3,475 : 3,386.)
 inline int wide_splits(int64_t workgroups, int64_t units, int64_t room, double unit_us, double start_us, double piece_us)
 {
     double best = 0.0;
@@ -1552,9 +1585,10 @@ inline int wide_splits(int64_t workgroups, int64_t units, int64_t room, double u
     return at;
 }
 
-// For the passes, by an estimate of their time in microseconds: rounds of the workgroups that are resident together, each with
+// For the passes, by an estimate of their time in microseconds (8,192 rows, 100k items of 50, loss alone: 392 us, in one piece 2,141; 100
+// rows, 1k items with gradients 46, in one piece 86): rounds of the workgroups that are resident together, each with
 // its start and its stages, whose cost grows with the wavefronts that share a SIMD; and what it takes to join the pieces.  More than
-// eight come in eights.
+// eight come in eights, so that the pieces of equal number share a die's cache.
 template <class Y, int KO, int ODD, int MODE> int pass_splits(int64_t still_tiles, int64_t stream_tiles, int cus)
 {
     typedef Shape<Y, KO, ODD, MODE> Z;
@@ -1796,7 +1830,7 @@ template <class Y> int64_t run_wide(const Call &C)
 {
     typedef typename Y::t T;
     const int KO = (int)((C.k + 31) / 32 + 1) / 2 * 2, KP = 32 * KO, CB = 2 * KO, kg = (KO + kProductB - 1) / kProductB;
-    const int64_t n_tiles = (C.n + 31) / 32, v_tiles = (C.v + 31) / 32, nt = tiles_padded(n_tiles), vt = tiles_padded(v_tiles), unit = (int64_t)2 * KO * Y::S * kUnit, row_unit = (int64_t)(CB + 1) * Y::S * kUnit;
+    const int64_t n_tiles = (C.n + 31) / 32, v_tiles = (C.v + 31) / 32, nt = tiles_padded(n_tiles), vt = tiles_padded(v_tiles), unit = (int64_t)2 * KO * Y::S * kUnit, row_unit = (int64_t)CB * Y::S * kUnit;
     const int64_t nr = n_tiles * 32, nb = (n_tiles + kWideB - 1) / kWideB, na = nt / kProductA, room = C.cus;   // the products' workgroups that are resident
     const int products = Y::S == 1 ? 1 : 6;
     // a group's product of 256 x 128 x K on half a compute unit, at two thirds of its rate, and its exponentials
@@ -1837,8 +1871,8 @@ template <class Y> int64_t run_wide(const Call &C)
         dw_part = S.take<float>(dw_splits_of(chunk) > 1 || dw_splits_of(last) > 1 ? dw_rows * KP * 4 : 4);
         dx_part = S.take<float>(dx_splits * nr * KP * 4);
         A.part_sum = S.take<float>(2 * nb * chunk * 32 * 4);
-        A.g_rows = S.take<char>(nt * (chunk * 2 + 1) * Y::S * kUnit);
-        A.g_items = S.take<char>(chunk * (nt * 2 + 1) * Y::S * kUnit);
+        A.g_rows = S.take<char>(nt * chunk * 2 * Y::S * kUnit);
+        A.g_items = S.take<char>(chunk * nt * 2 * Y::S * kUnit);
     }
     if (!C.ws)
         return S.used;
@@ -1846,8 +1880,8 @@ template <class Y> int64_t run_wide(const Call &C)
         return HPF_EINVAL;
 
     prepare_kernel<<<prepare_blocks(P), 256, 0, C.st>>>(P);
-    pack_wide_kernel<Y><<<dim3((unsigned)v_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mw, (int)C.k, CB, KO, CB + 1);
-    pack_wide_kernel<Y><<<dim3((unsigned)n_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mx, (int)C.k, CB, KO, CB + 1);
+    pack_wide_kernel<Y><<<dim3((unsigned)v_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mw, (int)C.k, CB, KO);
+    pack_wide_kernel<Y><<<dim3((unsigned)n_tiles, (unsigned)((KP + 127) / 128)), 256, 0, C.st>>>(mx, (int)C.k, CB, KO);
     A.w = mw.by_row;
     A.x = mx.by_row;
     A.bias = P.bias2;
@@ -1857,8 +1891,6 @@ template <class Y> int64_t run_wide(const Call &C)
     A.rows = nr;
     A.c = fabsf(C.scale) * kLog2e;
     A.CB = CB;
-    A.pitch = CB + 1;
-    A.g_items_pitch = n_tiles * 2 + 1;
     A.splits = row_splits;
     A.has_bias = C.bias != nullptr;
     wide_stats_kernel<Y><<<(unsigned)(nb * row_splits), 256, 0, C.st>>>(A);
@@ -1879,13 +1911,12 @@ template <class Y> int64_t run_wide(const Call &C)
         A.v_count = v_tiles - v0 < chunk ? v_tiles - v0 : chunk;
         const int dw_splits = dw_splits_of(A.v_count);
         const int64_t vg = (A.v_count + kWideA - 1) / kWideA, first = v0 * 32, count = C.v - first < A.v_count * 32 ? C.v - first : A.v_count * 32;
-        A.g_rows_pitch = A.v_count * 2 + 1;
         wide_g_kernel<Y><<<(unsigned)(nb * vg), 256, 0, C.st>>>(A);
         ProductArgs D = {};
         D.a = A.g_rows;
         D.b = mw.by_col + v0 * unit;
         D.a_tiles = n_tiles;
-        D.a_units = A.g_rows_pitch;
+        D.a_units = A.v_count * 2;
         D.tiles = A.v_count;
         D.KO = KO;
         D.splits = dx_splits;
@@ -1895,7 +1926,7 @@ template <class Y> int64_t run_wide(const Call &C)
         D.a = A.g_items;
         D.b = mx.by_col;
         D.a_tiles = A.v_count;
-        D.a_units = A.g_items_pitch;
+        D.a_units = n_tiles * 2;
         D.tiles = n_tiles;
         D.splits = dw_splits;
         D.part = dw_part;

@@ -115,7 +115,9 @@ class HipOps:
         return _NOTHING if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
 
     def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        # (what current_stream(...).cuda_stream gives, without the 2 us of making a Stream object of it)
+        index = self.device.index
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
     # -- every method mirrors one C entry point ------------------------------------------
     def sweep(self, side, tab_self, tab_other, part, k, ld, acc_rows=None, acc_ld=0, grid_blocks=None):

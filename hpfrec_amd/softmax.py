@@ -75,7 +75,8 @@ def softmax_nll(ops, x, items, target, bias=None, scale=1.0):
     bias    float32 [v] or None; -inf (or the type's lowest value) takes an item out, whatever its row holds.  A masked target's
             loss is +inf"""
     n, v, k, ldx, ldi = _inputs(ops, x, items, target, bias, scale)
-    loss, lse = (torch.empty(n, dtype=torch.float32, device=x.device) for _ in range(2))
+    loss = torch.empty(n, dtype=torch.float32, device=x.device)
+    lse = torch.empty_like(loss)
     if n:
         ops.softmax_nll(x, ldx, items, ldi, target, bias, float(scale), n, v, k, loss, lse)
     return loss, lse
