@@ -573,3 +573,88 @@ def test_more_than_2_to_the_32_logits(ops):
     want = torch.log(torch.exp(z).sum(dim=1) + (v - 300))
     assert bool(((lse.double() - want).abs() <= (64 + 4 * math.sqrt(v)) * U).all())
     assert bool(((loss.double() - (want - z[[0, 1], [299, 1]])).abs() <= (64 + 4 * math.sqrt(v)) * U).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("n, v, k", [(5, 40, 5000), (70, 300, 2049), (2, 9, 40000)])
+def test_very_wide_rows(ops, n, v, k, kind):
+    _check(ops, _case(n, v, k, kind, True, seed=n + k))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_rows_far_apart_and_one_table_for_both(ops, kind):
+    """Items 2^24 values apart, and rows that are some of the items themselves."""
+    c = _case(40, 40, 50, kind, True, seed=41)
+    flat = torch.empty(39 * 2 ** 24 + 50, dtype=kind, device="cuda:0")
+    far = flat.as_strided((40, 50), (2 ** 24, 1))
+    far.copy_(c["items"])
+    _check(ops, dict(c, items=far))
+    _check(ops, dict(c, items=far, x=far))
+    many = _case(10, 3000, 50, kind, True, seed=42)
+    many["x"] = many["items"][1000:1010]
+    _check(ops, many)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind, n, k", [(F32, 61, 100), (BF16, 61, 100), (F16, 1, 256)])
+def test_few_rows_streams_and_graphs(ops, kind, n, k):
+    """Equal bits on two streams at once, and in two captured calls' replays with eager work and synchronisations between them."""
+    c = {a: b for a, b in _case(n, 5000, k, kind, True, seed=43).items() if a != "weight"}
+    want = softmax.softmax_nll(ops, **c)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(softmax.softmax_nll(ops, **c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+    inputs = {a: b.clone() if torch.is_tensor(b) else b for a, b in c.items()}
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            outs.append(softmax.softmax_nll(ops, **inputs))
+    for r in range(3):
+        inputs["x"].copy_(c["x"] * (1 + r))
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = softmax.softmax_nll(ops, **dict(c, x=c["x"] * (1 + r)))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for o in outs for a, b in zip(o, eager))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v, k", [(2 ** 26 + 77, 33), (2 ** 22 + 5, 600)])
+def test_gradients_of_tables_of_over_2_to_the_31_values(ops, v, k):
+    """All items but the last 300 are zeros.  Shares, the matrices' products and the results are each rounded to the type (3 x 2^-8
+    of a term); sums of v shares of one size keep 4 sqrt(v) U."""
+    n = 70
+    gen = torch.Generator(device="cuda:0").manual_seed(2)
+    items = torch.zeros((v, k), dtype=BF16, device="cuda:0")
+    items[-300:] = torch.randn((300, k), device="cuda:0", generator=gen) * k ** -0.25
+    x = (torch.randn((n, k), device="cuda:0", generator=gen) * 3 * k ** -0.25).to(BF16)
+    target = v - 1 - torch.randint(0, 300, (n,), device="cuda:0", generator=gen)
+    target[0] = 5
+    loss, dx, ditems, _ = softmax.softmax_nll_grad(ops, x, items, target)
+    w = items[-300:].double()
+    z = x.double() @ w.t()
+    lse = torch.log(torch.exp(z).sum(dim=1) + (v - 300))
+    zt = torch.where(target == 5, 0.0, z.gather(1, (target - (v - 300)).clamp(min=0)[:, None])[:, 0])
+    assert bool(((loss.double() - (lse - zt)).abs() <= (64 + 4 * math.sqrt(v) + 40 * k ** 0.5) * U).all())
+    g = torch.exp(z - lse[:, None])
+    last = target != 5
+    g[last, (target - (v - 300))[last]] -= 1.0
+    rel = 3 * HALF[BF16] + (64 + 4 * math.sqrt(v)) * U
+    assert bool(((dx.double() - g @ w).abs() <= rel * (g.abs() @ w.abs()) + 1e-30).all())
+    assert bool(((ditems[-300:].double() - g.t() @ x.double()).abs() <= rel * (g.abs().t() @ x.double().abs())).all())
+    other = torch.exp(-lse)
+    rest = (other[:, None] * x.double())
+    for i in (0, 6, v // 2, v - 301):
+        assert bool(((ditems[i].double() - rest.sum(dim=0)).abs() <= rel * rest.abs().sum(dim=0)).all())
+    hit = rest.sum(dim=0) - x[0].double()
+    assert bool(((ditems[5].double() - hit).abs() <= rel * (rest.abs().sum(dim=0) + x[0].double().abs())).all())
