@@ -54,6 +54,7 @@ constexpr int kPadTiles = 8;              // packed matrices end on a multiple o
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 struct Bf {
     typedef __bf16 e;
@@ -449,7 +450,7 @@ template <class Y, int KO, int ODD, int MODE> struct Shape {
     static constexpr int waves = S == 2 && KO > 4 && MODE != kNll ? 1 : (S + (MODE == kNll ? 0 : 2)) * KO <= 9 ? 3 : 2;   // a SIMD
     static constexpr int NW = waves == 2 ? 8 : 4;                             // wavefronts of a workgroup
     static constexpr int RT = units <= 4 ? 4 : units <= 12 ? 2 : 1;           // streamed tiles a stage
-    static constexpr int side = RT * 64 * 4 * (MODE == kItems ? 2 : 1);       // reg_bias (and meta) of a stage: 64 values a tile, 32 of them its own
+    static constexpr int side = RT * 64 * 4 * (MODE == kItems ? 3 : 1);       // reg_bias (and meta, target_log) of a stage: 64 values a tile, 32 of them its own
     static constexpr int stage = RT * units * kUnit + side;
 };
 
@@ -606,8 +607,10 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
         }
         if (wave < RT) {
             stage_words(A.reg_bias + ((int64_t)g * RT + wave) * 32, &lds[buf][RT * Z::units * kUnit + wave * 256]);
-            if constexpr (MODE == kItems)
+            if constexpr (MODE == kItems) {
                 stage_words(A.meta + ((int64_t)g * RT + wave) * 32, &lds[buf][RT * Z::units * kUnit + (RT + wave) * 256]);
+                stage_words(A.target_log + ((int64_t)g * RT + wave) * 32, &lds[buf][RT * Z::units * kUnit + (2 * RT + wave) * 256]);
+            }
         }
     };
     auto fetch = [&](const char *unit) {
@@ -663,12 +666,15 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
                 const bool hit = __any(((meta & ~kNegative) >> 5) == (int)mine), negative = __any(meta & kNegative);
                 if (hit || negative) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int r = row_of(i, h), of = __shfl(meta, r);
-                        const bool own = (of & ~kNegative) == (int)mine * 32 + low;
-                        if (own)
-                            x[i] = A.target_log[(int64_t)tile * 32 + r] - lane_bias;
-                        flip |= (unsigned)(own != ((of & kNegative) != 0)) << i;
+                    for (int i = 0; i < 4; ++i) {
+                        const i32x4 of = *(const i32x4 *)(side + RT * 256 + (8 * i + 4 * h) * 4);
+                        const f32x4 log = *(const f32x4 *)(side + 2 * RT * 256 + (8 * i + 4 * h) * 4);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const bool own = (of[j] & ~kNegative) == (int)mine * 32 + low;
+                            x[4 * i + j] = own ? log[j] - lane_bias : x[4 * i + j];
+                            flip |= (unsigned)(own != ((of[j] & kNegative) != 0)) << (4 * i + j);
+                        }
                     }
                 }
                 if constexpr (Y::ranged) {
@@ -1738,7 +1744,7 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
             mx.col_top = P.zero + KP;
         }
         reg_bias = W.take<float>(nt * 32 * 4 + kOneTileMore);
-        target_log = W.take<float>(nt * 32 * 4);
+        target_log = W.take<float>(nt * 32 * 4 + kOneTileMore);
         const int64_t rows_part = row_splits * nr * KP * 4, items_part = item_splits > 1 ? item_splits * vr * KP * 4 : 0;
         part = W.take<float>(rows_part > items_part ? rows_part : items_part);   // (the rows' is read before the items' is written)
         if (item_splits > 1)
