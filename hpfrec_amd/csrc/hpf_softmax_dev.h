@@ -11,7 +11,7 @@
 //                unpacked.  64 rows, 100k items: of 100 in bf16 24.8 us against 39.9 by the passes, in 32 bits 44.8 : 55.2, of
 //                256 in bf16 49.3 : 64.1; one row, 27k items of 50 in 32 bits 21.0 : 27.8
 //   passes       rows of up to 256 values, which a wavefront's registers hold: of 60 in bf16 212 us against 762 by wide products,
-//                of 256 495 : 1,013; of 50 in 32 bits 391 : 1,970, of 200 1,370 : 2,840; 100 rows, 1k items: 46 : 115
+//                of 256 475 : 1,013; of 50 in 32 bits 395 : 1,970, of 200 1,350 : 2,840; 100 rows, 1k items: 42 : 115
 //   wide         wider ones
 //
 // PASSES.  A wavefront keeps 32 rows of one matrix in registers -- the STATIONARY rows -- and the other matrix streams by in tiles of
@@ -555,9 +555,9 @@ __device__ __forceinline__ float times_power(float x, float e) { return ldexpf(x
 
 // Bound by the matrix instructions where rows are wide and by the exponentials where they are narrow: a logit costs a wavefront's lane
 // about ten vector instructions and an exponential, and the two kinds of instruction were seen to take turns rather than to overlap
-// (raised priorities changed nothing).  8,192 x 380k of 100 in 32 bits: rows 3.40 ms, items 3.57 ms, 1.10 and 1.05 PFLOP/s of
-// half-precision products, while one of 8192 x 8192 x 8192 of the library runs at 1.16; loss alone, of 50: 1.25 ms.  8,192 x 100k of
-// 200 in bf16: 0.70 and 0.85 ms, 0.93 and 0.77 PFLOP/s.
+// (raised priorities changed nothing, logits made a tile ahead beside the exponentials cost 1 to 8 per cent).  8,192 x 380k of 100 in
+// 32 bits: rows 3.40 ms, items 3.57 ms, 1.10 and 1.05 PFLOP/s of half-precision products, while one of 8192 x 8192 x 8192 of the
+// library runs at 1.16; loss alone, of 50: 1.25 ms.  8,192 x 100k of 200 in bf16: 0.71 and 0.78 ms, 0.92 and 0.84 PFLOP/s.
 template <class Y, int KO, int ODD, int MODE>
 __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, ODD, MODE>::waves)) void pass_kernel(PassArgs A)
 {
