@@ -1202,36 +1202,48 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
         }
         return;
     }
-    // splits over the lanes: maxima first, then sums relative to them
+    const int64_t t = A.target[n], item = t >= 0 && t < A.V ? t : 0;
+    const float bias = A.bias ? A.bias[item] : 0.0f, given = GRAD && A.weight ? A.weight[n] : 1.0f;
+    // splits over the lanes, 256 at a time: all loads first, then maxima, then sums relative to them
     float top = kNothing, at = -INFINITY, others = 0.0f;
-#pragma unroll 4
-    for (int s = lane; s < A.splits; s += 64) {
-        top = fmaxf(top, A.stats[(3 * s + 0) * A.rows + n]);
-        at = larger(at, A.stats[(3 * s + 2) * A.rows + n]);
+    for (int s0 = 0; s0 < A.splits; s0 += 256) {
+        float tops[4], sums[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            tops[i] = kNothing;
+            sums[i] = 0.0f;
+            const int s = s0 + 64 * i + lane;
+            if (s < A.splits) {
+                const float *const from = A.stats + 3 * s * A.rows + n;
+                tops[i] = from[0];
+                sums[i] = from[A.rows];
+                at = larger(at, from[2 * A.rows]);
+            }
+        }
+        const float before = top;
+        top = wave_max(fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), top));
+        others = times_power(others, before - top);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            others += times_power(sums[i], tops[i] - top);
     }
     for (int d = 32; d; d >>= 1) {
-        top = fmaxf(top, __shfl_xor(top, d));
         at = larger(at, __shfl_xor(at, d));
-    }
-#pragma unroll 4
-    for (int s = lane; s < A.splits; s += 64)
-        others += times_power(A.stats[(3 * s + 1) * A.rows + n], A.stats[3 * s * A.rows + n] - top);
-    for (int d = 32; d; d >>= 1)
         others += __shfl_xor(others, d);
+    }
     others = ldexpf(others, -Y::shift);
 
     // `top` is that of the others; the target's own logit may be far above it
     const float peak = fmaxf(top, ceilf(at));
     const float rest = times_power(others, top - peak), own = __builtin_amdgcn_exp2f(at - peak), all = rest + own;
     const float lse2 = all > 0.0f || all != all ? peak + log2f(all) : -INFINITY;
-    const int64_t t = A.target[n];
     float loss = 0.0f;
     bool alive = t >= 0;
     if (t >= A.V) {                // no such item: said in the loss, and kept out of the gradients
         loss = __builtin_nanf("");
         alive = false;
     } else if (t >= 0) {
-        if ((A.bias && masks(A.bias[t])) || (!(at > kNothing) && at == at && all == all)) {   // a masked target
+        if ((A.bias && masks(bias)) || (!(at > kNothing) && at == at && all == all)) {   // a masked target
             loss = INFINITY;
             alive = false;
         } else if (own > 0.0f && rest < 0x1p20f * own) {
@@ -1246,7 +1258,7 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
             A.lse[n] = lse2 * kLn2;
     }
     if constexpr (GRAD) {
-        const float weight = alive ? (A.weight ? A.weight[n] : 1.0f) : 0.0f, share = ldexpf(fabsf(weight), -weight_exponent(A.weight_top));
+        const float weight = alive ? given : 0.0f, share = ldexpf(fabsf(weight), -weight_exponent(A.weight_top));
         if (lane == 0) {
             A.reg_bias[n] = alive ? log2f(share) - lse2 : -INFINITY;
             A.target_log[n] = alive ? log2f(share * (rest / all)) : -INFINITY;
@@ -1257,7 +1269,7 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
         // dx: four columns a lane, the splits over as many lanes as that leaves (KP / 4 = 8 KO lanes for a split, a power of two above)
         typedef typename Y::t T;
         T *dx = (T *)A.dx + n * A.lddx;
-        const T *w = (const T *)A.w + (alive ? t : 0) * A.ldw;
+        const T *w = (const T *)A.w + item * A.ldw;
         const int span = A.KP <= 32 ? 8 : A.KP <= 64 ? 16 : A.KP <= 128 ? 32 : 64, k = 4 * (lane & (span - 1)), step = 64 / span;
         f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
         if (alive && k < A.KP)
