@@ -658,3 +658,32 @@ def test_gradients_of_tables_of_over_2_to_the_31_values(ops, v, k):
         assert bool(((ditems[i].double() - rest.sum(dim=0)).abs() <= rel * rest.abs().sum(dim=0)).all())
     hit = rest.sum(dim=0) - x[0].double()
     assert bool(((ditems[5].double() - hit).abs() <= rel * (rest.abs().sum(dim=0) + x[0].double().abs())).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_batch_of_events_that_names_users_twice(ops, bits):
+    """Rows gathered from a table, their gradients added up to the table's, one step of all three tensors.  AdamW's first step moves a
+    value by lr g / (|g| + eps') -- lr times its gradient's sign, to 1e-4 of it where |g| > 1e4 eps (8-bit moments: the e4m3
+    rounding of the next step's moments does not reach this one)."""
+    c = _case(90, 400, 40, F32, True, seed=51)
+    gen = torch.Generator(device="cuda:0").manual_seed(3)
+    users = torch.randn((60, 40), device="cuda:0", generator=gen) * 0.2
+    batch = torch.randint(0, 50, (90,), device="cuda:0", generator=gen)
+    params = [users, c["items"].contiguous(), c["bias"]]
+    before = [p.clone() for p in params]
+    state = adamw.adamw_state(params, bits)
+    call = dict(c, x=users[batch], items=params[1])
+    e = _exact(**call)
+    b = _bounds(e, F32, c["bias"], c["scale"], 40)
+    loss, dx, ditems, dbias = softmax.softmax_nll_grad(ops, **call)
+    _close((loss, dx, ditems, dbias), e, b, ("loss", "dx", "ditems", "dbias"))
+    grads = [torch.zeros_like(users).index_add_(0, batch, dx), ditems, dbias]
+    want = torch.zeros((60, 40), dtype=torch.float64, device="cuda:0").index_add_(0, batch, e["dx"])
+    slack = torch.zeros_like(want).index_add_(0, batch, b["dx"] + 90 * U * e["dx"].abs())
+    assert bool(((grads[0].double() - want).abs() <= slack).all())
+    adamw.adamw_step(ops, params, grads, lr=1e-2, eps=1e-10, weight_decay=0.0, **state)
+    for p, q, g in zip(params, before, grads):
+        far = g.abs() > 1e-6
+        assert bool(((p - (q - 1e-2 * torch.sign(g)))[far].abs() <= 2e-6 + 4 * U * q[far].abs()).all())
+        assert bool((p == q)[g == 0].all())
