@@ -759,8 +759,8 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
 // a chunk at a time: at most kChunkBytes) and multiplied with the items (dx, summed over the chunks) and with x (dw).
 // Bound by the matrix instructions: 8 N V K operations.  Logits are made in 256 x 128 outputs a workgroup and 128 x 64 a wavefront,
 // two workgroups a compute unit: six operands read from shared memory for eight products (four for four, 64 x 64, keep shared
-// memory as busy as the matrix units).  2,048 x 50,001 of 1000 in half precision: statistics 251 us, G 255 us (0.82 and 0.80
-// PFLOP/s; a third stage on its way cost 5 per cent), each product with G about 240 us (0.85).
+// memory as busy as the matrix units).  2,048 x 50,001 of 1000 in half precision: statistics 247 us, G 252 us (0.83 and 0.81
+// PFLOP/s; a third stage on its way cost 5 per cent), the products with G 192 and 290.
 //   kChunkBytes  more is fewer launches and fuller last rounds, and memory: 4,096 x 50k of 600 in bf16 with 1 GB 1,572 us, with 512 MB
 //                1,743, with 2 GB 1,575
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1022,8 +1022,8 @@ struct ProductArgs {
 
 // 256 x 256 outputs a workgroup, 128 x 128 a wavefront and one wavefront a SIMD: eight operands for sixteen products, since shared memory
 // bounds smaller tiles.  Stages lie in a ring: while one is multiplied the first operands of the next are read, and the one after
-// that is known to have arrived.  2,048 x 50,001 x 1000 in half precision: 194 us with the items' results written directly, 1.06
-// PFLOP/s, and up to 300 where sums are written, joined over the chunks and pieces.
+// that is known to have arrived.  2,048 x 50,001 x 1000 in half precision: dx, one round of 256 workgroups
+// in eight pieces, 192 us, 1.07 PFLOP/s; dw, 784 workgroups or three rounds and a bit, 290.
 template <class Y> struct Ring {
     static constexpr int S = Y::S, KC = S == 1 ? 2 : 1, per = KC * S, tiles = 16;
     static constexpr int depth = S == 1 ? 4 : 3;               // 128 or 144 KB
