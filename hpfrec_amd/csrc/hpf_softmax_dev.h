@@ -7,9 +7,10 @@
 // Every product is a matrix instruction (32 x 32 x 16); a row's statistics are kept in base 2 (z log2(e)).
 //
 // THREE FORMS, chosen by sizes and types alone (times: 4,096 rows with gradients, 50k items, or what is said):
-//   few rows     loss alone, up to 64 rows (they fit shared memory as operands) of up to 256 values, 128 in 32 bits: items read once,
-//                unpacked.  64 rows, 100k items: of 100 in bf16 24.8 us against 39.9 by the passes, in 32 bits 44.8 : 55.2, of
-//                256 in bf16 49.3 : 64.1; one row, 27k items of 50 in 32 bits 21.0 : 27.8
+//   few rows     loss alone, up to 64 rows: items read once, unpacked; rows that shared memory holds beside tiles of items (256 values, 128
+//                in 32 bits) whole, wider ones in parts.  64 rows, 100k items: of 100 in bf16 24.8 us against 39.9 by the passes, in 32 bits 44.8 : 55.2, of
+//                256 in bf16 49.3 : 64.1; one row, 27k items of 50 in 32 bits 21.0 : 27.8, 380k of
+//                1000 395 : 1,911 by wide products; 64 rows, 100k items of 1000 in bf16 110 : 290
 //   passes       rows of up to 256 values, which a wavefront's registers hold: of 60 in bf16 212 us against 762 by wide products,
 //                of 256 475 : 1,013; of 50 in 32 bits 395 : 1,970, of 200 1,350 : 2,840; 100 rows, 1k items: 42 : 115
 //   wide         wider ones
@@ -1341,6 +1342,93 @@ template <class Y> __device__ __forceinline__ Parts<Y> parts_of(const Raw<typena
     return q;
 }
 
+// a tile's biases (base 2) as they belong to its logits' registers; `masked`: some lane's items are out, whatever their rows hold
+struct FewBias {
+    f32x4 b[4];
+    bool masked;
+};
+__device__ __forceinline__ FewBias few_bias(const FewArgs &A, int64_t tile, bool whole, int h)
+{
+    FewBias o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        o.b[i] = (f32x4)(0.0f);
+        if (whole && A.bias) {
+            __builtin_memcpy(&o.b[i], A.bias + tile * 32 + row_of(4 * i, h), 16);
+            o.b[i] *= kLog2e;
+        } else if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t v = tile * 32 + row_of(4 * i + j, h);
+                o.b[i][j] = v >= A.V ? -INFINITY : A.bias ? A.bias[v] * kLog2e : 0.0f;
+            }
+        }
+    }
+    float least = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        least = fminf(least, o.b[i >> 2][i & 3]);
+    o.masked = __any(least <= kNothing);
+    return o;
+}
+
+// 32 rows' statistics in a wavefront
+struct FewRows {
+    int target;
+    float top, at;
+    Sum sum;
+    __device__ __forceinline__ void begin(const FewArgs &A, int64_t n)
+    {
+        const int64_t t = n < A.N ? A.target[n] : -1;
+        target = t >= 0 && t < A.V ? (int)t : kNoTarget;
+        top = kNothing;
+        at = -INFINITY;
+        sum = {0.0f, 0.0f};
+    }
+    template <class Y> __device__ __forceinline__ void add(f32x16 x, const FewArgs &A, const FewBias &o, int tile, int h)
+    {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            x[i] = fmaf(x[i], A.c, o.b[i >> 2][i & 3]);
+        if (o.masked)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                x[i] = o.b[i >> 2][i & 3] <= kNothing ? -INFINITY : x[i];
+        take_target(x, 1.0f, tile, h, target, at);
+        exponentials<Y>(x, 1.0f, 0.0f, top, sum, [](float) {});
+        sum.add(sum16(x));
+    }
+};
+
+// the wavefronts' pieces become the workgroup's
+template <int QB, int WAVES> __device__ __forceinline__ void few_store(const FewArgs &A, const FewRows (&rows)[QB], float (&join)[WAVES][QB][3][32], int wave, int low, int h)
+{
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const float both = rows[q].sum.s + other_half(rows[q].sum.s), hit = larger(rows[q].at, other_half(rows[q].at));
+        if (h == 0) {
+            join[wave][q][0][low] = rows[q].top;
+            join[wave][q][1][low] = both;
+            join[wave][q][2][low] = hit;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 32 * QB) {
+        const int q = threadIdx.x >> 5;
+        float m = kNothing, all = 0.0f, hit = -INFINITY;
+        for (int i = 0; i < WAVES; ++i) {
+            m = fmaxf(m, join[i][q][0][low]);
+            hit = larger(hit, join[i][q][2][low]);
+        }
+        for (int i = 0; i < WAVES; ++i)
+            all += times_power(join[i][q][1][low], join[i][q][0][low] - m);
+        float *to = A.stats + (int64_t)blockIdx.x * 3 * A.rows + threadIdx.x;
+        to[0] = m;
+        to[A.rows] = all;
+        to[2 * A.rows] = hit;
+    }
+}
+
 // QB: tiles of 32 rows; CB: operands of a row, K / 16 or more (of six, since each is a kernel: 64 rows, 100k items of 200 in bf16 with 13
 // 42 us, with 16 48).  Eight wavefronts a workgroup where shared memory holds as many tiles beside the rows, else four; one workgroup a
 // compute unit.
@@ -1415,17 +1503,10 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__((FewShape<Y, QB,
         for (int s = 0; s < S; ++s)
             *(typename Y::m::v8 *)(lds + (u * S + s) * kUnit + lane * 16) = p.p[s];
     }
-    int target[QB];
-    float top[QB], at[QB];
-    Sum sum[QB];
+    FewRows rows[QB];
 #pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        const int64_t n = q * 32 + low, t = n < A.N ? A.target[n] : -1;
-        target[q] = t >= 0 && t < A.V ? (int)t : kNoTarget;
-        top[q] = kNothing;
-        at[q] = -INFINITY;
-        sum[q] = {0.0f, 0.0f};
-    }
+    for (int q = 0; q < QB; ++q)
+        rows[q].begin(A, q * 32 + low);
     __syncthreads();
     for (; tile < A.v_tiles; tile += step) {
         // (one wavefront's own memory: its accesses are served in order)
@@ -1435,27 +1516,7 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__((FewShape<Y, QB,
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (tile + step < fast)
             load(tile + step);
-        f32x4 b[4];
-        const bool whole = tile < fast;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            b[i] = (f32x4)(0.0f);
-            if (whole && A.bias) {
-                __builtin_memcpy(&b[i], A.bias + tile * 32 + row_of(4 * i, h), 16);
-                b[i] *= kLog2e;
-            } else if (!whole) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int64_t v = tile * 32 + row_of(4 * i + j, h);
-                    b[i][j] = v >= A.V ? -INFINITY : A.bias ? A.bias[v] * kLog2e : 0.0f;
-                }
-            }
-        }
-        float least = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            least = fminf(least, b[i >> 2][i & 3]);
-        const bool masked = __any(least <= kNothing);
+        const FewBias bias = few_bias(A, tile, tile < fast, h);
         f32x16 z[QB];
 #pragma unroll
         for (int q = 0; q < QB; ++q)
@@ -1485,45 +1546,111 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__((FewShape<Y, QB,
         if (tile + step >= fast && tile + step < A.v_tiles)      // (the slow way goes through `own`: the operands have been read)
             load(tile + step);
 #pragma unroll
-        for (int q = 0; q < QB; ++q) {
-            f32x16 &x = z[q];
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                x[i] = fmaf(x[i], A.c, b[i >> 2][i & 3]);
-            if (masked)              // whatever their rows hold
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    x[i] = b[i >> 2][i & 3] <= kNothing ? -INFINITY : x[i];
-            take_target(x, 1.0f, (int)tile, h, target[q], at[q]);
-            exponentials<Y>(x, 1.0f, 0.0f, top[q], sum[q], [](float) {});
-            sum[q].add(sum16(x));
-        }
+        for (int q = 0; q < QB; ++q)
+            rows[q].template add<Y>(z[q], A, bias, (int)tile, h);
     }
-    // the wavefronts' pieces become the workgroup's
+    few_store<QB, Z::waves>(A, rows, join, wave, low, h);
+}
+
+// The same for wider rows, 64 columns at a time; the rows, packed by a launch of their own, come from the caches.  One row, 380k items of
+// 1000 in 32 bits, 1.5 GB: 395 us, 3.84 TB/s; 50k, fewer tiles than wavefronts: 114 us, bound by the latency of a wavefront's parts.
+template <class Y, int QB> __global__ __launch_bounds__(512, 2) void few_wide_kernel(FewArgs A)
+{
+    typedef typename Y::t T;
+    constexpr int S = Y::S, CB = 4, NC = CB * (int)sizeof(T), waves = 8, columns = 16 * CB;
+    __shared__ __attribute__((aligned(1024))) char lds[waves][NC * 512];
+    __shared__ float join[waves][QB][3][32];
+    const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t step = (int64_t)gridDim.x * waves, fast = A.V >= 64 ? (A.V - 32) / 32 : 0;
+    const int parts = (A.K + columns - 1) / columns;
+    char *const own = lds[wave];
+
+    Chunk next[NC / 2];
+    uint32_t from[NC / 2];
 #pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        const float both = sum[q].s + other_half(sum[q].s), hit = larger(at[q], other_half(at[q]));
-        if (h == 0) {
-            join[wave][q][0][low] = top[q];
-            join[wave][q][1][low] = both;
-            join[wave][q][2][low] = hit;
+    for (int i = 0; i < NC / 2; ++i)
+        from[i] = (uint32_t)((64 * i + lane) / NC) * (uint32_t)(A.ldw * sizeof(T)) + (64 * i + lane) % NC * 16;
+    // columns 64 c on of a tile (a row's last ones reach beyond its end by less than a row: 32 rows follow)
+    auto load = [&](int64_t tile, int c) __attribute__((always_inline)) {
+        const char *const start = (const char *)A.w + (tile * 32 * A.ldw + c * columns) * (int64_t)sizeof(T);
+        if (tile < fast) {
+#pragma unroll
+            for (int i = 0; i < NC / 2; ++i)
+                next[i] = *(const LooseChunk *)(start + from[i]);
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < NC / 2; ++i) {
+                const int r = (64 * i + lane) / NC, k = c * columns + (64 * i + lane) % NC * (16 / (int)sizeof(T));
+#pragma unroll
+                for (int j = 0; j < (int)(16 / sizeof(T)); ++j)
+                    ((T *)(own + (64 * i + lane) * 16))[j] = tile * 32 + r < A.V && k + j < A.K ? ((const T *)A.w)[(tile * 32 + r) * A.ldw + k + j] : (T)0.0f;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int i = 0; i < NC / 2; ++i)
+                next[i] = *(const Chunk *)(own + (64 * i + lane) * 16);
         }
-    }
-    __syncthreads();
-    if (threadIdx.x < 32 * QB) {
-        const int q = threadIdx.x >> 5;
-        float m = kNothing, all = 0.0f, hit = -INFINITY;
-        for (int i = 0; i < Z::waves; ++i) {
-            m = fmaxf(m, join[i][q][0][low]);
-            hit = larger(hit, join[i][q][2][low]);
+    };
+    auto place = [&](int c, int r) { return own + c * 512 + ((r + c) & 31) * 16; };
+
+    int64_t tile = (int64_t)blockIdx.x * waves + wave;
+    if (tile < A.v_tiles)
+        load(tile, 0);
+    FewRows rows[QB];
+#pragma unroll
+    for (int q = 0; q < QB; ++q)
+        rows[q].begin(A, q * 32 + low);
+    for (; tile < A.v_tiles; tile += step) {
+        const FewBias bias = few_bias(A, tile, tile < fast, h);
+        f32x16 z[QB];
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+            z[q] = (f32x16)(0.0f);
+#pragma unroll 1
+        for (int c = 0; c < parts; ++c) {
+            Parts<Y> y[QB][CB];
+#pragma unroll
+            for (int q = 0; q < QB; ++q)
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb)
+                    for (int s = 0; s < S; ++s)
+                        y[q][cb].p[s] = *(const typename Y::m::v8 *)((const char *)A.x + (((int64_t)(q * parts + c) * CB + cb) * S + s) * kUnit + lane * 16);
+            // (one wavefront's own memory: its accesses are served in order)
+#pragma unroll
+            for (int i = 0; i < NC / 2; ++i)
+                *(Chunk *)place((64 * i + lane) % NC, (64 * i + lane) / NC) = next[i];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            const int64_t tile2 = c + 1 < parts ? tile : tile + step;
+            const int c2 = c + 1 < parts ? c + 1 : 0;
+            if (tile2 < fast)
+                load(tile2, c2);
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) {
+                Raw<T> raw;
+#pragma unroll
+                for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+                    const Chunk v = *(const Chunk *)place((2 * cb + h) * (int)sizeof(T) / 2 + i, low);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        raw.v[4 * i + j] = v[j];
+                }
+                if (c * columns + 16 * cb + 16 > A.K)
+                    zeros_from(raw, A.K - c * columns - 16 * cb - 8 * h);
+                const Parts<Y> a = parts_of<Y>(raw);
+#pragma unroll
+                for (int q = 0; q < QB; ++q)
+                    z[q] = product<Y>(a, y[q][cb], z[q]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (tile2 >= fast && tile2 < A.v_tiles)
+                load(tile2, c2);
         }
-        for (int i = 0; i < Z::waves; ++i)
-            all += times_power(join[i][q][1][low], join[i][q][0][low] - m);
-        float *to = A.stats + (int64_t)blockIdx.x * 3 * A.rows + threadIdx.x;
-        to[0] = m;
-        to[A.rows] = all;
-        to[2 * A.rows] = hit;
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+            rows[q].template add<Y>(z[q], A, bias, (int)tile, h);
     }
+    few_store<QB, waves>(A, rows, join, wave, low, h);
 }
 
 // Joins the splits of a product with G, bound by memory (27k x 64 in three pieces, 21 MB and 7 out, in 10 us): out = scale 2^weight_exponent sum, dbias = 2^weight_exponent sum (four columns a thread)
@@ -1971,8 +2098,10 @@ template <class Y> int64_t run_wide(const Call &C)
     return (int)hipGetLastError();
 }
 
-// a few rows, no gradients (Y as the products take it: W32 for 32 bits), as wide as shared memory has room for them and a tile
-template <class Y> bool is_few(const Call &C) { return !C.grad && C.n <= 64 && C.k <= (Y::S == 1 ? 256 : 128) && C.ldw < (1 << 24); }
+// a few rows, no gradients (Y as the products take it: W32 for 32 bits)
+template <class Y> bool is_few(const Call &C) { return !C.grad && C.n <= 64 && C.ldw < (1 << 24); }
+// of so many values shared memory has room for the rows and a tile
+template <class Y> bool few_are_wide(const Call &C) { return C.k > (Y::S == 1 ? 256 : 128); }
 
 template <class Y, int QB, int CB> void launch_few(FewArgs &A, int cus, hipStream_t st)
 {
@@ -2009,6 +2138,8 @@ template <class Y> int64_t run_few(const Call &C)
     A.K = (int)C.k;
     Space S = {C.ws, 0};
     A.stats = S.take<float>((int64_t)C.cus * 3 * A.rows * 4);
+    const int parts = (int)((C.k + 63) / 64);
+    char *const packed = S.take<char>(few_are_wide<Y>(C) ? A.rows / 32 * parts * 4 * Y::S * kUnit : 0);
     if (!C.ws)
         return S.used;
     if (C.ws_bytes < S.used)
@@ -2023,10 +2154,24 @@ template <class Y> int64_t run_few(const Call &C)
     A.ldw = C.ldw;
     A.c = fabsf(C.scale) * kLog2e;
     A.sign = C.scale < 0.0f ? -1.0f : 1.0f;
-    if (C.n <= 32)
+    if (few_are_wide<Y>(C)) {
+        Matrix w = {}, x = {};
+        fill_matrices(w, x, C);
+        x.by_row = packed;
+        pack_wide_kernel<Y><<<dim3((unsigned)((C.n + 31) / 32), (unsigned)((parts + 1) / 2)), 256, 0, C.st>>>(x, A.K, 4 * parts, 0);
+        A.x = packed;
+        A.sign = 1.0f;
+        const int64_t grid = (A.v_tiles + 7) / 8;
+        A.groups = (int)(grid > C.cus ? C.cus : grid);
+        if (C.n <= 32)
+            few_wide_kernel<Y, 1><<<A.groups, 512, 0, C.st>>>(A);
+        else
+            few_wide_kernel<Y, 2><<<A.groups, 512, 0, C.st>>>(A);
+    } else if (C.n <= 32) {
         launch_few_rows<Y, 1>(A, C.cus, C.st);
-    else
+    } else {
         launch_few_rows<Y, 2>(A, C.cus, C.st);
+    }
     FinishArgs F = {};
     fill_finish(F, C);
     F.stats = A.stats;

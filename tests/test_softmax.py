@@ -309,6 +309,23 @@ def test_few_rows(ops, n, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("n", [1, 32, 33, 64])
+def test_few_wide_rows(ops, n, kind):
+    """The same for rows that are taken in parts of 64 columns."""
+    for k in (129, 192, 257, 320, 1000, 1025):
+        for v in (1, 31, 33, 63, 64, 65, 95, 96, 97, 1000, 5003)[k % 2::2]:
+            c = _case(n, v, k, kind, v % 2 == 0, seed=n + k + v, pad=(0, 1, 3, 7)[k % 4])
+            if v % 3 == 0:
+                flat = torch.empty(v * (k + 5) + 1, dtype=kind, device="cuda:0")
+                flat[1:].view(v, k + 5)[:, :k].copy_(c["items"])
+                c["items"] = flat[1:].view(v, k + 5)[:, :k]
+            e = _exact(**c)
+            b = _bounds(e, kind, c["bias"], c["scale"], k, 4.0)
+            _close(softmax.softmax_nll(ops, **{a: x for a, x in c.items() if a != "weight"}), e, b, ("loss", "lse"))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("k", [50, 300])
 @pytest.mark.parametrize("kind", [F32, BF16])
 @pytest.mark.parametrize("lowest", [float("-inf"), torch.finfo(torch.float32).min])
