@@ -175,7 +175,7 @@ struct PrepArgs {
     const int64_t *target;
     const float *bias;
     int64_t N, V, np, vp;          // np, vp: padded
-    float *bias2;                  // bias in base 2, -inf beyond the catalogue
+    float *bias2;                  // bias in base 2, -inf beyond the catalogue and where it masks
     int32_t *meta;                 // targets as 32-bit numbers, kNoTarget where there is none or a masked one
     uint32_t *zero;                // what later launches take maxima into
     int zeros;
@@ -188,7 +188,7 @@ static __global__ __launch_bounds__(256) void prepare_kernel(PrepArgs A)
     if (i < A.zeros)
         A.zero[i] = 0;
     if (i < A.vp)
-        A.bias2[i] = i >= A.V ? -INFINITY : A.bias ? A.bias[i] * kLog2e : 0.0f;
+        A.bias2[i] = i >= A.V || (A.bias && masks(A.bias[i])) ? -INFINITY : A.bias ? A.bias[i] * kLog2e : 0.0f;
     if (i < A.np) {
         const int64_t t = i < A.N ? A.target[i] : -1;
         A.meta[i] = t >= 0 && t < A.V && !(A.bias && masks(A.bias[t])) ? (int32_t)t : kNoTarget;
@@ -412,7 +412,7 @@ struct PassArgs {
     const float *lane_bias;         // items pass: the stationary item's bias
     const int32_t *meta;            // items pass: per streamed row its target and flag; rows passes: per stationary row
     const float *target_log;        // items pass: per streamed row, log2 of |G| at its target
-    float *stats;                   // [split][3][still rows]: maximum, sum (rows: without the target), rows: target's logit
+    float *stats;                   // [split][3][still rows]: what sums are relative to (base 2), sum (rows: without the target), rows: target's logit
     float *part;                    // [split][still rows][32 KO]
     int64_t still_tiles, still_rows, stream_tiles;   // tiles of 32; still_rows = 32 still_tiles
     float c;                        // |scale| log2(e)
@@ -504,23 +504,45 @@ __device__ __forceinline__ float sum16(const f32x16 &x)
     return (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]))) + (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
 }
 
-// One block (lane: stationary row, register: streamed row) whose logarithms in base 2 are c x + more becomes its exponentials relative
-// to a running maximum, times 2^shift; `rescale(f)` is called where the maximum grew.  c > 0.
-template <class Y, class F> __device__ __forceinline__ void exponentials(f32x16 &x, float c, float more, float &top, Sum &sum, const F &rescale)
+// What a stationary row's exponentials are held relative to: they are 2^(z + down), and at most 2^shift.  `down` is a whole number, so that
+// rescaling changes no digit.  far: the same for all lanes, some of which hold logits so large that floats lie a whole number or more
+// apart and the shift would be lost in them: their largest is held as one, and every logit is rounded as the largest was.
+constexpr float kFar = 0x1p23f;
+struct Held {
+    float down;
+    bool far;
+    __device__ __forceinline__ void begin()
+    {
+        down = -kNothing;
+        far = false;
+    }
+};
+
+// One block (lane: stationary row, register: streamed row) whose logarithms in base 2 are c x becomes its exponentials relative to a
+// running maximum; `rescale(f)` is called where the maximum grew.  c > 0.
+template <class Y, class F> __device__ __forceinline__ void exponentials(f32x16 &x, float c, Held &held, Sum &sum, const F &rescale)
 {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i)
         m = fmaxf(m, x[i]);
-    m = fmaf(halves_max(m), c, more);
-    if (__any(m > top)) {
-        const float grown = m > top ? ceilf(m) : top, f = __builtin_amdgcn_exp2f(top - grown);
+    m = halves_max(m) * c;
+    if (__any(m + held.down > (float)Y::shift)) {
+        const float top = ceilf(m), down = m + held.down > (float)Y::shift ? fabsf(top) < kFar ? (float)Y::shift - top : -top : held.down;
+        const float f = __builtin_amdgcn_exp2f(down - held.down);
         sum.s *= f;
         sum.c *= f;
-        top = grown;
+        held.down = down;
+        held.far = __any(fabsf(down) >= kFar && down < -kNothing);
         rescale(f);
     }
-    const float down = ((float)Y::shift - top) + more;
+    if (held.far) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            x[i] *= c;
+        c = 1.0f;
+    }
+    const float down = held.down < -kNothing ? held.down : -INFINITY;     // (nothing yet: all of it is masked)
 #pragma unroll
     for (int i = 0; i < 16; ++i)
         x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], c, down));
@@ -541,11 +563,11 @@ __device__ __forceinline__ void take_target(f32x16 &x, float c, int tile, int h,
             }
 }
 
-__device__ __forceinline__ void store_stats(float *to, int64_t rows, int h, float top, const Sum &sum, float at)
+__device__ __forceinline__ void store_stats(float *to, int64_t rows, int h, const Held &held, const Sum &sum, float at)
 {
     const float both = sum.s + other_half(sum.s), hit = larger(at, other_half(at));
     if (h == 0) {
-        to[0] = top;
+        to[0] = -held.down;
         to[rows] = both;
         to[2 * rows] = hit;
     }
@@ -590,7 +612,10 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
     if constexpr (MODE != kNll)
         for (int ko = 0; ko < KO; ++ko)
             acc[ko] = (f32x16)(0.0f);
-    float top = MODE == kItems && !Y::ranged ? 0.0f : kNothing, at = -INFINITY;
+    float at = -INFINITY;
+    Held held = {0.0f, false};
+    if (MODE != kItems || Y::ranged)
+        held.begin();
     Sum sum = {0.0f, 0.0f};
 
     auto stage = [&](int g, int buf) {
@@ -662,6 +687,11 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
                         acc[ko] *= f;
             };
             if constexpr (MODE == kItems) {
+                // (the bias goes to the item's logits by themselves: a target's share and a large bias would lose each other's digits)
+                if (A.bias)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        x[i] += lane_bias;
                 const int meta = ((const int32_t *)(side + RT * 256))[low];
                 unsigned flip = 0;             // registers of negative G: negative weights, and targets of positive ones
                 const bool hit = __any(((meta & ~kNegative) >> 5) == (int)mine), negative = __any(meta & kNegative);
@@ -673,17 +703,17 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const bool own = (of[j] & ~kNegative) == (int)mine * 32 + low;
-                            x[4 * i + j] = own ? log[j] - lane_bias : x[4 * i + j];
+                            x[4 * i + j] = own ? log[j] : x[4 * i + j];
                             flip |= (unsigned)(own != ((of[j] & kNegative) != 0)) << (4 * i + j);
                         }
                     }
                 }
                 if constexpr (Y::ranged) {
-                    exponentials<Y>(x, c, lane_bias, top, sum, rescale);
+                    exponentials<Y>(x, c, held, sum, rescale);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        x[i] = __builtin_amdgcn_exp2f(x[i] + lane_bias);
+                        x[i] = __builtin_amdgcn_exp2f(x[i]);
                 }
                 if (hit || negative)
 #pragma unroll
@@ -693,7 +723,7 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
                     sum.add(sum16(x));
             } else {
                 take_target(x, c, tile, h, target, at);
-                exponentials<Y>(x, c, 0.0f, top, sum, rescale);
+                exponentials<Y>(x, c, held, sum, rescale);
                 sum.add(sum16(x));
             }
 
@@ -714,7 +744,7 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
         return;
     const int64_t row = mine * 32 + low;
     if (MODE == kItems && A.out) {             // the whole sum: the gradients themselves
-        const float both = sum.s + other_half(sum.s), e = top - (float)Y::shift + (float)weight_exponent(A.weight_top);
+        const float both = sum.s + other_half(sum.s), e = -held.down + (float)weight_exponent(A.weight_top);
         if (row < A.count) {
             if (A.dbias && h == 0)
                 A.dbias[row] = times_power(both, e);
@@ -741,7 +771,7 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
         }
         return;
     }
-    store_stats(A.stats + (int64_t)sp * 3 * A.still_rows + row, A.still_rows, h, top, sum, at);
+    store_stats(A.stats + (int64_t)sp * 3 * A.still_rows + row, A.still_rows, h, held, sum, at);
     if constexpr (MODE != kNll) {
         float *to = A.part + (sp * A.still_rows + row) * (32 * KO) + 4 * h;
 #pragma unroll
@@ -873,13 +903,14 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(W
     const int64_t n0 = (int64_t)(blockIdx.x / A.splits) * 4;
     const int64_t all = (A.v_tiles + kWideA - 1) / kWideA, g0 = all * sp / A.splits, g1 = all * (sp + 1) / A.splits;
     int target[2];
-    float top[2], at[2];
+    float at[2];
+    Held held[2];
     Sum sum[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int64_t tile = n0 + 2 * wb + j;
         target[j] = tile < A.n_tiles ? A.meta[tile * 32 + low] : kNoTarget;
-        top[j] = kNothing;
+        held[j].begin();
         sum[j] = {0.0f, 0.0f};
         at[j] = -INFINITY;
     }
@@ -898,7 +929,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(W
                     f32x16 &x = acc[i][j];
                     wide_bias(x, A, tile, h);
                     take_target(x, 1.0f, (int)tile, h, target[j], at[j]);
-                    exponentials<Y>(x, 1.0f, 0.0f, top[j], sum[j], [](float) {});
+                    exponentials<Y>(x, 1.0f, held[j], sum[j], [](float) {});
                     sum[j].add(sum16(x));
                 }
             }
@@ -907,7 +938,7 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_stats_kernel(W
     for (int j = 0; j < 2; ++j) {
         const int64_t tile = n0 + 2 * wb + j;
         if (tile < A.n_tiles)
-            store_stats(A.stats + (int64_t)(2 * sp + wa) * 3 * A.rows + tile * 32 + low, A.rows, h, top[j], sum[j], at[j]);
+            store_stats(A.stats + (int64_t)(2 * sp + wa) * 3 * A.rows + tile * 32 + low, A.rows, h, held[j], sum[j], at[j]);
     }
 }
 
@@ -1206,7 +1237,7 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
     const int64_t t = A.target[n], item = t >= 0 && t < A.V ? t : 0;
     const float bias = A.bias ? A.bias[item] : 0.0f, given = GRAD && A.weight ? A.weight[n] : 1.0f;
     // splits over the lanes, 256 at a time: all loads first, then maxima, then sums relative to them
-    float top = kNothing, at = -INFINITY, others = 0.0f;
+    float held = kNothing, at = -INFINITY, others = 0.0f;
     for (int s0 = 0; s0 < A.splits; s0 += 256) {
         float tops[4], sums[4];
 #pragma unroll
@@ -1221,20 +1252,21 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
                 at = larger(at, from[2 * A.rows]);
             }
         }
-        const float before = top;
-        top = wave_max(fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), top));
-        others = times_power(others, before - top);
+        const float before = held;
+        held = wave_max(fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), held));
+        others = times_power(others, before - held);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            others += times_power(sums[i], tops[i] - top);
+            others += times_power(sums[i], tops[i] - held);
     }
     for (int d = 32; d; d >>= 1) {
         at = larger(at, __shfl_xor(at, d));
         others += __shfl_xor(others, d);
     }
-    others = ldexpf(others, -Y::shift);
-
-    // `top` is that of the others; the target's own logit may be far above it
+    // `held` is below the others' largest by the shift, or (see Held) that itself; the target's own logit may be far above it
+    const int shift = fabsf(held) < kFar ? Y::shift : 0;
+    const float top = held + (float)shift;
+    others = ldexpf(others, -shift);
     const float peak = fmaxf(top, ceilf(at));
     const float rest = times_power(others, top - peak), own = __builtin_amdgcn_exp2f(at - peak), all = rest + own;
     const float lse2 = all > 0.0f || all != all ? peak + log2f(all) : -INFINITY;
@@ -1276,7 +1308,7 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
         if (alive && k < A.KP)
 #pragma unroll 4
             for (int s = lane / span; s < A.splits; s += step) {
-                const float down = A.stats[3 * s * A.rows + n] - top;
+                const float down = A.stats[3 * s * A.rows + n] - held;
                 const f32x4 p = *(const f32x4 *)(A.part + (s * A.rows + n) * A.KP + k);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -1291,7 +1323,7 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (k + j < A.K) {
-                    const float v = times_power(sum[j], top - peak - (float)Y::shift + ce[j]);
+                    const float v = times_power(sum[j], held - peak + ce[j]);
                     dx[k + j] = (T)(alive ? A.scale * weight * (v / all - rest / all * (float)w[k + j]) : 0.0f);
                 }
     }
@@ -1375,13 +1407,14 @@ __device__ __forceinline__ FewBias few_bias(const FewArgs &A, int64_t tile, bool
 // 32 rows' statistics in a wavefront
 struct FewRows {
     int target;
-    float top, at;
+    float at;
+    Held held;
     Sum sum;
     __device__ __forceinline__ void begin(const FewArgs &A, int64_t n)
     {
         const int64_t t = n < A.N ? A.target[n] : -1;
         target = t >= 0 && t < A.V ? (int)t : kNoTarget;
-        top = kNothing;
+        held.begin();
         at = -INFINITY;
         sum = {0.0f, 0.0f};
     }
@@ -1395,7 +1428,7 @@ struct FewRows {
             for (int i = 0; i < 16; ++i)
                 x[i] = o.b[i >> 2][i & 3] <= kNothing ? -INFINITY : x[i];
         take_target(x, 1.0f, tile, h, target, at);
-        exponentials<Y>(x, 1.0f, 0.0f, top, sum, [](float) {});
+        exponentials<Y>(x, 1.0f, held, sum, [](float) {});
         sum.add(sum16(x));
     }
 };
@@ -1407,7 +1440,7 @@ template <int QB, int WAVES> __device__ __forceinline__ void few_store(const Few
     for (int q = 0; q < QB; ++q) {
         const float both = rows[q].sum.s + other_half(rows[q].sum.s), hit = larger(rows[q].at, other_half(rows[q].at));
         if (h == 0) {
-            join[wave][q][0][low] = rows[q].top;
+            join[wave][q][0][low] = -rows[q].held.down;
             join[wave][q][1][low] = both;
             join[wave][q][2][low] = hit;
         }
@@ -1671,11 +1704,11 @@ template <class Y> __global__ __launch_bounds__(256) void join_kernel(JoinArgs A
     const int k = (int)(id - v * quads) * 4;
     if (v >= A.count)
         return;
-    float top = A.tops ? kNothing : 0.0f;
+    float top = A.tops ? kNothing : -(float)Y::shift;
     if (A.tops)
         for (int s = 0; s < A.splits; ++s)
             top = fmaxf(top, A.tops[3 * s * A.rows + v]);
-    const float e = top - (float)Y::shift + (float)weight_exponent(A.weight_top);
+    const float e = top + (float)weight_exponent(A.weight_top);
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int s = 0; s < A.splits; ++s) {

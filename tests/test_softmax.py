@@ -704,3 +704,120 @@ def test_a_batch_of_events_that_names_users_twice(ops, bits):
         far = g.abs() > 1e-6
         assert bool(((p - (q - 1e-2 * torch.sign(g)))[far].abs() <= 2e-6 + 4 * U * q[far].abs()).all())
         assert bool((p == q)[g == 0].all())
+
+
+# finite biases far from zero, above what masks
+FAR = (-1e4, -3e7, -5e7, -1e8, -1.5e8, -1e9, -1e20, -5e37)
+
+
+def _with_far_items(k, kind, weights, seed=61):
+    """A third of the items have biases far below the others'; every fifth row's target is one of them, and most are no row's target.
+    Returns the case, which items, and in 64 bits what it has to give: shares of exp(-800) are zero there as those of exp(-1e4) are."""
+    c = _case(200, 300, k, kind, True, seed=seed)
+    far = torch.arange(300, device="cuda:0") % 3 == 0
+    c["bias"] = torch.where(far, torch.tensor(FAR, device="cuda:0").repeat(100)[:300], c["bias"])
+    c["target"] = torch.where((c["target"] >= 0) & far[c["target"].clamp(min=0)], c["target"] + 1, c["target"])
+    c["target"][2::5] = 3 * (torch.arange(40, device="cuda:0") % 25)
+    gen = torch.Generator(device="cuda:0").manual_seed(7)
+    if weights == "spread":       # of both signs, from 2^-14 to 1
+        c["weight"] = torch.exp2(-14 * torch.rand(200, device="cuda:0", generator=gen)) * torch.sign(c["weight"])
+    else:
+        c["weight"] = torch.ones(200, device="cuda:0")
+    e = _exact(**dict(c, bias=torch.where(far, -800.0, c["bias"])))
+    # bounds as if the far items' logits were no further away than their row's lse: a share of zero and a target's of one owe nothing to
+    # the size of such a bias
+    e["z"] = torch.where(far, e["lse"][:, None], e["z"])
+    return c, far, e, _bounds(e, kind, torch.where(far, 0.0, c["bias"]), c["scale"], k, 2 * float(c["weight"].abs().max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [50, 200, 300])
+@pytest.mark.parametrize("weights", ["ones", "spread"])
+def test_targets_with_large_biases(ops, weights, k, kind):
+    """A target's share is its row's weight less nothing, however far below the others its item is."""
+    c, far, e, b = _with_far_items(k, kind, weights)
+    loss, dx, ditems, dbias = softmax.softmax_nll_grad(ops, **c)
+    near = (c["target"] < 0) | ~far[c["target"].clamp(min=0)]
+    _close((torch.where(near, loss, 0.0), dx), dict(e, loss=torch.where(near, e["loss"], 0.0)), b, ("loss", "dx"))
+    t = c["target"][~near]
+    z = c["scale"] * (c["x"][~near].double() * c["items"][t].double()).sum(dim=1) + c["bias"][t].double()
+    assert bool(((loss[~near].double() / (e["lse"][~near] - z) - 1).abs() <= 8 * U).all())
+    hit = torch.zeros(300, dtype=torch.bool, device="cuda:0")
+    hit[c["target"][c["target"] >= 0]] = True
+    for name, got in (("ditems", ditems), ("dbias", dbias)):
+        off = (got.double() - e[name]).abs() - b[name]
+        assert bool((off[hit | ~far] <= 0).all()), (name, float(off[hit | ~far].max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [50, 200, 300])
+def test_items_far_below_the_others(ops, k, kind):
+    """An item that is nobody's target and whose shares are zero in 32 bits gets gradients of zero."""
+    c, far, e, b = _with_far_items(k, kind, "spread")
+    _, _, ditems, dbias = softmax.softmax_nll_grad(ops, **c)
+    far[c["target"][c["target"] >= 0]] = False
+    assert int(far.sum()) >= 70 and not bool(ditems[far].any()) and not bool(dbias[far].any())
+    # rows none of which has weight to speak of but for these items
+    c["weight"] = torch.where(c["weight"].abs() > 0.5, c["weight"], 0.0)
+    for x in softmax.softmax_nll_grad(ops, **c)[1:]:
+        assert bool(torch.isfinite(x).all())
+
+
+AWAY = (-2e7, 2e7, -3e7, 5e7, -1e8, 1e8, -1.5e8, 1e9, -1e9, 1e12, -1e30, 1e37)
+
+
+def _away(n, k, kind, away):
+    """Logits that are `away` and a little, which 32 bits round to `away`: every item's share is 1 / v."""
+    c = _case(n, 300, k, kind, True, seed=71, spread=1e-3)
+    c["bias"] = torch.full((300,), away, device="cuda:0")
+    p = torch.full((n, 300), 1 / 300, dtype=torch.float64, device="cuda:0")
+    live = c["target"] >= 0
+    g = (p - torch.nn.functional.one_hot(c["target"].clamp(min=0), 300)) * (torch.where(live, c["weight"].double(), 0.0))[:, None]
+    x, w = c["x"].double(), c["items"].double()
+    flat = torch.full((n,), math.log(300.0), dtype=torch.float64, device="cuda:0")
+    e = dict(z=torch.zeros_like(g), lse=flat, loss=torch.where(live, flat, 0.0), g=g, dx=c["scale"] * (g @ w), ditems=c["scale"] * (g.t() @ x), dbias=g.sum(dim=0), x=x, w=w)
+    return c, e, _bounds(e, kind, None, c["scale"], k, 2 * float(c["weight"].abs().max()))
+
+
+def _check_away(ops, n, k, kind):
+    for away in AWAY:
+        c, e, b = _away(n, k, kind, away)
+        (loss, lse), grad = _both(ops, c)
+        _close((loss,), e, b, ("loss",))
+        _close(grad[:2], e, b, ("loss", "dx"))
+        assert bool(((lse.double() - away).abs() <= math.log(300.0) + 8 * U * abs(away)).all()), away
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [50, 200])
+@pytest.mark.parametrize("n", [40, 150])
+def test_rows_whose_logits_are_all_far_from_zero(ops, n, k, kind):
+    """Loss and dx know only differences; lse is off by a few units of its own last place."""
+    _check_away(ops, n, k, kind)
+
+
+def _check_products(ops, n, k, kind):
+    """One column whose product is far from zero, no bias.  All items are alike, so that logits that are rounded alike differ by nothing;
+    half precision's stay where floats are closer than one, and are rounded apart by up to a step each."""
+    big = 2.0 ** 7 if kind == F16 else 2.0 ** 14
+    step = 4 * U * big * big / 3 if kind == F16 else 0.0
+    x, items = torch.zeros((n, k), device="cuda:0", dtype=kind), torch.zeros((290, k), device="cuda:0", dtype=kind)
+    x[:, 0], items[:, 0] = big, -big
+    x[::2, 0] *= -1
+    target = torch.arange(n, device="cuda:0") % 290
+    loss, dx, ditems, _ = softmax.softmax_nll_grad(ops, x, items, target, scale=1.0 / 3)
+    want = math.log(290.0)
+    assert bool(((loss.double() - want).abs() <= 64 * U * want + step).all())
+    assert bool(torch.isfinite(dx).all()) and bool(torch.isfinite(ditems).all())
+    # all shares are 1 / 290 and the items alike: what is left of dx is rounding
+    assert bool((dx[:, 0].double().abs() <= big / 3 * (2 * HALF[kind] + 290 * U + step)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("n", [40, 150])
+def test_rows_far_from_zero_by_their_products(ops, n, kind):
+    _check_products(ops, n, 50, kind)
