@@ -50,7 +50,10 @@ namespace hpf_softmax {
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 constexpr float kNothing = -0x1p126f;     // a running maximum before anything: logits (base 2) at or below it are masked
 constexpr int kNoTarget = 0x3FFFFFFF;     // block 2^25 of 32 items: beyond every catalogue
-constexpr int kNegative = 0x40000000;     // flag beside a row's target: its weight is negative
+constexpr int kNegative = 0x40000000;     // flags beside a row's target: its weight is negative
+constexpr int kAway = -0x7FFFFFFF - 1;    //   its lse is over kAwayFrom in size: see FinishArgs::away
+constexpr int kTarget = 0x3FFFFFFF;       //   the target itself
+constexpr float kAwayFrom = 128.0f;
 constexpr int kPadTiles = 8;              // packed matrices end on a multiple of so many tiles: staging reads whole groups
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -408,10 +411,11 @@ struct PassArgs {
     const char *still;              // stationary matrix, by_row
     const char *by_row, *by_col;    // streamed matrix
     const int32_t *still_exp, *stream_exp;   // scaled: their tiles' (stationary rows without gradients: each row's)
-    const float *reg_bias;          // per streamed row: rows passes: its bias (base 2); items pass: log2(|weight|), less weight_exponent, less lse
+    const float *reg_bias;          // per streamed row: rows passes: its bias (base 2); items pass: log2(|weight|), less weight_exponent, less lse (less `away`)
     const float *lane_bias;         // items pass: the stationary item's bias
     const int32_t *meta;            // items pass: per streamed row its target and flag; rows passes: per stationary row
     const float *target_log;        // items pass: per streamed row, log2 of |G| at its target
+    const float *away;              //   and of rows whose meta has kAway: what is added ahead of reg_bias
     float *stats;                   // [split][3][still rows]: what sums are relative to (base 2), sum (rows: without the target), rows: target's logit
     float *part;                    // [split][still rows][32 KO]
     int64_t still_tiles, still_rows, stream_tiles;   // tiles of 32; still_rows = 32 still_tiles
@@ -563,6 +567,9 @@ __device__ __forceinline__ void take_target(f32x16 &x, float c, int tile, int h,
             }
 }
 
+// The logarithm of a share as it comes out of the roundings of its logit and its row's lse: no share is above one.  (NaN stays.)
+__device__ __forceinline__ float share_log(float x) { return __builtin_elementwise_minimum(x, 0.0f); }
+
 __device__ __forceinline__ void store_stats(float *to, int64_t rows, int h, const Held &held, const Sum &sum, float at)
 {
     const float both = sum.s + other_half(sum.s), hit = larger(at, other_half(at));
@@ -670,7 +677,17 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
             order_reads<S, 2 * S - 1, CB>();
 
             float c = Y::scaled ? ldexpf(A.c, stream_exp + still_exp) : A.c;
-            if (biased || __any(c == 0.0f)) {
+            const int meta = MODE == kItems ? ((const int32_t *)(side + RT * 256))[low] : 0;
+            if (MODE == kItems && __any(meta < 0)) {       // (logits first, then down to their row's, then shares: small numbers beside small ones)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 b = *(const f32x4 *)(side + (8 * i + 4 * h) * 4), away = *(const f32x4 *)(A.away + (int64_t)tile * 32 + 8 * i + 4 * h);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        x[4 * i + j] = share_log((fmaf(x[4 * i + j], c, lane_bias) + away[j]) + b[j]);
+                }
+                c = 1.0f;
+            } else if (biased || __any(c == 0.0f)) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const f32x4 b = *(const f32x4 *)(side + (8 * i + 4 * h) * 4);
@@ -678,6 +695,11 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
                     for (int j = 0; j < 4; ++j)
                         x[4 * i + j] = fmaf(x[4 * i + j], c, b[j]);
                 }
+                // (the bias goes to the item's logits by themselves: a target's share and a large bias would lose each other's digits)
+                if (MODE == kItems && A.bias)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        x[i] += lane_bias;
                 c = 1.0f;
             }
             const auto rescale = [&](float f) {
@@ -687,14 +709,8 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
                         acc[ko] *= f;
             };
             if constexpr (MODE == kItems) {
-                // (the bias goes to the item's logits by themselves: a target's share and a large bias would lose each other's digits)
-                if (A.bias)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        x[i] += lane_bias;
-                const int meta = ((const int32_t *)(side + RT * 256))[low];
                 unsigned flip = 0;             // registers of negative G: negative weights, and targets of positive ones
-                const bool hit = __any(((meta & ~kNegative) >> 5) == (int)mine), negative = __any(meta & kNegative);
+                const bool hit = __any(((meta & kTarget) >> 5) == (int)mine), negative = __any(meta & kNegative);
                 if (hit || negative) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -702,7 +718,7 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
                         const f32x4 log = *(const f32x4 *)(side + 2 * RT * 256 + (8 * i + 4 * h) * 4);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const bool own = (of[j] & ~kNegative) == (int)mine * 32 + low;
+                            const bool own = (of[j] & kTarget) == (int)mine * 32 + low;
                             x[4 * i + j] = own ? log[j] : x[4 * i + j];
                             flip |= (unsigned)(own != ((of[j] & kNegative) != 0)) << (4 * i + j);
                         }
@@ -866,7 +882,7 @@ __device__ __forceinline__ void wide_core(char *lds, int64_t groups, int steps, 
 
 struct WideArgs {
     const char *w, *x;              // by_row units
-    const float *bias, *reg_bias, *target_log;
+    const float *bias, *reg_bias, *target_log, *away;
     const int32_t *meta;
     float *stats, *part_sum;
     char *g_rows, *g_items;         // G of a chunk: rows n / contraction v, and rows v / contraction n
@@ -954,13 +970,14 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
     e(*const turn)[36] = (e(*)[36])(lds + wave * 2304);      // a block a wavefront, to exchange its lanes and registers: where the stages were
     const int64_t ngroups = (A.n_tiles + 3) / 4, n0 = blockIdx.x % ngroups * 4, vg = blockIdx.x / ngroups * kWideA;   // vg: within the chunk
     int meta[2];
-    float down[2], tg[2];
+    float down[2], tg[2], away[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int64_t tile = n0 + 2 * wb + j;
         const bool in = tile < A.n_tiles;
         meta[j] = in ? A.meta[tile * 32 + low] : kNoTarget;
         down[j] = in ? A.reg_bias[tile * 32 + low] : -INFINITY;
+        away[j] = meta[j] < 0 ? A.away[tile * 32 + low] : 0.0f;
         tg[j] = in ? A.target_log[tile * 32 + low] : 0.0f;
     }
     wide_core<Y, Z>(
@@ -982,15 +999,21 @@ template <class Y> __global__ __launch_bounds__(256, 2) void wide_g_kernel(WideA
                         break;
                     f32x16 &x = acc[i][j];
                     wide_bias(x, A, tile, h);
+                    if (__any(meta[j] < 0)) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        x[r] += down[j];
-                    const bool hit = __any(((meta[j] & ~kNegative) >> 5) == (int)tile);
+                        for (int r = 0; r < 16; ++r)
+                            x[r] = share_log((x[r] + away[j]) + down[j]);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            x[r] += down[j];
+                    }
+                    const bool hit = __any(((meta[j] & kTarget) >> 5) == (int)tile);
                     unsigned flip = meta[j] & kNegative ? 0xFFFFu : 0u;
                     if (hit)
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
-                            if ((meta[j] & ~kNegative) == (int)tile * 32 + row_of(r, h)) {
+                            if ((meta[j] & kTarget) == (int)tile * 32 + row_of(r, h)) {
                                 x[r] = tg[j];
                                 flip ^= 1u << r;
                             }
@@ -1214,6 +1237,8 @@ struct FinishArgs {
     const void *w;                 // items, for the target's own row
     const uint32_t *col_top;
     float *loss, *lse, *reg_bias, *target_log;
+    float *away;                   // Shares come from z - lse, and what the lse adds to a large maximum would be lost in it: for such rows minus
+                                   // the maximum (others: 0), and reg_bias is relative to it
     int32_t *meta;
     void *dx;
     int64_t N, V, rows, ldw, lddx;
@@ -1230,6 +1255,7 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
     if (n >= A.N) {                // rows that only fill the last tile: no share of any sum
         if (GRAD && lane == 0) {
             A.reg_bias[n] = A.target_log[n] = -INFINITY;
+            A.away[n] = 0.0f;
             A.meta[n] = kNoTarget;
         }
         return;
@@ -1293,9 +1319,11 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
     if constexpr (GRAD) {
         const float weight = alive ? given : 0.0f, share = ldexpf(fabsf(weight), -weight_exponent(A.weight_top));
         if (lane == 0) {
-            A.reg_bias[n] = alive ? log2f(share) - lse2 : -INFINITY;
+            const bool away = alive && fabsf(lse2) > kAwayFrom;
+            A.reg_bias[n] = alive ? log2f(share) - (away ? log2f(all) : lse2) : -INFINITY;
+            A.away[n] = away ? -peak : 0.0f;
             A.target_log[n] = alive ? log2f(share * (rest / all)) : -INFINITY;
-            A.meta[n] = alive ? (int32_t)t | (weight < 0.0f ? kNegative : 0) : kNoTarget;
+            A.meta[n] = alive ? (int32_t)t | (weight < 0.0f ? kNegative : 0) | (away ? kAway : 0) : kNoTarget;
         }
         if (!A.dx)
             return;
@@ -1904,7 +1932,7 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
         mw.exps = W.take<int32_t>(vt * 4);
         mx.exps = W.take<int32_t>(nt * (C.grad ? 4 : 32 * 4));
     }
-    float *const stats = W.take<float>((int64_t)row_splits * 3 * nr * 4), *reg_bias = nullptr, *target_log = nullptr, *item_stats = nullptr, *part = nullptr;
+    float *const stats = W.take<float>((int64_t)row_splits * 3 * nr * 4), *reg_bias = nullptr, *target_log = nullptr, *away = nullptr, *item_stats = nullptr, *part = nullptr;
     if (C.grad) {
         mw.by_col = W.take<char>(vt * col_unit);
         mx.by_col = W.take<char>(nt * col_unit);
@@ -1917,6 +1945,7 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
         }
         reg_bias = W.take<float>(nt * 32 * 4 + kOneTileMore);
         target_log = W.take<float>(nt * 32 * 4 + kOneTileMore);
+        away = W.take<float>(nr * 4);
         const int64_t rows_part = row_splits * nr * KP * 4, items_part = item_splits > 1 ? item_splits * vr * KP * 4 : 0;
         part = W.take<float>(rows_part > items_part ? rows_part : items_part);   // (the rows' is read before the items' is written)
         if (item_splits > 1)
@@ -1958,6 +1987,7 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
     F.col_top = mw.col_top;
     F.reg_bias = reg_bias;
     F.target_log = target_log;
+    F.away = away;
     F.meta = P.meta;
     F.dx = C.dx;
     F.rows = nr;
@@ -1979,6 +2009,7 @@ template <class Y, int KO, int ODD> int64_t run_narrow(const Call &C)
     A.reg_bias = reg_bias;
     A.lane_bias = P.bias2;
     A.target_log = target_log;
+    A.away = away;
     A.stats = item_stats;
     A.still_tiles = v_tiles;
     A.still_rows = vr;
@@ -2044,6 +2075,7 @@ template <class Y> int64_t run_wide(const Call &C)
         mx.by_col = S.take<char>(nt * unit);
         F.reg_bias = S.take<float>(nt * 32 * 4);
         F.target_log = S.take<float>(nt * 32 * 4);
+        F.away = S.take<float>(nr * 4);
         P.zeros = 1;
         P.zero = mx.weight_top = S.take<uint32_t>(4);
         dw_part = S.take<float>(dw_splits_of(chunk) > 1 || dw_splits_of(last) > 1 ? dw_rows * KP * 4 : 4);
@@ -2084,6 +2116,7 @@ template <class Y> int64_t run_wide(const Call &C)
     finish_rows_kernel<Y, true><<<blocks_of((nr + 3) / 4), 256, 0, C.st>>>(F);
     A.reg_bias = F.reg_bias;
     A.target_log = F.target_log;
+    A.away = F.away;
     for (int64_t v0 = 0; v0 < v_tiles; v0 += chunk) {
         A.v0 = v0;
         A.v_count = v_tiles - v0 < chunk ? v_tiles - v0 : chunk;

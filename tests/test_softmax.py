@@ -821,3 +821,47 @@ def _check_products(ops, n, k, kind):
 @pytest.mark.parametrize("n", [40, 150])
 def test_rows_far_from_zero_by_their_products(ops, n, kind):
     _check_products(ops, n, 50, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("n", [40, 150])
+def test_wide_rows_far_from_zero(ops, n, kind):
+    """Rows over 256 wide, whose dx comes from the shares that the items' gradients come from."""
+    _check_away(ops, n, 300, kind)
+    _check_products(ops, n, 300, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [50, 200, 300])
+def test_items_of_rows_far_from_zero(ops, k, kind):
+    """The items' gradients too know only differences of logits, and the rows' weights."""
+    for away in AWAY + (300.0, -5000.0):
+        c, e, b = _away(150, k, kind, away)
+        if abs(away) < 1e6:      # (there logits keep their own differences: up to a 32-bit step of `away`, twice)
+            b = {name: x + 8 * U * abs(away) * (e["g"].abs().sum(dim=0)[:, None] * 0.1 if name == "ditems" else e["g"].abs().sum(dim=0)) if name in ("ditems", "dbias") else x for name, x in b.items()}
+            e = _exact(**c)
+        _, _, ditems, dbias = softmax.softmax_nll_grad(ops, **c)
+        _close((ditems, dbias), e, b, ("ditems", "dbias"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [50, 300])
+def test_an_item_far_above_the_others(ops, k, kind):
+    """It has every row's share, with its row's weight: what it gets is the sum of the others' weights, to their rounding.  (A logit of z
+    is rounded to U z, in both passes by itself; from 1e8 on the products are lost in it, and it is the bias in both.)"""
+    for above in (200.0, 5e3, 1e6, 1e8, 1e9, 1e20):
+        c = _case(150, 300, k, kind, True, seed=72)
+        c["bias"][17] = above
+        c["target"][2::5] = 17
+        c["weight"] = torch.exp2(torch.round(c["weight"] * 3))
+        loss, dx, ditems, dbias = softmax.softmax_nll_grad(ops, **c)
+        w = torch.where((c["target"] >= 0) & (c["target"] != 17), c["weight"].double(), 0.0)
+        assert bool((loss[c["target"] == 17] == 0).all()) and bool(torch.isfinite(dx).all()) and bool(torch.isfinite(ditems).all())
+        step = 4 * U * above if above < 1e7 else 0.0
+        assert abs(float(dbias[17]) / float(w.sum()) - 1) <= 64 * U + step, above
+        want = c["scale"] * (w @ c["x"].double())
+        slack = abs(c["scale"]) * (w @ c["x"].double().abs()) * (64 * U + step + 2 * HALF[kind])
+        assert bool(((ditems[17].double() - want).abs() <= slack).all()), above
