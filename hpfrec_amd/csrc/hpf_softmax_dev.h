@@ -1375,6 +1375,10 @@ struct FewArgs {
     float c, sign;
 };
 
+// The tiles that are read 16 bytes a lane, at 32-bit offsets from the tile's start: 32 rows follow each (see `load`).  Items 2^24 values
+// apart or more -- a few thousand fill the memory -- are read value by value.
+__device__ __forceinline__ int64_t few_fast(const FewArgs &A) { return A.V >= 64 && A.ldw < (1 << 24) ? (A.V - 32) / 32 : 0; }
+
 // 8 values as words
 template <class T> struct Raw { uint32_t v[2 * sizeof(T)]; };
 typedef uint32_t Chunk __attribute__((ext_vector_type(4)));
@@ -1508,7 +1512,7 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__((FewShape<Y, QB,
     __shared__ float join[Z::waves][QB][3][32];
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t step = (int64_t)gridDim.x * Z::waves, fast = A.V >= 64 ? (A.V - 32) / 32 : 0;
+    const int64_t step = (int64_t)gridDim.x * Z::waves, fast = few_fast(A);
     char *const own = lds + Z::rows_bytes + wave * Z::own;
 
     // chunk p = 64 i + lane of a tile: row p / NC, bytes 16 (p % NC) on.  A row's last chunks reach beyond its end: where 32 rows or more
@@ -1623,7 +1627,7 @@ template <class Y, int QB> __global__ __launch_bounds__(512, 2) void few_wide_ke
     __shared__ float join[waves][QB][3][32];
     const int lane = threadIdx.x & 63, low = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t step = (int64_t)gridDim.x * waves, fast = A.V >= 64 ? (A.V - 32) / 32 : 0;
+    const int64_t step = (int64_t)gridDim.x * waves, fast = few_fast(A);
     const int parts = (A.K + columns - 1) / columns;
     char *const own = lds[wave];
 
@@ -2164,8 +2168,8 @@ template <class Y> int64_t run_wide(const Call &C)
     return (int)hipGetLastError();
 }
 
-// a few rows, no gradients (Y as the products take it: W32 for 32 bits)
-template <class Y> bool is_few(const Call &C) { return !C.grad && C.n <= 64 && C.ldw < (1 << 24); }
+// a few rows, no gradients (a choice by what the workspace's size is asked for with, so not by strides)
+inline bool is_few(const Call &C) { return !C.grad && C.n <= 64; }
 // of so many values shared memory has room for the rows and a tile
 template <class Y> bool few_are_wide(const Call &C) { return C.k > (Y::S == 1 ? 256 : 128); }
 

@@ -3,7 +3,7 @@
 
 int64_t hpf_softmax::run_f16(const Call &C)
 {
-    if (is_few<H16>(C))
+    if (is_few(C))
         return run_few<H16>(C);
     return C.k <= 256 ? run_any_narrow<H16>(C) : run_wide<H16>(C);
 }

@@ -865,3 +865,35 @@ def test_an_item_far_above_the_others(ops, k, kind):
         want = c["scale"] * (w @ c["x"].double())
         slack = abs(c["scale"]) * (w @ c["x"].double().abs()) * (64 * U + step + 2 * HALF[kind])
         assert bool(((ditems[17].double() - want).abs() <= slack).all()), above
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="shows, without a GPU, that nothing is refused ahead of the first launch")
+@pytest.mark.parametrize("n, v, k, kind", [(4, 1000, 50, 0), (64, 500, 100, 0), (64, 40, 300, 0), (4, 300, 200, 1), (64, 3000, 300, 2)])
+def test_a_workspace_of_the_size_asked_for_is_enough_for_every_stride(n, v, k, kind):
+    L = ctypes.CDLL(_lib.build())
+    vp, i64, ci, cf = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+    L.hpf_hip_softmax_workspace.argtypes, L.hpf_hip_softmax_workspace.restype = [i64, i64, i64, ci, ci, ci], i64
+    L.hpf_hip_softmax_nll.argtypes = [vp, i64, vp, i64, vp, vp, cf, i64, i64, i64, ci, vp, vp, vp, i64, ci, vp]
+    buf = ctypes.create_string_buffer(1024)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    size = L.hpf_hip_softmax_workspace(n, v, k, kind, 0, 256)
+    for ld in (k, 2 ** 24 - 1, 2 ** 24, 2 ** 33):
+        rc = L.hpf_hip_softmax_nll(p, k, p, ld, p, None, 1.0, n, v, k, kind, p, None, p, size, 256, None)
+        assert rc > 0, ld      # the runtime's word that there is no device; -1 would be a refusal
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [4, 64])
+@pytest.mark.parametrize("v, k, kind", [(40, 300, F32), (150, 100, F32), (300, 200, BF16), (70, 600, F16), (66, 31, BF16)])
+def test_few_rows_of_items_far_apart(ops, n, v, k, kind):
+    """Items 2^24 values apart and one value less, for the paths that take a few rows."""
+    c = _case(n, v, k, kind, True, seed=n + v + k)
+    args = {a: b for a, b in c.items() if a != "weight"}
+    e = _exact(**c)
+    b = _bounds(e, kind, c["bias"], c["scale"], k, 4.0)
+    for ld in (2 ** 24, 2 ** 24 - 1):
+        flat = torch.empty((v - 1) * ld + k, dtype=kind, device="cuda:0")
+        far = flat.as_strided((v, k), (ld, 1))
+        far.copy_(c["items"])
+        _close(softmax.softmax_nll(ops, **dict(args, items=far)), e, b, ("loss", "lse"))
+        del flat, far
