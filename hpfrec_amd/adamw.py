@@ -84,7 +84,7 @@ def adamw_step(ops, params, grads, m, v, step, masters=None, m_scale=None, v_sca
     device = step.device if torch.is_tensor(step) else None
     if device is None or step.dtype != torch.int64 or step.numel() != 1:
         raise ValueError("step must be an int64 tensor of one element")
-    if device != ops.device and (ops.device.index is not None or device.type != ops.device.type):
+    if device != ops.device:
         raise ValueError("step is on %s, expected %s" % (device, ops.device))
     if torch.is_tensor(lr):
         if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:

@@ -98,7 +98,9 @@ class HipOps:
         if not torch.cuda.is_available():
             raise _lib.HpfHipError("hpfrec_amd: no ROCm device visible (torch.cuda.is_available() is False); "
                                    "the HIP path has no CPU fallback")
-        self.device = torch.device(device if device is not None else "cuda:%d" % torch.cuda.current_device())
+        self.device = torch.device(device if device is not None else "cuda")
+        if self.device.index is None:      # the current one as of now: tensors and launches are held against it
+            self.device = torch.device(self.device.type, torch.cuda.current_device())
         self.L = _lib.lib()
         with torch.cuda.device(self.device):
             self.cu_count, self.arch = _lib.device_info()
@@ -111,13 +113,11 @@ class HipOps:
 
     def _on_device(self):
         """A context in which launches go to this object's device (nothing to do where it is the current one)."""
-        index = self.device.index
-        return _NOTHING if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
+        return _NOTHING if self.device.index == torch.cuda.current_device() else torch.cuda.device(self.device.index)
 
     def _stream(self):
         # (what current_stream(...).cuda_stream gives, without the 2 us of making a Stream object of it)
-        index = self.device.index
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     # -- every method mirrors one C entry point ------------------------------------------
     def sweep(self, side, tab_self, tab_other, part, k, ld, acc_rows=None, acc_ld=0, grid_blocks=None):

@@ -40,7 +40,7 @@ def _vector(t, name, ops, dtype, n):
 
 
 def _on(t, name, ops):
-    if t.device != ops.device and (ops.device.index is not None or t.device.type != ops.device.type):
+    if t.device != ops.device:
         raise ValueError("%s is on %s, expected %s" % (name, t.device, ops.device))
 
 

@@ -438,3 +438,15 @@ def test_more_than_2_to_the_32_values(ops):
     (want, _, _), (bound, _, _) = _wide(torch.tensor(0.25), torch.tensor(f(1e-3)), torch.tensor(0.0), torch.tensor(0.0), t=1)
     for i in (0, 2 ** 31, 2 ** 32 - 1, 2 ** 32, n - 1):
         assert abs(float(p[i]) - float(want)) <= float(bound)
+
+
+def test_a_step_on_another_device_is_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = _Recorder()
+    for device in ("cuda", "cuda:0"):
+        ops.device = torch.device(device)
+        with FakeTensorMode():
+            p = [torch.empty(5, 3, device="cuda:1")]
+            with pytest.raises(ValueError, match="expected cuda"):
+                adamw.adamw_step(ops, p, [torch.empty(5, 3, device="cuda:1")], **adamw.adamw_state(p))
+    assert ops.calls == []

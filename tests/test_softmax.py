@@ -897,3 +897,32 @@ def test_few_rows_of_items_far_apart(ops, n, v, k, kind):
         far.copy_(c["items"])
         _close(softmax.softmax_nll(ops, **dict(args, items=far)), e, b, ("loss", "lse"))
         del flat, far
+
+
+@pytest.mark.parametrize("device", ["cuda", "cuda:0"])
+@pytest.mark.parametrize("call", [softmax.softmax_nll, softmax.softmax_nll_grad])
+def test_tensors_of_another_device_are_refused(call, device):
+    """Also where the operators' device was given without a number, and where one tensor alone is elsewhere."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops = _Recorder()
+    ops.device = torch.device(device)
+    with FakeTensorMode():
+        for at in (("cuda:1",) * 4, ("cuda:0", "cuda:1", "cuda:0", "cuda:0"), ("cuda:0", "cuda:0", "cuda:1", "cuda:0"), ("cuda:0",) * 3 + ("cuda:1",)):
+            args = dict(x=torch.empty(4, 5, device=at[0]), items=torch.empty(7, 5, device=at[1]), target=torch.empty(4, dtype=torch.int64, device=at[2]),
+                        bias=torch.empty(7, device=at[3]))
+            with pytest.raises(ValueError, match="expected cuda"):
+                call(ops, **args)
+    assert ops.calls == []
+
+
+def test_operators_without_a_device_number_are_those_of_the_current_device(monkeypatch):
+    import contextlib
+    from hpfrec_amd import ops_hip
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(_lib, "lib", lambda: None)
+    monkeypatch.setattr(_lib, "device_info", lambda: (256, "gfx950"))
+    for given in (None, "cuda", torch.device("cuda"), "cuda:3"):
+        assert ops_hip.HipOps(given).device == torch.device("cuda", 3)
+    assert ops_hip.HipOps("cuda:1").device == torch.device("cuda", 1)
