@@ -84,7 +84,8 @@ template <class Y> struct Parts { typename Y::m::v8 p[Y::S]; };   // 8 values of
 template <class Y> __device__ __forceinline__ void split(float x, Parts<Y> &to, int j)
 {
     typedef typename Y::m::e e;
-    to.p[0][j] = (e)x;
+    // (three bfloat16 parts: a value above bfloat16's largest would round to infinity and leave minus infinity)
+    to.p[0][j] = (e)(Y::S == 3 ? __builtin_amdgcn_fmed3f(x, -0x1.FEp127f, 0x1.FEp127f) : x);
     if constexpr (Y::S > 1) {
         const float r = x - (float)to.p[0][j];
         to.p[1][j] = (e)r;

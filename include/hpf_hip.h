@@ -737,7 +737,9 @@ int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors, int param_
  *   - An item whose bias is below -5.9e37 (-2^126 ln 2; -inf, or the type's lowest value) is masked: probability zero,
  *     whatever its row holds.  So is a single logit down there.  A row whose target is masked -- or everything -- has loss
  *     +inf and takes no part in the gradients; lse of nothing is -inf.
- *   - NaN and +inf logits of other items give NaN losses and gradients; so do weights that are infinite or NaN.
+ *   - NaN and +inf logits of other items give NaN losses and gradients; so do weights that are infinite or NaN.  An infinite
+ *     value of x or items that takes part gives logits of NaN in HPF_F32 (whose values are multiplied in parts), in the other
+ *     types what its products are -- -inf is masked -- and gradients of NaN in all.
  *   - float32, k <= 256: values below 2^-17 of the largest of their 32 rows (of 32 consecutive rows of items, or of x in the
  *     gradients) or of their column are held to 2^-40 of it.  HPF_F16, k > 256: G below 2^-38 of the largest weight is zero.
  * workspace: hpf_hip_softmax_workspace bytes (same sizes, type, grad and cu_count) at a multiple of 256; free again when

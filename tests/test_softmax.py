@@ -926,3 +926,53 @@ def test_operators_without_a_device_number_are_those_of_the_current_device(monke
     for given in (None, "cuda", torch.device("cuda"), "cuda:3"):
         assert ops_hip.HipOps(given).device == torch.device("cuda", 3)
     assert ops_hip.HipOps("cuda:1").device == torch.device("cuda", 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n, k", [(40, 50), (40, 300), (100, 50), (100, 300)])
+def test_the_largest_32_bit_values(ops, n, k):
+    """Items up to the largest number of the type -- its upper 2^-8 is beyond bfloat16 --, rows small enough for ordinary logits."""
+    gen = torch.Generator(device="cuda:0").manual_seed(9)
+    items = torch.zeros((200, k), device="cuda:0")
+    items[:, 0] = torch.finfo(F32).max * (1 - 2.0 ** -8 * torch.rand(200, device="cuda:0", generator=gen))
+    items[::2, 0] *= -1
+    items[0, 0] = torch.finfo(F32).max
+    x = torch.zeros((n, k), device="cuda:0")
+    x[:, 0] = 2.0 ** -125 * (1 + torch.arange(n, device="cuda:0") % 4)     # (one set bit or two: its second part is zero)
+    target = torch.arange(n, device="cuda:0") % 200
+    e = _exact(x, items, target, None, None, 1.0)
+    b = _bounds(e, F32, None, 1.0, k)
+    _close(softmax.softmax_nll(ops, x, items, target), e, b, ("loss", "lse"))
+    loss, _, ditems, _ = softmax.softmax_nll_grad(ops, x, items, target)
+    _close((loss,), e, b, ("loss",))
+    assert bool(torch.isfinite(ditems).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("n, k", [(40, 50), (40, 300), (100, 50), (100, 300)])
+def test_infinite_values(ops, n, k, kind):
+    """32 bits: logits of NaN.  16 bits: what the products are, so that -inf is masked."""
+    c = _case(n, 200, k, kind, True, seed=33)
+    c["x"][:, 3] = c["x"][:, 3].abs() + 0.25
+    live = c["target"] >= 0
+    c["target"] = torch.where(live & (c["target"] == 70), 71, c["target"])
+    c["items"][70, 3] = -float("inf")
+    nll = {a: b for a, b in c.items() if a != "weight"}
+    loss, lse = softmax.softmax_nll(ops, **nll)
+    if kind == F32:
+        assert bool(torch.isnan(loss[live]).all()) and bool(torch.isnan(lse).all())
+        assert bool(torch.isnan(softmax.softmax_nll_grad(ops, **c)[0][live]).all())
+    else:
+        bias = c["bias"].clone()
+        bias[70] = -float("inf")
+        want = softmax.softmax_nll(ops, **dict(nll, bias=bias))
+        assert torch.equal(loss, want[0]) and torch.equal(lse, want[1])
+        loss, dx, _, _ = softmax.softmax_nll_grad(ops, **c)
+        assert torch.equal(loss, softmax.softmax_nll_grad(ops, **dict(c, bias=bias))[0]) and bool(torch.isnan(dx[live, 3]).all())
+    c["items"][70, 3] = float("inf")
+    assert bool(torch.isnan(softmax.softmax_nll(ops, **nll)[0][live]).all())
+    c["items"][70, 3] = 0.0
+    c["x"][6, 3] = float("inf")          # one row alone
+    loss = softmax.softmax_nll(ops, **nll)[0]
+    assert math.isnan(float(loss[6])) and bool(torch.isfinite(loss[torch.arange(n, device="cuda:0") != 6]).all())
