@@ -32,6 +32,7 @@ namespace {
 constexpr int kBlock = 256;              // values per wavefront pass = values per scale of an 8-bit moment
 constexpr int kAtOnce = 2;               // blocks of a wavefront in flight
 constexpr int kMaxTensors = 40;          // per launch: their descriptors travel in the kernel's arguments
+constexpr int64_t kMaxBlocks = 0x7FFFFF00;   // per launch, and per tensor: 2^39 values, less 2^16
 constexpr int kTicketShift = 40;         // the step counter's upper bits count the workgroups that are done
 constexpr int kMaxGrid = 1 << 22;        // what fits there
 
@@ -355,6 +356,8 @@ extern "C" int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors,
             return HPF_EINVAL;
         if (t.n == 0)
             continue;
+        if ((t.n - 1) / kBlock >= kMaxBlocks)
+            return HPF_EUNSUPPORTED;           // (here, so that a refused call has changed nothing)
         if (!t.param || !t.grad || !t.m || !t.v || (param_type != HPF_F32) != (t.master != nullptr))
             return HPF_EINVAL;
         if (state_bits == 8 ? (!t.m_scale || !t.v_scale) : (t.m_scale || t.v_scale))
@@ -380,11 +383,8 @@ extern "C" int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors,
             if (t.n == 0)
                 continue;
             const int64_t mine = (t.n + kBlock - 1) / kBlock;
-            if (blocks + mine > 0x7FFFFF00) {
-                if (blocks == 0)
-                    return HPF_EUNSUPPORTED;   // one tensor of over 2^38 values
+            if (blocks + mine > kMaxBlocks)
                 break;
-            }
             Tensor &d = A.t[A.ntensors++];
             d.p = t.param;
             d.g = t.grad;

@@ -450,3 +450,19 @@ def test_a_step_on_another_device_is_refused():
             with pytest.raises(ValueError, match="expected cuda"):
                 adamw.adamw_step(ops, p, [torch.empty(5, 3, device="cuda:1")], **adamw.adamw_state(p))
     assert ops.calls == []
+
+
+def test_c_entry_refuses_a_tensor_that_is_too_large_before_it_moves_any():
+    """A tensor of over 2^39 - 2^16 values behind an ordinary one: refused ahead of every launch, which would give the runtime's word
+    that there is no device (and on one would read these host addresses)."""
+    from hpfrec_amd.ops_hip import AdamwTensor
+    L = ctypes.CDLL(_lib.build())
+    vp, ci, cd = ctypes.c_void_p, ctypes.c_int, ctypes.c_double
+    L.hpf_hip_adamw_step.argtypes = [vp, ci, ci, ci, ci, vp, ci, vp, cd, cd, cd, cd, ctypes.c_uint64, ci, vp]
+    buf = ctypes.create_string_buffer(256)
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    if torch.cuda.is_available():
+        pytest.skip("shown without a GPU")
+    for n in (2 ** 39 - 2 ** 16 + 1, 2 ** 39, 2 ** 62, 2 ** 63 - 1):
+        d = (AdamwTensor * 2)((p, p, p, p, None, None, None, 3, 0.0, 0, 0), (p, p, p, p, None, None, None, n, 0.0, 1, 0))
+        assert L.hpf_hip_adamw_step(d, 2, 0, 0, 32, p, 1, None, 1e-3, 0.9, 0.999, 1e-8, 0, 8, None) == -2, n
