@@ -10,7 +10,7 @@ import math
 
 import torch
 
-from .ops_hip import TYPE_CODES
+from .ops_hip import TYPE_CODES, changed
 
 #: consecutive values of an 8-bit moment that share a scale (HPF_ADAMW_BLOCK)
 BLOCK = 256
@@ -71,7 +71,8 @@ def adamw_step(ops, params, grads, m, v, step, masters=None, m_scale=None, v_sca
                   in the list, index) alone, so that equal calls give equal results
 
     Tensors of different types may share a call; those of one combination of types share launches.  No two of them may
-    overlap.  Empty tensors are allowed."""
+    overlap.  Empty tensors are allowed.  Parameters may require gradients: the step is no part of their graph, but moves
+    their version, so that a backward pass that still needs the old values says so."""
     count = len(params)
     for name, x in (("grads", grads), ("m", m), ("v", v), ("masters", masters), ("m_scale", m_scale), ("v_scale", v_scale)):
         if x is not None and len(x) != count:
@@ -139,3 +140,4 @@ def adamw_step(ops, params, grads, m, v, step, masters=None, m_scale=None, v_sca
     last = len(groups) - 1
     for j, ((ptype, gtype, bits), tensors) in enumerate(groups.items()):
         ops.adamw_step(tensors, ptype, gtype, bits, step, j == last, lr, b1, b2, eps, seed)
+    changed([*params, *masters] if masters is not None else params)

@@ -91,6 +91,11 @@ AdamwTensor = _adamw_tensor_struct()
 TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+def changed(tensors):
+    """Tells torch that a kernel has written these tensors (None among them: nothing): their version moves, as by an in-place operation."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None and not t.is_inference()])
+
+
 class HipOps:
     name = "hip"
 

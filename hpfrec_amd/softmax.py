@@ -3,14 +3,15 @@
 
 Logits are scale * <x[n], items[v]> + bias[v]; they are made and used in pieces and never stored.  Results are torch tensors on
 the device of `ops`; calls are asynchronous on the current stream, take their scratch memory from torch's allocator and keep
-nothing.  The definitions, and what happens to rows without a target, masked items and NaN, are in include/hpf_hip.h
+nothing.  They are no part of autograd's graph: results require no gradients, whatever the inputs do, and
+softmax_nll_grad gives them.  The definitions, and what happens to rows without a target, masked items and NaN, are in include/hpf_hip.h
 (hpf_hip_softmax_nll, hpf_hip_softmax_nll_grad).
 """
 import math
 
 import torch
 
-from .ops_hip import TYPE_CODES
+from .ops_hip import TYPE_CODES, changed
 
 
 def _matrix(t, name, ops, dtype=None, shape=None):
@@ -122,4 +123,6 @@ def softmax_nll_grad(ops, x, items, target, weight=None, bias=None, scale=1.0, d
                 raise ValueError("dx, ditems or dbias overlaps another tensor of the call")
     loss = torch.empty(n, dtype=torch.float32, device=x.device)
     ops.softmax_nll_grad(x, ldx, items, ldi, target, weight, bias, float(scale), n, v, k, loss, dx, lddx, ditems, lddi, dbias)
+    if given:
+        changed(given)
     return loss, dx, ditems, dbias

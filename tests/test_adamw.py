@@ -466,3 +466,16 @@ def test_c_entry_refuses_a_tensor_that_is_too_large_before_it_moves_any():
     for n in (2 ** 39 - 2 ** 16 + 1, 2 ** 39, 2 ** 62, 2 ** 63 - 1):
         d = (AdamwTensor * 2)((p, p, p, p, None, None, None, 3, 0.0, 0, 0), (p, p, p, p, None, None, None, n, 0.0, 1, 0))
         assert L.hpf_hip_adamw_step(d, 2, 0, 0, 32, p, 1, None, 1e-3, 0.9, 0.999, 1e-8, 0, 8, None) == -2, n
+
+
+def test_parameters_are_known_to_have_changed():
+    p = [torch.full((5, 3), 2.0, requires_grad=True), torch.ones(4, dtype=torch.bfloat16)]
+    st = adamw.adamw_state(p)
+    late = (p[0] * p[0]).sum()                  # its backward pass needs the parameter as it was
+    _call(params=p, grads=[torch.ones(5, 3), torch.ones(4)], **st)
+    assert p[0]._version == p[1]._version == st["masters"][1]._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        late.backward()
+    with torch.inference_mode():
+        p = [torch.ones(3)]
+        _call(params=p, grads=[torch.ones(3)], **adamw.adamw_state(p))

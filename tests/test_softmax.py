@@ -976,3 +976,20 @@ def test_infinite_values(ops, n, k, kind):
     c["x"][6, 3] = float("inf")          # one row alone
     loss = softmax.softmax_nll(ops, **nll)[0]
     assert math.isnan(float(loss[6])) and bool(torch.isfinite(loss[torch.arange(n, device="cuda:0") != 6]).all())
+
+
+def test_given_outputs_are_known_to_have_changed_and_no_graph_is_made():
+    a = _good(x=torch.ones(4, 5, requires_grad=True), items=torch.ones(7, 5, requires_grad=True))
+    loss, lse = softmax.softmax_nll(**a)
+    out = dict(dx=torch.ones(4, 8)[:, :5], ditems=torch.ones(7, 5), dbias=torch.ones(7))
+    got = softmax.softmax_nll_grad(**a, **out)
+    assert not any(t.requires_grad for t in (loss, lse) + got)
+    assert all(t._version == 1 for t in out.values()) and a["x"]._version == a["items"]._version == a["bias"]._version == 0
+    table = torch.full((7, 5), 2.0, requires_grad=True)
+    late = (table * table).sum()                # its backward pass needs the table as it was
+    with torch.no_grad():
+        softmax.softmax_nll_grad(**a, ditems=table)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        late.backward()
+    with torch.inference_mode():
+        softmax.softmax_nll_grad(**a, ditems=torch.ones(7, 5))
