@@ -9,6 +9,8 @@ int64_t run(int type, const Call &C) { return type == HPF_F32 ? hpf_softmax::run
 
 bool sizes_ok(int64_t n, int64_t v, int64_t k) { return n >= 0 && v > 0 && k > 0 && n < hpf_softmax::kNoTarget - 31 && v < hpf_softmax::kNoTarget - 31 && k < (1 << 20); }
 
+bool scale_ok(float scale) { return fabsf(scale) < 0x1p127f; }    // (times log2(e) it is a number)
+
 }  // namespace
 
 extern "C" int64_t hpf_hip_softmax_workspace(int64_t n, int64_t v, int64_t k, int type, int grad, int cu_count)
@@ -32,7 +34,7 @@ extern "C" int hpf_hip_softmax_nll(const void *x, int64_t ldx, const void *items
                                    float scale, int64_t n, int64_t v, int64_t k, int type, float *loss, float *lse, void *workspace,
                                    int64_t workspace_bytes, int cu_count, void *stream)
 {
-    if (!sizes_ok(n, v, k) || cu_count <= 0 || ldx < k || ld_items < k)
+    if (!sizes_ok(n, v, k) || cu_count <= 0 || ldx < k || ld_items < k || !scale_ok(scale))
         return HPF_EINVAL;
     if (type < HPF_F32 || type > HPF_F16)
         return HPF_EUNSUPPORTED;
@@ -65,7 +67,7 @@ extern "C" int hpf_hip_softmax_nll_grad(const void *x, int64_t ldx, const void *
                                         float *loss, void *dx, int64_t ld_dx, void *ditems, int64_t ld_ditems, float *dbias, void *workspace,
                                         int64_t workspace_bytes, int cu_count, void *stream)
 {
-    if (!sizes_ok(n, v, k) || cu_count <= 0 || ldx < k || ld_items < k || ld_dx < k || ld_ditems < k)
+    if (!sizes_ok(n, v, k) || cu_count <= 0 || ldx < k || ld_items < k || ld_dx < k || ld_ditems < k || !scale_ok(scale))
         return HPF_EINVAL;
     if (type < HPF_F32 || type > HPF_F16)
         return HPF_EUNSUPPORTED;

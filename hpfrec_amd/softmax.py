@@ -7,8 +7,6 @@ nothing.  They are no part of autograd's graph: results require no gradients, wh
 softmax_nll_grad gives them.  The definitions, and what happens to rows without a target, masked items and NaN, are in include/hpf_hip.h
 (hpf_hip_softmax_nll, hpf_hip_softmax_nll_grad).
 """
-import math
-
 import torch
 
 from .ops_hip import TYPE_CODES, changed
@@ -61,8 +59,8 @@ def _inputs(ops, x, items, target, bias, scale):
     _vector(target, "target", ops, torch.int64, n)
     if bias is not None:
         _vector(bias, "bias", ops, torch.float32, v)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if not abs(scale) < 2.0 ** 127:      # (32 bits hold it times log2(e))
+        raise ValueError("scale must be a number below 2^127 in size")
     return n, v, k, ldx, ldi
 
 

@@ -730,7 +730,7 @@ int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors, int param_
  *   z[i][j] = scale <x[i], items[j]> + bias[j];   lse[i] = log sum_j exp z[i][j];   loss[i] = lse[i] - z[i][target[i]]
  *   G[i][j] = weight[i] (exp(z[i][j] - lse[i]) - [j == target[i]])
  *   dx = scale G items;   ditems = scale G^T x;   dbias[j] = sum_i G[i][j]
- * x [n][k] and items [v][k], both of `type` (HPF_F32 / HPF_BF16 / HPF_F16), with row strides in values; target int64;
+ * |scale| < 2^127.  x [n][k] and items [v][k], both of `type` (HPF_F32 / HPF_BF16 / HPF_F16), with row strides in values; target int64;
  * weight (NULL: ones), bias (NULL: none), loss, lse (nll only, may be NULL) and dbias (given exactly when bias is) float32.
  * Sums and statistics are float32; dx and ditems are rounded once, to `type`.  Equal calls give equal results.
  *   - target < 0: loss 0; target >= v: loss NaN.  Neither takes part in the gradients, whatever its x holds.

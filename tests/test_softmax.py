@@ -993,3 +993,27 @@ def test_given_outputs_are_known_to_have_changed_and_no_graph_is_made():
         late.backward()
     with torch.inference_mode():
         softmax.softmax_nll_grad(**a, ditems=torch.ones(7, 5))
+
+
+@pytest.mark.parametrize("call", [softmax.softmax_nll, softmax.softmax_nll_grad])
+@pytest.mark.parametrize("scale", [1e39, -1e39, 3.5e38, 1e300, 2.0 ** 127, -3e38])
+def test_scales_that_32_bits_do_not_hold_are_refused(call, scale):
+    a = _good(scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        call(**a)
+    assert a["ops"].calls == []
+    call(**_good(scale=-1.7e38))
+
+
+def test_c_entries_refuse_such_a_scale():
+    if torch.cuda.is_available():
+        pytest.skip("shown without a GPU: a call that is not refused would read host addresses")
+    L = ctypes.CDLL(_lib.build())
+    vp, i64, ci, cf = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+    L.hpf_hip_softmax_nll.argtypes = [vp, i64, vp, i64, vp, vp, cf, i64, i64, i64, ci, vp, vp, vp, i64, ci, vp]
+    L.hpf_hip_softmax_nll_grad.argtypes = [vp, i64, vp, i64, vp, vp, vp, cf, i64, i64, i64, ci, vp, vp, i64, vp, i64, vp, vp, i64, ci, vp]
+    buf = ctypes.create_string_buffer(1024)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    for scale in (float("inf"), -float("inf"), float("nan"), 2.0 ** 127):
+        assert L.hpf_hip_softmax_nll(p, 5, p, 5, p, None, scale, 4, 7, 5, 0, p, None, p, 1 << 40, 256, None) == -1
+        assert L.hpf_hip_softmax_nll_grad(p, 5, p, 5, p, None, None, scale, 4, 7, 5, 0, p, p, 5, p, 5, None, p, 1 << 40, 256, None) == -1
