@@ -96,7 +96,7 @@ def adamw_step(ops, params, grads, m, v, step, masters=None, m_scale=None, v_sca
     decay = [float(weight_decay)] * count if one else [float(w) for w in weight_decay]
     if len(decay) != count or not all(math.isfinite(w) and w >= 0.0 for w in (decay[:1] if one else decay)):
         raise ValueError("weight_decay must be a finite number that is not negative, or one for each of params")
-    groups, written, read = {}, [(step.data_ptr(), 8)], []
+    groups, written, read = {}, [(step.data_ptr(), 8)], [(lr.data_ptr(), 4, "lr")] if torch.is_tensor(lr) else []
     for i in range(count):
         p = params[i]
         at = _held(p, "params", i, getattr(p, "shape", None), _PARAM_TYPES, device)
@@ -126,15 +126,15 @@ def adamw_step(ops, params, grads, m, v, step, masters=None, m_scale=None, v_sca
             written.append((at_w, 4 * n))
         if eight:
             written += [(at_ms, 4 * scales[0]), (at_vs, 4 * scales[0])]
-        read.append((g, (4 if grads[i].dtype == torch.float32 else 2) * n))
+        read.append((g, (4 if grads[i].dtype == torch.float32 else 2) * n, "a gradient"))
         groups.setdefault((p.dtype, grads[i].dtype, 8 if eight else 32), []).append((at, g, at_m, at_v, at_w, at_ms, at_vs, n, decay[i], i, 0))
     written.sort()
     if any(a + size > b for (a, size), (b, _) in zip(written, written[1:])):
         raise ValueError("two of the tensors that the step writes overlap")
-    for a, size in read:
+    for a, size, name in read:
         j = bisect.bisect_left(written, (a + size,))
         if j and written[j - 1][0] + written[j - 1][1] > a:
-            raise ValueError("a gradient overlaps a tensor that the step writes")
+            raise ValueError("%s overlaps a tensor that the step writes" % name)
     if not groups:
         groups[torch.float32, torch.float32, 32] = []   # nothing to move, yet a step
     last = len(groups) - 1

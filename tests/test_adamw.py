@@ -479,3 +479,13 @@ def test_parameters_are_known_to_have_changed():
     with torch.inference_mode():
         p = [torch.ones(3)]
         _call(params=p, grads=[torch.ones(3)], **adamw.adamw_state(p))
+
+
+def test_a_rate_inside_what_the_step_writes_is_refused():
+    p = torch.ones(8)
+    st = adamw.adamw_state([p])
+    for lr in (p[3:4], st["m"][0][:1], st["v"][0][7:]):
+        with pytest.raises(ValueError, match="lr overlaps"):
+            _call(params=[p], grads=[torch.ones(8)], lr=lr, **st)
+    g = torch.full((8,), 1e-3)
+    assert len(_call(params=[p], grads=[g], lr=g[:1], **st)) == 1      # read twice: allowed
