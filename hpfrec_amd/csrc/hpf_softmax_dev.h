@@ -233,12 +233,13 @@ __device__ __forceinline__ void largest_weight(const Matrix &M, int64_t tile, ui
         atomicMax(M.weight_top, __float_as_uint(top));
 }
 
-// G is held as a share of the power of two above every |weight| (2^-100 .. 2^100; 1 where there is none or no finite one)
+// G is held as a share of the power of two above every |weight| (2^-100 .. 2^127, so that no share is above two; 1 where there is none or
+// no finite weight)
 __device__ __forceinline__ int weight_exponent(const uint32_t *top)
 {
     const uint32_t bits = *top;
     const int e = (int)(bits >> 23) - 126;
-    return bits == 0 || bits >= 0x7F800000u ? 0 : e > 100 ? 100 : e < -100 ? -100 : e;
+    return bits == 0 || bits >= 0x7F800000u ? 0 : e > 127 ? 127 : e < -100 ? -100 : e;
 }
 
 // Largest magnitudes of the columns of both matrices; a wavefront reads whole rows, 8 at a time.  One workgroup of 16 wavefronts a
@@ -568,8 +569,9 @@ __device__ __forceinline__ void take_target(f32x16 &x, float c, int tile, int h,
             }
 }
 
-// The logarithm of a share as it comes out of the roundings of its logit and its row's lse: no share is above one.  (NaN stays.)
-__device__ __forceinline__ float share_log(float x) { return __builtin_elementwise_minimum(x, 0.0f); }
+// The logarithm of a share as it comes out of the roundings of its logit and its row's lse: no share is above two (weight_exponent).
+// (NaN stays.)
+__device__ __forceinline__ float share_log(float x) { return __builtin_elementwise_minimum(x, 1.0f); }
 
 __device__ __forceinline__ void store_stats(float *to, int64_t rows, int h, const Held &held, const Sum &sum, float at)
 {

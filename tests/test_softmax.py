@@ -1017,3 +1017,21 @@ def test_c_entries_refuse_such_a_scale():
     for scale in (float("inf"), -float("inf"), float("nan"), 2.0 ** 127):
         assert L.hpf_hip_softmax_nll(p, 5, p, 5, p, None, scale, 4, 7, 5, 0, p, None, p, 1 << 40, 256, None) == -1
         assert L.hpf_hip_softmax_nll_grad(p, 5, p, 5, p, None, None, scale, 4, 7, 5, 0, p, p, 5, p, 5, None, p, 1 << 40, 256, None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [50, 300])
+@pytest.mark.parametrize("power", [-120, -100, 98, 110, 125])
+def test_weights_of_any_size(ops, power, k, kind):
+    """Largest weights of 2^power to 2^(power + 2), and a scale that brings the tables' gradients back to ordinary sizes (logits are biases)."""
+    c = _case(90, 300, k, kind, True, seed=81)
+    c["weight"] = (c["weight"].clamp(-2, 2) * 2.0 ** power).float()
+    c["scale"] = 2.0 ** (-power if power > 0 else 0)
+    e = _exact(**c)
+    b = _bounds(e, kind, c["bias"], c["scale"], k, 2 * float(c["weight"].abs().max()))
+    _, dx, ditems, dbias = softmax.softmax_nll_grad(ops, **c)
+    # sums of numbers below the normal ones; and a result below 2^-126 is rounded by up to half of the type's least number, which for
+    # bfloat16 (7 bits of mantissa) is 2^-133 (half precision's 2^-24 is in the bounds)
+    least = 2.0 ** -149 * 90 + (2.0 ** -134 if kind == BF16 else 0.0)
+    _close((dx, ditems, dbias), e, {name: x + least for name, x in b.items()}, ("dx", "ditems", "dbias"))
