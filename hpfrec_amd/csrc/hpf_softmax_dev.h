@@ -49,7 +49,7 @@ namespace hpf_softmax {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 constexpr float kNothing = -0x1p126f;     // a running maximum before anything: logits (base 2) at or below it are masked
-constexpr int kNoTarget = 0x3FFFFFFF;     // block 2^25 of 32 items: beyond every catalogue
+constexpr int kNoTarget = 0x3FFFFFFF;     // in tile 2^25 - 1 of 32 items: the one behind the largest catalogue's last
 constexpr int kNegative = 0x40000000;     // flags beside a row's target: its weight is negative
 constexpr int kAway = -0x7FFFFFFF - 1;    //   its lse is over kAwayFrom in size: see FinishArgs::away
 constexpr int kTarget = 0x3FFFFFFF;       //   the target itself
@@ -512,7 +512,8 @@ __device__ __forceinline__ float sum16(const f32x16 &x)
 
 // What a stationary row's exponentials are held relative to: they are 2^(z + down), and at most 2^shift.  `down` is a whole number, so that
 // rescaling changes no digit.  far: the same for all lanes, some of which hold logits so large that floats lie a whole number or more
-// apart and the shift would be lost in them: their largest is held as one, and every logit is rounded as the largest was.
+// apart and the shift would be lost in them: their largest is held as one, and every logit is rounded as the largest was (later blocks
+// come with c = 1).
 constexpr float kFar = 0x1p23f;
 struct Held {
     float down;
@@ -541,12 +542,12 @@ template <class Y, class F> __device__ __forceinline__ void exponentials(f32x16 
         held.down = down;
         held.far = __any(fabsf(down) >= kFar && down < -kNothing);
         rescale(f);
-    }
-    if (held.far) {
+        if (held.far) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            x[i] *= c;
-        c = 1.0f;
+            for (int i = 0; i < 16; ++i)
+                x[i] *= c;
+            c = 1.0f;
+        }
     }
     const float down = held.down < -kNothing ? held.down : -INFINITY;     // (nothing yet: all of it is masked)
 #pragma unroll
@@ -690,7 +691,7 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
                         x[4 * i + j] = share_log((fmaf(x[4 * i + j], c, lane_bias) + away[j]) + b[j]);
                 }
                 c = 1.0f;
-            } else if (biased || __any(c == 0.0f)) {
+            } else if (biased || held.far || __any(c == 0.0f)) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const f32x4 b = *(const f32x4 *)(side + (8 * i + 4 * h) * 4);
@@ -806,7 +807,8 @@ __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, O
 // ---------------------------------------------------------------------------------------------------------------------
 // Rows too wide for a wavefront's registers (k > 256): plain tiled products of packed matrices, the catalogue in chunks.  The
 // statistics come from a first run over all logits; then, chunk by chunk, G is written in both operand layouts (16-bit parts,
-// a chunk at a time: at most kChunkBytes) and multiplied with the items (dx, summed over the chunks) and with x (dw).
+// a chunk at a time) and multiplied with the items (dx, summed over the chunks) and with x (dw).  Rows are not cut, so a chunk is
+// kChunkBytes or, from a million rows on (350k in 32 bits), the least that a workgroup takes, 256 items: 1 KB a row, 3 in 32 bits.
 // Bound by the matrix instructions: 8 N V K operations.  Logits are made in 256 x 128 outputs a workgroup and 128 x 64 a wavefront,
 // two workgroups a compute unit: six operands read from shared memory for eight products (four for four, 64 x 64, keep shared
 // memory as busy as the matrix units).  2,048 x 50,001 of 1000 in half precision: statistics 247 us, G 252 us (0.83 and 0.81
