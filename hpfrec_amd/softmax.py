@@ -89,7 +89,9 @@ def _span(t):
 
 def softmax_nll_grad(ops, x, items, target, weight=None, bias=None, scale=1.0, dx=None, ditems=None, dbias=None):
     """(loss, dx, ditems, dbias): softmax_nll's loss of each event, and the gradients of sum_n weight[n] * loss[n] in x, items and
-    (None without a bias) bias.  dx and ditems are of x's type, each value rounded once; loss and dbias are float32.
+    (None without a bias) bias.  dx and ditems are of x's type; loss and dbias are float32.  Sums are float32 and results are rounded
+    once; with 16-bit tables each event's factor in a sum is rounded to their type before (by up to 2^-8 of it in bfloat16, 2^-11
+    in float16), as the tables are.
 
     weight  float32 [n] or None (ones); any sign
     dx, ditems, dbias  tensors to write to (dx and ditems may have a stride between rows; what lies between is left as it is);

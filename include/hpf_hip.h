@@ -732,7 +732,9 @@ int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors, int param_
  *   dx = scale G items;   ditems = scale G^T x;   dbias[j] = sum_i G[i][j]
  * |scale| < 2^127.  x [n][k] and items [v][k], both of `type` (HPF_F32 / HPF_BF16 / HPF_F16), with row strides in values; target int64;
  * weight (NULL: ones), bias (NULL: none), loss, lse (nll only, may be NULL) and dbias (given exactly when bias is) float32.
- * Sums and statistics are float32; dx and ditems are rounded once, to `type`.  Equal calls give equal results.
+ * Sums and statistics are float32, each result is rounded once, to `type`.  What is multiplied with items and x is G, as a share of its
+ * row's largest, its item's or the largest weight: in HPF_BF16 and HPF_F16 rounded to that type (up to 2^-8 or 2^-11 of each term,
+ * of either sign), in HPF_F32 held in two or three parts.  Equal calls give equal results.
  *   - target < 0: loss 0; target >= v: loss NaN.  Neither takes part in the gradients, whatever its x holds.
  *   - An item whose bias is below -5.9e37 (-2^126 ln 2; -inf, or the type's lowest value) is masked: probability zero,
  *     whatever its row holds.  So is a single logit down there.  A row whose target is masked -- or everything -- has loss
@@ -742,8 +744,8 @@ int hpf_hip_adamw_step(const hpf_adamw_tensor *tensors, int ntensors, int param_
  *     types what its products are -- -inf is masked -- and gradients of NaN in all.
  *   - float32, k <= 256: values below 2^-17 of the largest of their 32 rows (of 32 consecutive rows of items, or of x in the
  *     gradients) or of their column are held to 2^-40 of it.  HPF_F16, k > 256: G below 2^-38 of the largest weight is zero.
- * workspace: hpf_hip_softmax_workspace bytes (same sizes, type, grad and cu_count) at a multiple of 256; free again when
- * the call's work is done.  n, v < 2^30 - 32, k < 2^20.  cu_count: compute units the launch grids are made for.
+ * workspace: hpf_hip_softmax_workspace bytes (same sizes, type, grad and cu_count; enough for any strides) at a multiple of 256; free
+ * again when the call's work is done.  n, v < 2^30 - 32, k < 2^20.  cu_count: compute units the launch grids are made for.
  */
 int64_t hpf_hip_softmax_workspace(int64_t n, int64_t v, int64_t k, int type, int grad, int cu_count);
 int hpf_hip_softmax_nll(const void *x, int64_t ldx, const void *items, int64_t ld_items, const int64_t *target,
