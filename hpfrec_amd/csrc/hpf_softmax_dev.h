@@ -589,9 +589,10 @@ __device__ __forceinline__ float times_power(float x, float e) { return ldexpf(x
 
 // Bound by the matrix instructions where rows are wide and by the exponentials where they are narrow: a logit costs a wavefront's lane
 // about ten vector instructions and an exponential, and the two kinds of instruction were seen to take turns rather than to overlap
-// (raised priorities changed nothing, logits made a tile ahead beside the exponentials cost 1 to 8 per cent).  8,192 x 380k of 100 in
-// 32 bits: rows 3.40 ms, items 3.57 ms, 1.10 and 1.05 PFLOP/s of half-precision products, while one of 8192 x 8192 x 8192 of the
-// library runs at 1.16; loss alone, of 50: 1.25 ms.  8,192 x 100k of 200 in bf16: 0.71 and 0.78 ms, 0.92 and 0.84 PFLOP/s.
+// (raised priorities changed nothing, logits made a tile ahead beside the exponentials cost 1 to 8 per cent).  Least and mean of six calls,
+// 8,192 x 380k of 100 in 32 bits: rows 3.45 and 3.59 ms, items 3.58 and 3.75 ms, 1.04 and 1.00 PFLOP/s of half-precision products in the mean,
+// while one of 8192 x 8192 x 8192 of the library runs at 1.16; loss alone, of 50: 1.28 and 1.43 ms.  8,192 x 100k of 200 in bf16: 0.72 and
+// 0.76, 0.80 and 0.84 ms, 0.86 and 0.78 PFLOP/s.  Rows away from zero (kAway) cost the items 2 to 8 per cent of the call.
 template <class Y, int KO, int ODD, int MODE>
 __global__ __launch_bounds__((Shape<Y, KO, ODD, MODE>::NW * 64), (Shape<Y, KO, ODD, MODE>::waves)) void pass_kernel(PassArgs A)
 {
@@ -1367,8 +1368,9 @@ template <class Y, bool GRAD> __global__ __launch_bounds__(256) void finish_rows
 // wavefront reads a tile of 32 items as it lies in the table, 16 bytes a lane and neighbours side by side (reading operands -- 16 bytes
 // of each row -- fetched every line four times), turns it into operands through shared memory of its own, and splits it as it goes;
 // the rows lie in shared memory as operands.  (Three bfloat16 parts for 32-bit matrices: they need no scale, and the matrix
-// instructions have time to spare.)  61 rows, 380k items of 100 in bf16, 76 MB: 29 us, 2.6 TB/s with the launch's start and end (a
-// sum of a large tensor reads 4.0 TB/s), 42 by operands; one row, 27k of 50 in 32 bits: 8 us, which is latency.
+// instructions have time to spare.)  61 rows, 380k items of 100 in bf16, 76 MB: 30 us, 2.5 TB/s with the launch's start and end (a
+// sum of a large tensor reads 4.0 TB/s), 42 by operands; one row, 27k of 50 in 32 bits: 8 us.  Against 64 items alone they take 12 and 7.6 us:
+// the last one or two tiles, their biases and the end of the rows' operands are read value by value, each waited for before the next.
 // ---------------------------------------------------------------------------------------------------------------------
 struct FewArgs {
     const void *x, *w;
@@ -1623,7 +1625,8 @@ template <class Y, int QB, int CB> __global__ __launch_bounds__((FewShape<Y, QB,
 }
 
 // The same for wider rows, 64 columns at a time; the rows, packed by a launch of their own, come from the caches.  One row, 380k items of
-// 1000 in 32 bits, 1.5 GB: 395 us, 3.84 TB/s; 50k, fewer tiles than wavefronts: 114 us, bound by the latency of a wavefront's parts.
+// 1000 in 32 bits, 1.5 GB: 395 us, 3.84 TB/s; 50k, fewer tiles than wavefronts: 100 us; 64: 66 us,
+// which is the last tiles' value by value.
 template <class Y, int QB> __global__ __launch_bounds__(512, 2) void few_wide_kernel(FewArgs A)
 {
     typedef typename Y::t T;
