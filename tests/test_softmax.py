@@ -1035,3 +1035,41 @@ def test_weights_of_any_size(ops, power, k, kind):
     # bfloat16 (7 bits of mantissa) is 2^-133 (half precision's 2^-24 is in the bounds)
     least = 2.0 ** -149 * 90 + (2.0 ** -134 if kind == BF16 else 0.0)
     _close((dx, ditems, dbias), e, {name: x + least for name, x in b.items()}, ("dx", "ditems", "dbias"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("n, k", [(20, 50), (300, 50), (300, 300)])
+def test_far_and_near_pieces_of_a_long_catalogue(ops, n, k, kind):
+    """Most items far below, a few near zero in one piece of the catalogue alone, the targets among either: shares are those of the
+    near ones, and the far pieces' sums vanish beside them.  Then one item far above all: it has every share."""
+    v, near = 30000, torch.arange(17000, 17040, device="cuda:0")
+    c = _case(n, v, k, kind, True, seed=91)
+    bias = torch.full((v,), -1e8, device="cuda:0")
+    bias[near] = c["bias"][near]
+    live = c["target"] >= 0
+    c["target"] = torch.where(live, near[torch.arange(n, device="cuda:0") % 40], c["target"])
+    c["target"][7] = 3                       # far, whatever the others
+    few = dict(c, items=c["items"][near], bias=bias[near], target=torch.where(live, c["target"] - 17000, c["target"]))
+    few["target"][7] = -1
+    e = _exact(**few)
+    b = _bounds(e, kind, few["bias"], c["scale"], k, 2 * float(c["weight"].abs().max()))
+    (loss, lse), (gloss, dx, ditems, dbias) = _both(ops, dict(c, bias=bias))
+    rest = torch.arange(n, device="cuda:0") != 7
+    _close((torch.where(rest, loss, 0.0), lse), e, b, ("loss", "lse"))
+    _close((torch.where(rest, gloss, 0.0), torch.where(rest[:, None], dx, 0.0)), e, b, ("loss", "dx"))
+    assert abs(float(loss[7]) / 1e8 - 1) < 1e-6 and bool(torch.isfinite(dx[7]).all())
+    g7 = c["weight"][7] * torch.softmax(e["z"][7], 0)       # row 7's shares, which `few` left out
+    got = ditems[near].double() - c["scale"] * g7[:, None] * c["x"][7].double()
+    assert bool(((got - e["ditems"]).abs() <= b["ditems"] + (2 * HALF[kind] + 1e-4) * (abs(c["scale"]) * g7.abs()[:, None] * c["x"][7].double().abs() + e["ditems"].abs())).all())
+    assert bool(((dbias[near].double() - g7 - e["dbias"]).abs() <= b["dbias"] + 1e-4 * g7.abs()).all())
+    far = torch.ones(v, dtype=torch.bool, device="cuda:0")
+    far[near] = False
+    far[3] = False
+    assert not bool(ditems[far].any()) and not bool(dbias[far].any())
+    assert abs(float(dbias[3]) + float(c["weight"][7])) <= 64 * U * abs(float(c["weight"][7]))
+    bias[29990] = 3e8
+    (loss, lse), (_, _, ditems, dbias) = _both(ops, dict(c, bias=bias))
+    w = torch.where(live, c["weight"].double(), 0.0)
+    assert bool(((lse.double() / 3e8 - 1).abs() <= 8 * U).all()) and abs(float(dbias[29990]) - float(w.sum())) <= 64 * U * float(w.abs().sum())
+    assert bool(((ditems[29990].double() - c["scale"] * (w @ c["x"].double())).abs() <= abs(c["scale"]) * (w.abs() @ c["x"].double().abs()) * (64 * U + 2 * HALF[kind])).all())
