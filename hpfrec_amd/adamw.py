@@ -7,6 +7,7 @@ include/hpf_hip.h (hpf_hip_adamw_step).
 """
 import bisect
 import math
+import numbers
 
 import torch
 
@@ -92,7 +93,7 @@ def adamw_step(ops, params, grads, m, v, step, masters=None, m_scale=None, v_sca
             raise ValueError("lr must be a number or a float32 tensor of one element on %s" % device)
     elif not (math.isfinite(lr) and lr >= 0.0):
         raise ValueError("lr must be finite and not negative")
-    one = isinstance(weight_decay, (int, float))
+    one = isinstance(weight_decay, (int, float)) or isinstance(weight_decay, numbers.Real)
     decay = [float(weight_decay)] * count if one else [float(w) for w in weight_decay]
     if len(decay) != count or not all(math.isfinite(w) and w >= 0.0 for w in (decay[:1] if one else decay)):
         raise ValueError("weight_decay must be a finite number that is not negative, or one for each of params")

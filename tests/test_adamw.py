@@ -489,3 +489,8 @@ def test_a_rate_inside_what_the_step_writes_is_refused():
             _call(params=[p], grads=[torch.ones(8)], lr=lr, **st)
     g = torch.full((8,), 1e-3)
     assert len(_call(params=[p], grads=[g], lr=g[:1], **st)) == 1      # read twice: allowed
+
+
+@pytest.mark.parametrize("number", [np.float32(0.25), np.float64(0.25), np.int64(1), 1, True])
+def test_numbers_of_numpy_are_numbers(number):
+    assert len(_call(weight_decay=number, lr=number)) == 2
